@@ -164,7 +164,7 @@ def _plain_recurrence(s):
         return {"h": h[0].to(dt), "h_n": h_n}
     if case["mode"] == "forward":
         return {"h": h.to(dt), "h_n": h_n}
-    g = s["dh"].float()
+    g = s["dh"].to(torch.float32, copy=True)
     g[-1] += s["dh_n"]
     after = torch.cat((keep[1:], torch.zeros_like(keep[:1])))
     e = _scan(after.flip(0), g.flip(0)).flip(0)
