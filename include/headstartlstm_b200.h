@@ -50,7 +50,8 @@ enum {
   HS_ERR_WORKSPACE = 2,     /* workspace missing or smaller than required     */
   HS_ERR_UNSUPPORTED = 3,   /* shape outside what the kernels implement       */
   HS_ERR_CUDA = 4,          /* a CUDA runtime call or launch failed           */
-  HS_ERR_DEVICE_TIMEOUT = 5 /* a device-side bounded wait gave up             */
+  HS_ERR_DEVICE_TIMEOUT = 5, /* a device-side bounded wait gave up            */
+  HS_ERR_INDEX = 6           /* a token id outside its table or vocabulary    */
 };
 
 /* Library identity and diagnostics. */
@@ -468,6 +469,94 @@ HS_API int hs_recurrent_backward_bf16(const float *x, const float *w_ih, const f
                                       float *dw_hh, float *db_ih, float *db_hh, float *da, int64_t T,
                                       int64_t B, int64_t D, int64_t H, void *workspace,
                                       size_t workspace_bytes, int *dev_status, hs_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Language-model operators: what a model of token sequences needs before,
+ * beside and after the recurrent layers above.  No counterpart in the
+ * reference, whose package holds the recurrent layer alone.
+ *
+ * Tensors of these calls are float32, bfloat16 or float16 (`dtype`, one type
+ * for all `void *` tensors of a call) and aligned to their element; all
+ * arithmetic, states and sums are float32.  Extents may be 0.  Every result
+ * has one fixed order of operations: the same bits from run to run.
+ * ---------------------------------------------------------------------- */
+enum { HS_F32 = 0, HS_BF16 = 1, HS_F16 = 2 };
+enum {
+  HS_RECURRENCE_GATED = 0, /* f = sigmoid(z), b = (1 - f) x */
+  HS_RECURRENCE_LINEAR = 1 /* f = z, b = x                  */
+};
+
+/* Gated linear recurrence along time,
+ *   h_t = f_t k_t h_{t-1} + b_t,   k_t = 0 where starts[t][b] != 0, else 1,
+ * from the state h0 [B,H] (NULL = zeros).  z, x and h are [T,B,H] with the
+ * last axis contiguous; *_t and *_b are the element strides of a step and of a
+ * sequence, so [B,T,H] tensors and slices of wider ones are passed as they
+ * are.  starts (NULL = none) are bytes with strides starts_t, starts_b: a step
+ * marked so begins a new sequence and nothing before it, not even an infinity
+ * or NaN, reaches it.  h_n [B,H] (NULL = not wanted) is the state after the
+ * last step; it may be h0 itself.  checkpoints (NULL = no backward will
+ * follow): hs_recurrence_checkpoint_bytes(T, B, H) bytes for the backward.
+ * T = 1 is the single-token step of serving. */
+HS_API size_t hs_recurrence_checkpoint_bytes(int64_t T, int64_t B, int64_t H);
+HS_API int hs_recurrence_forward(int dtype, int form, const void *z, int64_t z_t, int64_t z_b, const void *x,
+                                 int64_t x_t, int64_t x_b, const float *h0, const unsigned char *starts,
+                                 int64_t starts_t, int64_t starts_b, void *h, int64_t h_t, int64_t h_b,
+                                 float *h_n, float *checkpoints, int64_t T, int64_t B, int64_t H,
+                                 hs_stream_t stream);
+/* Its gradient: dh [T,B,H] and dh_n [B,H] (either may be NULL = zeros) to dz,
+ * dx [T,B,H] and dh0 [B,H] (NULL = not wanted).  Reads the forward's
+ * checkpoints, not h: the states are recomputed in float32. */
+HS_API int hs_recurrence_backward(int dtype, int form, const void *z, int64_t z_t, int64_t z_b, const void *x,
+                                  int64_t x_t, int64_t x_b, const float *checkpoints,
+                                  const unsigned char *starts, int64_t starts_t, int64_t starts_b,
+                                  const void *dh, int64_t dh_t, int64_t dh_b, const float *dh_n, void *dz,
+                                  int64_t dz_t, int64_t dz_b, void *dx, int64_t dx_t, int64_t dx_b, float *dh0,
+                                  int64_t T, int64_t B, int64_t H, hs_stream_t stream);
+
+/* out[n] = scale * weight[tokens[n]], weight [V,D] with rows weight_ld
+ * elements apart, out [N,D].  tokens are 64-bit (token_bits = 64) or 32-bit
+ * whole numbers.  An id outside [0, V) gives a row of zeros and sets
+ * HS_ERR_INDEX in *dev_status. */
+HS_API int hs_embedding_forward(int dtype, const void *weight, int64_t weight_ld, int token_bits,
+                                const void *tokens, double scale, void *out, int64_t N, int64_t V, int64_t D,
+                                int *dev_status, hs_stream_t stream);
+/* dweight[v] = scale * sum of dout[n] over the n with tokens[n] = v, in the
+ * order of n, rounded once; rows of no token, and the row padding_idx (-1 =
+ * none), are zero.  dout [N,D], dweight [V,D], every element written.
+ * workspace: hs_embedding_workspace_bytes, 256-byte aligned. */
+HS_API size_t hs_embedding_workspace_bytes(int64_t N, int64_t V, int64_t D);
+HS_API int hs_embedding_backward(int dtype, const void *dout, int token_bits, const void *tokens,
+                                 int64_t padding_idx, double scale, void *dweight, int64_t N, int64_t V,
+                                 int64_t D, void *workspace, size_t workspace_bytes, int *dev_status,
+                                 hs_stream_t stream);
+
+/* Log probabilities of given tokens under softmax(logits / temperature), with
+ * the distribution's entropy and its `top` (0 to HS_MAX_TOP) most likely
+ * tokens.  logits [N,V], rows logits_ld elements apart.  logprob and entropy
+ * [N] in nats; top_logprob, top_index [N,top], ordered by logit, equal ones by
+ * the lower index; stats [N,2] for the backward (any of these but logprob may
+ * be NULL; top_* must be given where top > 0).
+ *   - A row whose token is ignore_index is not read: logprob, entropy and
+ *     top_logprob 0, top_index -1, gradient 0.
+ *   - Logits of -inf are masked out.  A row of nothing else: logprob and
+ *     top_logprob -inf, entropy 0, gradient 0.
+ *   - A row with a NaN or +inf: NaN everywhere, top_index -1.
+ *   - A token outside [0, V): NaN logprob, and HS_ERR_INDEX in *dev_status;
+ *     the rest of the row is unaffected, its gradient is that of the rest. */
+enum { HS_MAX_TOP = 32 };
+HS_API int hs_token_logprobs_forward(int dtype, const void *logits, int64_t logits_ld, int token_bits,
+                                     const void *tokens, int64_t ignore_index, float temperature, int top,
+                                     float *logprob, float *entropy, float *top_logprob, int64_t *top_index,
+                                     float *stats, int64_t N, int64_t V, int *dev_status, hs_stream_t stream);
+/* dlogits [N,V] (rows dlogits_ld apart) from the gradients of logprob,
+ * entropy [N] and top_logprob [N,top] (each may be NULL = zeros), with the
+ * forward's stats, entropy and top_index. */
+HS_API int hs_token_logprobs_backward(int dtype, const void *logits, int64_t logits_ld, int token_bits,
+                                      const void *tokens, int64_t ignore_index, float temperature, int top,
+                                      const float *stats, const float *entropy, const int64_t *top_index,
+                                      const float *dlogprob, const float *dentropy, const float *dtop_logprob,
+                                      void *dlogits, int64_t dlogits_ld, int64_t N, int64_t V,
+                                      hs_stream_t stream);
 
 #ifdef __cplusplus
 }

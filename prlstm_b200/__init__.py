@@ -11,6 +11,10 @@ return shapes.  The two hot paths run in ``libhsb200.so``:
 * parallel mode: input-projection GEMM, a fused activation + chunked
   decoupled-look-back scan over T, and its reverse-time counterpart.
 
+Beside the module, the operators that make a language model of it: the gated
+linear recurrence with general coefficients, the embedding with its gradient,
+and log probabilities of given tokens (``_lm_functions.py``).
+
 There is one implementation and no CPU fallback: tensors must live on a CUDA
 device; ``backend`` and ``compile_cell`` are accepted for signature
 compatibility and validated like the reference validates them.
@@ -26,6 +30,8 @@ import torch.nn as nn
 from . import _lib
 from ._functions import EPS, headstartlstm_parallel, headstartlstm_recurrent
 from ._lib import check_device_status, clear_device_status
+from ._lm_functions import (TokenLogprobs, embedding, gated_recurrence, gated_recurrence_step, linear_recurrence,
+                            linear_recurrence_step, token_logprobs)
 
 __version__ = "0.1.0"
 
@@ -129,4 +135,6 @@ def library_path() -> str:
 
 
 __all__ = ["HeadStartLSTM", "headstartlstm_recurrent", "headstartlstm_parallel",
+           "gated_recurrence", "gated_recurrence_step", "linear_recurrence", "linear_recurrence_step",
+           "embedding", "token_logprobs", "TokenLogprobs",
            "check_device_status", "clear_device_status", "library_path", "EPS", "__version__"]

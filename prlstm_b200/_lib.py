@@ -27,6 +27,7 @@ _c_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 _sz = ctypes.c_size_t
 
 # name -> (restype, argtypes); must match include/headstartlstm_b200.h
@@ -87,6 +88,19 @@ SIGNATURES = {
     "hs_recurrent_backward": (_i32, [_c_p] * 17 + [_i64] * 4 + [_c_p, _sz, _c_p, _c_p]),
     "hs_recurrent_forward_bf16": (_i32, [_c_p] * 11 + [_i64] * 4 + [_c_p, _sz, _c_p, _c_p]),
     "hs_recurrent_backward_bf16": (_i32, [_c_p] * 17 + [_i64] * 4 + [_c_p, _sz, _c_p, _c_p]),
+    "hs_recurrence_checkpoint_bytes": (_sz, [_i64] * 3),
+    "hs_recurrence_forward": (_i32, [_i32] * 2 + [_c_p, _i64, _i64] * 2 + [_c_p] + [_c_p, _i64, _i64] * 2
+                              + [_c_p] * 2 + [_i64] * 3 + [_c_p]),
+    "hs_recurrence_backward": (_i32, [_i32] * 2 + [_c_p, _i64, _i64] * 2 + [_c_p] + [_c_p, _i64, _i64] * 2 + [_c_p]
+                               + [_c_p, _i64, _i64] * 2 + [_c_p] + [_i64] * 3 + [_c_p]),
+    "hs_embedding_forward": (_i32, [_i32, _c_p, _i64, _i32, _c_p, _f64, _c_p] + [_i64] * 3 + [_c_p] * 2),
+    "hs_embedding_workspace_bytes": (_sz, [_i64] * 3),
+    "hs_embedding_backward": (_i32, [_i32, _c_p, _i32, _c_p, _i64, _f64, _c_p] + [_i64] * 3
+                              + [_c_p, _sz, _c_p, _c_p]),
+    "hs_token_logprobs_forward": (_i32, [_i32, _c_p, _i64, _i32, _c_p, _i64, _f32, _i32] + [_c_p] * 5 + [_i64] * 2
+                                  + [_c_p] * 2),
+    "hs_token_logprobs_backward": (_i32, [_i32, _c_p, _i64, _i32, _c_p, _i64, _f32, _i32] + [_c_p] * 7
+                                   + [_i64] * 3 + [_c_p]),
 }
 
 _lib = None
@@ -138,19 +152,32 @@ _status = {}
 _pending = {}
 
 
-def status_word(device: torch.device) -> torch.Tensor:
-    """Per-device sticky device-status int the kernels report bounded-wait
-    failures into."""
+def _status_words(device: torch.device):
+    """Per device: both status words as one tensor, and each as a view.  The
+    first is for bounded waits that gave up (a nonzero one makes later waits
+    give up at once); the second for token ids out of range, which must not
+    disturb them."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     t = _status.get(idx)
     if t is None:
-        t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
-        _status[idx] = t
+        both = torch.zeros(2, dtype=torch.int32, device=torch.device("cuda", idx))
+        t = _status[idx] = (both, both[:1], both[1:])
     return t
 
 
+def status_word(device: torch.device) -> torch.Tensor:
+    """Per-device sticky device-status int the kernels report bounded-wait
+    failures into."""
+    return _status_words(device)[1]
+
+
+def token_status_word(device: torch.device) -> torch.Tensor:
+    """Per-device sticky int the kernels report token ids out of range into."""
+    return _status_words(device)[2]
+
+
 def note_launch(device: torch.device):
-    """Queue an asynchronous read-back of the status word; the value is
+    """Queue an asynchronous read-back of the status words; the values are
     checked (without a sync) the next time the library is called.  Skipped
     while the stream is being captured into a CUDA graph (an event query is
     not allowed there): a graphed step reports through check_device_status."""
@@ -158,8 +185,8 @@ def note_launch(device: torch.device):
         return
     idx = device.index if device.index is not None else torch.cuda.current_device()
     poll(device)
-    host = torch.empty(1, dtype=torch.int32, pin_memory=True)
-    host.copy_(status_word(device), non_blocking=True)
+    host = torch.empty(2, dtype=torch.int32, pin_memory=True)
+    host.copy_(_status_words(device)[0], non_blocking=True)
     ev = torch.cuda.Event()
     ev.record()
     _pending[idx] = (host, ev)
@@ -181,22 +208,26 @@ def poll(device: torch.device):
     host, ev = item
     if ev.query():
         del _pending[idx]
-        if int(host.item()) != HS_OK:
-            _raise_status(int(host.item()))
+        for code in host.tolist():
+            if code != HS_OK:
+                _raise_status(code)
 
 
 def check_device_status(device=None):
-    """Synchronously read the device status word; raise if a kernel gave up."""
+    """Synchronously read the device status words; raise if a kernel gave up
+    or met a token id out of range."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    out = ctypes.c_int(-1)
-    call("hs_read_status", ptr(status_word(device)), ctypes.byref(out), stream_ptr(device))
-    if out.value != HS_OK:
-        _raise_status(out.value)
+    for word in (status_word(device), token_status_word(device)):
+        out = ctypes.c_int(-1)
+        call("hs_read_status", ptr(word), ctypes.byref(out), stream_ptr(device))
+        if out.value != HS_OK:
+            _raise_status(out.value)
 
 
 def clear_device_status(device=None):
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    call("hs_clear_status", ptr(status_word(device)), stream_ptr(device))
+    for word in (status_word(device), token_status_word(device)):
+        call("hs_clear_status", ptr(word), stream_ptr(device))
     idx = device.index if device.index is not None else torch.cuda.current_device()
     _pending.pop(idx, None)
 

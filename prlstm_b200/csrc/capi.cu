@@ -504,6 +504,7 @@ const char *hs_status_string(int status) {
     case HS_ERR_UNSUPPORTED: return "unsupported shape";
     case HS_ERR_CUDA: return "CUDA error";
     case HS_ERR_DEVICE_TIMEOUT: return "device-side wait timed out";
+    case HS_ERR_INDEX: return "token id out of range";
     default: return "unknown status";
   }
 }

@@ -1,0 +1,582 @@
+// Embedding lookup with scaling, and its gradient by sorted tokens.
+//
+//   out_n = s W[tok_n],   dW[v] = s sum_{n : tok_n = v} dout_n
+//
+// Bound: memory.  The lookup reads N rows and writes N rows; the gradient
+// reads the N rows of dout once and writes the V rows of dW once.
+//
+// Gradient, three launches:
+//   1. One cluster sorts the N ids with their positions (stable, least
+//      significant digit first, up to 9 bits a pass: two passes for any vocabulary
+//      below 2^18) and marks the ids that occur in a bitmap.
+//   2. Pieces of 32 consecutive sorted entries x 32 lanes of up to 16 bytes:
+//      each warp sums the runs of equal ids in its piece in float32.  A run
+//      inside the piece is a finished row of dW; one that crosses a piece
+//      boundary leaves its part in the workspace.  The work of a warp does not depend on
+//      how often a token occurs, so a frequent token costs no more than rare
+//      ones.  Further CTAs write the zero rows of the ids that do not occur.
+//   3. The parts of each crossing run are added in order.
+// dW is therefore written once (no clearing pass), there are no atomics on
+// floating-point data, and the order of every sum follows from the tokens alone.
+#include <algorithm>
+
+#include "lm_types.cuh"
+
+namespace hs {
+namespace {
+
+constexpr int kPiece = 32;        // sorted entries per warp of the summing kernel
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortCluster = 8;   // CTAs of the sorting cluster at most
+constexpr int kMaxBits = 9;       // bits of a sorting pass at most
+
+template <int BYTES> struct Chunk;  // one lane's bytes of a row
+template <> struct Chunk<16> { using type = uint4; };
+template <> struct Chunk<8> { using type = uint2; };
+template <> struct Chunk<4> { using type = unsigned; };
+template <> struct Chunk<2> { using type = unsigned short; };
+
+// The scale as a sum of two float32, so that a product with it is rounded
+// once although the scale (the root of a width, say) is no float32.
+struct Scale {
+  float hi, lo;
+};
+HS_DEV float scaled(float v, Scale s) { return fmaf(v, s.hi, v * s.lo); }
+Scale make_scale(double s) {
+  const float hi = (float)s;
+  const double lo = s - (double)hi;
+  return {hi, lo == lo && lo - lo == 0.0 ? (float)lo : 0.f};
+}
+
+template <typename T, int BYTES> HS_DEV void chunk_to_f32(const typename Chunk<BYTES>::type &c, float *v) {
+  if constexpr (BYTES == 2) {
+    v[0] = to_f32<T>(*reinterpret_cast<const T *>(&c));
+  } else {
+    const unsigned *w = reinterpret_cast<const unsigned *>(&c);
+#pragma unroll
+    for (int i = 0; i < BYTES / 4; ++i) unpack_word<T>(w[i], v + i * PerWord<T>::value);
+  }
+}
+template <typename T, int BYTES> HS_DEV typename Chunk<BYTES>::type chunk_of_f32(const float *v) {
+  typename Chunk<BYTES>::type c;
+  if constexpr (BYTES == 2) {
+    *reinterpret_cast<T *>(&c) = from_f32<T>(v[0]);
+  } else {
+    unsigned *w = reinterpret_cast<unsigned *>(&c);
+#pragma unroll
+    for (int i = 0; i < BYTES / 4; ++i) w[i] = pack_word<T>(v + i * PerWord<T>::value);
+  }
+  return c;
+}
+
+// ------------------------------------------------------------------ lookup
+// One thread per row chunk and four chunks per thread, a CTA's width apart.
+template <typename T, int BYTES, typename TOK>
+__global__ void __launch_bounds__(256) emb_lookup_kernel(const char *w, int64_t ld_bytes, const TOK *tok, Scale scale,
+                                                         char *out, int64_t total, int chunks, int64_t V, int *status) {
+  using C = typename Chunk<BYTES>::type;
+  constexpr int E = BYTES / (int)sizeof(T);
+  const int64_t i0 = (int64_t)blockIdx.x * (256 * 4) + threadIdx.x;
+  C c[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int64_t i = i0 + k * 256;
+    if (i < total) {
+      const int64_t n = i / chunks;
+      const int64_t t = (int64_t)tok[n];
+      if (t >= 0 && t < V) {
+        c[k] = *reinterpret_cast<const C *>(w + t * ld_bytes + (i - n * chunks) * BYTES);
+      } else {
+        c[k] = C{};
+        set_status(status, HS_ERR_INDEX);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int64_t i = i0 + k * 256;
+    if (i < total) {
+      float v[E];
+      chunk_to_f32<T, BYTES>(c[k], v);
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = scaled(v[e], scale);
+      *reinterpret_cast<C *>(out + i * BYTES) = chunk_of_f32<T, BYTES>(v);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ sort
+HS_DEV void cluster_sync_all() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+HS_DEV void st_cluster_u32(const void *p, int rank, unsigned v) {
+  const unsigned a = (unsigned)__cvta_generic_to_shared(p);
+  asm volatile(
+      "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, %1;\n\tst.shared::cluster.u32 [r], %2;\n\t}" ::"r"(a),
+      "r"(rank), "r"(v)
+      : "memory");
+}
+
+struct SortArgs {
+  const void *tok;
+  int64_t N, V, pad;
+  unsigned *key[2], *pos[2];
+  unsigned *seen;     // bitmap of the ids that occur
+  int passes, bits;
+  int *status;
+};
+
+// A stable counting sort per pass.  Every warp owns a contiguous part of the
+// entries: it counts its digits, the counts are added up over warps, CTAs and
+// digits, and it then places its entries in order, so entries of one digit
+// keep their order.  Ids out of range and the padding id sort as V, last.
+template <typename TOK>
+__global__ void __launch_bounds__(kSortThreads, 1) emb_sort_kernel(const SortArgs p) {
+  extern __shared__ __align__(16) unsigned sm[];
+  const int D = 1 << p.bits;
+  unsigned *hist = sm;                         // [warps][D]
+  unsigned *tot = hist + kSortWarps * D;       // [cluster][D], written by the cluster's CTAs
+  unsigned *base = tot + kSortCluster * D;     // [D]
+  __shared__ unsigned wsum[kSortWarps];
+  const int C = gridDim.x, rank = blockIdx.x;  // one cluster
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t per = (p.N + (int64_t)C * kSortThreads - 1) / ((int64_t)C * kSortThreads) * 32;
+  const int64_t lo = min(p.N, ((int64_t)rank * kSortWarps + warp) * per), hi = min(p.N, lo + per);
+  const int64_t words = (p.V + 31) / 32;
+  for (int64_t i = (int64_t)rank * kSortThreads + tid; i < words; i += (int64_t)C * kSortThreads) p.seen[i] = 0;
+  const TOK *tok = static_cast<const TOK *>(p.tok);
+  for (int pass = 0; pass < p.passes; ++pass) {
+    const int shift = pass * p.bits;
+    const unsigned *ksrc = p.key[(pass + 1) & 1], *psrc = p.pos[(pass + 1) & 1];
+    unsigned *kdst = p.key[pass & 1], *pdst = p.pos[pass & 1];
+    auto key_at = [&](int64_t i) -> unsigned {
+      if (pass) return __ldcg(ksrc + i);
+      const int64_t t = (int64_t)tok[i];
+      if (t >= 0 && t < p.V) return t == p.pad ? (unsigned)p.V : (unsigned)t;
+      set_status(p.status, HS_ERR_INDEX);
+      return (unsigned)p.V;
+    };
+    unsigned *h = hist + warp * D;
+    for (int i = lane; i < D; i += 32) h[i] = 0;
+    __syncwarp();
+    for (int64_t b = lo; b < hi; b += 32) {
+      const bool ok = b + lane < hi;
+      const unsigned dig = ok ? (key_at(b + lane) >> shift) & (D - 1) : 0xffffffffu;
+      const unsigned same = __match_any_sync(0xffffffffu, dig);
+      if (ok && lane == __ffs(same) - 1) h[dig] += __popc(same);
+      __syncwarp();
+    }
+    if (pass == 0 && C > 1) cluster_sync_all();  // every CTA has started before its memory is written
+    __syncthreads();
+    if (tid < D) {  // over the warps of this CTA, then to every CTA
+      unsigned run = 0;
+      for (int w = 0; w < kSortWarps; ++w) {
+        const unsigned c = hist[w * D + tid];
+        hist[w * D + tid] = run;
+        run += c;
+      }
+      if (C == 1)
+        tot[tid] = run;
+      else
+        for (int r = 0; r < C; ++r) st_cluster_u32(tot + rank * D + tid, r, run);
+    }
+    if (C > 1) cluster_sync_all(); else __syncthreads();
+    unsigned before = 0, all = 0;
+    if (tid < D) {
+      for (int r = 0; r < C; ++r) {
+        const unsigned c = tot[r * D + tid];
+        if (r < rank) before += c;
+        all += c;
+      }
+    }
+    unsigned inc = all;  // exclusive sums over the digits
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    if (tid < D) {
+      unsigned less = 0;
+      for (int w = 0; w < warp; ++w) less += wsum[w];
+      base[tid] = less + inc - all + before;
+    }
+    __syncthreads();
+    for (int64_t b = lo; b < hi; b += 32) {
+      const bool ok = b + lane < hi;
+      const int64_t i = b + lane;
+      const unsigned key = ok ? key_at(i) : 0u;
+      const unsigned pos = ok ? (pass ? __ldcg(psrc + i) : (unsigned)i) : 0u;
+      const unsigned dig = ok ? (key >> shift) & (D - 1) : 0xffffffffu;
+      const unsigned same = __match_any_sync(0xffffffffu, dig);
+      unsigned at = 0;
+      if (ok) at = base[dig] + h[dig] + __popc(same & ((1u << lane) - 1u));
+      __syncwarp();
+      if (ok && lane == __ffs(same) - 1) h[dig] += __popc(same);
+      __syncwarp();
+      if (ok) {
+        kdst[at] = key;
+        pdst[at] = pos;
+      }
+    }
+    if (C > 1) cluster_sync_all(); else __syncthreads();
+  }
+  const unsigned *sk = p.key[(p.passes + 1) & 1];
+  for (int64_t i = lo + lane; i < hi; i += 32) {
+    const unsigned k = __ldcg(sk + i);
+    if (k < (unsigned)p.V && (i == 0 || __ldcg(sk + i - 1) != k)) atomicOr(p.seen + (k >> 5), 1u << (k & 31));
+  }
+}
+
+// ------------------------------------------------------------------ sums of runs
+struct SumArgs {
+  const unsigned *key, *pos, *seen;
+  const char *dout;
+  char *dw;
+  float *head, *tail;  // [pieces][D]: the part of a run that came in / goes on
+  int64_t N, V, D, pieces;
+  int slices;          // lane groups of a row
+  int chunks;          // lane chunks of a row
+  int64_t sum_blocks;  // CTAs of the sums; the others write zero rows
+  Scale scale;
+};
+
+template <typename T, int BYTES>
+__global__ void __launch_bounds__(256) emb_sum_kernel(const SumArgs p) {
+  using C = typename Chunk<BYTES>::type;
+  constexpr int E = BYTES / (int)sizeof(T);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row_bytes = p.D * (int64_t)sizeof(T);
+  if ((int64_t)blockIdx.x >= p.sum_blocks) {
+    // 32 ids per warp: rows of those that do not occur
+    const int64_t g = ((int64_t)blockIdx.x - p.sum_blocks) * 8 + warp;
+    if (g * 32 >= p.V) return;
+    unsigned none = ~p.seen[g];
+    if (g * 32 + 32 > p.V) none &= (1u << (p.V - g * 32)) - 1u;
+    const C zero = {};
+    while (none) {
+      const int r = __ffs(none) - 1;
+      none &= none - 1;
+      C *row = reinterpret_cast<C *>(p.dw + (g * 32 + r) * row_bytes);
+      for (int c = lane; c < p.chunks; c += 32) row[c] = zero;
+    }
+    return;
+  }
+  const int64_t unit = (int64_t)blockIdx.x * 8 + warp;
+  if (unit >= p.pieces * p.slices) return;
+  const int64_t piece = unit / p.slices;
+  const int chunk = (int)(unit - piece * p.slices) * 32 + lane;
+  const bool live = chunk < p.chunks;
+  const int64_t first = piece * kPiece, mine = first + lane;
+  const unsigned none = (unsigned)p.V;
+  const unsigned key = mine < p.N ? p.key[mine] : none;
+  const unsigned pos = mine < p.N ? p.pos[mine] : 0u;
+  const unsigned prev = first > 0 ? p.key[first - 1] : none;
+  const unsigned next = first + kPiece < p.N ? p.key[first + kPiece] : none;
+  const int count = __popc(__ballot_sync(0xffffffffu, key != none));  // valid entries come first
+  float acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  unsigned cur = __shfl_sync(0xffffffffu, key, 0);
+  bool from_prev = cur == prev;
+  constexpr int U = 8;
+  for (int j0 = 0; j0 < count; j0 += U) {
+    C c[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const unsigned n = __shfl_sync(0xffffffffu, pos, (j0 + u) & 31);
+      if (live && j0 + u < count) c[u] = *reinterpret_cast<const C *>(p.dout + (int64_t)n * row_bytes + (int64_t)chunk * BYTES);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (j0 + u >= count) break;
+      float v[E];
+      chunk_to_f32<T, BYTES>(c[u], v);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += v[e];
+      const int j = j0 + u;
+      const unsigned after = j + 1 < kPiece ? __shfl_sync(0xffffffffu, key, (j + 1) & 31) : next;
+      if (after != cur || j + 1 == kPiece) {  // the run, or its part in this piece, ends here
+        const bool goes_on = after == cur;
+        if (live) {
+          if (from_prev || goes_on) {
+            float *part = (from_prev ? p.head : p.tail) + piece * p.D + (int64_t)chunk * E;
+#pragma unroll
+            for (int e = 0; e < E; ++e) part[e] = acc[e];
+          } else {
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = scaled(acc[e], p.scale);
+            *reinterpret_cast<C *>(p.dw + (int64_t)cur * row_bytes + (int64_t)chunk * BYTES) = chunk_of_f32<T, BYTES>(acc);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = 0.f;
+        cur = after;
+        from_prev = false;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ crossing runs
+// A warp per piece whose last run goes on into the next piece and began in
+// this one: it adds the run's parts in order.  Runs over more than kLong
+// pieces are left to the whole CTA, each warp adding a contiguous share.
+constexpr int kJoinWarps = 16, kLong = 32;
+
+template <typename T, int BYTES>
+__global__ void __launch_bounds__(32 * kJoinWarps) emb_join_kernel(const SumArgs p) {
+  using C = typename Chunk<BYTES>::type;
+  constexpr int E = BYTES / (int)sizeof(T);
+  __shared__ float share[kJoinWarps][E][32];
+  __shared__ int64_t long_first, long_last;
+  __shared__ unsigned long_key;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t group = blockIdx.x / p.slices;
+  const int chunk = (int)(blockIdx.x % p.slices) * 32 + lane;
+  const bool live = chunk < p.chunks;
+  const int64_t piece = group * kJoinWarps + warp;
+  const unsigned none = (unsigned)p.V;
+  if (threadIdx.x == 0) long_first = -1;
+  __syncthreads();
+  auto add_heads = [&](int64_t a, int64_t b, float *acc) {  // head parts of pieces a..b
+    int64_t j = a;
+    for (; j + 4 <= b + 1; j += 4) {
+      float v[4][E];
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[u][e] = live ? p.head[(j + u) * p.D + (int64_t)chunk * E + e] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += v[u][e];
+    }
+    for (; j <= b; ++j)
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += live ? p.head[j * p.D + (int64_t)chunk * E + e] : 0.f;
+  };
+  auto write_row = [&](unsigned v, float *acc) {
+    if (!live) return;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = scaled(acc[e], p.scale);
+    *reinterpret_cast<C *>(p.dw + (int64_t)v * p.D * (int64_t)sizeof(T) + (int64_t)chunk * BYTES) = chunk_of_f32<T, BYTES>(acc);
+  };
+  const int64_t end = (piece + 1) * kPiece;
+  if (piece < p.pieces && end < p.N) {
+    const unsigned k = p.key[end - 1];
+    const bool crosses = k != none && p.key[end] == k;
+    const bool began = p.key[piece * kPiece] != k || piece == 0 || p.key[piece * kPiece - 1] != k;
+    if (crosses && began) {
+      // last piece whose first entry is still k: by groups of 32, then halving
+      auto starts_with = [&](int64_t j) { return j < p.pieces && p.key[j * kPiece] == k; };
+      const unsigned run = __ballot_sync(0xffffffffu, starts_with(piece + 1 + lane));
+      if (run != 0xffffffffu) {
+        const int64_t last = piece + __popc(run);  // the pieces of a run are consecutive
+        float acc[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = live ? p.tail[piece * p.D + (int64_t)chunk * E + e] : 0.f;
+        add_heads(piece + 1, last, acc);
+        write_row(k, acc);
+      } else if (lane == 0) {
+        int64_t a = piece + kLong, b = p.pieces;  // starts_with(a), not starts_with(b)
+        while (b - a > 1) {
+          const int64_t m = (a + b) / 2;
+          if (starts_with(m)) a = m; else b = m;
+        }
+        long_first = piece;  // 16 pieces hold the beginning of one such run at most
+        long_last = a;
+        long_key = k;
+      }
+    }
+  }
+  __syncthreads();
+  if (long_first < 0) return;
+  const int64_t n = long_last - long_first, per = (n + kJoinWarps - 1) / kJoinWarps;
+  const int64_t a = long_first + 1 + warp * per, b = min(long_last, a + per - 1);
+  float acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = warp == 0 && live ? p.tail[long_first * p.D + (int64_t)chunk * E + e] : 0.f;
+  add_heads(a, b, acc);
+#pragma unroll
+  for (int e = 0; e < E; ++e) share[warp][e][lane] = acc[e];
+  __syncthreads();
+  if (warp == 0) {
+    for (int w = 1; w < kJoinWarps; ++w)
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += share[w][e][lane];
+    write_row(long_key, acc);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+struct Layout {
+  size_t key[2], pos[2], seen, head, tail, total;
+};
+Layout layout(int64_t N, int64_t V, int64_t D) {
+  Layout l;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at += round_up(bytes, 256);
+    return o;
+  };
+  for (int i = 0; i < 2; ++i) l.key[i] = take((size_t)N * 4), l.pos[i] = take((size_t)N * 4);
+  l.seen = take((size_t)((V + 31) / 32) * 4);
+  const size_t parts = (size_t)((N + kPiece - 1) / kPiece) * (size_t)D * sizeof(float);
+  l.head = take(parts);
+  l.tail = take(parts);
+  l.total = at;
+  return l;
+}
+
+// The widest lane chunk that divides the row and the alignments.
+int chunk_bytes(int64_t row_bytes, std::initializer_list<const void *> ptrs, int64_t ld_bytes, size_t es) {
+  int b = 16;
+  auto fits = [&](int c) {
+    if (row_bytes % c || ld_bytes % c) return false;
+    for (const void *p : ptrs)
+      if (!aligned(p, c)) return false;
+    return true;
+  };
+  while (b > (int)es && !fits(b)) b /= 2;
+  return b;
+}
+
+template <typename F> int by_chunk(int dtype, int bytes, F f) {
+  auto at = [&](auto tag) -> int {
+    using T = decltype(tag);
+    if (bytes == 16) return f(tag, std::integral_constant<int, 16>{});
+    if (bytes == 8) return f(tag, std::integral_constant<int, 8>{});
+    if constexpr (sizeof(T) == 2)
+      if (bytes == 2) return f(tag, std::integral_constant<int, 2>{});
+    return f(tag, std::integral_constant<int, 4>{});
+  };
+  if (dtype == HS_F32) return at(float{});
+  if (dtype == HS_BF16) return at(__nv_bfloat16{});
+  return at(__half{});
+}
+
+int check_ids(const char *who, int dtype, int token_bits, const void *tokens, int64_t N, int64_t V, int64_t D,
+              const int *status) {
+  if (!dtype_ok(dtype)) return fail(HS_ERR_INVALID_ARG, "%s: unknown dtype %d", who, dtype);
+  if (token_bits != 32 && token_bits != 64) return fail(HS_ERR_INVALID_ARG, "%s: token_bits is 32 or 64", who);
+  if (N < 0 || V < 0 || D < 0) return fail(HS_ERR_INVALID_ARG, "%s: negative N, V or D", who);
+  if (N > 0x7fffffff || V > 0x7ffffffe) return fail(HS_ERR_UNSUPPORTED, "%s: N or V is 2^31 or more", who);
+  if (N && (!tokens || !aligned(tokens, token_bits / 8))) return fail(HS_ERR_INVALID_ARG, "%s: null or misaligned tokens", who);
+  if (!status) return fail(HS_ERR_INVALID_ARG, "%s: null dev_status", who);
+  return HS_OK;
+}
+
+}  // namespace
+}  // namespace hs
+
+extern "C" {
+
+int hs_embedding_forward(int dtype, const void *weight, int64_t weight_ld, int token_bits, const void *tokens,
+                         double scale, void *out, int64_t N, int64_t V, int64_t D, int *dev_status,
+                         hs_stream_t stream) {
+  using namespace hs;
+  if (int e = check_ids("hs_embedding_forward", dtype, token_bits, tokens, N, V, D, dev_status)) return e;
+  if (N == 0 || D == 0) return HS_OK;
+  const size_t es = dtype_bytes(dtype);
+  if ((V && !weight) || !out || !aligned(weight, es) || !aligned(out, es))
+    return fail(HS_ERR_INVALID_ARG, "hs_embedding_forward: null or misaligned weight or out");
+  if (weight_ld < D && V > 1) return fail(HS_ERR_INVALID_ARG, "hs_embedding_forward: weight_ld is below D");
+  const int bytes = chunk_bytes(D * (int64_t)es, {weight, out}, V > 1 ? weight_ld * (int64_t)es : 0, es);
+  const int64_t chunks = D * (int64_t)es / bytes, total = chunks * N, blocks = (total + 1023) / 1024;
+  if (chunks > 0x7fffffff || blocks > 0x7fffffff) return fail(HS_ERR_UNSUPPORTED, "hs_embedding_forward: N * D is too large");
+  return by_chunk(dtype, bytes, [&](auto tag, auto b) -> int {
+    using T = decltype(tag);
+    constexpr int BYTES = decltype(b)::value;
+    if (token_bits == 64)
+      emb_lookup_kernel<T, BYTES, int64_t><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(
+          (const char *)weight, weight_ld * (int64_t)es, (const int64_t *)tokens, make_scale(scale), (char *)out, total, (int)chunks, V, dev_status);
+    else
+      emb_lookup_kernel<T, BYTES, int><<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(
+          (const char *)weight, weight_ld * (int64_t)es, (const int *)tokens, make_scale(scale), (char *)out, total, (int)chunks, V, dev_status);
+    return check_launch("emb_lookup_kernel");
+  });
+}
+
+size_t hs_embedding_workspace_bytes(int64_t N, int64_t V, int64_t D) {
+  if (N <= 0 || V <= 0 || D <= 0) return 0;
+  return hs::layout(N, V, D).total;
+}
+
+int hs_embedding_backward(int dtype, const void *dout, int token_bits, const void *tokens, int64_t padding_idx,
+                          double scale, void *dweight, int64_t N, int64_t V, int64_t D, void *workspace,
+                          size_t workspace_bytes, int *dev_status, hs_stream_t stream) {
+  using namespace hs;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (int e = check_ids("hs_embedding_backward", dtype, token_bits, tokens, N, V, D, dev_status)) return e;
+  if (V == 0 || D == 0) return HS_OK;
+  const size_t es = dtype_bytes(dtype);
+  if (!dweight || !aligned(dweight, es) || (N && !dout) || !aligned(dout, es))
+    return fail(HS_ERR_INVALID_ARG, "hs_embedding_backward: null or misaligned dout or dweight");
+  if (N == 0) {
+    const cudaError_t e = cudaMemsetAsync(dweight, 0, (size_t)V * D * es, st);
+    return e == cudaSuccess ? HS_OK : fail(HS_ERR_CUDA, "hs_embedding_backward: %s", cudaGetErrorString(e));
+  }
+  const Layout l = layout(N, V, D);
+  if (!workspace || workspace_bytes < l.total || !aligned(workspace, 256))
+    return fail(HS_ERR_WORKSPACE, "hs_embedding_backward: workspace %zu < %zu bytes, or not 256-byte aligned", workspace_bytes, l.total);
+  char *ws = static_cast<char *>(workspace);
+
+  SortArgs s = {};
+  s.tok = tokens, s.N = N, s.V = V, s.pad = padding_idx, s.status = dev_status;
+  for (int i = 0; i < 2; ++i) s.key[i] = (unsigned *)(ws + l.key[i]), s.pos[i] = (unsigned *)(ws + l.pos[i]);
+  s.seen = (unsigned *)(ws + l.seen);
+  int key_bits = 1;
+  while ((V >> key_bits) != 0) ++key_bits;  // ids 0..V
+  s.passes = (key_bits + kMaxBits - 1) / kMaxBits;
+  s.bits = (key_bits + s.passes - 1) / s.passes;
+  int cluster = 1;
+  while (cluster < kSortCluster && (int64_t)cluster * kSortThreads < N) cluster *= 2;
+  const void *sort = token_bits == 64 ? (const void *)emb_sort_kernel<int64_t> : (const void *)emb_sort_kernel<int>;
+  static std::atomic<unsigned long long> done64{0}, done32{0};
+  if (int e = allow_dynamic_smem(sort, sizeof(unsigned) * (kSortWarps + kSortCluster + 1) << kMaxBits,
+                                 token_bits == 64 ? &done64 : &done32))
+    return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cluster);
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = sizeof(unsigned) * (kSortWarps + kSortCluster + 1) << s.bits;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  void *args[] = {&s};
+  if (cudaLaunchKernelExC(&cfg, sort, args) != cudaSuccess) return check_launch("emb_sort_kernel");
+
+  SumArgs p = {};
+  p.key = s.key[(s.passes + 1) & 1], p.pos = s.pos[(s.passes + 1) & 1], p.seen = s.seen;
+  p.dout = (const char *)dout, p.dw = (char *)dweight;
+  p.head = (float *)(ws + l.head), p.tail = (float *)(ws + l.tail);
+  p.N = N, p.V = V, p.D = D, p.pieces = (N + kPiece - 1) / kPiece, p.scale = make_scale(scale);
+  const int bytes = chunk_bytes(D * (int64_t)es, {dout, dweight}, 0, es);
+  const int64_t chunks = D * (int64_t)es / bytes, slices = (chunks + 31) / 32;
+  p.sum_blocks = (p.pieces * slices + 7) / 8;
+  const int64_t zero_blocks = (V + 255) / 256, join_blocks = (p.pieces + kJoinWarps - 1) / kJoinWarps * slices;
+  if (chunks > 0x7fffffff || p.sum_blocks + zero_blocks > 0x7fffffff || join_blocks > 0x7fffffff)
+    return fail(HS_ERR_UNSUPPORTED, "hs_embedding_backward: N * D is too large");
+  p.chunks = (int)chunks, p.slices = (int)slices;
+  return by_chunk(dtype, bytes, [&](auto tag, auto b) -> int {
+    using T = decltype(tag);
+    constexpr int BYTES = decltype(b)::value;
+    emb_sum_kernel<T, BYTES><<<(unsigned)(p.sum_blocks + zero_blocks), 256, 0, st>>>(p);
+    if (int e = check_launch("emb_sum_kernel")) return e;
+    if (p.pieces > 1) {
+      emb_join_kernel<T, BYTES><<<(unsigned)join_blocks, 32 * kJoinWarps, 0, st>>>(p);
+      return check_launch("emb_join_kernel");
+    }
+    return HS_OK;
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,654 @@
+// Gated linear recurrence over time, forward and backward.
+//
+//   h_t = k_t f_t h_{t-1} + b_t,   k_t = 0 where a sequence starts, else 1
+//   gated:  f_t = 1 / (1 + e^-z_t), b_t = (1 - f_t) x_t
+//   linear: f_t and b_t are given
+//
+// A run of steps maps the state entering it to the state leaving it as
+// h -> A h + B, and such maps compose, so the runs of a long sequence are
+// summarised at once and only the maps are chained.  The backward is the same
+// construction from the last step to the first on u_t = k_t f_t (g_t + u_{t+1}),
+// the gradient reaching h_{t-1}:
+//   e_t = g_t + u_{t+1},  dx_t = e_t (1 - f_t),  dz_t = e_t (k_t h_{t-1} - x_t) f_t (1 - f_t)
+//   (linear: db_t = e_t,  df_t = e_t k_t h_{t-1}),  dh0 = u_0.
+//
+// Bound: memory.  The forward reads two words and writes one per element; the
+// backward reads three (z, x, g) and writes two.  It does not read h: the
+// forward keeps the float32 state entering each run of 16 steps (1/16 of a
+// float32 tensor) and the backward recomputes the states inside the run from
+// it, which moves less than reading h back and leaves no 16-bit rounding of h
+// in the gradient.
+//
+// Split: a warp owns 16 consecutive steps of one 128-byte word row (32 lanes
+// of one 32-bit word: 32 float32 or 64 16-bit columns).  The warps of a CTA
+// stack along time, the CTAs of a cluster continue the stack, and a cluster
+// walks the sequence in waves of 16 x warps x CTAs steps.  Each warp summarises its
+// run, the maps meet in shared memory (distributed over the cluster), and
+// every warp then knows its entering state and writes its outputs from the
+// values it still holds, so every tensor is read and written once.  The order of
+// operations is fixed by the shape alone: results are the same bit for bit
+// from run to run.  No CTA waits on one outside its own cluster.
+#include "lm_types.cuh"
+
+namespace hs {
+namespace {
+
+constexpr int kRun = 16;       // steps per warp and per saved state
+constexpr int kMaxWarps = 8;   // warps of a CTA along time
+constexpr int kMaxCluster = 8; // CTAs of a cluster along time
+
+struct RecShape {
+  int64_t T, n;         // steps; columns of one row
+  int64_t groups;       // word-row groups of one row
+  int nchunk;           // runs of 16 steps
+  int waves;
+  int cluster;
+};
+
+struct FwdArgs {
+  RecShape s;
+  const char *z, *x;
+  char *h;
+  const float *h0;
+  float *h_n, *ckpt;
+  const unsigned char *starts;
+  int64_t zt, zb, xt, xb, ht, hb, st, sb;  // strides in elements
+  int64_t state_b;                         // row stride of h0 and h_n (columns)
+  int64_t ckpt_t;                          // columns of one saved state (B * H)
+};
+
+struct BwdArgs {
+  RecShape s;
+  const char *z, *x, *g;
+  char *dz, *dx;
+  const float *ckpt, *dh_n;
+  float *dh0;
+  const unsigned char *starts;
+  int64_t zt, zb, xt, xb, gt, gb, dzt, dzb, dxt, dxb, st, sb;
+  int64_t state_b, ckpt_t;
+};
+
+HS_DEV unsigned smem_u32(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
+HS_DEV void cp_async4(unsigned dst, const void *src, bool valid) {
+  const int n = valid ? 4 : 0;  // 0 bytes read: the word is filled with zeros
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+HS_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> HS_DEV void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+HS_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+HS_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+HS_DEV void st_cluster(unsigned addr, int rank, float v) {
+  asm volatile(
+      "{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %0, %1;\n\tst.shared::cluster.f32 [r], %2;\n\t}" ::"r"(addr),
+      "r"(rank), "f"(v)
+      : "memory");
+}
+
+// f = 1/(1+e^-z) and 1-f, each to a few float32 ulps of its own size: with
+// t = e^-|z| they are 1/(1+t) and t/(1+t), whichever way round z's sign says.
+// The reciprocal is refined by one Newton step (as in sigf: its rounding
+// compounds over thousands of steps).
+HS_DEV void gate(float z, float &f, float &om) {
+  const float t = __expf(-fabsf(z));
+  const float d = 1.0f + t;
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  r = fmaf(r, fmaf(-d, r, 1.0f), r);
+  const float tr = t * r;
+  f = z >= 0.f ? r : tr;
+  om = z >= 0.f ? tr : r;
+}
+
+// a * h where a may have overflowed or underflowed as a product of many
+// coefficients: from a zero state nothing arrives, as step by step.
+HS_DEV float carry(float a, float h) { return h == 0.f ? 0.f : a * h; }
+
+// Row of one warp: base pointers advance by whole steps.
+template <typename T, int VEC> HS_DEV void fetch_word(unsigned dst, const char *src, bool valid) {
+  if constexpr (VEC == PerWord<T>::value) {
+    cp_async4(dst, src, valid);
+  } else {  // one 16-bit value per lane: rows that are not 4-byte aligned
+    unsigned w = 0;
+    if (valid) w = *reinterpret_cast<const unsigned short *>(src);
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst), "r"(w) : "memory");
+  }
+}
+template <typename T, int VEC> HS_DEV void read_word(unsigned src, float *v) {
+  unsigned w;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(src) : "memory");
+  if constexpr (VEC == PerWord<T>::value) {
+    unpack_word<T>(w, v);
+  } else {
+    float t[2];
+    unpack_word<T>(w, t);
+    v[0] = t[0];
+  }
+}
+template <typename T, int VEC> HS_DEV void write_word(char *dst, const float *v) {
+  if constexpr (VEC == PerWord<T>::value)
+    *reinterpret_cast<unsigned *>(dst) = pack_word<T>(v);
+  else
+    *reinterpret_cast<T *>(dst) = from_f32<T>(v[0]);
+}
+
+// The maps of the warps of a CTA and of the CTAs of a cluster.  Both buffers
+// alternate between two copies, so one barrier per wave separates a wave's
+// writes from the reads two waves before.
+template <int VEC> struct Maps {
+  float a[2][kMaxWarps][VEC][32], b[2][kMaxWarps][VEC][32];
+  float ca[2][kMaxCluster][VEC][32], cb[2][kMaxCluster][VEC][32];
+  float cut[2][kMaxWarps], ccut[2][kMaxCluster];  // 1: nothing passes (a start lies inside)
+};
+
+template <int VEC, bool STARTS>
+HS_DEV void apply_map(const float (&a)[VEC][32], const float (&b)[VEC][32], float cut, int lane, float *h) {
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) {
+    const float c = STARTS && cut != 0.f ? 0.f : carry(a[v][lane], h[v]);
+    h[v] = c + b[v][lane];
+  }
+}
+
+// Publishes the warp's map (A, B, cut) and returns the state entering the
+// warp's run in `in`; `state`, the same in every thread of a column, moves
+// from the wave's entry to its end.
+template <int VEC, bool STARTS>
+HS_DEV void exchange(Maps<VEC> &m, int p, int warps, int warp, int lane, int cluster, int rank, const float *A,
+                     const float *B, bool cut, float *state, float *in) {
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) {
+    m.a[p][warp][v][lane] = A[v];
+    m.b[p][warp][v][lane] = B[v];
+  }
+  if (STARTS && lane == 0) m.cut[p][warp] = cut ? 1.f : 0.f;
+  __syncthreads();
+  if (cluster == 1) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) in[v] = state[v];
+    for (int j = 0; j < warps; ++j) {
+      apply_map<VEC, STARTS>(m.a[p][j], m.b[p][j], m.cut[p][j], lane, state);
+      if (j + 1 == warp) {
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) in[v] = state[v];
+      }
+    }
+    return;
+  }
+  if (warp == warps - 1) {  // the CTA's map, to every CTA of the cluster
+    float ta[VEC], tb[VEC], tc = 0.f;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) ta[v] = 1.f, tb[v] = 0.f;
+    for (int j = 0; j < warps; ++j) {
+      const bool c = STARTS && m.cut[p][j] != 0.f;
+      if (c) tc = 1.f;
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        const float a = m.a[p][j][v][lane];
+        ta[v] = c ? 0.f : carry(a, ta[v]);
+        tb[v] = (c ? 0.f : carry(a, tb[v])) + m.b[p][j][v][lane];
+      }
+    }
+    for (int r = 0; r < cluster; ++r) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        st_cluster(smem_u32(&m.ca[p][rank][v][lane]), r, ta[v]);
+        st_cluster(smem_u32(&m.cb[p][rank][v][lane]), r, tb[v]);
+      }
+      if (STARTS && lane == 0) st_cluster(smem_u32(&m.ccut[p][rank]), r, tc);
+    }
+  }
+  cluster_arrive();
+  cluster_wait();
+  for (int r = 0; r < cluster; ++r) {
+    if (r == rank) {
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) in[v] = state[v];
+    }
+    apply_map<VEC, STARTS>(m.ca[p][r], m.cb[p][r], m.ccut[p][r], lane, state);
+  }
+  for (int j = 0; j < warp; ++j) apply_map<VEC, STARTS>(m.a[p][j], m.b[p][j], m.cut[p][j], lane, in);
+}
+
+template <int VEC> HS_DEV void load_state(const float *p, int64_t at, bool live, float *v) {
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = p && live ? p[at + i] : 0.f;
+}
+
+// ------------------------------------------------------------------ forward
+// Shared memory: `stages` buffers of [2 tensors][16 steps][warps][32 words],
+// each lane's words private to it (copied in and read by the same thread).
+template <typename T, int VEC, bool GATED, bool STARTS>
+__global__ void __launch_bounds__(32 * kMaxWarps, 2) rec_fwd_kernel(const FwdArgs p, int stages) {
+  extern __shared__ __align__(16) unsigned char dyn[];
+  __shared__ Maps<VEC> maps;
+  const int lane = threadIdx.x, warp = threadIdx.y, warps = blockDim.y;
+  const int cluster = p.s.cluster, rank = (int)(blockIdx.x % cluster);
+  const int64_t gid = blockIdx.x / cluster;
+  const int64_t row = gid / p.s.groups, col = (gid % p.s.groups) * 32 * VEC + lane * VEC;
+  const bool live = col < p.s.n;  // VEC > 1 only where n is a multiple of VEC
+  const int64_t T_ = p.s.T;
+  const char *zp = p.z + (row * p.zb + col) * sizeof(T), *xp = p.x + (row * p.xb + col) * sizeof(T);
+  char *hp = p.h + (row * p.hb + col) * sizeof(T);
+  const int64_t zs = p.zt * (int64_t)sizeof(T), xs = p.xt * (int64_t)sizeof(T), hs = p.ht * (int64_t)sizeof(T);
+  const unsigned buf = smem_u32(dyn) + (warp * 32 + lane) * 4;
+  const unsigned step = warps * 128u, tensor = kRun * step, stage = 2 * tensor;
+
+  float state[VEC];
+  load_state<VEC>(p.h0, row * p.state_b + col, live, state);
+  if (cluster > 1) cluster_arrive();  // met before the first exchange: every CTA has started
+
+  unsigned next_start = 0;
+  auto fetch = [&](int w) {
+    const int64_t t0 = ((int64_t)(w * cluster + rank) * warps + warp) * kRun;
+    const unsigned d = buf + (unsigned)(w % stages) * stage;
+    const char *zq = zp + t0 * zs, *xq = xp + t0 * xs;
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+      const bool ok = live && t0 + k < T_;
+      fetch_word<T, VEC>(d + k * step, ok ? zq + k * zs : p.z, ok);
+      fetch_word<T, VEC>(d + tensor + k * step, ok ? xq + k * xs : p.x, ok);
+    }
+    cp_commit();
+  };
+  auto fetch_starts = [&](int w) -> unsigned {
+    const int64_t t = ((int64_t)(w * cluster + rank) * warps + warp) * kRun + lane;
+    return lane < kRun && t < T_ ? p.starts[t * p.st + row * p.sb] : 0;
+  };
+
+  for (int w = 0; w < stages - 1; ++w) {
+    if (w < p.s.waves) fetch(w); else cp_commit();
+  }
+  if (STARTS) next_start = fetch_starts(0);
+  for (int w = 0; w < p.s.waves; ++w) {
+    if (w + stages - 1 < p.s.waves) fetch(w + stages - 1); else cp_commit();
+    unsigned mask = 0;
+    if (STARTS) {
+      mask = __ballot_sync(0xffffffffu, next_start != 0);
+      if (w + 1 < p.s.waves) next_start = fetch_starts(w + 1);
+    }
+    if (stages == 3) cp_wait<2>(); else if (stages == 2) cp_wait<1>(); else cp_wait<0>();
+    const int64_t t0 = ((int64_t)(w * cluster + rank) * warps + warp) * kRun;
+    const unsigned d = buf + (unsigned)(w % stages) * stage;
+    const int len = (int)min((int64_t)kRun, T_ - t0);  // may be <= 0
+    float f[kRun][VEC], b[kRun][VEC], A[VEC], B[VEC], in[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) A[v] = 1.f, B[v] = 0.f;
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+      read_word<T, VEC>(d + k * step, f[k]);
+      read_word<T, VEC>(d + tensor + k * step, b[k]);
+      const bool cut = STARTS && ((mask >> k) & 1);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        if (GATED) {
+          float om;
+          gate(f[k][v], f[k][v], om);
+          b[k][v] *= om;
+        }
+        if (k >= len) f[k][v] = 1.f, b[k][v] = 0.f;
+        A[v] = cut ? 0.f : A[v] * f[k][v];
+        B[v] = cut ? b[k][v] : fmaf(f[k][v], B[v], b[k][v]);
+      }
+    }
+    if (cluster > 1 && w == 0) cluster_wait();
+    exchange<VEC, STARTS>(maps, w & 1, warps, warp, lane, cluster, rank, A, B, mask != 0, state, in);
+    if (live && len > 0) {
+      if (p.ckpt) {
+        float *c = p.ckpt + (t0 / kRun) * p.ckpt_t + row * p.state_b + col;
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) c[v] = in[v];
+      }
+      char *hq = hp + t0 * hs;
+#pragma unroll
+      for (int k = 0; k < kRun; ++k) {
+        const bool cut = STARTS && ((mask >> k) & 1);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) in[v] = cut ? b[k][v] : fmaf(f[k][v], in[v], b[k][v]);
+        if (k < len) write_word<T, VEC>(hq + k * hs, in);
+      }
+    }
+  }
+  if (p.h_n && live && rank == 0 && warp == 0) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) p.h_n[row * p.state_b + col + v] = state[v];
+  }
+}
+
+// ------------------------------------------------------------------ backward
+// Shared memory: [3 tensors][16 steps][warps][32 words] per stage; a stage is
+// in use until its outputs are written (g is read twice), so the next one is
+// fetched beside it.
+template <typename T, int VEC, bool GATED, bool STARTS>
+__global__ void __launch_bounds__(32 * kMaxWarps, 2) rec_bwd_kernel(const BwdArgs p, int stages) {
+  extern __shared__ __align__(16) unsigned char dyn[];
+  __shared__ Maps<VEC> maps;
+  // float32 keeps both f and 1-f; the 16-bit types keep 1-f alone and take
+  // f = 1 - (1-f), whose error (2^-25) only enters u, far below their rounding
+  constexpr bool kBoth = GATED && sizeof(T) == 4;
+  const int lane = threadIdx.x, warp = threadIdx.y, warps = blockDim.y;
+  const int cluster = p.s.cluster, rank = (int)(blockIdx.x % cluster);
+  const int64_t gid = blockIdx.x / cluster;
+  const int64_t row = gid / p.s.groups, col = (gid % p.s.groups) * 32 * VEC + lane * VEC;
+  const bool live = col < p.s.n;
+  const int64_t T_ = p.s.T;
+  const char *zp = p.z + (row * p.zb + col) * sizeof(T), *xp = p.x + (row * p.xb + col) * sizeof(T);
+  const char *gp = p.g + (row * p.gb + col) * sizeof(T);
+  char *dzp = p.dz + (row * p.dzb + col) * sizeof(T), *dxp = p.dx + (row * p.dxb + col) * sizeof(T);
+  const int64_t zs = p.zt * (int64_t)sizeof(T), xs = p.xt * (int64_t)sizeof(T), gs = p.gt * (int64_t)sizeof(T);
+  const int64_t dzs = p.dzt * (int64_t)sizeof(T), dxs = p.dxt * (int64_t)sizeof(T);
+  const unsigned buf = smem_u32(dyn) + (warp * 32 + lane) * 4;
+  const unsigned step = warps * 128u, tensor = kRun * step, stage = 3 * tensor;
+
+  float state[VEC];
+  load_state<VEC>(p.dh_n, row * p.state_b + col, live, state);
+  if (cluster > 1) cluster_arrive();  // met before the first exchange: every CTA has started
+
+  // chunks from the last to the first; below 0: past the beginning, nothing
+  auto chunk_of = [&](int w) { return p.s.nchunk - 1 - ((w * cluster + rank) * warps + warp); };
+  auto fetch = [&](int w) {
+    const int c = chunk_of(w);
+    const int64_t t0 = (int64_t)c * kRun;
+    const unsigned d = buf + (unsigned)(w % stages) * stage;
+    const char *zq = zp + t0 * zs, *xq = xp + t0 * xs, *gq = gp + t0 * gs;
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+      const bool ok = live && c >= 0 && t0 + k < T_, okg = ok && p.g != nullptr;
+      fetch_word<T, VEC>(d + k * step, ok ? zq + k * zs : p.z, ok);
+      fetch_word<T, VEC>(d + tensor + k * step, ok ? xq + k * xs : p.z, ok);
+      fetch_word<T, VEC>(d + 2 * tensor + k * step, okg ? gq + k * gs : p.z, okg);
+    }
+    cp_commit();
+  };
+  auto fetch_starts = [&](int w) -> unsigned {
+    const int64_t t = (int64_t)chunk_of(w) * kRun + lane;
+    return lane < kRun && t >= 0 && t < T_ ? p.starts[t * p.st + row * p.sb] : 0;
+  };
+  auto fetch_ckpt = [&](int w, float *h) {
+    const int c = chunk_of(w);
+    load_state<VEC>(p.ckpt, c * p.ckpt_t + row * p.state_b + col, live && c >= 0, h);
+  };
+
+  unsigned next_start = 0;
+  float next_h[VEC];
+  for (int w = 0; w < stages - 1; ++w) {
+    if (w < p.s.waves) fetch(w); else cp_commit();
+  }
+  fetch_ckpt(0, next_h);
+  if (STARTS) next_start = fetch_starts(0);
+  for (int w = 0; w < p.s.waves; ++w) {
+    if (w + stages - 1 < p.s.waves) fetch(w + stages - 1); else cp_commit();
+    unsigned mask = 0;
+    if (STARTS) {
+      mask = __ballot_sync(0xffffffffu, next_start != 0);
+      if (w + 1 < p.s.waves) next_start = fetch_starts(w + 1);
+    }
+    float h[VEC];
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) h[v] = next_h[v];
+    if (w + 1 < p.s.waves) fetch_ckpt(w + 1, next_h);
+    if (stages == 3) cp_wait<2>(); else if (stages == 2) cp_wait<1>(); else cp_wait<0>();
+    const int c = chunk_of(w);
+    const int64_t t0 = (int64_t)c * kRun;
+    const unsigned d = buf + (unsigned)(w % stages) * stage;
+    const int len = c < 0 ? 0 : (int)min((int64_t)kRun, T_ - t0);
+    // keep: 1-f (gated) or f (linear); q: the factor of e in df
+    float keep[kRun][VEC], both[kBoth ? kRun : 1][VEC], q[kRun][VEC], A[VEC], B[VEC], u[VEC];
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+      float zz[VEC], xx[VEC];
+      read_word<T, VEC>(d + k * step, zz);
+      read_word<T, VEC>(d + tensor + k * step, xx);
+      const bool cut = STARTS && ((mask >> k) & 1);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        const float before = cut ? 0.f : h[v];
+        if (GATED) {
+          float f, om;
+          gate(zz[v], f, om);
+          q[k][v] = (before - xx[v]) * f * om;
+          h[v] = fmaf(f, before, om * xx[v]);
+          if (k >= len) om = 0.f, f = 1.f;
+          keep[k][v] = om;
+          if (kBoth) both[k][v] = f;
+        } else {
+          q[k][v] = before;
+          h[v] = fmaf(zz[v], before, xx[v]);
+          keep[k][v] = k >= len ? 1.f : zz[v];
+        }
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) A[v] = 1.f, B[v] = 0.f;
+#pragma unroll
+    for (int k = kRun - 1; k >= 0; --k) {
+      float g[VEC];
+      read_word<T, VEC>(d + 2 * tensor + k * step, g);
+      const bool cut = STARTS && ((mask >> k) & 1);
+#pragma unroll
+      for (int v = 0; v < VEC; ++v) {
+        const float f = kBoth ? both[kBoth ? k : 0][v] : GATED ? 1.f - keep[k][v] : keep[k][v];
+        B[v] = cut ? 0.f : f * (g[v] + B[v]);
+        A[v] = cut ? 0.f : A[v] * f;
+      }
+    }
+    if (cluster > 1 && w == 0) cluster_wait();
+    exchange<VEC, STARTS>(maps, w & 1, warps, warp, lane, cluster, rank, A, B, mask != 0, state, u);
+    if (live && len > 0) {
+      char *dzq = dzp + t0 * dzs, *dxq = dxp + t0 * dxs;
+#pragma unroll
+      for (int k = kRun - 1; k >= 0; --k) {
+        float g[VEC], dz[VEC], dx[VEC];
+        read_word<T, VEC>(d + 2 * tensor + k * step, g);
+        const bool cut = STARTS && ((mask >> k) & 1);
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) {
+          const float f = kBoth ? both[kBoth ? k : 0][v] : GATED ? 1.f - keep[k][v] : keep[k][v];
+          const float e = g[v] + u[v];
+          dz[v] = e * q[k][v];
+          dx[v] = GATED ? e * keep[k][v] : e;
+          u[v] = cut ? 0.f : f * e;
+        }
+        if (k < len) {
+          write_word<T, VEC>(dzq + k * dzs, dz);
+          write_word<T, VEC>(dxq + k * dxs, dx);
+        }
+      }
+    }
+  }
+  if (p.dh0 && live && rank == 0 && warp == 0) {
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) p.dh0[row * p.state_b + col + v] = state[v];
+  }
+}
+
+// ------------------------------------------------------------------ launch
+struct Plan {
+  int warps, cluster, stages;
+  size_t smem;
+};
+
+// Warps and CTAs along time: enough of both that the column groups times the
+// cluster fill the SMs twice (two CTAs each), and no more than the sequence
+// has runs for.
+Plan make_plan(int64_t rows_groups, int nchunk, int tensors) {
+  Plan pl;
+  pl.warps = 1;
+  while (pl.warps < kMaxWarps && pl.warps < nchunk) pl.warps *= 2;
+  pl.cluster = 1;
+  while (pl.cluster < kMaxCluster && pl.cluster * pl.warps < nchunk && rows_groups * pl.cluster < 2 * 148) pl.cluster *= 2;
+  pl.stages = tensors == 2 ? 3 : 2;
+  const int waves = (nchunk + pl.warps * pl.cluster - 1) / (pl.warps * pl.cluster);
+  if (waves < pl.stages) pl.stages = waves;
+  pl.smem = (size_t)pl.stages * tensors * kRun * pl.warps * 128;
+  return pl;
+}
+
+template <typename Args, typename K>
+int launch(K kernel, const Args &args, const Plan &pl, int64_t groups, cudaStream_t st, const char *what,
+           std::atomic<unsigned long long> *done) {
+  if (int e = allow_dynamic_smem((const void *)kernel, (size_t)3 * 2 * kRun * kMaxWarps * 128, done)) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(groups * pl.cluster));
+  cfg.blockDim = dim3(32, pl.warps);
+  cfg.dynamicSmemBytes = pl.smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)pl.cluster;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, kernel, args, pl.stages) != cudaSuccess) return check_launch(what);
+  return check_launch(what);
+}
+
+template <typename T, int VEC, bool GATED, bool STARTS> int launch_fwd(const FwdArgs &a, const Plan &pl, int64_t groups, cudaStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  return launch(rec_fwd_kernel<T, VEC, GATED, STARTS>, a, pl, groups, st, "rec_fwd_kernel", &done);
+}
+template <typename T, int VEC, bool GATED, bool STARTS> int launch_bwd(const BwdArgs &a, const Plan &pl, int64_t groups, cudaStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  return launch(rec_bwd_kernel<T, VEC, GATED, STARTS>, a, pl, groups, st, "rec_bwd_kernel", &done);
+}
+
+#define HS_REC_DISPATCH(FN, args)                                                                       \
+  [&]() -> int {                                                                                        \
+    const bool gated = form == HS_RECURRENCE_GATED, cuts = starts != nullptr;                           \
+    auto go = [&](auto tag, auto vec) -> int {                                                          \
+      using E = decltype(tag);                                                                          \
+      constexpr int V = decltype(vec)::value;                                                           \
+      if (gated) return cuts ? FN<E, V, true, true>(args, pl, groups, st) : FN<E, V, true, false>(args, pl, groups, st); \
+      return cuts ? FN<E, V, false, true>(args, pl, groups, st) : FN<E, V, false, false>(args, pl, groups, st);          \
+    };                                                                                                  \
+    if (dtype == HS_F32) return go(float{}, std::integral_constant<int, 1>{});                          \
+    if (dtype == HS_BF16)                                                                               \
+      return vec == 2 ? go(__nv_bfloat16{}, std::integral_constant<int, 2>{})                           \
+                      : go(__nv_bfloat16{}, std::integral_constant<int, 1>{});                          \
+    return vec == 2 ? go(__half{}, std::integral_constant<int, 2>{}) : go(__half{}, std::integral_constant<int, 1>{});   \
+  }()
+
+int check_common(const char *who, int dtype, int form, int64_t T, int64_t B, int64_t H) {
+  if (!dtype_ok(dtype)) return fail(HS_ERR_INVALID_ARG, "%s: unknown dtype %d", who, dtype);
+  if (form != HS_RECURRENCE_GATED && form != HS_RECURRENCE_LINEAR)
+    return fail(HS_ERR_INVALID_ARG, "%s: unknown form %d", who, form);
+  if (T < 0 || B < 0 || H < 0) return fail(HS_ERR_INVALID_ARG, "%s: negative T, B or H", who);
+  if (T > (int64_t)1 << 30) return fail(HS_ERR_UNSUPPORTED, "%s: T=%lld is above 2^30", who, (long long)T);
+  if (H > 0 && B > ((int64_t)1 << 31) / H)
+    return fail(HS_ERR_UNSUPPORTED, "%s: B * H = %lld * %lld is above 2^31", who, (long long)B, (long long)H);
+  return HS_OK;
+}
+
+// One row of B * H columns when every tensor stores its batch rows back to
+// back and no start mask tells them apart; else B rows of H.
+bool one_row(const void *starts, int64_t H, std::initializer_list<int64_t> batch_strides) {
+  if (starts) return false;
+  for (int64_t s : batch_strides)
+    if (s != H) return false;
+  return true;
+}
+
+// 16-bit tensors move two columns per lane where every row is 4-byte aligned.
+int vec_of(int dtype, int64_t n, std::initializer_list<const void *> ptrs, std::initializer_list<int64_t> strides) {
+  if (dtype == HS_F32) return 1;
+  if (n % 2) return 1;
+  for (const void *p : ptrs)
+    if (p && !aligned(p, 4)) return 1;
+  for (int64_t s : strides)
+    if (s % 2) return 1;
+  return 2;
+}
+
+}  // namespace
+}  // namespace hs
+
+extern "C" {
+
+size_t hs_recurrence_checkpoint_bytes(int64_t T, int64_t B, int64_t H) {
+  if (T <= 0 || B <= 0 || H <= 0) return 0;
+  return (size_t)((T + hs::kRun - 1) / hs::kRun) * (size_t)B * (size_t)H * sizeof(float);
+}
+
+int hs_recurrence_forward(int dtype, int form, const void *z, int64_t z_t, int64_t z_b, const void *x, int64_t x_t,
+                          int64_t x_b, const float *h0, const unsigned char *starts, int64_t starts_t,
+                          int64_t starts_b, void *h, int64_t h_t, int64_t h_b, float *h_n, float *checkpoints,
+                          int64_t T, int64_t B, int64_t H, hs_stream_t stream) {
+  using namespace hs;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (int e = check_common("hs_recurrence_forward", dtype, form, T, B, H)) return e;
+  if (B == 0 || H == 0) return HS_OK;
+  if (T == 0) {
+    if (!h_n || h_n == h0) return HS_OK;
+    const size_t bytes = (size_t)B * H * sizeof(float);
+    const cudaError_t e = h0 ? cudaMemcpyAsync(h_n, h0, bytes, cudaMemcpyDeviceToDevice, st) : cudaMemsetAsync(h_n, 0, bytes, st);
+    return e == cudaSuccess ? HS_OK : fail(HS_ERR_CUDA, "hs_recurrence_forward: %s", cudaGetErrorString(e));
+  }
+  if (!z || !x || !h) return fail(HS_ERR_INVALID_ARG, "hs_recurrence_forward: null z, x or h");
+  const size_t es = dtype_bytes(dtype);
+  if (!aligned(z, es) || !aligned(x, es) || !aligned(h, es) || !aligned(h0, 4) || !aligned(h_n, 4) || !aligned(checkpoints, 4))
+    return fail(HS_ERR_INVALID_ARG, "hs_recurrence_forward: misaligned tensor");
+  const bool flat = one_row(starts, H, {z_b, x_b, h_b});
+  FwdArgs a = {};
+  a.s.T = T;
+  a.s.n = flat ? B * H : H;
+  const int vec = vec_of(dtype, a.s.n, {z, x, h}, {z_t, x_t, h_t, flat ? 0 : z_b, flat ? 0 : x_b, flat ? 0 : h_b});
+  const int per = 32 * (dtype == HS_F32 ? 1 : vec);
+  a.s.groups = (a.s.n + per - 1) / per;
+  const int64_t groups = a.s.groups * (flat ? 1 : B);
+  a.s.nchunk = (int)((T + kRun - 1) / kRun);
+  const Plan pl = make_plan(groups, a.s.nchunk, 2);
+  if (groups * pl.cluster > 0x7fffffff) return fail(HS_ERR_UNSUPPORTED, "hs_recurrence_forward: too many columns");
+  a.s.cluster = pl.cluster;
+  a.s.waves = (a.s.nchunk + pl.warps * pl.cluster - 1) / (pl.warps * pl.cluster);
+  a.z = (const char *)z, a.x = (const char *)x, a.h = (char *)h;
+  a.h0 = h0, a.h_n = h_n, a.ckpt = checkpoints, a.starts = starts;
+  a.zt = z_t, a.zb = z_b, a.xt = x_t, a.xb = x_b, a.ht = h_t, a.hb = h_b, a.st = starts_t, a.sb = starts_b;
+  a.state_b = H, a.ckpt_t = B * H;
+  return HS_REC_DISPATCH(launch_fwd, a);
+}
+
+int hs_recurrence_backward(int dtype, int form, const void *z, int64_t z_t, int64_t z_b, const void *x, int64_t x_t,
+                           int64_t x_b, const float *checkpoints, const unsigned char *starts, int64_t starts_t,
+                           int64_t starts_b, const void *dh, int64_t dh_t, int64_t dh_b, const float *dh_n, void *dz,
+                           int64_t dz_t, int64_t dz_b, void *dx, int64_t dx_t, int64_t dx_b, float *dh0, int64_t T,
+                           int64_t B, int64_t H, hs_stream_t stream) {
+  using namespace hs;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (int e = check_common("hs_recurrence_backward", dtype, form, T, B, H)) return e;
+  if (B == 0 || H == 0) return HS_OK;
+  if (T == 0) {
+    if (!dh0 || dh0 == dh_n) return HS_OK;
+    const size_t bytes = (size_t)B * H * sizeof(float);
+    const cudaError_t e = dh_n ? cudaMemcpyAsync(dh0, dh_n, bytes, cudaMemcpyDeviceToDevice, st) : cudaMemsetAsync(dh0, 0, bytes, st);
+    return e == cudaSuccess ? HS_OK : fail(HS_ERR_CUDA, "hs_recurrence_backward: %s", cudaGetErrorString(e));
+  }
+  if (!z || !x || !checkpoints || !dz || !dx)
+    return fail(HS_ERR_INVALID_ARG, "hs_recurrence_backward: null z, x, checkpoints, dz or dx");
+  const size_t es = dtype_bytes(dtype);
+  if (!aligned(z, es) || !aligned(x, es) || !aligned(dh, es) || !aligned(dz, es) || !aligned(dx, es) ||
+      !aligned(checkpoints, 4) || !aligned(dh_n, 4) || !aligned(dh0, 4))
+    return fail(HS_ERR_INVALID_ARG, "hs_recurrence_backward: misaligned tensor");
+  if (!dh) dh_t = dz_t, dh_b = dz_b;
+  const bool flat = one_row(starts, H, {z_b, x_b, dh_b, dz_b, dx_b});
+  BwdArgs a = {};
+  a.s.T = T;
+  a.s.n = flat ? B * H : H;
+  const int vec = vec_of(dtype, a.s.n, {z, x, dh, dz, dx},
+                         {z_t, x_t, dh_t, dz_t, dx_t, flat ? 0 : z_b, flat ? 0 : x_b, flat ? 0 : dh_b, flat ? 0 : dz_b, flat ? 0 : dx_b});
+  const int per = 32 * (dtype == HS_F32 ? 1 : vec);
+  a.s.groups = (a.s.n + per - 1) / per;
+  const int64_t groups = a.s.groups * (flat ? 1 : B);
+  a.s.nchunk = (int)((T + kRun - 1) / kRun);
+  const Plan pl = make_plan(groups, a.s.nchunk, 3);
+  if (groups * pl.cluster > 0x7fffffff) return fail(HS_ERR_UNSUPPORTED, "hs_recurrence_backward: too many columns");
+  a.s.cluster = pl.cluster;
+  a.s.waves = (a.s.nchunk + pl.warps * pl.cluster - 1) / (pl.warps * pl.cluster);
+  a.z = (const char *)z, a.x = (const char *)x, a.g = (const char *)dh, a.dz = (char *)dz, a.dx = (char *)dx;
+  a.ckpt = checkpoints, a.dh_n = dh_n, a.dh0 = dh0, a.starts = starts;
+  a.zt = z_t, a.zb = z_b, a.xt = x_t, a.xb = x_b, a.gt = dh_t, a.gb = dh_b;
+  a.dzt = dz_t, a.dzb = dz_b, a.dxt = dx_t, a.dxb = dx_b, a.st = starts_t, a.sb = starts_b;
+  a.state_b = H, a.ckpt_t = B * H;
+  return HS_REC_DISPATCH(launch_bwd, a);
+}
+
+}  // extern "C"

@@ -1,0 +1,52 @@
+// Element types of the language-model operators (gated_recurrence.cu,
+// embedding.cu, token_logprobs.cu): float32, bfloat16 and float16 tensors,
+// float32 arithmetic.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "hs_common.cuh"
+
+namespace hs {
+
+inline bool dtype_ok(int dtype) { return dtype == HS_F32 || dtype == HS_BF16 || dtype == HS_F16; }
+inline size_t dtype_bytes(int dtype) { return dtype == HS_F32 ? 4 : 2; }
+
+template <typename T> HS_DEV float to_f32(T v);
+template <> HS_DEV float to_f32<float>(float v) { return v; }
+template <> HS_DEV float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> HS_DEV float to_f32<__half>(__half v) { return __half2float(v); }
+
+template <typename T> HS_DEV T from_f32(float v);
+template <> HS_DEV float from_f32<float>(float v) { return v; }
+template <> HS_DEV __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> HS_DEV __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+// The values held by one 32-bit word: one float32 or two 16-bit values.
+template <typename T> HS_DEV void unpack_word(unsigned w, float *v);
+template <> HS_DEV void unpack_word<float>(unsigned w, float *v) { v[0] = __uint_as_float(w); }
+template <> HS_DEV void unpack_word<__nv_bfloat16>(unsigned w, float *v) {
+  v[0] = __uint_as_float(w << 16);
+  v[1] = __uint_as_float(w & 0xffff0000u);
+}
+template <> HS_DEV void unpack_word<__half>(unsigned w, float *v) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+  v[0] = f.x;
+  v[1] = f.y;
+}
+
+template <typename T> HS_DEV unsigned pack_word(const float *v);
+template <> HS_DEV unsigned pack_word<float>(const float *v) { return __float_as_uint(v[0]); }
+template <> HS_DEV unsigned pack_word<__nv_bfloat16>(const float *v) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(v[0], v[1]);
+  return *reinterpret_cast<const unsigned *>(&p);
+}
+template <> HS_DEV unsigned pack_word<__half>(const float *v) {
+  const __half2 p = __floats2half2_rn(v[0], v[1]);
+  return *reinterpret_cast<const unsigned *>(&p);
+}
+
+template <typename T> struct PerWord { static constexpr int value = 4 / (int)sizeof(T); };
+
+}  // namespace hs

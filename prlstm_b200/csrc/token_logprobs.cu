@@ -1,0 +1,611 @@
+// Log probabilities of given tokens with entropy and top alternatives, and
+// the gradient of the logits.
+//
+// With c = log2(e) / temperature, m = max x, t_v = (x_v - m) c (base-2 logits):
+//   S = sum 2^t_v, U = sum t_v 2^t_v
+//   log p_v = ln2 (t_v - log2 S),  entropy = ln2 (log2 S - U / S)
+//   dx_v = (1/temperature) (sum of the gradients that name v - p_v (G + ge (log p_v + entropy))),
+//   G the sum of all gradients of the row's log probabilities, ge the entropy's.
+//
+// Bound: memory, the logits read once (and, for the gradient, read once more
+// and written once).  The forward keeps a running maximum per thread and
+// rescales S and U where a batch of values exceeds it; each value costs one
+// hardware exp2 and a few FMAs, below the memory time for 16-bit logits too.
+//
+// Top alternatives cost the pass nothing: the running maximum already says
+// where each thread's best value lies.  The k-th best of the threads' bests
+// (k distinct values are at least that) bounds the k-th best of the row from
+// below, and only the k threads whose best reaches it can hold alternatives.
+// Those threads' values, k / 256 of the row, are read again (from L2) and
+// merged into a warp-wide list of 32 sorted keys.  A key is the value's
+// monotone 32-bit image with the complement of its index below it, so the
+// order is by value and, for equal values, by the lower index.
+//
+// Split: a CTA of 256 threads per row, a cluster of CTAs per row where there
+// are few rows (the parts meet in distributed shared memory), a warp per row
+// where the rows are short.
+#include "lm_types.cuh"
+
+namespace hs {
+namespace {
+
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kMaxCluster = 8;
+constexpr float kFloor = -150.f;  // 2^-150 is 0 in float32: smaller exponents change nothing
+
+HS_DEV float max_nan(float a, float b) {  // the maximum, NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+HS_DEV float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float kNegInf = -__builtin_huge_valf();
+
+// Running (maximum, S, U) of a set of values; S and U are relative to m.
+struct Stat {
+  float m, s, u;
+};
+HS_DEV float rel(float m) { return m == kNegInf ? 0.f : m; }  // nothing but -inf so far: 2^(-inf) terms, all 0
+// Moves (s, u) from reference `from` to the larger reference `to`.
+HS_DEV void rescale(Stat &a, float to, float c) {
+  const bool none = a.m == kNegInf;
+  const float d = none ? 0.f : max_nan((a.m - to) * c, kFloor);
+  const float f = none ? 0.f : ex2(d);  // (a NaN s stays NaN)
+  a.u = (a.u + d * a.s) * f;
+  a.s *= f;
+  a.m = to;
+}
+HS_DEV void merge(Stat &a, Stat b, float c) {
+  const float m = fmaxf(a.m, b.m);
+  if (a.m != m) rescale(a, m, c);
+  if (b.m != m) rescale(b, m, c);
+  a.s += b.s;
+  a.u += b.u;
+}
+HS_DEV Stat shfl_xor(const Stat &a, int o) {
+  return {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o)};
+}
+
+// ------------------------------------------------------------------ keys
+using Key = unsigned long long;  // 0: none
+HS_DEV unsigned order_bits(float v) {
+  const unsigned b = __float_as_uint(v + 0.0f);  // -0 counts as +0
+  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+HS_DEV float value_of(Key k) {
+  const unsigned b = (unsigned)(k >> 32);
+  return __uint_as_float((b & 0x80000000u) ? b ^ 0x80000000u : ~b);
+}
+HS_DEV int index_of(Key k) { return (int)(0xffffffffu - (unsigned)k); }
+HS_DEV Key make_key(float v, int i) { return ((Key)order_bits(v) << 32) | (0xffffffffu - (unsigned)i); }
+
+HS_DEV Key order_pair(Key k, int o, bool keep_max) {
+  const Key other = __shfl_xor_sync(0xffffffffu, k, o);
+  return ((k > other) == keep_max) ? k : other;
+}
+// The warp's 32 keys in descending order of lanes (bitonic network).
+HS_DEV Key sort_desc(Key k, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll
+    for (int o = size >> 1; o; o >>= 1) k = order_pair(k, o, ((lane & o) == 0) == ((lane & size) == 0));
+  return k;
+}
+// The 32 largest of two descending lists, descending.
+HS_DEV Key merge_desc(Key a, Key b, int lane) {
+  const Key r = __shfl_sync(0xffffffffu, b, 31 - lane);
+  Key k = a > r ? a : r;  // bitonic
+#pragma unroll
+  for (int o = 16; o; o >>= 1) k = order_pair(k, o, (lane & o) == 0);
+  return k;
+}
+
+// ------------------------------------------------------------------ a row
+// The row as [head scalars | 16-byte vectors | tail scalars]; CTA `rank` of
+// `C` takes a contiguous share of the vectors, the first the head, the last
+// the tail.  Thread j of n holds head scalar j, vectors lo+j, lo+j+n, .. and
+// tail scalar j, in ascending order of index.
+template <typename T> struct Row {
+  static constexpr int E = 16 / (int)sizeof(T);
+  const T *x;
+  int head, lo, hi, tail0, ntail;
+  HS_DEV Row(const T *row, int64_t V, int rank, int C) : x(row) {
+    const int off = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+    const int h = off ? min((int64_t)(E - off), V) : 0;
+    const int nv = (int)((V - h) / E);
+    head = rank == 0 ? h : 0;
+    base = h;
+    lo = (int)((int64_t)nv * rank / C);
+    hi = (int)((int64_t)nv * (rank + 1) / C);
+    tail0 = h + nv * E;
+    ntail = rank == C - 1 ? (int)(V - tail0) : 0;
+  }
+  int base;  // index of vector 0's first value
+  HS_DEV const uint4 *vec(int i) const { return reinterpret_cast<const uint4 *>(x + base) + i; }
+  HS_DEV int index(int i, int e) const { return base + i * E + e; }
+};
+
+template <typename T> HS_DEV void unpack_vec(const uint4 &c, float *v) {
+  constexpr int P = PerWord<T>::value;
+  unpack_word<T>(c.x, v);
+  unpack_word<T>(c.y, v + P);
+  unpack_word<T>(c.z, v + 2 * P);
+  unpack_word<T>(c.w, v + 3 * P);
+}
+
+struct FwdArgs {
+  const void *x;
+  int64_t ld;
+  const void *tok;
+  int token64;
+  int64_t ignore;
+  float c, inv_t;  // log2(e) / temperature, 1 / temperature
+  int top;
+  float *lp, *ent, *top_lp;
+  int64_t *top_id;
+  float *stats;
+  int64_t N, V;
+  int cluster;
+  int *status;
+};
+
+HS_DEV int64_t token_at(const void *tok, int token64, int64_t n) {
+  return token64 ? static_cast<const int64_t *>(tok)[n] : (int64_t)static_cast<const int *>(tok)[n];
+}
+
+// What a thread knows of its values.
+template <typename T> struct Scan {
+  Stat a{kNegInf, 0.f, 0.f};
+  int best = -1;  // where the maximum was first met: vector i as i, head scalar as -2, tail scalar as -3
+  HS_DEV void scalar(float v, float c, int where) {
+    if (best == -1) best = where;
+    if (v > a.m) {
+      rescale(a, v, c);
+      best = where;
+    }
+    const float t = max_nan((v - rel(a.m)) * c, kFloor), e = ex2(t);
+    a.s += e;
+    a.u = fmaf(e, t, a.u);
+  }
+  // U vectors, the first at index i0, `stride` apart; n of them are there
+  template <int U> HS_DEV void vectors(const uint4 (&q)[U], int n, int i0, int stride, float c) {
+    constexpr int E = Row<T>::E;
+    if (best == -1) best = i0;
+    float bm = kNegInf;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (k >= n) break;
+      float v[E];
+      unpack_vec<T>(q[k], v);
+#pragma unroll
+      for (int e = 0; e < E; ++e) bm = fmaxf(bm, v[e]);
+    }
+    if (bm > a.m) {
+      rescale(a, bm, c);
+#pragma unroll
+      for (int k = U - 1; k >= 0; --k) {
+        if (k >= n) continue;
+        float v[E], m = kNegInf;
+        unpack_vec<T>(q[k], v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) m = fmaxf(m, v[e]);
+        if (m == bm) best = i0 + k * stride;
+      }
+    }
+    const float r = rel(a.m);
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (k >= n) break;
+      float v[E];
+      unpack_vec<T>(q[k], v);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float t = max_nan((v[e] - r) * c, kFloor), p = ex2(t);
+        a.s += p;
+        a.u = fmaf(p, t, a.u);
+      }
+    }
+  }
+};
+
+// Shared memory of a CTA per row (a warp per row uses none of it).
+struct Shared {
+  Stat stat[kWarps];
+  Key list[kWarps][32];
+  int chosen[32];
+  int nchosen;
+  Key bound;
+  Stat cstat[kMaxCluster];          // written by the cluster's CTAs
+  Key clist[kMaxCluster][32];
+};
+
+HS_DEV unsigned remote(const void *p, int rank) {
+  unsigned r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((unsigned)__cvta_generic_to_shared(p)), "r"(rank));
+  return r;
+}
+HS_DEV void st_remote(const float *p, int rank, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote(p, rank)), "f"(v) : "memory");
+}
+HS_DEV void st_remote(const Key *p, int rank, Key v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote(p, rank)), "l"(v) : "memory");
+}
+
+// W: warps per row (1 or kWarps).
+template <typename T, int W, bool TOP>
+__global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) logprobs_fwd_kernel(const FwdArgs p) {
+  __shared__ Shared sh;
+  constexpr int NT = 32 * W, U = 4, E = Row<T>::E;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tid = W == 1 ? lane : (int)threadIdx.x;
+  const int C = W == 1 ? 1 : p.cluster, rank = (int)(blockIdx.x % C);
+  const int64_t n = W == 1 ? (int64_t)blockIdx.x * kWarps + warp : blockIdx.x / C;
+  if (W == 1 && n >= p.N) return;
+  const T *row = static_cast<const T *>(p.x) + n * p.ld;
+  const int64_t tok = token_at(p.tok, p.token64, n);
+  if (tok == p.ignore) {  // the whole cluster
+    if (rank == 0) {
+      if (tid == 0) {
+        p.lp[n] = 0.f;
+        if (p.ent) p.ent[n] = 0.f;
+        if (p.stats) p.stats[2 * n] = p.stats[2 * n + 1] = 0.f;
+      }
+      if (TOP && tid < p.top) {
+        p.top_lp[n * p.top + tid] = 0.f;
+        p.top_id[n * p.top + tid] = -1;
+      }
+    }
+    return;
+  }
+  if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  const Row<T> r(row, p.V, rank, C);
+  Scan<T> scan;
+  if (tid < r.head) scan.scalar(to_f32<T>(row[tid]), p.c, -2);
+  for (int i = r.lo + tid; i < r.hi; i += U * NT) {
+    uint4 q[U];
+    const int left = (r.hi - i + NT - 1) / NT, here = left < U ? left : U;
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (k < here) q[k] = __ldg(r.vec(i + k * NT));
+    scan.template vectors<U>(q, here, i, NT, p.c);
+  }
+  if (tid < r.ntail) scan.scalar(to_f32<T>(row[r.tail0 + tid]), p.c, -3);
+
+  // the row's statistics
+  Stat a = scan.a;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) merge(a, shfl_xor(a, o), p.c);
+  if (W > 1) {
+    if (lane == 0) sh.stat[warp] = a;
+    if (threadIdx.x == 0) sh.nchosen = 0;
+  }
+
+  Key list = 0;
+  if constexpr (TOP) {
+    // this thread's best value and its lowest index
+    Key mine = 0;
+    if (scan.best == -2) mine = make_key(to_f32<T>(row[tid]), tid);
+    if (scan.best == -3) mine = make_key(to_f32<T>(row[r.tail0 + tid]), r.tail0 + tid);
+    if (scan.best >= 0) {
+      float v[E];
+      unpack_vec<T>(*r.vec(scan.best), v);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const Key k = make_key(v[e], r.index(scan.best, e));
+        if (v[e] == scan.a.m && k > mine) mine = k;
+      }
+      if (mine == 0) mine = make_key(kNegInf, r.index(scan.best, 0));  // NaN alone (the row's results are NaN)
+    }
+    Key bests = sort_desc(mine, lane);
+    if (W > 1) {
+      sh.list[warp][lane] = bests;
+      __syncthreads();
+#pragma unroll
+      for (int half = W / 2; half; half >>= 1) {
+        if (warp < half) {
+          bests = merge_desc(bests, sh.list[warp + half][lane], lane);
+          sh.list[warp][lane] = bests;
+        }
+        __syncthreads();
+      }
+      if (warp == 0 && lane == p.top - 1) sh.bound = bests;
+      __syncthreads();
+    }
+    const Key bound = W > 1 ? sh.bound : __shfl_sync(0xffffffffu, bests, p.top - 1);
+    // read the sets of the threads that reach the bound (0: fewer sets than alternatives, all of them)
+    auto add = [&](Key k) {
+      if (__ballot_sync(0xffffffffu, k >= bound && k > 0) == 0) return;
+      list = merge_desc(list, sort_desc(k >= bound ? k : 0, lane), lane);
+    };
+    auto read_set = [&](int t) {
+      if (t < r.head) add(lane == 0 ? make_key(to_f32<T>(row[t]), t) : 0);
+      for (int i0 = r.lo + t; i0 < r.hi; i0 += 32 * NT) {
+        const int i = i0 + lane * NT;
+        float v[E];
+        const bool ok = i < r.hi;
+        if (ok) unpack_vec<T>(__ldg(r.vec(i)), v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) add(ok && !isnan(v[e]) ? make_key(v[e], r.index(i, e)) : 0);
+      }
+      if (t < r.ntail) add(lane == 0 ? make_key(to_f32<T>(row[r.tail0 + t]), r.tail0 + t) : 0);
+    };
+    if (W == 1) {
+      unsigned who = __ballot_sync(0xffffffffu, mine >= bound && mine > 0);
+      while (who) {
+        const int t = __ffs(who) - 1;
+        who &= who - 1;
+        read_set(t);
+      }
+    } else {
+      if (mine >= bound && mine > 0) {
+        const int at = atomicAdd(&sh.nchosen, 1);  // the order does not matter: keys are merged
+        if (at < 32) sh.chosen[at] = (int)threadIdx.x;
+      }
+      __syncthreads();
+      if (bound > 0) {
+        for (int j = warp; j < min(sh.nchosen, 32); j += W) read_set(sh.chosen[j]);
+      } else {
+        for (int t = warp; t < NT; t += W) read_set(t);
+      }
+      sh.list[warp][lane] = list;
+      __syncthreads();
+#pragma unroll
+      for (int half = W / 2; half; half >>= 1) {
+        if (warp < half) {
+          list = merge_desc(list, sh.list[warp + half][lane], lane);
+          sh.list[warp][lane] = list;
+        }
+        __syncthreads();
+      }
+    }
+  } else if (W > 1) {
+    __syncthreads();
+  }
+  if (W > 1) {
+    if (warp != 0 && C == 1) return;
+    if (warp == 0) {
+      a = sh.stat[lane & (W - 1)];
+#pragma unroll
+      for (int o = W / 2; o; o >>= 1) merge(a, shfl_xor(a, o), p.c);
+    }
+    if (C > 1) {
+      asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA has started
+      if (warp == 0) {
+        if (lane == 0) {
+          st_remote(&sh.cstat[rank].m, 0, a.m);
+          st_remote(&sh.cstat[rank].s, 0, a.s);
+          st_remote(&sh.cstat[rank].u, 0, a.u);
+        }
+        if (TOP) st_remote(&sh.clist[rank][lane], 0, list);
+      }
+      asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+      if (rank != 0 || warp != 0) return;
+      a = sh.cstat[0];
+      for (int j = 1; j < C; ++j) merge(a, sh.cstat[j], p.c);
+      if (TOP) {
+        list = sh.clist[0][lane];
+        for (int j = 1; j < C; ++j) list = merge_desc(list, sh.clist[j][lane], lane);
+      }
+    }
+  }
+  const float kLn2 = 0.69314718055994531f;
+  const bool empty = a.m == kNegInf && a.s == 0.f, bad = isnan(a.s);  // only -inf; a NaN or +inf
+  const float ls = log2f(a.s);
+  auto logp = [&](float x) { return empty ? kNegInf : bad ? a.s : fmaf(x - a.m, p.inv_t, -kLn2 * ls); };
+  if (lane == 0) {
+    if (tok >= 0 && tok < p.V) {
+      p.lp[n] = logp(to_f32<T>(row[tok]));
+    } else {
+      p.lp[n] = __int_as_float(0x7fc00000);
+      set_status(p.status, HS_ERR_INDEX);
+    }
+    if (p.ent) p.ent[n] = empty ? 0.f : kLn2 * (ls - a.u / a.s);
+    if (p.stats) {
+      p.stats[2 * n] = bad ? a.s : a.m;
+      p.stats[2 * n + 1] = ls;
+    }
+  }
+  if (TOP && lane < p.top) {
+    p.top_lp[n * p.top + lane] = logp(value_of(list));
+    p.top_id[n * p.top + lane] = bad ? -1 : index_of(list);
+  }
+}
+
+// ------------------------------------------------------------------ gradient
+struct BwdArgs {
+  const void *x;
+  int64_t ld;
+  const void *tok;
+  int token64;
+  int64_t ignore;
+  float c, inv_t;
+  int top;
+  const float *stats, *ent, *g, *ge, *gt;
+  const int64_t *top_id;
+  void *dx;
+  int64_t dld;
+  int64_t N, V;
+  int parts;  // CTAs per row
+};
+
+template <typename T, int W>
+__global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs p) {
+  constexpr int NT = 32 * W, U = 4, E = Row<T>::E;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int tid = W == 1 ? lane : (int)threadIdx.x;
+  const int C = W == 1 ? 1 : p.parts, rank = (int)(blockIdx.x % C);
+  const int64_t n = W == 1 ? (int64_t)blockIdx.x * kWarps + warp : blockIdx.x / C;
+  if (W == 1 && n >= p.N) return;
+  const T *row = static_cast<const T *>(p.x) + n * p.ld;
+  T *out = static_cast<T *>(p.dx) + n * p.dld;
+  const int64_t tok = token_at(p.tok, p.token64, n);
+  const float m = p.stats[2 * n], ls = p.stats[2 * n + 1];
+  const bool zero = tok == p.ignore || m == kNegInf;
+  const float kLn2 = 0.69314718055994531f;
+  const bool named = tok >= 0 && tok < p.V;
+  const float g = p.g && named ? p.g[n] : 0.f;
+  float sum = g;  // G: every gradient of a log probability of this row
+  if (p.gt && !zero)
+    for (int j = 0; j < p.top; ++j)
+      if (p.top_id[n * p.top + j] >= 0) sum += p.gt[n * p.top + j];
+  const float ge = p.ge && !zero ? p.ge[n] : 0.f;
+  // dx = -inv_t p (sum + ge (ln2 t + entropy)) = p (k0 + k1 t)
+  const float k0 = ge != 0.f ? -p.inv_t * fmaf(ge, p.ent[n], sum) : -p.inv_t * sum, k1 = -p.inv_t * ge * kLn2;
+  auto grad = [&](float x) {
+    const float t = max_nan(fmaf(x - m, p.c, -ls), kFloor);
+    return ex2(t) * fmaf(k1, t, k0);
+  };
+  const Row<T> r(row, p.V, rank, C);
+  // vectors where the output's row is aligned like the input's, else one value at a time
+  const bool vec = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  if (tid < r.head) out[tid] = from_f32<T>(zero ? 0.f : grad(to_f32<T>(row[tid])));
+  if (vec) {
+    uint4 *o = reinterpret_cast<uint4 *>(out + r.base);
+    for (int i = r.lo + tid; i < r.hi; i += U * NT) {
+      uint4 q[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        q[k] = uint4{};
+        if (!zero && i + k * NT < r.hi) q[k] = __ldg(r.vec(i + k * NT));
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        if (i + k * NT >= r.hi) break;
+        float v[E];
+        unpack_vec<T>(q[k], v);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = zero ? 0.f : grad(v[e]);
+        constexpr int P = PerWord<T>::value;
+        o[i + k * NT] = make_uint4(pack_word<T>(v), pack_word<T>(v + P), pack_word<T>(v + 2 * P), pack_word<T>(v + 3 * P));
+      }
+    }
+  } else {
+    for (int i = r.index(r.lo, 0) + tid; i < r.index(r.hi, 0); i += NT) out[i] = from_f32<T>(zero ? 0.f : grad(to_f32<T>(row[i])));
+  }
+  if (tid < r.ntail) out[r.tail0 + tid] = from_f32<T>(zero ? 0.f : grad(to_f32<T>(row[r.tail0 + tid])));
+  if (zero) return;
+  // the values that the gradients name, whole: written again by the CTA that wrote them
+  if (W == 1) __syncwarp(); else __syncthreads();
+  const int a = rank == 0 ? 0 : r.index(r.lo, 0), b = rank == C - 1 ? (int)p.V : r.index(r.hi, 0);
+  for (int j = tid; j <= p.top; j += NT) {
+    const int64_t v = j < p.top ? (p.gt ? p.top_id[n * p.top + j] : -1) : (named ? tok : -1);
+    if (v < a || v >= b) continue;
+    float add = v == tok ? g : 0.f;
+    if (p.gt)
+      for (int k = 0; k < p.top; ++k)
+        if (p.top_id[n * p.top + k] == v) add += p.gt[n * p.top + k];
+    out[v] = from_f32<T>(fmaf(p.inv_t, add, grad(to_f32<T>(row[v]))));
+  }
+}
+
+// ------------------------------------------------------------------ launch
+// Rows up to this many bytes are taken by one warp each.
+constexpr int64_t kShortRow = 4096;
+
+int parts_of(int64_t N, int64_t row_bytes, int most) {
+  // CTAs per row: until the rows fill the SMs several times over, and no
+  // part below 8 KB
+  int c = 1;
+  while (c < most && N * c < 4 * 148 && row_bytes / (2 * c) >= 8192) c *= 2;
+  return c;
+}
+
+int check_rows(const char *who, int dtype, const void *x, int64_t ld, int token_bits, const void *tok, float temperature,
+               int top, int64_t N, int64_t V) {
+  if (!dtype_ok(dtype)) return fail(HS_ERR_INVALID_ARG, "%s: unknown dtype %d", who, dtype);
+  if (token_bits != 32 && token_bits != 64) return fail(HS_ERR_INVALID_ARG, "%s: token_bits is 32 or 64", who);
+  if (N < 0 || V < 0) return fail(HS_ERR_INVALID_ARG, "%s: negative N or V", who);
+  if (V > (int64_t)1 << 30 || N > (int64_t)1 << 27) return fail(HS_ERR_UNSUPPORTED, "%s: V above 2^30 or N above 2^27", who);
+  if (!(temperature > 0.f) || !(temperature < 3.0e38f)) return fail(HS_ERR_INVALID_ARG, "%s: the temperature must be positive", who);
+  if (top < 0 || top > HS_MAX_TOP || top > V) return fail(HS_ERR_INVALID_ARG, "%s: top=%d outside 0..min(%d, V)", who, top, HS_MAX_TOP);
+  if (N == 0) return HS_OK;
+  if (V == 0) return fail(HS_ERR_INVALID_ARG, "%s: rows of no logits", who);
+  if (!x || !aligned(x, dtype_bytes(dtype)) || !tok || !aligned(tok, token_bits / 8))
+    return fail(HS_ERR_INVALID_ARG, "%s: null or misaligned logits or tokens", who);
+  if (ld < V && N > 1) return fail(HS_ERR_INVALID_ARG, "%s: rows %lld apart hold %lld logits", who, (long long)ld, (long long)V);
+  return HS_OK;
+}
+
+template <typename F> int by_type(int dtype, F f) {
+  if (dtype == HS_F32) return f(float{});
+  if (dtype == HS_BF16) return f(__nv_bfloat16{});
+  return f(__half{});
+}
+
+}  // namespace
+}  // namespace hs
+
+extern "C" {
+
+int hs_token_logprobs_forward(int dtype, const void *logits, int64_t logits_ld, int token_bits, const void *tokens,
+                              int64_t ignore_index, float temperature, int top, float *logprob, float *entropy,
+                              float *top_logprob, int64_t *top_index, float *stats, int64_t N, int64_t V,
+                              int *dev_status, hs_stream_t stream) {
+  using namespace hs;
+  if (int e = check_rows("hs_token_logprobs_forward", dtype, logits, logits_ld, token_bits, tokens, temperature, top, N, V)) return e;
+  if (N == 0) return HS_OK;
+  if (!logprob || (top && (!top_logprob || !top_index)) || !dev_status)
+    return fail(HS_ERR_INVALID_ARG, "hs_token_logprobs_forward: null output or dev_status");
+  FwdArgs a = {};
+  a.x = logits, a.ld = logits_ld, a.tok = tokens, a.token64 = token_bits == 64, a.ignore = ignore_index;
+  a.c = (float)(1.4426950408889634 / (double)temperature), a.inv_t = (float)(1.0 / (double)temperature);
+  a.top = top, a.lp = logprob, a.ent = entropy, a.top_lp = top_logprob, a.top_id = top_index, a.stats = stats;
+  a.N = N, a.V = V, a.status = dev_status;
+  const int64_t bytes = V * (int64_t)dtype_bytes(dtype);
+  const bool short_row = bytes <= kShortRow;
+  a.cluster = short_row ? 1 : parts_of(N, bytes, kMaxCluster);
+  return by_type(dtype, [&](auto tag) -> int {
+    using T = decltype(tag);
+    auto kernel = short_row ? (top ? logprobs_fwd_kernel<T, 1, true> : logprobs_fwd_kernel<T, 1, false>)
+                            : (top ? logprobs_fwd_kernel<T, kWarps, true> : logprobs_fwd_kernel<T, kWarps, false>);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(short_row ? (N + kWarps - 1) / kWarps : N * a.cluster));
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = (cudaStream_t)stream;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)a.cluster;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    (void)cudaLaunchKernelEx(&cfg, kernel, a);
+    return check_launch("logprobs_fwd_kernel");
+  });
+}
+
+int hs_token_logprobs_backward(int dtype, const void *logits, int64_t logits_ld, int token_bits, const void *tokens,
+                               int64_t ignore_index, float temperature, int top, const float *stats,
+                               const float *entropy, const int64_t *top_index, const float *dlogprob,
+                               const float *dentropy, const float *dtop_logprob, void *dlogits, int64_t dlogits_ld,
+                               int64_t N, int64_t V, hs_stream_t stream) {
+  using namespace hs;
+  if (int e = check_rows("hs_token_logprobs_backward", dtype, logits, logits_ld, token_bits, tokens, temperature, top, N, V)) return e;
+  if (N == 0) return HS_OK;
+  if (!stats || !dlogits || !aligned(dlogits, dtype_bytes(dtype)) || (dentropy && !entropy) || (dtop_logprob && top && !top_index))
+    return fail(HS_ERR_INVALID_ARG, "hs_token_logprobs_backward: null or misaligned tensor");
+  if (dlogits_ld < V && N > 1) return fail(HS_ERR_INVALID_ARG, "hs_token_logprobs_backward: dlogits rows overlap");
+  BwdArgs a = {};
+  a.x = logits, a.ld = logits_ld, a.tok = tokens, a.token64 = token_bits == 64, a.ignore = ignore_index;
+  a.c = (float)(1.4426950408889634 / (double)temperature), a.inv_t = (float)(1.0 / (double)temperature);
+  a.top = top, a.stats = stats, a.ent = entropy, a.top_id = top_index;
+  a.g = dlogprob, a.ge = dentropy, a.gt = top ? dtop_logprob : nullptr;
+  a.dx = dlogits, a.dld = dlogits_ld, a.N = N, a.V = V;
+  const int64_t bytes = V * (int64_t)dtype_bytes(dtype);
+  const bool short_row = bytes <= kShortRow;
+  a.parts = short_row ? 1 : parts_of(N, bytes, 256);
+  const unsigned grid = (unsigned)(short_row ? (N + kWarps - 1) / kWarps : N * a.parts);
+  return by_type(dtype, [&](auto tag) -> int {
+    using T = decltype(tag);
+    if (short_row)
+      logprobs_bwd_kernel<T, 1><<<grid, kThreads, 0, (cudaStream_t)stream>>>(a);
+    else
+      logprobs_bwd_kernel<T, kWarps><<<grid, kThreads, 0, (cudaStream_t)stream>>>(a);
+    return check_launch("logprobs_bwd_kernel");
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,320 @@
+"""The gated linear recurrence against its definition, step by step in 64 bits.
+
+Tolerances, from the float32 arithmetic: a gate carries a relative error of a
+few units 2^-24, and an error made in one step lasts as long as the state's
+memory, 1 / (1 - |f|) steps at most.  So a state, or a gradient, is off by at
+most about 8 units x (memory + 4) of the tensor's largest value, and results
+stored in 16 bits by half a unit in their last place more."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = torch.device("cuda", 0)
+UNIT = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.float32: 0.0, torch.bfloat16: 0.0, torch.float16: 2.0 ** -25}
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def make(T, B, H, dtype, form, seed=0, starts=False):
+    g = torch.Generator().manual_seed(seed)
+    if form == "gated":
+        a = (1.5 * torch.randn(T, B, H, generator=g) + 1.0).clamp(-6, 5)
+    else:
+        a = 1.9 * torch.rand(T, B, H, generator=g) - 0.95
+    b = torch.randn(T, B, H, generator=g)
+    h0 = torch.randn(B, H, generator=g)
+    dh, dh_n = torch.randn(T, B, H, generator=g), torch.randn(B, H, generator=g)
+    s = torch.rand(T, B, generator=g) < 0.05 if starts else None
+    return a.to(dtype), b.to(dtype), h0, s, dh.to(dtype), dh_n
+
+
+def truth(a, b, h0, s, dh, dh_n, form):
+    """h, h_n and the gradients in 64 bits, by the definition, and the memory."""
+    a, x, h0 = a.double().cpu(), b.double().cpu(), h0.double().cpu()
+    T = a.shape[0]
+    f = torch.sigmoid(a) if form == "gated" else a
+    om = torch.sigmoid(-a) if form == "gated" else None
+    keep = f.clone()
+    cut = torch.zeros(a.shape[:2], dtype=torch.bool) if s is None else s.cpu()
+    keep[cut] = 0
+    inp = om * x if form == "gated" else x
+    h, before, state = torch.empty_like(a), torch.empty_like(a), h0
+    for t in range(T):
+        before[t] = torch.where(cut[t][:, None], 0.0, state)
+        state = torch.where(cut[t][:, None], 0.0, f[t] * state) + inp[t]
+        h[t] = state
+    u = torch.zeros_like(h0) if dh_n is None else dh_n.double().cpu()
+    da, db = torch.empty_like(a), torch.empty_like(a)
+    for t in range(T - 1, -1, -1):
+        e = u + (0 if dh is None else dh[t].double().cpu())
+        da[t] = e * (before[t] - x[t]) * f[t] * om[t] if form == "gated" else e * before[t]
+        db[t] = e * om[t] if form == "gated" else e
+        u = keep[t] * e
+    memory = float(1 / (1 - f.abs().max())) if T else 1.0
+    return dict(h=h, h_n=state, da=da, db=db, dh0=u), min(memory, T)
+
+
+def check(got, want, memory, what, dtype=None):
+    dtype = dtype or got.dtype
+    assert got.dtype == dtype and got.shape == want.shape, what
+    if not want.numel():
+        return
+    err = (got.double().cpu() - want).abs()
+    tol = 8 * 2.0 ** -24 * (memory + 4) * want.abs().max() + TINY[dtype]
+    if dtype != torch.float32:
+        tol = tol + UNIT[dtype] * want.abs()
+    worst = float((err - tol).max())
+    assert worst <= 0, f"{what}: off by {float(err.max()):.3e}, {worst:.3e} over"
+
+
+def call(form):
+    import prlstm_b200 as P
+
+    return P.gated_recurrence if form == "gated" else P.linear_recurrence
+
+
+def run(a, b, h0, s, dh, dh_n, form, batch_first=False):
+    leaves = [t.to(DEV).requires_grad_(True) if t is not None else None for t in (a, b, h0)]
+    h, h_n = call(form)(*leaves[:2], leaves[2], starts=None if s is None else s.to(DEV), batch_first=batch_first)
+    outs = [(o, g.to(DEV)) for o, g in ((h, dh), (h_n, dh_n)) if g is not None]
+    torch.autograd.backward([o for o, _ in outs], [g for _, g in outs])
+    return dict(h=h.detach(), h_n=h_n.detach(), da=leaves[0].grad, db=leaves[1].grad,
+                dh0=None if h0 is None else leaves[2].grad)
+
+
+def check_all(got, want, memory, what):
+    for k in ("h", "h_n", "da", "db", "dh0"):
+        if got[k] is not None:
+            check(got[k], want[k], memory, f"{what} {k}")
+
+
+SHAPES = [(1, 1, 1), (1, 3, 5), (2, 1, 33), (15, 2, 64), (16, 2, 64), (17, 3, 31), (33, 1, 34), (129, 1, 96),
+          (300, 4, 7), (1000, 2, 130), (2049, 1, 64), (5000, 1, 32), (64, 40, 256)]
+
+
+@pytest.mark.parametrize("form", ["gated", "linear"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_forward_and_gradient(shape, dtype, form):
+    for starts in (False, True):
+        a, b, h0, s, dh, dh_n = make(*shape, dtype, form, seed=sum(shape), starts=starts)
+        want, memory = truth(a, b, h0, s, dh, dh_n, form)
+        check_all(run(a, b, h0, s, dh, dh_n, form), want, memory, f"{shape} starts={starts}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_batch_first_is_the_transpose(dtype):
+    a, b, h0, s, dh, dh_n = make(77, 3, 40, dtype, "gated", seed=3, starts=True)
+    want, memory = truth(a, b, h0, s, dh, dh_n, "gated")
+    t = lambda x: x.transpose(0, 1).contiguous()  # noqa: E731
+    got = run(t(a), t(b), h0, t(s), t(dh), dh_n, "gated", batch_first=True)
+    for k in ("h", "da", "db"):
+        assert got[k].is_contiguous()
+        got[k] = got[k].transpose(0, 1)
+    check_all(got, want, memory, "batch first")
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_slices_and_odd_alignment_are_read_in_place(dtype):
+    """z and x as the halves of one projection, as every second sequence, and
+    one element off alignment; gradients of an expanded tensor."""
+    T, B, H = 40, 6, 24
+    a, b, h0, s, dh, dh_n = make(T, B, H, dtype, "gated", seed=5)
+    want, memory = truth(a, b, h0, None, dh, dh_n, "gated")
+    both = torch.cat((a, b), 2).to(DEV)
+    z, x = both.chunk(2, 2)
+    assert not z.is_contiguous()
+    h, h_n = call("gated")(z, x, h0.to(DEV))
+    check(h, want["h"], memory, "halves")
+    wide = torch.zeros(T, 2 * B, H, dtype=dtype, device=DEV)
+    wide[:, ::2] = a.to(DEV)
+    h, _ = call("gated")(wide[:, ::2], x, h0.to(DEV))
+    check(h, want["h"], memory, "every second sequence")
+    off = torch.zeros(T * B * H + 1, dtype=dtype, device=DEV)[1:].view(T, B, H)
+    off.copy_(a)
+    z = off.requires_grad_(True)
+    h, h_n = call("gated")(z, x, h0.to(DEV))
+    torch.autograd.backward((h, h_n), (dh.to(DEV), dh_n.to(DEV)))
+    check(h.detach(), want["h"], memory, "odd alignment")
+    check(z.grad, want["da"], memory, "odd alignment da")
+    ones, _ = truth(a, b, h0, None, torch.ones_like(dh), None, "gated")
+    z2, x2 = a.to(DEV).requires_grad_(True), b.to(DEV).requires_grad_(True)
+    call("gated")(z2, x2, h0.to(DEV))[0].sum().backward()  # an expanded gradient
+    check(z2.grad, ones["da"], memory, "expanded da")
+    check(x2.grad, ones["db"], memory, "expanded db")
+
+
+@pytest.mark.parametrize("form", ["gated", "linear"])
+def test_optional_inputs_and_gradients(form):
+    a, b, h0, s, dh, dh_n = make(50, 2, 36, torch.float32, form, seed=7)
+    zero = torch.zeros_like(h0)
+    for d, dn, start in ((dh, None, None), (None, dh_n, h0), (dh, dh_n, h0.bfloat16())):
+        want, memory = truth(a, b, zero if start is None else start, None, d, dn, form)
+        got = run(a, b, start, None, d, dn, form)
+        if start is not None and start.dtype != torch.float32:
+            assert got["dh0"].dtype == start.dtype
+            check(got["dh0"], want["dh0"], memory, "dh0 in its own type", start.dtype)
+            got["dh0"] = None
+        check_all(got, want, memory, f"{form} {d is None} {dn is None}")
+
+
+def test_empty_extents():
+    for T, B, H in ((0, 3, 8), (4, 0, 8), (4, 3, 0), (0, 0, 0)):
+        z = torch.randn(T, B, H, device=DEV, requires_grad=True)
+        x = torch.randn(T, B, H, device=DEV, requires_grad=True)
+        h0 = torch.randn(B, H, device=DEV, requires_grad=True)
+        h, h_n = call("gated")(z, x, h0)
+        assert h.shape == (T, B, H) and h_n.shape == (B, H)
+        if T == 0:
+            assert torch.equal(h_n, h0)
+        (h.sum() + 3 * h_n.sum()).backward()
+        assert z.grad.shape == z.shape
+        if T == 0:
+            assert torch.equal(h0.grad, torch.full_like(h0, 3))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_nothing_passes_a_start(dtype):
+    """NaN and infinities in one document leave the next one untouched, in
+    both directions, wherever the boundary lies among tiles."""
+    for T, at in ((40, 7), (40, 16), (700, 513), (3000, 1600)):
+        a, b, h0, s, dh, dh_n = make(T, 2, 64, dtype, "gated", seed=at)
+        s = torch.zeros(T, 2, dtype=torch.bool)
+        s[at] = True
+        clean, memory = truth(a, b, h0, s, dh, dh_n, "gated")
+        for bad in (float("nan"), float("inf"), -float("inf")):
+            bb, hh = b.clone(), h0.clone()
+            bb[:at] = bad
+            hh[:] = bad
+            got = run(a, bb, hh, s, dh, dh_n, "gated")
+            check(got["h"][at:], clean["h"][at:], memory, f"h after {bad}")
+            check(got["da"][at:], clean["da"][at:], memory, f"da after {bad}")
+            check(got["db"], clean["db"], memory, f"db with {bad}")  # does not depend on x
+            d = dh.clone()
+            d[at:] = bad
+            got = run(a, b, h0, s, d, dh_n, "gated")
+            check(got["da"][:at], clean["da"][:at], memory, f"da before {bad}")
+            check(got["db"][:at], clean["db"][:at], memory, f"db before {bad}")
+
+
+def test_nan_spreads_as_step_by_step():
+    """Without a start a NaN reaches every later state of its column only."""
+    a, b, h0, s, dh, dh_n = make(900, 1, 70, torch.float32, "gated", seed=9)
+    b[300, 0, 5] = float("nan")
+    h, h_n = call("gated")(a.to(DEV), b.to(DEV), h0.to(DEV))
+    bad = torch.isnan(h).cpu()
+    assert bad[300:, 0, 5].all() and not bad[:300].any() and int(bad.sum()) == 600
+    assert torch.isnan(h_n[0, 5])
+
+
+def test_extreme_gates_and_zero_states():
+    T, H = 2100, 32
+    z = torch.full((T, 1, H), 200.0, device=DEV)  # f = 1: the state is carried unchanged
+    x = torch.randn(T, 1, H, device=DEV)
+    h0 = torch.randn(1, H, device=DEV)
+    h, h_n = call("gated")(z, x, h0)
+    assert torch.equal(h_n, h0) and torch.equal(h, h0.expand(T, 1, H))
+    h, h_n = call("gated")(-z, x, h0)  # f = 0: the input passes
+    assert torch.equal(h, x)
+    # from a zero state, coefficients above 1 whose product overflows give 0
+    h, h_n = call("linear")(torch.full((T, 1, H), 2.0, device=DEV), torch.zeros(T, 1, H, device=DEV))
+    assert torch.equal(h, torch.zeros_like(h)) and torch.equal(h_n, torch.zeros_like(h_n))
+
+
+@pytest.mark.parametrize("form", ["gated", "linear"])
+def test_gradient_against_differences(form):
+    """Central differences of the float32 results: with a step of 2^-5 the
+    third-order term is about 2^-10 / 6 of the gradient's scale and the
+    rounding of the loss (summed in 64 bits) far below it."""
+    a, b, h0, s, dh, dh_n = make(35, 2, 6, torch.float32, form, seed=11, starts=True)
+    got = run(a, b, h0, s, dh, dh_n, form)
+    step = 2.0 ** -5
+
+    def loss(a, b, h0):
+        h, h_n = call(form)(a.to(DEV), b.to(DEV), h0.to(DEV), starts=s.to(DEV))
+        return float((h.double().cpu() * dh).sum() + (h_n.double().cpu() * dh_n).sum())
+
+    g = torch.Generator().manual_seed(1)
+    for name, k in (("da", 0), ("db", 1), ("dh0", 2)):
+        flat = got[name].cpu().reshape(-1)
+        for i in torch.randint(0, flat.numel(), (12,), generator=g).tolist():
+            d = []
+            for sign in (1, -1):
+                v = [a.clone(), b.clone(), h0.clone()]
+                v[k].view(-1)[i] += sign * step
+                d.append(loss(*v))
+            diff = (d[0] - d[1]) / (2 * step)
+            assert abs(diff - float(flat[i])) <= 2.0 ** -9 * float(flat.abs().max()), (name, i)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_step_equals_the_recurrence(dtype):
+    import prlstm_b200 as P
+
+    a, b, h0, _, _, _ = make(6, 5, 70, dtype, "gated", seed=13)
+    h, h_n = P.gated_recurrence(a.to(DEV), b.to(DEV), h0.to(DEV))
+    state, fresh = h0.to(DEV).clone(), h0.to(DEV)
+    for t in range(6):
+        o, new = P.gated_recurrence_step(a[t].to(DEV), b[t].to(DEV), fresh)
+        out, same = P.gated_recurrence_step(a[t].to(DEV), b[t].to(DEV), state, out_state=state)
+        assert same.data_ptr() == state.data_ptr() and torch.equal(state, new) and torch.equal(o, out)
+        fresh = new
+        want, memory = truth(a[:t + 1], b[:t + 1], h0, None, None, None, "gated")
+        check(o, want["h"][t], memory, "step")
+    check(state, want["h_n"], memory, "state")
+    check(h_n, want["h_n"], memory, "h_n")
+
+
+def test_same_bits_every_run_and_on_another_stream():
+    a, b, h0, s, dh, dh_n = make(1500, 2, 200, torch.bfloat16, "gated", seed=17, starts=True)
+    first = run(a, b, h0, s, dh, dh_n, "gated")
+    side = torch.cuda.Stream(DEV)
+    side.wait_stream(torch.cuda.current_stream(DEV))
+    with torch.cuda.stream(side):
+        again = run(a, b, h0, s, dh, dh_n, "gated")
+    side.synchronize()
+    for k in first:
+        assert torch.equal(first[k], again[k]), k
+
+
+def test_long_offsets():
+    """A tensor whose offsets pass 2^31 elements, read through a slice."""
+    T, B, H, W = 3, 2, 64, 600_000_000
+    big = torch.empty(5 * W + H, dtype=torch.bfloat16, device=DEV).as_strided((T, B, H), (2 * W, W, 1))
+    a, b, h0, _, _, _ = make(T, B, H, torch.bfloat16, "gated", seed=19)
+    big.copy_(a)
+    want, memory = truth(a, b, h0, None, None, None, "gated")
+    h, _ = call("gated")(big, b.to(DEV), h0.to(DEV))
+    check(h, want["h"], memory, "long offsets")
+
+
+def test_refusals():
+    import prlstm_b200 as P
+
+    z = torch.randn(4, 2, 8, device=DEV)
+    with pytest.raises(TypeError):
+        P.gated_recurrence(z.double(), z.double())
+    with pytest.raises(TypeError):
+        P.gated_recurrence(z, z.bfloat16())
+    with pytest.raises(RuntimeError):
+        P.gated_recurrence(z, z[:, :1])
+    with pytest.raises(RuntimeError):
+        P.gated_recurrence(z[0], z[0])
+    with pytest.raises(RuntimeError):
+        P.gated_recurrence(z, z, torch.zeros(3, 8, device=DEV))
+    with pytest.raises(RuntimeError):
+        P.gated_recurrence(z, z, starts=torch.zeros(2, 4, dtype=torch.bool, device=DEV))
+    with pytest.raises(RuntimeError):
+        P.gated_recurrence(z, z, starts=torch.zeros(4, 2, device=DEV))
+    with pytest.raises(RuntimeError):
+        P.gated_recurrence(z.cpu(), z.cpu())
+    with pytest.raises(RuntimeError):
+        P.gated_recurrence(z, z, torch.zeros(2, 8))
+    with pytest.raises(TypeError):
+        P.gated_recurrence_step(z[0], z[0], torch.zeros(2, 8, device=DEV, dtype=torch.bfloat16))
+    with pytest.raises(RuntimeError):
+        P.gated_recurrence_step(z[0], z[0], torch.zeros(2, 8, device=DEV), out_state=torch.zeros(2, 16, device=DEV)[:, ::2])
+    with pytest.raises(RuntimeError):
+        P.gated_recurrence_step(z[0].requires_grad_(True), z[0], torch.zeros(2, 8, device=DEV))
