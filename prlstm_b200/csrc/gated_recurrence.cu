@@ -84,19 +84,69 @@ HS_DEV void st_cluster(unsigned addr, int rank, float v) {
       : "memory");
 }
 
-// f = 1/(1+e^-z) and 1-f, each to a few float32 ulps of its own size: with
-// t = e^-|z| they are 1/(1+t) and t/(1+t), whichever way round z's sign says.
-// The reciprocal is refined by one Newton step (as in sigf: its rounding
-// compounds over thousands of steps).
-HS_DEV void gate(float z, float &f, float &om) {
-  const float t = __expf(-fabsf(z));
-  const float d = 1.0f + t;
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-  r = fmaf(r, fmaf(-d, r, 1.0f), r);
-  const float tr = t * r;
-  f = z >= 0.f ? r : tr;
-  om = z >= 0.f ? tr : r;
+// The columns of one lane: one float32, or two as one pair of registers that
+// sm_100a's packed float32 instructions take at once.
+template <int VEC> struct Cols;
+template <> struct Cols<1> {
+  float v;
+  HS_DEV static Cols all(float a) { return {a}; }
+  HS_DEV static Cols of(const float *a) { return {a[0]}; }
+  HS_DEV void get(float *a) const { a[0] = v; }
+};
+template <> struct Cols<2> {
+  unsigned long long v;
+  HS_DEV static Cols of(const float *a) {
+    Cols r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a[0]), "f"(a[1]));
+    return r;
+  }
+  HS_DEV static Cols all(float a) {
+    const float t[2] = {a, a};
+    return of(t);
+  }
+  HS_DEV void get(float *a) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a[0]), "=f"(a[1]) : "l"(v)); }
+};
+HS_DEV Cols<1> operator+(Cols<1> a, Cols<1> b) { return {a.v + b.v}; }
+HS_DEV Cols<1> operator-(Cols<1> a, Cols<1> b) { return {a.v - b.v}; }
+HS_DEV Cols<1> operator*(Cols<1> a, Cols<1> b) { return {__fmul_rn(a.v, b.v)}; }
+HS_DEV Cols<1> fma(Cols<1> a, Cols<1> b, Cols<1> c) { return {fmaf(a.v, b.v, c.v)}; }
+HS_DEV Cols<2> fma(Cols<2> a, Cols<2> b, Cols<2> c) {
+  Cols<2> r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+HS_DEV Cols<2> operator+(Cols<2> a, Cols<2> b) {
+  Cols<2> r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+HS_DEV Cols<2> operator*(Cols<2> a, Cols<2> b) {
+  Cols<2> r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+HS_DEV Cols<2> operator-(Cols<2> a, Cols<2> b) { return fma(b, Cols<2>::all(-1.f), a); }
+
+// f = 1/(1+e^-z) and 1-f = e^-z/(1+e^-z), each to a few float32 ulps of its own
+// size.  e^-z is held to 2^126, so that both stay finite (f is 0 to float32's
+// smallest normal number there); a NaN stays one.  The reciprocal is refined by
+// one Newton step (as in sigf: its rounding compounds over thousands of steps).
+template <int VEC> HS_DEV void gate(const float *z, Cols<VEC> &f, Cols<VEC> &om) {
+  float t[VEC], r[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) {
+    float x = z[v] * -1.44269504088896341f;
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(126.f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t[v]) : "f"(x));
+  }
+  const Cols<VEC> e = Cols<VEC>::of(t), d = e + Cols<VEC>::all(1.f);
+  float dd[VEC];
+  d.get(dd);
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r[v]) : "f"(dd[v]));
+  const Cols<VEC> rr = Cols<VEC>::of(r), nd = d * Cols<VEC>::all(-1.f);
+  f = fma(rr, fma(nd, rr, Cols<VEC>::all(1.f)), rr);
+  om = e * f;
 }
 
 // a * h where a may have overflowed or underflowed as a product of many
@@ -209,9 +259,9 @@ HS_DEV void exchange(Maps<VEC> &m, int p, int warps, int warp, int lane, int clu
   for (int j = 0; j < warp; ++j) apply_map<VEC, STARTS>(m.a[p][j], m.b[p][j], m.cut[p][j], lane, in);
 }
 
-template <int VEC> HS_DEV void load_state(const float *p, int64_t at, bool live, float *v) {
+template <int VEC> HS_DEV void load_state(const float *p, int64_t at, float *v) {
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) v[i] = p && live ? p[at + i] : 0.f;
+  for (int i = 0; i < VEC; ++i) v[i] = p ? p[at + i] : 0.f;
 }
 
 // ------------------------------------------------------------------ forward
@@ -224,8 +274,10 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) rec_fwd_kernel(const FwdArg
   const int lane = threadIdx.x, warp = threadIdx.y, warps = blockDim.y;
   const int cluster = p.s.cluster, rank = (int)(blockIdx.x % cluster);
   const int64_t gid = blockIdx.x / cluster;
-  const int64_t row = gid / p.s.groups, col = (gid % p.s.groups) * 32 * VEC + lane * VEC;
+  const int64_t row = gid / p.s.groups;
+  int64_t col = (gid % p.s.groups) * 32 * VEC + lane * VEC;
   const bool live = col < p.s.n;  // VEC > 1 only where n is a multiple of VEC
+  if (!live) col = p.s.n - VEC;   // reads what a live lane reads, writes nothing
   const int64_t T_ = p.s.T;
   const char *zp = p.z + (row * p.zb + col) * sizeof(T), *xp = p.x + (row * p.xb + col) * sizeof(T);
   char *hp = p.h + (row * p.hb + col) * sizeof(T);
@@ -234,7 +286,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) rec_fwd_kernel(const FwdArg
   const unsigned step = warps * 128u, tensor = kRun * step, stage = 2 * tensor;
 
   float state[VEC];
-  load_state<VEC>(p.h0, row * p.state_b + col, live, state);
+  load_state<VEC>(p.h0, row * p.state_b + col, state);
   if (cluster > 1) cluster_arrive();  // met before the first exchange: every CTA has started
 
   unsigned next_start = 0;
@@ -242,11 +294,19 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) rec_fwd_kernel(const FwdArg
     const int64_t t0 = ((int64_t)(w * cluster + rank) * warps + warp) * kRun;
     const unsigned d = buf + (unsigned)(w % stages) * stage;
     const char *zq = zp + t0 * zs, *xq = xp + t0 * xs;
+    if (t0 + kRun <= T_) {
 #pragma unroll
-    for (int k = 0; k < kRun; ++k) {
-      const bool ok = live && t0 + k < T_;
-      fetch_word<T, VEC>(d + k * step, ok ? zq + k * zs : p.z, ok);
-      fetch_word<T, VEC>(d + tensor + k * step, ok ? xq + k * xs : p.x, ok);
+      for (int k = 0; k < kRun; ++k, zq += zs, xq += xs) {
+        fetch_word<T, VEC>(d + k * step, zq, true);
+        fetch_word<T, VEC>(d + tensor + k * step, xq, true);
+      }
+    } else {
+#pragma unroll 1
+      for (int k = 0; k < kRun; ++k, zq += zs, xq += xs) {
+        const bool ok = t0 + k < T_;
+        fetch_word<T, VEC>(d + k * step, ok ? zq : zp, ok);
+        fetch_word<T, VEC>(d + tensor + k * step, ok ? xq : xp, ok);
+      }
     }
     cp_commit();
   };
@@ -270,26 +330,45 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) rec_fwd_kernel(const FwdArg
     const int64_t t0 = ((int64_t)(w * cluster + rank) * warps + warp) * kRun;
     const unsigned d = buf + (unsigned)(w % stages) * stage;
     const int len = (int)min((int64_t)kRun, T_ - t0);  // may be <= 0
-    float f[kRun][VEC], b[kRun][VEC], A[VEC], B[VEC], in[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) A[v] = 1.f, B[v] = 0.f;
+    using C = Cols<VEC>;
+    C f[kRun], b[kRun];
 #pragma unroll
     for (int k = 0; k < kRun; ++k) {
-      read_word<T, VEC>(d + k * step, f[k]);
-      read_word<T, VEC>(d + tensor + k * step, b[k]);
-      const bool cut = STARTS && ((mask >> k) & 1);
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        if (GATED) {
-          float om;
-          gate(f[k][v], f[k][v], om);
-          b[k][v] *= om;
-        }
-        if (k >= len) f[k][v] = 1.f, b[k][v] = 0.f;
-        A[v] = cut ? 0.f : A[v] * f[k][v];
-        B[v] = cut ? b[k][v] : fmaf(f[k][v], B[v], b[k][v]);
+      float zv[VEC], xv[VEC];
+      read_word<T, VEC>(d + k * step, zv);
+      read_word<T, VEC>(d + tensor + k * step, xv);
+      if (GATED) {
+        C om;
+        gate<VEC>(zv, f[k], om);
+        b[k] = om * C::of(xv);
+      } else {
+        f[k] = C::of(zv);
+        b[k] = C::of(xv);
       }
     }
+    if (len < kRun) {
+#pragma unroll
+      for (int k = 0; k < kRun; ++k)
+        if (k >= len) f[k] = C::all(1.f), b[k] = C::all(0.f);
+    }
+    C mapA = C::all(1.f), mapB = C::all(0.f);
+    if (STARTS && mask) {
+#pragma unroll
+      for (int k = 0; k < kRun; ++k) {
+        const bool cut = (mask >> k) & 1;
+        mapA = cut ? C::all(0.f) : mapA * f[k];
+        mapB = cut ? b[k] : fma(f[k], mapB, b[k]);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kRun; ++k) {
+        mapA = mapA * f[k];
+        mapB = fma(f[k], mapB, b[k]);
+      }
+    }
+    float A[VEC], B[VEC], in[VEC];
+    mapA.get(A);
+    mapB.get(B);
     if (cluster > 1 && w == 0) cluster_wait();
     exchange<VEC, STARTS>(maps, w & 1, warps, warp, lane, cluster, rank, A, B, mask != 0, state, in);
     if (live && len > 0) {
@@ -299,12 +378,25 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) rec_fwd_kernel(const FwdArg
         for (int v = 0; v < VEC; ++v) c[v] = in[v];
       }
       char *hq = hp + t0 * hs;
+      C h = C::of(in);
+      auto put = [&] {
+        float hv[VEC];
+        h.get(hv);
+        write_word<T, VEC>(hq, hv);
+        hq += hs;
+      };
+      if (len < kRun || (STARTS && mask)) {
 #pragma unroll
-      for (int k = 0; k < kRun; ++k) {
-        const bool cut = STARTS && ((mask >> k) & 1);
+        for (int k = 0; k < kRun; ++k) {
+          h = STARTS && ((mask >> k) & 1) ? b[k] : fma(f[k], h, b[k]);
+          if (k < len) put();
+        }
+      } else {
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) in[v] = cut ? b[k][v] : fmaf(f[k][v], in[v], b[k][v]);
-        if (k < len) write_word<T, VEC>(hq + k * hs, in);
+        for (int k = 0; k < kRun; ++k) {
+          h = fma(f[k], h, b[k]);
+          put();
+        }
       }
     }
   }
@@ -328,8 +420,10 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) rec_bwd_kernel(const BwdArg
   const int lane = threadIdx.x, warp = threadIdx.y, warps = blockDim.y;
   const int cluster = p.s.cluster, rank = (int)(blockIdx.x % cluster);
   const int64_t gid = blockIdx.x / cluster;
-  const int64_t row = gid / p.s.groups, col = (gid % p.s.groups) * 32 * VEC + lane * VEC;
+  const int64_t row = gid / p.s.groups;
+  int64_t col = (gid % p.s.groups) * 32 * VEC + lane * VEC;
   const bool live = col < p.s.n;
+  if (!live) col = p.s.n - VEC;
   const int64_t T_ = p.s.T;
   const char *zp = p.z + (row * p.zb + col) * sizeof(T), *xp = p.x + (row * p.xb + col) * sizeof(T);
   const char *gp = p.g + (row * p.gb + col) * sizeof(T);
@@ -340,7 +434,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) rec_bwd_kernel(const BwdArg
   const unsigned step = warps * 128u, tensor = kRun * step, stage = 3 * tensor;
 
   float state[VEC];
-  load_state<VEC>(p.dh_n, row * p.state_b + col, live, state);
+  load_state<VEC>(p.dh_n, row * p.state_b + col, state);
   if (cluster > 1) cluster_arrive();  // met before the first exchange: every CTA has started
 
   // chunks from the last to the first; below 0: past the beginning, nothing
@@ -350,12 +444,21 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) rec_bwd_kernel(const BwdArg
     const int64_t t0 = (int64_t)c * kRun;
     const unsigned d = buf + (unsigned)(w % stages) * stage;
     const char *zq = zp + t0 * zs, *xq = xp + t0 * xs, *gq = gp + t0 * gs;
+    if (c >= 0 && t0 + kRun <= T_ && p.g) {
 #pragma unroll
-    for (int k = 0; k < kRun; ++k) {
-      const bool ok = live && c >= 0 && t0 + k < T_, okg = ok && p.g != nullptr;
-      fetch_word<T, VEC>(d + k * step, ok ? zq + k * zs : p.z, ok);
-      fetch_word<T, VEC>(d + tensor + k * step, ok ? xq + k * xs : p.z, ok);
-      fetch_word<T, VEC>(d + 2 * tensor + k * step, okg ? gq + k * gs : p.z, okg);
+      for (int k = 0; k < kRun; ++k, zq += zs, xq += xs, gq += gs) {
+        fetch_word<T, VEC>(d + k * step, zq, true);
+        fetch_word<T, VEC>(d + tensor + k * step, xq, true);
+        fetch_word<T, VEC>(d + 2 * tensor + k * step, gq, true);
+      }
+    } else if (c >= 0) {
+#pragma unroll 1
+      for (int k = 0; k < kRun; ++k, zq += zs, xq += xs, gq += gs) {
+        const bool ok = t0 + k < T_, okg = ok && p.g;
+        fetch_word<T, VEC>(d + k * step, ok ? zq : zp, ok);
+        fetch_word<T, VEC>(d + tensor + k * step, ok ? xq : xp, ok);
+        fetch_word<T, VEC>(d + 2 * tensor + k * step, okg ? gq : zp, okg);
+      }
     }
     cp_commit();
   };
@@ -365,7 +468,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) rec_bwd_kernel(const BwdArg
   };
   auto fetch_ckpt = [&](int w, float *h) {
     const int c = chunk_of(w);
-    load_state<VEC>(p.ckpt, c * p.ckpt_t + row * p.state_b + col, live && c >= 0, h);
+    load_state<VEC>(c >= 0 ? p.ckpt : nullptr, c * p.ckpt_t + row * p.state_b + col, h);
   };
 
   unsigned next_start = 0;
@@ -391,67 +494,92 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) rec_bwd_kernel(const BwdArg
     const int64_t t0 = (int64_t)c * kRun;
     const unsigned d = buf + (unsigned)(w % stages) * stage;
     const int len = c < 0 ? 0 : (int)min((int64_t)kRun, T_ - t0);
-    // keep: 1-f (gated) or f (linear); q: the factor of e in df
-    float keep[kRun][VEC], both[kBoth ? kRun : 1][VEC], q[kRun][VEC], A[VEC], B[VEC], u[VEC];
-#pragma unroll
-    for (int k = 0; k < kRun; ++k) {
-      float zz[VEC], xx[VEC];
-      read_word<T, VEC>(d + k * step, zz);
-      read_word<T, VEC>(d + tensor + k * step, xx);
-      const bool cut = STARTS && ((mask >> k) & 1);
-#pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const float before = cut ? 0.f : h[v];
-        if (GATED) {
-          float f, om;
-          gate(zz[v], f, om);
-          q[k][v] = (before - xx[v]) * f * om;
-          h[v] = fmaf(f, before, om * xx[v]);
-          if (k >= len) om = 0.f, f = 1.f;
-          keep[k][v] = om;
-          if (kBoth) both[k][v] = f;
-        } else {
-          q[k][v] = before;
-          h[v] = fmaf(zz[v], before, xx[v]);
-          keep[k][v] = k >= len ? 1.f : zz[v];
-        }
-      }
-    }
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) A[v] = 1.f, B[v] = 0.f;
-#pragma unroll
-    for (int k = kRun - 1; k >= 0; --k) {
+    using C = Cols<VEC>;
+    const C one = C::all(1.f), zero = C::all(0.f);
+    // keep: 1-f (gated) or f (linear); q: the factor of e in df (set where the
+    // warp has a run, c >= 0, and read only there)
+#pragma nv_diag_suppress 549
+    C keep[kRun], both[kBoth ? kRun : 1], q[kRun];
+    auto coef = [&](int k) { return kBoth ? both[kBoth ? k : 0] : GATED ? one - keep[k] : keep[k]; };
+    auto grad = [&](int k) {
       float g[VEC];
       read_word<T, VEC>(d + 2 * tensor + k * step, g);
-      const bool cut = STARTS && ((mask >> k) & 1);
+      return C::of(g);
+    };
+    C A = one, B = zero;
+    if (c >= 0) {
+      C s = C::of(h);
 #pragma unroll
-      for (int v = 0; v < VEC; ++v) {
-        const float f = kBoth ? both[kBoth ? k : 0][v] : GATED ? 1.f - keep[k][v] : keep[k][v];
-        B[v] = cut ? 0.f : f * (g[v] + B[v]);
-        A[v] = cut ? 0.f : A[v] * f;
+      for (int k = 0; k < kRun; ++k) {
+        float zv[VEC], xv[VEC];
+        read_word<T, VEC>(d + k * step, zv);
+        read_word<T, VEC>(d + tensor + k * step, xv);
+        const C x = C::of(xv);
+        if (STARTS && ((mask >> k) & 1)) s = zero;
+        if (GATED) {
+          C f, om;
+          gate<VEC>(zv, f, om);
+          q[k] = (s - x) * (f * om);
+          s = fma(f, s, om * x);
+          keep[k] = om;
+          if (kBoth) both[k] = f;
+        } else {
+          q[k] = s;
+          keep[k] = C::of(zv);
+          s = fma(keep[k], s, x);
+        }
+      }
+      if (len < kRun) {
+#pragma unroll
+        for (int k = 0; k < kRun; ++k)
+          if (k >= len) {
+            keep[k] = GATED ? zero : one;
+            if (kBoth) both[k] = one;
+          }
+      }
+      if (STARTS && mask) {
+#pragma unroll
+        for (int k = kRun - 1; k >= 0; --k) {
+          const bool cut = (mask >> k) & 1;
+          B = cut ? zero : coef(k) * (grad(k) + B);
+          A = cut ? zero : A * coef(k);
+        }
+      } else {
+#pragma unroll
+        for (int k = kRun - 1; k >= 0; --k) {
+          const C f = coef(k);
+          B = f * (grad(k) + B);
+          A = A * f;
+        }
       }
     }
+    float Av[VEC], Bv[VEC], u[VEC];
+    A.get(Av);
+    B.get(Bv);
     if (cluster > 1 && w == 0) cluster_wait();
-    exchange<VEC, STARTS>(maps, w & 1, warps, warp, lane, cluster, rank, A, B, mask != 0, state, u);
+    exchange<VEC, STARTS>(maps, w & 1, warps, warp, lane, cluster, rank, Av, Bv, mask != 0, state, u);
     if (live && len > 0) {
-      char *dzq = dzp + t0 * dzs, *dxq = dxp + t0 * dxs;
-#pragma unroll
-      for (int k = kRun - 1; k >= 0; --k) {
-        float g[VEC], dz[VEC], dx[VEC];
-        read_word<T, VEC>(d + 2 * tensor + k * step, g);
-        const bool cut = STARTS && ((mask >> k) & 1);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-          const float f = kBoth ? both[kBoth ? k : 0][v] : GATED ? 1.f - keep[k][v] : keep[k][v];
-          const float e = g[v] + u[v];
-          dz[v] = e * q[k][v];
-          dx[v] = GATED ? e * keep[k][v] : e;
-          u[v] = cut ? 0.f : f * e;
+      char *dzq = dzp + (t0 + kRun - 1) * dzs, *dxq = dxp + (t0 + kRun - 1) * dxs;
+      C uu = C::of(u);
+      auto put = [&](int k, bool cut, bool write) {
+        const C e = grad(k) + uu;
+        uu = cut ? zero : coef(k) * e;
+        if (write) {
+          float dz[VEC], dx[VEC];
+          (e * q[k]).get(dz);
+          (GATED ? e * keep[k] : e).get(dx);
+          write_word<T, VEC>(dzq, dz);
+          write_word<T, VEC>(dxq, dx);
         }
-        if (k < len) {
-          write_word<T, VEC>(dzq + k * dzs, dz);
-          write_word<T, VEC>(dxq + k * dxs, dx);
-        }
+        dzq -= dzs;
+        dxq -= dxs;
+      };
+      if (len < kRun || (STARTS && mask)) {
+#pragma unroll
+        for (int k = kRun - 1; k >= 0; --k) put(k, STARTS && ((mask >> k) & 1), k < len);
+      } else {
+#pragma unroll
+        for (int k = kRun - 1; k >= 0; --k) put(k, false, true);
       }
     }
   }
