@@ -502,7 +502,7 @@ HS_API int hs_recurrence_forward(int dtype, int form, const void *z, int64_t z_t
                                  int64_t x_t, int64_t x_b, const float *h0, const unsigned char *starts,
                                  int64_t starts_t, int64_t starts_b, void *h, int64_t h_t, int64_t h_b,
                                  float *h_n, float *checkpoints, int64_t T, int64_t B, int64_t H,
-                                 hs_stream_t stream);
+                                 int *dev_status, hs_stream_t stream);
 /* Its gradient: dh [T,B,H] and dh_n [B,H] (either may be NULL = zeros) to dz,
  * dx [T,B,H] and dh0 [B,H] (NULL = not wanted).  Reads the forward's
  * checkpoints, not h: the states are recomputed in float32. */
@@ -511,7 +511,7 @@ HS_API int hs_recurrence_backward(int dtype, int form, const void *z, int64_t z_
                                   const unsigned char *starts, int64_t starts_t, int64_t starts_b,
                                   const void *dh, int64_t dh_t, int64_t dh_b, const float *dh_n, void *dz,
                                   int64_t dz_t, int64_t dz_b, void *dx, int64_t dx_t, int64_t dx_b, float *dh0,
-                                  int64_t T, int64_t B, int64_t H, hs_stream_t stream);
+                                  int64_t T, int64_t B, int64_t H, int *dev_status, hs_stream_t stream);
 
 /* out[n] = scale * weight[tokens[n]], weight [V,D] with rows weight_ld
  * elements apart, out [N,D].  tokens are 64-bit (token_bits = 64) or 32-bit

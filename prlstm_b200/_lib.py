@@ -90,9 +90,9 @@ SIGNATURES = {
     "hs_recurrent_backward_bf16": (_i32, [_c_p] * 17 + [_i64] * 4 + [_c_p, _sz, _c_p, _c_p]),
     "hs_recurrence_checkpoint_bytes": (_sz, [_i64] * 3),
     "hs_recurrence_forward": (_i32, [_i32] * 2 + [_c_p, _i64, _i64] * 2 + [_c_p] + [_c_p, _i64, _i64] * 2
-                              + [_c_p] * 2 + [_i64] * 3 + [_c_p]),
+                              + [_c_p] * 2 + [_i64] * 3 + [_c_p] * 2),
     "hs_recurrence_backward": (_i32, [_i32] * 2 + [_c_p, _i64, _i64] * 2 + [_c_p] + [_c_p, _i64, _i64] * 2 + [_c_p]
-                               + [_c_p, _i64, _i64] * 2 + [_c_p] + [_i64] * 3 + [_c_p]),
+                               + [_c_p, _i64, _i64] * 2 + [_c_p] + [_i64] * 3 + [_c_p] * 2),
     "hs_embedding_forward": (_i32, [_i32, _c_p, _i64, _i32, _c_p, _f64, _c_p] + [_i64] * 3 + [_c_p] * 2),
     "hs_embedding_workspace_bytes": (_sz, [_i64] * 3),
     "hs_embedding_backward": (_i32, [_i32, _c_p, _i32, _c_p, _i64, _f64, _c_p] + [_i64] * 3

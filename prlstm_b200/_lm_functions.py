@@ -82,7 +82,7 @@ def _recurrence_forward(form, z, x, h0, starts, batch_first, keep, h_n=None):
     zs, xs, hs = _strides(z, batch_first), _strides(x, batch_first), _strides(h, batch_first)
     ss = (0, 0) if starts is None else _strides(starts, batch_first)
     _call("hs_recurrence_forward", dev, _CODE[z.dtype], form, _p(z), *zs, _p(x), *xs, _p(h0), _p(starts), *ss,
-          _p(h), *hs, _p(h_n), _p(ckpt), T, B, H)
+          _p(h), *hs, _p(h_n), _p(ckpt), T, B, H, _p(_lib.status_word(dev)))
     return h, h_n, ckpt
 
 
@@ -112,7 +112,7 @@ class RecurrenceFn(torch.autograd.Function):
         ss = (0, 0) if starts is None else _strides(starts, bf)
         _call("hs_recurrence_backward", dev, _CODE[z.dtype], ctx.form, _p(z), *_strides(z, bf), _p(x),
               *_strides(x, bf), _p(ckpt), _p(starts), *ss, _p(dh), *gs, _p(dh_n), _p(dz), *_strides(dz, bf),
-              _p(dx), *_strides(dx, bf), _p(dh0), T, B, H)
+              _p(dx), *_strides(dx, bf), _p(dh0), T, B, H, _p(_lib.status_word(dev)))
         return dz, dx, None if dh0 is None else dh0.to(ctx.h0_dtype), None, None, None
 
 
