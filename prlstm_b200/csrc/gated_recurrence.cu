@@ -32,16 +32,24 @@
 
 #include <algorithm>
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
 #include "lm_types.cuh"
+
+// Arrays filled and read by fully unrolled loops read as "used before set" to
+// the compiler's front end.
+#pragma nv_diag_suppress 549
 
 namespace hs {
 namespace {
 
 constexpr int kRun = 16;       // steps per warp and per saved state
-constexpr int kMaxWarps = 8;   // warps of a CTA along time
+constexpr int kMaxWarps = 4;   // warps of a CTA along time
 constexpr int kMaxCluster = 8; // CTAs of a cluster along time
-constexpr int kFwdStages = 3, kBwdStages = 2;
-constexpr unsigned kStep = 128, kTensor = kRun * kStep;  // shared memory of one warp: a step, a run of one tensor
+constexpr int kStages = 2;     // waves of inputs in shared memory
+constexpr unsigned kStep = 128, kSlab = kRun * kStep;  // bytes of a step's words, and of a warp's run of one tensor
+constexpr int kFwdCtas = 4, kBwdCtas = 3;  // CTAs per SM (registers, shared memory)
 
 struct RecShape {
   int64_t T, n;         // steps; columns of one row
@@ -62,6 +70,7 @@ struct FwdArgs {
   int64_t state_b;                         // row stride of h0 and h_n (columns)
   int64_t ckpt_t;                          // columns of one saved state (B * H)
   int *status;
+  CUtensorMap zm, xm, hm;                  // where the tensors suit TMA
 };
 
 struct BwdArgs {
@@ -74,12 +83,12 @@ struct BwdArgs {
   int64_t zt, zb, xt, xb, gt, gb, dzt, dzb, dxt, dxb, st, sb;
   int64_t state_b, ckpt_t;
   int *status;
+  CUtensorMap zm, xm, gm, dzm, dxm;
 };
 
 HS_DEV unsigned smem_u32(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
-HS_DEV void cp_async4(unsigned dst, const void *src, bool valid) {
-  const int n = valid ? 4 : 0;  // 0 bytes read: the word is filled with zeros
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+HS_DEV void cp_async4(unsigned dst, const void *src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 HS_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> HS_DEV void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -125,6 +134,23 @@ HS_DEV unsigned cluster_addr(const void *p, int rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
   return r;
 }
+
+// A box of a [T][rows][columns] tensor into shared memory, counted on bar (out
+// of range: zeros), and a warp's run back (out of range: dropped).
+HS_DEV void tma_load(unsigned dst, const CUtensorMap *tm, uint64_t *bar, int col, int row, int t) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(tm), "r"(col), "r"(row), "r"(t), "r"(smem_u32(bar))
+      : "memory");
+}
+HS_DEV void tma_store(const CUtensorMap *tm, unsigned src, int col, int row, int t) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(tm), "r"(col),
+               "r"(row), "r"(t), "r"(src)
+               : "memory");
+}
+HS_DEV void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+HS_DEV void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+HS_DEV void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // The columns of one lane: one float32, or two as one pair of registers that
 // sm_100a's packed float32 instructions take at once.
@@ -191,19 +217,21 @@ template <int VEC> HS_DEV void gate(const float *z, Cols<VEC> &f, Cols<VEC> &om)
   om = e * f;
 }
 
-// Row of one warp: base pointers advance by whole steps.
-template <typename T, int VEC> HS_DEV void fetch_word(unsigned dst, const char *src, bool valid) {
+// One lane's word of a step, copied by the lane itself.
+template <typename T, int VEC> HS_DEV void fetch_word(unsigned dst, const char *src) {
   if constexpr (VEC == PerWord<T>::value) {
-    cp_async4(dst, src, valid);
+    cp_async4(dst, src);
   } else {  // one 16-bit value per lane: rows that are not 4-byte aligned
-    unsigned w = 0;
-    if (valid) w = *reinterpret_cast<const unsigned short *>(src);
+    const unsigned w = *reinterpret_cast<const unsigned short *>(src);
     asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst), "r"(w) : "memory");
   }
 }
-template <typename T, int VEC> HS_DEV void read_word(unsigned src, float *v) {
+HS_DEV unsigned read_raw(unsigned src) {
   unsigned w;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(src) : "memory");
+  return w;
+}
+template <typename T, int VEC> HS_DEV void unpack_lane(unsigned w, float *v) {
   if constexpr (VEC == PerWord<T>::value) {
     unpack_word<T>(w, v);
   } else {
@@ -211,6 +239,10 @@ template <typename T, int VEC> HS_DEV void read_word(unsigned src, float *v) {
     unpack_word<T>(w, t);
     v[0] = t[0];
   }
+}
+template <typename T, int VEC> HS_DEV void read_word(unsigned src, float *v) { unpack_lane<T, VEC>(read_raw(src), v); }
+template <typename T> HS_DEV void stage_word(unsigned dst, const float *v) {
+  asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst), "r"(pack_word<T>(v)) : "memory");
 }
 template <typename T, int VEC> HS_DEV void write_word(char *dst, const float *v) {
   if constexpr (VEC == PerWord<T>::value)
@@ -249,12 +281,14 @@ template <int VEC, bool GATED> HS_DEV Cols<VEC> held(Cols<VEC> a) {
 // stores.  A CTA sends the map of wave w+2 only after all of wave w+1 have
 // arrived, and each of those was sent after its sender's last read of wave w.
 template <int VEC> struct Maps {
-  Map<VEC> warp[2][kMaxWarps][32], cta[2][kMaxCluster][32];
+  Map<VEC> warp[2][kMaxWarps][32];
   uint64_t bar[2];
+  Map<VEC> *cta;  // [2][cluster][32], behind the tiles (where the cluster has more than one CTA)
 };
 
 // Sets up the maps; met by exchange_ready() before the first publish.
-template <int VEC> HS_DEV void exchange_init(Maps<VEC> &m, int warps, int warp, int lane, int cluster) {
+template <int VEC> HS_DEV void exchange_init(Maps<VEC> &m, unsigned char *behind, int warps, int warp, int lane, int cluster) {
+  if (warp == 0 && lane == 0) m.cta = reinterpret_cast<Map<VEC> *>(behind);
   Map<VEC> one;
 #pragma unroll
   for (int v = 0; v < VEC; ++v) one.a[v] = 1.f, one.b[v] = 0.f;
@@ -301,7 +335,7 @@ HS_DEV void publish(Maps<VEC> &m, int w, int warps, int warp, int lane, int clus
     tb.get(t.b);
     if (STARTS && any) t.a[0] = __int_as_float(0x7f800000);
     for (int r = 0; r < cluster; ++r) {
-      const unsigned to = cluster_addr(&m.cta[p][rank][lane], r), bar = cluster_addr(&m.bar[p], r);
+      const unsigned to = cluster_addr(&m.cta[(p * cluster + rank) * 32 + lane], r), bar = cluster_addr(&m.bar[p], r);
       if constexpr (VEC == 2)
         asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to),
                      "f"(t.a[0]), "f"(t.a[1]), "f"(t.b[0]), "f"(t.b[1]), "r"(bar)
@@ -333,7 +367,7 @@ HS_DEV Cols<VEC> resolve(Maps<VEC> &m, int w, int warp, int lane, int cluster, i
   for (int r = 0; r < kMaxCluster; ++r) {
     if (r < cluster) {
       if (r == rank) in = state;
-      state = apply<VEC, STARTS>(m.cta[p][r][lane], state);
+      state = apply<VEC, STARTS>(m.cta[(p * cluster + r) * 32 + lane], state);
     }
   }
 #pragma unroll
@@ -347,192 +381,194 @@ template <int VEC> HS_DEV void load_state(const float *p, int64_t at, float *v) 
   for (int i = 0; i < VEC; ++i) v[i] = p ? p[at + i] : 0.f;
 }
 
-// ------------------------------------------------------------------ forward
-// Shared memory: kFwdStages buffers of [2 tensors][16 steps][32 words] per warp,
-// each lane's words private to it (copied in and read by the same thread).
-//
-// A wave is summarised before the previous one is finished: its gates and
-// its map are computed while the previous wave's maps travel, then the
-// previous wave's outputs are written, then its own map is published.  Between the
-// two a 16-bit lane keeps 1-f alone and reads x again from shared memory
-// (f = 1 - (1-f) is off by 2^-25 at most); a float32 lane keeps f and b.
-template <typename T, int VEC, bool GATED, bool STARTS> struct FwdRun {
-  static constexpr bool kBoth = sizeof(T) == 4;
-  using C = Cols<VEC>;
-  C keep[GATED || kBoth ? kRun : 1], b[kBoth ? kRun : 1];
-  unsigned mask;
-  C A, B;
-
-  // gates and map of the run staged at d; steps from len on are the identity
-  HS_DEV void summarise(unsigned d, int len) {
-    A = C::all(1.f), B = C::all(0.f);
-    auto one = [&](int k, bool cut) {
-      float zv[VEC], xv[VEC];
-      read_word<T, VEC>(d + k * kStep, zv);
-      read_word<T, VEC>(d + kTensor + k * kStep, xv);
-      C f, bb;
-      if (GATED) {
-        C om;
-        gate<VEC>(zv, f, om);
-        bb = om * C::of(xv);
-        keep[k] = kBoth ? f : om;
-      } else {
-        f = C::of(zv);
-        bb = C::of(xv);
-        if (kBoth) keep[k] = f;
-      }
-      if (kBoth) b[k] = bb;
-      A = cut ? C::all(0.f) : A * f;
-      B = cut ? bb : fma(f, B, bb);
-    };
-    if (len < kRun) {
-#pragma unroll
-      for (int k = 0; k < kRun; ++k)
-        if (k < len) one(k, STARTS && ((mask >> k) & 1));
-    } else if (STARTS && mask) {
-#pragma unroll
-      for (int k = 0; k < kRun; ++k) one(k, (mask >> k) & 1);
-    } else {
-#pragma unroll
-      for (int k = 0; k < kRun; ++k) one(k, false);
-    }
-  }
-
-  // the states of the run from the one entering it
-  HS_DEV void write(unsigned d, int len, C h, char *hq, int64_t hs) const {
-    auto one = [&](int k, bool cut) {
-      C f, bb;
-      if (kBoth) {
-        f = keep[k], bb = b[k];
-      } else {
-        float xv[VEC];
-        read_word<T, VEC>(d + kTensor + k * kStep, xv);
-        bb = C::of(xv);
-        if (GATED) {
-          f = C::all(1.f) - keep[k];
-          bb = keep[k] * bb;
-        } else {
-          float zv[VEC];
-          read_word<T, VEC>(d + k * kStep, zv);
-          f = C::of(zv);
-        }
-      }
-      h = cut ? bb : fma(f, h, bb);
-      float hv[VEC];
-      h.get(hv);
-      write_word<T, VEC>(hq, hv);
-      hq += hs;
-    };
-    if (len < kRun) {
-#pragma unroll
-      for (int k = 0; k < kRun; ++k)
-        if (k < len) one(k, STARTS && ((mask >> k) & 1));
-    } else if (STARTS && mask) {
-#pragma unroll
-      for (int k = 0; k < kRun; ++k) one(k, (mask >> k) & 1);
-    } else {
-#pragma unroll
-      for (int k = 0; k < kRun; ++k) one(k, false);
-    }
+// ------------------------------------------------------------------ inputs
+// Shared memory of a CTA: kStages x [N tensors][warps][16 steps][32 words] of
+// inputs, then [outputs][warps][16 steps][32 words] where TMA writes them.
+// A tile of all warps' runs comes in by one TMA copy per tensor (TMA), or each
+// lane copies and reads its own words (tensors or strides off 16 bytes).
+template <typename T, int VEC, bool TMA, int N> struct Inputs {
+  unsigned base, tensor;  // this lane's first word of its slab; bytes between tensors
+  uint64_t *full;
+  int *status;
+  HS_DEV unsigned at(int w) const { return base + (unsigned)(w % kStages) * (N * tensor); }
+  // Waits until wave w is there.
+  HS_DEV void wait(int w) const {
+    if constexpr (TMA)
+      mbar_wait(full + w % kStages, (w / kStages) & 1, status);
+    else
+      cp_wait<kStages - 1>();
   }
 };
 
-template <typename T, int VEC, bool GATED, bool STARTS>
-__global__ void __launch_bounds__(32 * kMaxWarps, 2) rec_fwd_kernel(const FwdArgs p) {
-  extern __shared__ __align__(16) unsigned char dyn[];
+HS_DEV void barriers_init(uint64_t *full, int warp, int lane) {
+  if (warp == 0 && lane == 0) {
+    for (int i = 0; i < kStages; ++i) mbar_init(full + i);
+    fence_mbar_init();
+    fence_async();
+  }
+  __syncthreads();
+}
+
+// ------------------------------------------------------------------ forward
+template <typename T, int VEC, bool GATED, bool STARTS, bool TMA>
+__global__ void __launch_bounds__(32 * kMaxWarps, kFwdCtas) rec_fwd_kernel(const __grid_constant__ FwdArgs p) {
+  extern __shared__ __align__(128) unsigned char dyn[];
   __shared__ Maps<VEC> maps;
+  __shared__ uint64_t full[kStages];
   using C = Cols<VEC>;
   const int lane = threadIdx.x, warp = threadIdx.y, warps = blockDim.y;
   const int cluster = p.s.cluster, rank = (int)(blockIdx.x % cluster), waves = p.s.waves;
   const int64_t gid = blockIdx.x / cluster;
   const int64_t row = gid / p.s.groups;
-  int64_t col = (gid % p.s.groups) * 32 * VEC + lane * VEC;
+  const int64_t col0 = (gid % p.s.groups) * 32 * VEC;
+  int64_t col = col0 + lane * VEC;
   const bool live = col < p.s.n;  // VEC > 1 only where n is a multiple of VEC
   if (!live) col = p.s.n - VEC;   // reads what a live lane reads, writes nothing
   const int64_t T_ = p.s.T;
-  const char *zp = p.z + (row * p.zb + col) * sizeof(T), *xp = p.x + (row * p.xb + col) * sizeof(T);
-  char *hp = p.h + (row * p.hb + col) * sizeof(T);
-  const int64_t zs = p.zt * (int64_t)sizeof(T), xs = p.xt * (int64_t)sizeof(T), hs = p.ht * (int64_t)sizeof(T);
-  constexpr unsigned stage = 2 * kTensor;
-  const unsigned buf = smem_u32(dyn) + warp * (kFwdStages * stage) + lane * 4;
+  Inputs<T, VEC, TMA, 2> in;
+  in.tensor = warps * kSlab, in.full = full, in.status = p.status;
+  in.base = smem_u32(dyn) + warp * kSlab + lane * 4;
+  const unsigned slab = in.base + kStages * 2 * in.tensor;  // this lane's words of the outputs
 
   auto start_of = [&](int w) { return ((int64_t)(w * cluster + rank) * warps + warp) * kRun; };
   auto fetch = [&](int w) {
-    if (w < waves) {
-      const int64_t t0 = start_of(w);
-      const unsigned d = buf + (unsigned)(w % kFwdStages) * stage;
-      const char *zq = zp + t0 * zs, *xq = xp + t0 * xs;
-      if (t0 + kRun <= T_) {
+    if constexpr (TMA) {
+      if (warp == 0 && lane == 0 && w < waves) {
+        uint64_t *bar = full + w % kStages;
+        const unsigned d = in.at(w);
+        const int t = (int)start_of(w);
+        mbar_expect(bar, 2 * in.tensor);
+        tma_load(d, &p.zm, bar, (int)col0, (int)row, t);
+        tma_load(d + in.tensor, &p.xm, bar, (int)col0, (int)row, t);
+      }
+    } else {
+      if (w < waves) {
+        const int64_t t0 = start_of(w), zs = p.zt * (int64_t)sizeof(T), xs = p.xt * (int64_t)sizeof(T);
+        const unsigned d = in.at(w);
+        const char *zq = p.z + (row * p.zb + col) * (int64_t)sizeof(T) + t0 * zs;
+        const char *xq = p.x + (row * p.xb + col) * (int64_t)sizeof(T) + t0 * xs;
+        if (t0 + kRun <= T_) {
 #pragma unroll
-        for (int k = 0; k < kRun; ++k, zq += zs, xq += xs) {
-          fetch_word<T, VEC>(d + k * kStep, zq, true);
-          fetch_word<T, VEC>(d + kTensor + k * kStep, xq, true);
-        }
-      } else {
+          for (int k = 0; k < kRun; ++k, zq += zs, xq += xs) {
+            fetch_word<T, VEC>(d + k * kStep, zq);
+            fetch_word<T, VEC>(d + in.tensor + k * kStep, xq);
+          }
+        } else {
 #pragma unroll 1
-        for (int k = 0; k < kRun && t0 + k < T_; ++k, zq += zs, xq += xs) {
-          fetch_word<T, VEC>(d + k * kStep, zq, true);
-          fetch_word<T, VEC>(d + kTensor + k * kStep, xq, true);
+          for (int k = 0; k < kRun && t0 + k < T_; ++k, zq += zs, xq += xs) {
+            fetch_word<T, VEC>(d + k * kStep, zq);
+            fetch_word<T, VEC>(d + in.tensor + k * kStep, xq);
+          }
         }
       }
+      cp_commit();
     }
-    cp_commit();
   };
   auto fetch_starts = [&](int w) -> unsigned {
     const int64_t t = start_of(w) + lane;
     return w < waves && lane < kRun && t < T_ ? p.starts[t * p.st + row * p.sb] : 0;
   };
-  auto length = [&](int w) { return (int)max((int64_t)0, min((int64_t)kRun, T_ - start_of(w))); };
-  auto staged = [&](int w) { return buf + (unsigned)(w % kFwdStages) * stage; };
 
-  exchange_init(maps, warps, warp, lane, cluster);
+  exchange_init(maps, dyn + (kStages * 2 + (TMA ? 1 : 0)) * in.tensor, warps, warp, lane, cluster);
+  if (TMA) barriers_init(full, warp, lane);
+  fetch(0);
+  fetch(1);
+  unsigned next = STARTS ? fetch_starts(0) : 0;
   float s0[VEC];
   load_state<VEC>(p.h0, row * p.state_b + col, s0);
   C state = C::of(s0);
-  unsigned next = 0;
-  fetch(0);
-  fetch(1);
-  if (STARTS) next = fetch_starts(0);
 
-  FwdRun<T, VEC, GATED, STARTS> run[2];
-  auto summarise = [&](FwdRun<T, VEC, GATED, STARTS> &r, int w) {
-    r.mask = 0;
+  for (int w = 0; w < waves; ++w) {
+    const int64_t t0 = start_of(w);
+    const int len = (int)max((int64_t)0, min((int64_t)kRun, T_ - t0));
+    unsigned mask = 0;
     if (STARTS) {
-      r.mask = __ballot_sync(0xffffffffu, next != 0);
+      mask = __ballot_sync(0xffffffffu, next != 0);
       next = fetch_starts(w + 1);
     }
-    r.summarise(staged(w), length(w));
-  };
-  auto put = [&](const FwdRun<T, VEC, GATED, STARTS> &r, int w) {
-    publish<VEC, GATED, STARTS>(maps, w, warps, warp, lane, cluster, rank, r.A, r.B, r.mask != 0);
-  };
-  // wave w is published, wave w+1 staged; ends with w+1 published
-  auto wave = [&](FwdRun<T, VEC, GATED, STARTS> &cur, FwdRun<T, VEC, GATED, STARTS> &nxt, int w) {
-    fetch(w + 2);
-    cp_wait<1>();
-    if (w + 1 < waves) summarise(nxt, w + 1);
-    const C in = resolve<VEC, STARTS>(maps, w, warp, lane, cluster, rank, state, p.status);
-    const int64_t t0 = start_of(w);
-    const int len = length(w);
-    if (live && len > 0) {
-      if (p.ckpt) {
+    in.wait(w);
+    const unsigned d = in.at(w);
+    C f[kRun], b[kRun];
+    C A = C::all(1.f), B = C::all(0.f);
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+      float zv[VEC], xv[VEC];
+      read_word<T, VEC>(d + k * kStep, zv);
+      read_word<T, VEC>(d + in.tensor + k * kStep, xv);
+      if (GATED) {
+        C om;
+        gate<VEC>(zv, f[k], om);
+        b[k] = om * C::of(xv);
+      } else {
+        f[k] = C::of(zv);
+        b[k] = C::of(xv);
+      }
+    }
+    if (len < kRun) {
+#pragma unroll
+      for (int k = 0; k < kRun; ++k)
+        if (k >= len) f[k] = C::all(1.f), b[k] = C::all(0.f);
+    }
+    if (STARTS && mask) {
+#pragma unroll
+      for (int k = 0; k < kRun; ++k) {
+        const bool cut = (mask >> k) & 1;
+        A = cut ? C::all(0.f) : A * f[k];
+        B = cut ? b[k] : fma(f[k], B, b[k]);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kRun; ++k) {
+        A = A * f[k];
+        B = fma(f[k], B, b[k]);
+      }
+    }
+    if (w == 0) exchange_ready(cluster);
+    // (every warp has read its inputs once all have published)
+    publish<VEC, GATED, STARTS>(maps, w, warps, warp, lane, cluster, rank, A, B, mask != 0);
+    fetch(w + kStages);
+    C h = resolve<VEC, STARTS>(maps, w, warp, lane, cluster, rank, state, p.status);
+    if (len > 0) {
+      if (p.ckpt && live) {
         float *c = p.ckpt + (t0 / kRun) * p.ckpt_t + row * p.state_b + col;
         float v[VEC];
-        in.get(v);
+        h.get(v);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) c[i] = v[i];
       }
-      cur.write(staged(w), len, in, hp + t0 * hs, hs);
+      if constexpr (TMA) {
+        if (lane == 0) bulk_wait_read();  // the previous wave's copy has left the slab
+        __syncwarp();
+      }
+      const int64_t hs = p.ht * (int64_t)sizeof(T);
+      char *hq = p.h + (row * p.hb + col) * (int64_t)sizeof(T) + t0 * hs;
+      auto put = [&](int k, bool cut) {
+        h = cut ? b[k] : fma(f[k], h, b[k]);
+        float v[VEC];
+        h.get(v);
+        if constexpr (TMA) {
+          stage_word<T>(slab + k * kStep, v);
+        } else {
+          if (live && k < len) write_word<T, VEC>(hq, v);
+          hq += hs;
+        }
+      };
+      if (STARTS && mask) {
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) put(k, (mask >> k) & 1);
+      } else {
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) put(k, false);
+      }
+      if constexpr (TMA) {
+        fence_async();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store(&p.hm, slab, (int)col0, (int)row, (int)t0);
+          bulk_commit();
+        }
+      }
     }
-    if (w + 1 < waves) put(nxt, w + 1);
-  };
-  cp_wait<1>();
-  summarise(run[0], 0);
-  exchange_ready(cluster);
-  put(run[0], 0);
-  for (int w = 0; w < waves; w += 2) {
-    wave(run[0], run[1], w);
-    if (w + 1 < waves) wave(run[1], run[0], w + 1);
   }
   if (p.h_n && live && rank == 0 && warp == 0) {
     float v[VEC];
@@ -540,6 +576,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) rec_fwd_kernel(const FwdArg
 #pragma unroll
     for (int i = 0; i < VEC; ++i) p.h_n[row * p.state_b + col + i] = v[i];
   }
+  if (TMA && lane == 0) bulk_wait_read();
   if (cluster > 1) {  // no CTA leaves before the others are done with its memory
     cluster_arrive_relaxed();
     cluster_wait();
@@ -547,175 +584,206 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) rec_fwd_kernel(const FwdArg
 }
 
 // ------------------------------------------------------------------ backward
-// Shared memory: [3 tensors][16 steps][32 words] per warp and stage; a stage is
-// in use until its outputs are written (g is read twice), so the next one is
-// fetched beside it.
-template <typename T, int VEC, bool GATED, bool STARTS>
-__global__ void __launch_bounds__(32 * kMaxWarps, 2) rec_bwd_kernel(const BwdArgs p) {
-  extern __shared__ __align__(16) unsigned char dyn[];
+template <typename T, int VEC, bool GATED, bool STARTS, bool TMA>
+__global__ void __launch_bounds__(32 * kMaxWarps, kBwdCtas) rec_bwd_kernel(const __grid_constant__ BwdArgs p) {
+  extern __shared__ __align__(128) unsigned char dyn[];
   __shared__ Maps<VEC> maps;
+  __shared__ uint64_t full[kStages];
+  using C = Cols<VEC>;
   // float32 keeps both f and 1-f; the 16-bit types keep 1-f alone and take
   // f = 1 - (1-f), whose error (2^-25) only enters u, far below their rounding
   constexpr bool kBoth = GATED && sizeof(T) == 4;
   const int lane = threadIdx.x, warp = threadIdx.y, warps = blockDim.y;
-  const int cluster = p.s.cluster, rank = (int)(blockIdx.x % cluster);
+  const int cluster = p.s.cluster, rank = (int)(blockIdx.x % cluster), waves = p.s.waves;
   const int64_t gid = blockIdx.x / cluster;
   const int64_t row = gid / p.s.groups;
-  int64_t col = (gid % p.s.groups) * 32 * VEC + lane * VEC;
+  const int64_t col0 = (gid % p.s.groups) * 32 * VEC;
+  int64_t col = col0 + lane * VEC;
   const bool live = col < p.s.n;
   if (!live) col = p.s.n - VEC;
   const int64_t T_ = p.s.T;
-  const char *zp = p.z + (row * p.zb + col) * sizeof(T), *xp = p.x + (row * p.xb + col) * sizeof(T);
-  const char *gp = p.g + (row * p.gb + col) * sizeof(T);
-  char *dzp = p.dz + (row * p.dzb + col) * sizeof(T), *dxp = p.dx + (row * p.dxb + col) * sizeof(T);
-  const int64_t zs = p.zt * (int64_t)sizeof(T), xs = p.xt * (int64_t)sizeof(T), gs = p.gt * (int64_t)sizeof(T);
-  const int64_t dzs = p.dzt * (int64_t)sizeof(T), dxs = p.dxt * (int64_t)sizeof(T);
-  constexpr unsigned stage = 3 * kTensor;
-  const unsigned buf = smem_u32(dyn) + warp * (kBwdStages * stage) + lane * 4;
-
-  exchange_init(maps, warps, warp, lane, cluster);
-  float s0[VEC];
-  load_state<VEC>(p.dh_n, row * p.state_b + col, s0);
-  Cols<VEC> state = Cols<VEC>::of(s0);
+  const bool has_g = p.g != nullptr;
+  Inputs<T, VEC, TMA, 3> in;
+  in.tensor = warps * kSlab, in.full = full, in.status = p.status;
+  // warps go back in time, so the first warp's run is the last of a tile
+  in.base = smem_u32(dyn) + (warps - 1 - warp) * kSlab + lane * 4;
+  const unsigned slab = in.base + kStages * 3 * in.tensor;
 
   // chunks from the last to the first; below 0: past the beginning, nothing
   auto chunk_of = [&](int w) { return p.s.nchunk - 1 - ((w * cluster + rank) * warps + warp); };
   auto fetch = [&](int w) {
-    const int c = chunk_of(w);
-    const int64_t t0 = (int64_t)c * kRun;
-    const unsigned d = buf + (unsigned)(w % kBwdStages) * stage;
-    const char *zq = zp + t0 * zs, *xq = xp + t0 * xs, *gq = gp + t0 * gs;
-    if (c >= 0 && t0 + kRun <= T_ && p.g) {
+    if constexpr (TMA) {
+      if (warp == warps - 1 && lane == 0 && w < waves) {  // (the warp whose slab is the tile's first)
+        uint64_t *bar = full + w % kStages;
+        const unsigned d = in.at(w);
+        const int t = chunk_of(w) * kRun;  // negative in the last wave's tail: zeros
+        mbar_expect(bar, (has_g ? 3 : 2) * in.tensor);
+        tma_load(d, &p.zm, bar, (int)col0, (int)row, t);
+        tma_load(d + in.tensor, &p.xm, bar, (int)col0, (int)row, t);
+        if (has_g) tma_load(d + 2 * in.tensor, &p.gm, bar, (int)col0, (int)row, t);
+      }
+    } else {
+      const int c = w < waves ? chunk_of(w) : -1;
+      if (c >= 0) {
+        const int64_t t0 = (int64_t)c * kRun;
+        const int64_t zs = p.zt * (int64_t)sizeof(T), xs = p.xt * (int64_t)sizeof(T), gs = p.gt * (int64_t)sizeof(T);
+        const unsigned d = in.at(w);
+        const char *zq = p.z + (row * p.zb + col) * (int64_t)sizeof(T) + t0 * zs;
+        const char *xq = p.x + (row * p.xb + col) * (int64_t)sizeof(T) + t0 * xs;
+        const char *gq = p.g + (row * p.gb + col) * (int64_t)sizeof(T) + t0 * gs;
+        if (t0 + kRun <= T_ && has_g) {
 #pragma unroll
-      for (int k = 0; k < kRun; ++k, zq += zs, xq += xs, gq += gs) {
-        fetch_word<T, VEC>(d + k * kStep, zq, true);
-        fetch_word<T, VEC>(d + kTensor + k * kStep, xq, true);
-        fetch_word<T, VEC>(d + 2 * kTensor + k * kStep, gq, true);
-      }
-    } else if (c >= 0) {
+          for (int k = 0; k < kRun; ++k, zq += zs, xq += xs, gq += gs) {
+            fetch_word<T, VEC>(d + k * kStep, zq);
+            fetch_word<T, VEC>(d + in.tensor + k * kStep, xq);
+            fetch_word<T, VEC>(d + 2 * in.tensor + k * kStep, gq);
+          }
+        } else {
 #pragma unroll 1
-      for (int k = 0; k < kRun; ++k, zq += zs, xq += xs, gq += gs) {
-        const bool ok = t0 + k < T_, okg = ok && p.g;
-        fetch_word<T, VEC>(d + k * kStep, ok ? zq : zp, ok);
-        fetch_word<T, VEC>(d + kTensor + k * kStep, ok ? xq : xp, ok);
-        fetch_word<T, VEC>(d + 2 * kTensor + k * kStep, okg ? gq : zp, okg);
+          for (int k = 0; k < kRun && t0 + k < T_; ++k, zq += zs, xq += xs, gq += gs) {
+            fetch_word<T, VEC>(d + k * kStep, zq);
+            fetch_word<T, VEC>(d + in.tensor + k * kStep, xq);
+            if (has_g) fetch_word<T, VEC>(d + 2 * in.tensor + k * kStep, gq);
+          }
+        }
       }
+      cp_commit();
     }
-    cp_commit();
   };
   auto fetch_starts = [&](int w) -> unsigned {
     const int64_t t = (int64_t)chunk_of(w) * kRun + lane;
-    return lane < kRun && t >= 0 && t < T_ ? p.starts[t * p.st + row * p.sb] : 0;
+    return w < waves && lane < kRun && t >= 0 && t < T_ ? p.starts[t * p.st + row * p.sb] : 0;
   };
   auto fetch_ckpt = [&](int w, float *h) {
-    const int c = chunk_of(w);
+    const int c = w < waves ? chunk_of(w) : -1;
     load_state<VEC>(c >= 0 ? p.ckpt : nullptr, c * p.ckpt_t + row * p.state_b + col, h);
   };
 
-  unsigned next_start = 0;
-  float next_h[VEC];
+  exchange_init(maps, dyn + (kStages * 3 + (TMA ? 2 : 0)) * in.tensor, warps, warp, lane, cluster);
+  if (TMA) barriers_init(full, warp, lane);
   fetch(0);
+  fetch(1);
+  float next_h[VEC], s0[VEC];
   fetch_ckpt(0, next_h);
-  if (STARTS) next_start = fetch_starts(0);
-  for (int w = 0; w < p.s.waves; ++w) {
-    if (w + 1 < p.s.waves) fetch(w + 1); else cp_commit();
+  unsigned next_start = STARTS ? fetch_starts(0) : 0;
+  load_state<VEC>(p.dh_n, row * p.state_b + col, s0);
+  C state = C::of(s0);
+  const C one = C::all(1.f), zero = C::all(0.f);
+
+  for (int w = 0; w < waves; ++w) {
     unsigned mask = 0;
     if (STARTS) {
       mask = __ballot_sync(0xffffffffu, next_start != 0);
-      if (w + 1 < p.s.waves) next_start = fetch_starts(w + 1);
+      next_start = fetch_starts(w + 1);
     }
-    float h[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) h[v] = next_h[v];
-    if (w + 1 < p.s.waves) fetch_ckpt(w + 1, next_h);
-    cp_wait<1>();
+    C s = C::of(next_h);
+    fetch_ckpt(w + 1, next_h);
+    in.wait(w);
     const int c = chunk_of(w);
     const int64_t t0 = (int64_t)c * kRun;
-    const unsigned d = buf + (unsigned)(w % kBwdStages) * stage;
+    const unsigned d = in.at(w);
     const int len = c < 0 ? 0 : (int)min((int64_t)kRun, T_ - t0);
-    using C = Cols<VEC>;
-    const C one = C::all(1.f), zero = C::all(0.f);
-    // keep: 1-f (gated) or f (linear); q: the factor of e in df (set where the
-    // warp has a run, c >= 0, and read only there)
-#pragma nv_diag_suppress 549
+    // keep: 1-f (gated) or f (linear); q: the factor of e in df; raw: g as stored
     C keep[kRun], both[kBoth ? kRun : 1], q[kRun];
+    unsigned raw[kRun];
     auto coef = [&](int k) { return kBoth ? both[kBoth ? k : 0] : GATED ? one - keep[k] : keep[k]; };
     auto grad = [&](int k) {
       float g[VEC];
-      read_word<T, VEC>(d + 2 * kTensor + k * kStep, g);
+      unpack_lane<T, VEC>(raw[k], g);
       return C::of(g);
     };
-    C A = one, B = zero;
-    if (c >= 0) {
-      C s = C::of(h);
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) {
+      float zv[VEC], xv[VEC];
+      read_word<T, VEC>(d + k * kStep, zv);
+      read_word<T, VEC>(d + in.tensor + k * kStep, xv);
+      raw[k] = read_raw(d + 2 * in.tensor + k * kStep);
+      const C x = C::of(xv);
+      if (STARTS && ((mask >> k) & 1)) s = zero;
+      if (GATED) {
+        C f, om;
+        gate<VEC>(zv, f, om);
+        q[k] = (s - x) * (f * om);
+        s = fma(f, s, om * x);
+        keep[k] = om;
+        if (kBoth) both[k] = f;
+      } else {
+        q[k] = s;
+        keep[k] = C::of(zv);
+        s = fma(keep[k], s, x);
+      }
+    }
+    if (len < kRun || !has_g) {
 #pragma unroll
       for (int k = 0; k < kRun; ++k) {
-        float zv[VEC], xv[VEC];
-        read_word<T, VEC>(d + k * kStep, zv);
-        read_word<T, VEC>(d + kTensor + k * kStep, xv);
-        const C x = C::of(xv);
-        if (STARTS && ((mask >> k) & 1)) s = zero;
-        if (GATED) {
-          C f, om;
-          gate<VEC>(zv, f, om);
-          q[k] = (s - x) * (f * om);
-          s = fma(f, s, om * x);
-          keep[k] = om;
-          if (kBoth) both[k] = f;
-        } else {
-          q[k] = s;
-          keep[k] = C::of(zv);
-          s = fma(keep[k], s, x);
+        if (k >= len) {
+          keep[k] = GATED ? zero : one;
+          if (kBoth) both[k] = one;
         }
+        if (k >= len || !has_g) raw[k] = 0;
       }
-      if (len < kRun) {
+    }
+    C A = one, B = zero;
+    if (STARTS && mask) {
 #pragma unroll
-        for (int k = 0; k < kRun; ++k)
-          if (k >= len) {
-            keep[k] = GATED ? zero : one;
-            if (kBoth) both[k] = one;
-          }
+      for (int k = kRun - 1; k >= 0; --k) {
+        const bool cut = (mask >> k) & 1;
+        B = cut ? zero : coef(k) * (grad(k) + B);
+        A = cut ? zero : A * coef(k);
       }
-      if (STARTS && mask) {
+    } else {
 #pragma unroll
-        for (int k = kRun - 1; k >= 0; --k) {
-          const bool cut = (mask >> k) & 1;
-          B = cut ? zero : coef(k) * (grad(k) + B);
-          A = cut ? zero : A * coef(k);
-        }
-      } else {
-#pragma unroll
-        for (int k = kRun - 1; k >= 0; --k) {
-          const C f = coef(k);
-          B = f * (grad(k) + B);
-          A = A * f;
-        }
+      for (int k = kRun - 1; k >= 0; --k) {
+        const C f = coef(k);
+        B = f * (grad(k) + B);
+        A = A * f;
       }
     }
     if (w == 0) exchange_ready(cluster);
     publish<VEC, GATED, STARTS>(maps, w, warps, warp, lane, cluster, rank, A, B, mask != 0);
-    C uu = resolve<VEC, STARTS>(maps, w, warp, lane, cluster, rank, state, p.status);
-    if (live && len > 0) {
-      char *dzq = dzp + (t0 + kRun - 1) * dzs, *dxq = dxp + (t0 + kRun - 1) * dxs;
-      auto put = [&](int k, bool cut, bool write) {
-        const C e = grad(k) + uu;
-        uu = cut ? zero : coef(k) * e;
-        if (write) {
-          float dz[VEC], dx[VEC];
-          (e * q[k]).get(dz);
-          (GATED ? e * keep[k] : e).get(dx);
-          write_word<T, VEC>(dzq, dz);
-          write_word<T, VEC>(dxq, dx);
+    fetch(w + kStages);
+    C u = resolve<VEC, STARTS>(maps, w, warp, lane, cluster, rank, state, p.status);
+    if (len > 0) {
+      if constexpr (TMA) {
+        if (lane == 0) bulk_wait_read();
+        __syncwarp();
+      }
+      const int64_t dzs = p.dzt * (int64_t)sizeof(T), dxs = p.dxt * (int64_t)sizeof(T);
+      char *dzq = p.dz + (row * p.dzb + col) * (int64_t)sizeof(T) + (t0 + kRun - 1) * dzs;
+      char *dxq = p.dx + (row * p.dxb + col) * (int64_t)sizeof(T) + (t0 + kRun - 1) * dxs;
+      auto put = [&](int k, bool cut) {
+        const C e = grad(k) + u;
+        u = cut ? zero : coef(k) * e;
+        float dz[VEC], dx[VEC];
+        (e * q[k]).get(dz);
+        (GATED ? e * keep[k] : e).get(dx);
+        if constexpr (TMA) {
+          stage_word<T>(slab + k * kStep, dz);
+          stage_word<T>(slab + in.tensor + k * kStep, dx);
+        } else {
+          if (live && k < len) {
+            write_word<T, VEC>(dzq, dz);
+            write_word<T, VEC>(dxq, dx);
+          }
+          dzq -= dzs;
+          dxq -= dxs;
         }
-        dzq -= dzs;
-        dxq -= dxs;
       };
-      if (len < kRun || (STARTS && mask)) {
+      if (STARTS && mask) {
 #pragma unroll
-        for (int k = kRun - 1; k >= 0; --k) put(k, STARTS && ((mask >> k) & 1), k < len);
+        for (int k = kRun - 1; k >= 0; --k) put(k, (mask >> k) & 1);
       } else {
 #pragma unroll
-        for (int k = kRun - 1; k >= 0; --k) put(k, false, true);
+        for (int k = kRun - 1; k >= 0; --k) put(k, false);
+      }
+      if constexpr (TMA) {
+        fence_async();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store(&p.dzm, slab, (int)col0, (int)row, (int)t0);
+          tma_store(&p.dxm, slab + in.tensor, (int)col0, (int)row, (int)t0);
+          bulk_commit();
+        }
       }
     }
   }
@@ -725,6 +793,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) rec_bwd_kernel(const BwdArg
 #pragma unroll
     for (int v = 0; v < VEC; ++v) p.dh0[row * p.state_b + col + v] = last[v];
   }
+  if (TMA && lane == 0) bulk_wait_read();
   if (cluster > 1) {  // no CTA leaves before the others are done with its memory
     cluster_arrive_relaxed();
     cluster_wait();
@@ -733,37 +802,108 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 2) rec_bwd_kernel(const BwdArg
 
 // ------------------------------------------------------------------ launch
 struct Plan {
-  int warps, cluster;
+  int vec, warps, cluster, waves;
+  bool flat, tma;
+  int64_t groups;  // of all rows
   size_t smem;
 };
 
-// Warps and CTAs along time: up to 8 warps as the sequence has runs for, then
+// Warps and CTAs along time: up to 4 warps as the sequence has runs for, then
 // the cluster size of the least time in units of one wave: the rounds in
-// which the CTAs pass through the SMs (two at a time each) times the waves of a
-// round, with 1.5 for its start and end.
-Plan make_plan(int64_t groups, int nchunk, int tensors, int stages) {
-  Plan pl;
+// which the CTAs pass through the SMs times the waves of a round, with 1.5 for
+// its start and end.
+void split_time(Plan &pl, int nchunk, int inputs, int outputs, int per_sm) {
   pl.warps = 1;
   while (pl.warps < kMaxWarps && pl.warps < nchunk) pl.warps *= 2;
-  const int64_t slots = 2 * 148;
+  const int64_t slots = per_sm * 148;
   const int most = std::min(kMaxCluster, (nchunk + pl.warps - 1) / pl.warps);
   double best = 0;
   for (int c = 1; c <= most; ++c) {
-    const int64_t rounds = (groups * c + slots - 1) / slots;
+    const int64_t rounds = (pl.groups * c + slots - 1) / slots;
     const int waves = (nchunk + pl.warps * c - 1) / (pl.warps * c);
     const double time = (double)rounds * (waves + 1.5);
     if (c == 1 || time < best) best = time, pl.cluster = c;
   }
-  pl.smem = (size_t)stages * tensors * kRun * pl.warps * 128;
+  pl.waves = (nchunk + pl.warps * pl.cluster - 1) / (pl.warps * pl.cluster);
+  pl.smem = (size_t)(kStages * inputs + (pl.tma ? outputs : 0)) * pl.warps * kSlab;
+  if (pl.cluster > 1) pl.smem += (size_t)2 * pl.cluster * 32 * 8 * pl.vec;
+}
+
+struct Tensor3 {  // [T][rows][n] with contiguous n; null: not there
+  const void *p;
+  int64_t t, b;
+};
+
+// One row of B * H columns when every tensor stores its batch rows back to
+// back and no start mask tells them apart; else B rows of H.  16-bit tensors
+// move two columns per lane where every row is 4-byte aligned, and all move by
+// TMA where bases and strides are multiples of 16 bytes and there is more than
+// one run (a single run, the serving step, is faster without the copies' set-up).
+Plan make_plan(int dtype, const void *starts, int64_t T, int64_t B, int64_t H, const Tensor3 *ts, int n, int nchunk,
+               int inputs, int outputs, int per_sm) {
+  Plan pl = {};
+  const int64_t es = (int64_t)dtype_bytes(dtype);
+  pl.flat = starts == nullptr;
+  for (int i = 0; i < n; ++i)
+    if (ts[i].p && ts[i].b != H && B > 1) pl.flat = false;
+  const int64_t rows = pl.flat ? 1 : B, cols = pl.flat ? B * H : H;
+  auto fits = [&](int64_t bytes) {
+    for (int i = 0; i < n; ++i) {
+      if (!ts[i].p) continue;
+      if (!aligned(ts[i].p, bytes) || ts[i].t * es % bytes || (rows > 1 && ts[i].b * es % bytes)) return false;
+    }
+    return true;
+  };
+  pl.vec = dtype != HS_F32 && cols % 2 == 0 && fits(4) ? 2 : 1;
+  pl.tma = nchunk > 1 && pl.vec == 4 / es && fits(16) && cols <= 0x7fffffff && B <= 0x7fffffff;
+  for (int i = 0; i < n; ++i)  // strides a tensor map can hold
+    if (ts[i].p && (ts[i].t <= 0 || ts[i].t * es >= (int64_t)1 << 40 || (rows > 1 && (ts[i].b <= 0 || ts[i].b * es >= (int64_t)1 << 40)))) pl.tma = false;
+  const int per = 32 * pl.vec;
+  pl.groups = (cols + per - 1) / per * rows;
+  split_time(pl, nchunk, inputs, outputs, per_sm);
   return pl;
 }
 
+RecShape shape_of(const Plan &pl, int64_t T, int64_t B, int64_t H, int nchunk) {
+  RecShape s;
+  s.T = T, s.n = pl.flat ? B * H : H;
+  s.groups = pl.flat ? pl.groups : pl.groups / B;
+  s.nchunk = nchunk, s.waves = pl.waves, s.cluster = pl.cluster;
+  return s;
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void *p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }();
+  return fn;
+}
+
+// The tensor as a map of boxes of `steps` x 1 row x one word row.
+bool encode(CUtensorMap *m, const Tensor3 &t, int dtype, const Plan &pl, int64_t T, int64_t B, int64_t H, int steps) {
+  if (!t.p) return true;
+  const cuuint64_t es = dtype_bytes(dtype);
+  const cuuint64_t dims[3] = {(cuuint64_t)(pl.flat ? B * H : H), (cuuint64_t)(pl.flat ? 1 : B), (cuuint64_t)T};
+  const cuuint64_t strides[2] = {dims[1] > 1 ? (cuuint64_t)t.b * es : (cuuint64_t)t.t * es, (cuuint64_t)t.t * es};
+  const cuuint32_t box[3] = {(cuuint32_t)(32 * pl.vec), 1, (cuuint32_t)steps}, elem[3] = {1, 1, 1};
+  const CUtensorMapDataType type = dtype == HS_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == HS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                      : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return encoder() && encoder()(m, type, 3, const_cast<void *>(t.p), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename Args, typename K>
-int launch(K kernel, const Args &args, const Plan &pl, int64_t groups, cudaStream_t st, const char *what,
+int launch(K kernel, const Args &args, const Plan &pl, cudaStream_t st, const char *what,
            std::atomic<unsigned long long> *done) {
-  if (int e = allow_dynamic_smem((const void *)kernel, (size_t)6 * kRun * kMaxWarps * 128, done)) return e;
+  if (int e = allow_dynamic_smem((const void *)kernel, (size_t)(kStages * 3 + 2) * kMaxWarps * kSlab + 2 * kMaxCluster * 32 * 16, done)) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(groups * pl.cluster));
+  cfg.gridDim = dim3((unsigned)(pl.groups * pl.cluster));
   cfg.blockDim = dim3(32, pl.warps);
   cfg.dynamicSmemBytes = pl.smem;
   cfg.stream = st;
@@ -774,34 +914,37 @@ int launch(K kernel, const Args &args, const Plan &pl, int64_t groups, cudaStrea
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kernel, args) != cudaSuccess) return check_launch(what);
+  (void)cudaLaunchKernelEx(&cfg, kernel, args);
   return check_launch(what);
 }
 
-template <typename T, int VEC, bool GATED, bool STARTS> int launch_fwd(const FwdArgs &a, const Plan &pl, int64_t groups, cudaStream_t st) {
-  static std::atomic<unsigned long long> done{0};
-  return launch(rec_fwd_kernel<T, VEC, GATED, STARTS>, a, pl, groups, st, "rec_fwd_kernel", &done);
-}
-template <typename T, int VEC, bool GATED, bool STARTS> int launch_bwd(const BwdArgs &a, const Plan &pl, int64_t groups, cudaStream_t st) {
-  static std::atomic<unsigned long long> done{0};
-  return launch(rec_bwd_kernel<T, VEC, GATED, STARTS>, a, pl, groups, st, "rec_bwd_kernel", &done);
-}
+template <typename T, int VEC, bool GATED, bool STARTS, bool TMA> struct Kernel {
+  static int run(const FwdArgs &a, const Plan &pl, cudaStream_t st) {
+    static std::atomic<unsigned long long> done{0};
+    return launch(rec_fwd_kernel<T, VEC, GATED, STARTS, TMA>, a, pl, st, "rec_fwd_kernel", &done);
+  }
+  static int run(const BwdArgs &a, const Plan &pl, cudaStream_t st) {
+    static std::atomic<unsigned long long> done{0};
+    return launch(rec_bwd_kernel<T, VEC, GATED, STARTS, TMA>, a, pl, st, "rec_bwd_kernel", &done);
+  }
+};
 
-#define HS_REC_DISPATCH(FN, args)                                                                       \
-  [&]() -> int {                                                                                        \
-    const bool gated = form == HS_RECURRENCE_GATED, cuts = starts != nullptr;                           \
-    auto go = [&](auto tag, auto vec) -> int {                                                          \
-      using E = decltype(tag);                                                                          \
-      constexpr int V = decltype(vec)::value;                                                           \
-      if (gated) return cuts ? FN<E, V, true, true>(args, pl, groups, st) : FN<E, V, true, false>(args, pl, groups, st); \
-      return cuts ? FN<E, V, false, true>(args, pl, groups, st) : FN<E, V, false, false>(args, pl, groups, st);          \
-    };                                                                                                  \
-    if (dtype == HS_F32) return go(float{}, std::integral_constant<int, 1>{});                          \
-    if (dtype == HS_BF16)                                                                               \
-      return vec == 2 ? go(__nv_bfloat16{}, std::integral_constant<int, 2>{})                           \
-                      : go(__nv_bfloat16{}, std::integral_constant<int, 1>{});                          \
-    return vec == 2 ? go(__half{}, std::integral_constant<int, 2>{}) : go(__half{}, std::integral_constant<int, 1>{});   \
-  }()
+template <typename T, int VEC, bool TMA, typename Args>
+int by_form(int form, const Args &a, const Plan &pl, cudaStream_t st) {
+  const bool gated = form == HS_RECURRENCE_GATED, cuts = a.starts != nullptr;
+  if (gated) return cuts ? Kernel<T, VEC, true, true, TMA>::run(a, pl, st) : Kernel<T, VEC, true, false, TMA>::run(a, pl, st);
+  return cuts ? Kernel<T, VEC, false, true, TMA>::run(a, pl, st) : Kernel<T, VEC, false, false, TMA>::run(a, pl, st);
+}
+template <typename Args> int dispatch(int dtype, int form, const Args &a, const Plan &pl, cudaStream_t st) {
+  if (dtype == HS_F32) return pl.tma ? by_form<float, 1, true>(form, a, pl, st) : by_form<float, 1, false>(form, a, pl, st);
+  if (dtype == HS_BF16)
+    return pl.tma        ? by_form<__nv_bfloat16, 2, true>(form, a, pl, st)
+           : pl.vec == 2 ? by_form<__nv_bfloat16, 2, false>(form, a, pl, st)
+                         : by_form<__nv_bfloat16, 1, false>(form, a, pl, st);
+  return pl.tma        ? by_form<__half, 2, true>(form, a, pl, st)
+         : pl.vec == 2 ? by_form<__half, 2, false>(form, a, pl, st)
+                       : by_form<__half, 1, false>(form, a, pl, st);
+}
 
 int check_common(const char *who, int dtype, int form, int64_t T, int64_t B, int64_t H) {
   if (!dtype_ok(dtype)) return fail(HS_ERR_INVALID_ARG, "%s: unknown dtype %d", who, dtype);
@@ -812,26 +955,6 @@ int check_common(const char *who, int dtype, int form, int64_t T, int64_t B, int
   if (H > 0 && B > ((int64_t)1 << 31) / H)
     return fail(HS_ERR_UNSUPPORTED, "%s: B * H = %lld * %lld is above 2^31", who, (long long)B, (long long)H);
   return HS_OK;
-}
-
-// One row of B * H columns when every tensor stores its batch rows back to
-// back and no start mask tells them apart; else B rows of H.
-bool one_row(const void *starts, int64_t H, std::initializer_list<int64_t> batch_strides) {
-  if (starts) return false;
-  for (int64_t s : batch_strides)
-    if (s != H) return false;
-  return true;
-}
-
-// 16-bit tensors move two columns per lane where every row is 4-byte aligned.
-int vec_of(int dtype, int64_t n, std::initializer_list<const void *> ptrs, std::initializer_list<int64_t> strides) {
-  if (dtype == HS_F32) return 1;
-  if (n % 2) return 1;
-  for (const void *p : ptrs)
-    if (p && !aligned(p, 4)) return 1;
-  for (int64_t s : strides)
-    if (s % 2) return 1;
-  return 2;
 }
 
 }  // namespace
@@ -862,24 +985,21 @@ int hs_recurrence_forward(int dtype, int form, const void *z, int64_t z_t, int64
   const size_t es = dtype_bytes(dtype);
   if (!aligned(z, es) || !aligned(x, es) || !aligned(h, es) || !aligned(h0, 4) || !aligned(h_n, 4) || !aligned(checkpoints, 4))
     return fail(HS_ERR_INVALID_ARG, "hs_recurrence_forward: misaligned tensor");
-  const bool flat = one_row(starts, H, {z_b, x_b, h_b});
+  const int nchunk = (int)((T + kRun - 1) / kRun);
+  const Tensor3 ts[3] = {{z, z_t, z_b}, {x, x_t, x_b}, {h, h_t, h_b}};
+  const Plan pl = make_plan(dtype, starts, T, B, H, ts, 3, nchunk, 2, 1, kFwdCtas);
+  if (pl.groups * pl.cluster > 0x7fffffff) return fail(HS_ERR_UNSUPPORTED, "hs_recurrence_forward: too many columns");
   FwdArgs a = {};
-  a.s.T = T;
-  a.s.n = flat ? B * H : H;
-  const int vec = vec_of(dtype, a.s.n, {z, x, h}, {z_t, x_t, h_t, flat ? 0 : z_b, flat ? 0 : x_b, flat ? 0 : h_b});
-  const int per = 32 * (dtype == HS_F32 ? 1 : vec);
-  a.s.groups = (a.s.n + per - 1) / per;
-  const int64_t groups = a.s.groups * (flat ? 1 : B);
-  a.s.nchunk = (int)((T + kRun - 1) / kRun);
-  const Plan pl = make_plan(groups, a.s.nchunk, 2, kFwdStages);
-  if (groups * pl.cluster > 0x7fffffff) return fail(HS_ERR_UNSUPPORTED, "hs_recurrence_forward: too many columns");
-  a.s.cluster = pl.cluster;
-  a.s.waves = (a.s.nchunk + pl.warps * pl.cluster - 1) / (pl.warps * pl.cluster);
+  a.s = shape_of(pl, T, B, H, nchunk);
   a.z = (const char *)z, a.x = (const char *)x, a.h = (char *)h;
   a.h0 = h0, a.h_n = h_n, a.ckpt = checkpoints, a.starts = starts;
   a.zt = z_t, a.zb = z_b, a.xt = x_t, a.xb = x_b, a.ht = h_t, a.hb = h_b, a.st = starts_t, a.sb = starts_b;
   a.state_b = H, a.ckpt_t = B * H, a.status = dev_status;
-  return HS_REC_DISPATCH(launch_fwd, a);
+  const int tile = pl.warps * kRun;
+  if (pl.tma && !(encode(&a.zm, ts[0], dtype, pl, T, B, H, tile) && encode(&a.xm, ts[1], dtype, pl, T, B, H, tile) &&
+                  encode(&a.hm, ts[2], dtype, pl, T, B, H, kRun)))
+    return fail(HS_ERR_CUDA, "hs_recurrence_forward: cannot describe a tensor to TMA");
+  return dispatch(dtype, form, a, pl, st);
 }
 
 int hs_recurrence_backward(int dtype, int form, const void *z, int64_t z_t, int64_t z_b, const void *x, int64_t x_t,
@@ -903,27 +1023,23 @@ int hs_recurrence_backward(int dtype, int form, const void *z, int64_t z_t, int6
   if (!aligned(z, es) || !aligned(x, es) || !aligned(dh, es) || !aligned(dz, es) || !aligned(dx, es) ||
       !aligned(checkpoints, 4) || !aligned(dh_n, 4) || !aligned(dh0, 4))
     return fail(HS_ERR_INVALID_ARG, "hs_recurrence_backward: misaligned tensor");
-  if (!dh) dh_t = dz_t, dh_b = dz_b;
-  const bool flat = one_row(starts, H, {z_b, x_b, dh_b, dz_b, dx_b});
+  const int nchunk = (int)((T + kRun - 1) / kRun);
+  const Tensor3 ts[5] = {{z, z_t, z_b}, {x, x_t, x_b}, {dh, dh_t, dh_b}, {dz, dz_t, dz_b}, {dx, dx_t, dx_b}};
+  const Plan pl = make_plan(dtype, starts, T, B, H, ts, 5, nchunk, 3, 2, kBwdCtas);
+  if (pl.groups * pl.cluster > 0x7fffffff) return fail(HS_ERR_UNSUPPORTED, "hs_recurrence_backward: too many columns");
   BwdArgs a = {};
-  a.s.T = T;
-  a.s.n = flat ? B * H : H;
-  const int vec = vec_of(dtype, a.s.n, {z, x, dh, dz, dx},
-                         {z_t, x_t, dh_t, dz_t, dx_t, flat ? 0 : z_b, flat ? 0 : x_b, flat ? 0 : dh_b, flat ? 0 : dz_b, flat ? 0 : dx_b});
-  const int per = 32 * (dtype == HS_F32 ? 1 : vec);
-  a.s.groups = (a.s.n + per - 1) / per;
-  const int64_t groups = a.s.groups * (flat ? 1 : B);
-  a.s.nchunk = (int)((T + kRun - 1) / kRun);
-  const Plan pl = make_plan(groups, a.s.nchunk, 3, kBwdStages);
-  if (groups * pl.cluster > 0x7fffffff) return fail(HS_ERR_UNSUPPORTED, "hs_recurrence_backward: too many columns");
-  a.s.cluster = pl.cluster;
-  a.s.waves = (a.s.nchunk + pl.warps * pl.cluster - 1) / (pl.warps * pl.cluster);
+  a.s = shape_of(pl, T, B, H, nchunk);
   a.z = (const char *)z, a.x = (const char *)x, a.g = (const char *)dh, a.dz = (char *)dz, a.dx = (char *)dx;
   a.ckpt = checkpoints, a.dh_n = dh_n, a.dh0 = dh0, a.starts = starts;
   a.zt = z_t, a.zb = z_b, a.xt = x_t, a.xb = x_b, a.gt = dh_t, a.gb = dh_b;
   a.dzt = dz_t, a.dzb = dz_b, a.dxt = dx_t, a.dxb = dx_b, a.st = starts_t, a.sb = starts_b;
   a.state_b = H, a.ckpt_t = B * H, a.status = dev_status;
-  return HS_REC_DISPATCH(launch_bwd, a);
+  const int tile = pl.warps * kRun;
+  if (pl.tma && !(encode(&a.zm, ts[0], dtype, pl, T, B, H, tile) && encode(&a.xm, ts[1], dtype, pl, T, B, H, tile) &&
+                  encode(&a.gm, ts[2], dtype, pl, T, B, H, tile) && encode(&a.dzm, ts[3], dtype, pl, T, B, H, kRun) &&
+                  encode(&a.dxm, ts[4], dtype, pl, T, B, H, kRun)))
+    return fail(HS_ERR_CUDA, "hs_recurrence_backward: cannot describe a tensor to TMA");
+  return dispatch(dtype, form, a, pl, st);
 }
 
 }  // extern "C"
