@@ -45,11 +45,11 @@ namespace hs {
 namespace {
 
 constexpr int kRun = 16;       // steps per warp and per saved state
-constexpr int kMaxWarps = 4;   // warps of a CTA along time
+constexpr int kFwdWarps = 16, kBwdWarps = 12;  // warps of an SM (128 and 168 registers a thread), of a CTA at most
 constexpr int kMaxCluster = 8; // CTAs of a cluster along time
 constexpr int kStages = 2;     // waves of inputs in shared memory
 constexpr unsigned kStep = 128, kSlab = kRun * kStep;  // bytes of a step's words, and of a warp's run of one tensor
-constexpr int kFwdCtas = 4, kBwdCtas = 3;  // CTAs per SM (registers, shared memory)
+
 
 struct RecShape {
   int64_t T, n;         // steps; columns of one row
@@ -281,18 +281,18 @@ template <int VEC, bool GATED> HS_DEV Cols<VEC> held(Cols<VEC> a) {
 // stores.  A CTA sends the map of wave w+2 only after all of wave w+1 have
 // arrived, and each of those was sent after its sender's last read of wave w.
 template <int VEC> struct Maps {
-  Map<VEC> warp[2][kMaxWarps][32];
-  uint64_t bar[2];
-  Map<VEC> *cta;  // [2][cluster][32], behind the tiles (where the cluster has more than one CTA)
+  uint64_t *bar;   // [2]
+  Map<VEC> *warp;  // [2][warps][32]
+  Map<VEC> *cta;   // [2][cluster][32], where the cluster has more than one CTA
 };
 
-// Sets up the maps; met by exchange_ready() before the first publish.
-template <int VEC> HS_DEV void exchange_init(Maps<VEC> &m, unsigned char *behind, int warps, int warp, int lane, int cluster) {
-  if (warp == 0 && lane == 0) m.cta = reinterpret_cast<Map<VEC> *>(behind);
-  Map<VEC> one;
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) one.a[v] = 1.f, one.b[v] = 0.f;
-  for (int j = warps + warp; j < kMaxWarps; j += warps) m.warp[0][j][lane] = m.warp[1][j][lane] = one;  // absent warps
+// Sets up the maps behind the tiles; met by exchange_ready() before the first publish.
+template <int VEC>
+HS_DEV Maps<VEC> exchange_init(uint64_t *bar, unsigned char *behind, int warps, int warp, int lane, int cluster) {
+  Maps<VEC> m;
+  m.bar = bar;
+  m.warp = reinterpret_cast<Map<VEC> *>(behind) + lane;
+  m.cta = m.warp + 2 * warps * 32;
   if (cluster > 1) {
     if (warp == 0 && lane == 0) {
       mbar_init(&m.bar[0]);
@@ -301,6 +301,7 @@ template <int VEC> HS_DEV void exchange_init(Maps<VEC> &m, unsigned char *behind
     }
     cluster_arrive();
   }
+  return m;
 }
 HS_DEV void exchange_ready(int cluster) {
   if (cluster > 1) cluster_wait();  // every CTA has started and set up its barriers
@@ -308,14 +309,15 @@ HS_DEV void exchange_ready(int cluster) {
 
 // Publishes this warp's map of wave w.
 template <int VEC, bool GATED, bool STARTS>
-HS_DEV void publish(Maps<VEC> &m, int w, int warps, int warp, int lane, int cluster, int rank, Cols<VEC> A, Cols<VEC> B,
+HS_DEV void publish(const Maps<VEC> &m, int w, int warps, int warp, int lane, int cluster, int rank, Cols<VEC> A, Cols<VEC> B,
                     bool cut) {
   const int p = w & 1;
   Map<VEC> mine;
   held<VEC, GATED>(A).get(mine.a);
   B.get(mine.b);
   if (STARTS && cut) mine.a[0] = __int_as_float(0x7f800000);
-  m.warp[p][warp][lane] = mine;
+  const Map<VEC> *all = m.warp + p * warps * 32;
+  m.warp[(p * warps + warp) * 32] = mine;
   __syncthreads();
   if (cluster == 1) return;
   if (warp == 0 && lane == 0) mbar_expect(&m.bar[p], cluster * 32 * (unsigned)sizeof(Map<VEC>));
@@ -323,9 +325,9 @@ HS_DEV void publish(Maps<VEC> &m, int w, int warps, int warp, int lane, int clus
     const Cols<VEC> none = Cols<VEC>::all(0.f);
     Cols<VEC> ta = Cols<VEC>::all(1.f), tb = none;
     bool any = false;
-#pragma unroll
-    for (int j = 0; j < kMaxWarps; ++j) {
-      const Map<VEC> e = m.warp[p][j][lane];
+#pragma unroll 4
+    for (int j = 0; j < warps; ++j) {
+      const Map<VEC> e = all[j * 32];
       if (STARTS && e.a[0] == __int_as_float(0x7f800000)) any = true;
       tb = apply<VEC, STARTS>(e, tb);
       ta = held<VEC, GATED>(Cols<VEC>::of(e.a) * ta);
@@ -335,7 +337,7 @@ HS_DEV void publish(Maps<VEC> &m, int w, int warps, int warp, int lane, int clus
     tb.get(t.b);
     if (STARTS && any) t.a[0] = __int_as_float(0x7f800000);
     for (int r = 0; r < cluster; ++r) {
-      const unsigned to = cluster_addr(&m.cta[(p * cluster + rank) * 32 + lane], r), bar = cluster_addr(&m.bar[p], r);
+      const unsigned to = cluster_addr(&m.cta[(p * cluster + rank) * 32], r), bar = cluster_addr(&m.bar[p], r);
       if constexpr (VEC == 2)
         asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to),
                      "f"(t.a[0]), "f"(t.a[1]), "f"(t.b[0]), "f"(t.b[1]), "r"(bar)
@@ -351,14 +353,15 @@ HS_DEV void publish(Maps<VEC> &m, int w, int warps, int warp, int lane, int clus
 // The state entering this warp's run of wave w; `state`, the same in every
 // thread of a column, moves from the wave's entry to its end.
 template <int VEC, bool STARTS>
-HS_DEV Cols<VEC> resolve(Maps<VEC> &m, int w, int warp, int lane, int cluster, int rank, Cols<VEC> &state, int *status) {
+HS_DEV Cols<VEC> resolve(const Maps<VEC> &m, int w, int warps, int warp, int lane, int cluster, int rank, Cols<VEC> &state, int *status) {
   const int p = w & 1;
+  const Map<VEC> *all = m.warp + p * warps * 32;
   Cols<VEC> in = state;
   if (cluster == 1) {
-#pragma unroll
-    for (int j = 0; j < kMaxWarps; ++j) {
+#pragma unroll 4
+    for (int j = 0; j < warps; ++j) {
       if (j == warp) in = state;
-      state = apply<VEC, STARTS>(m.warp[p][j][lane], state);
+      state = apply<VEC, STARTS>(all[j * 32], state);
     }
     return in;
   }
@@ -367,12 +370,11 @@ HS_DEV Cols<VEC> resolve(Maps<VEC> &m, int w, int warp, int lane, int cluster, i
   for (int r = 0; r < kMaxCluster; ++r) {
     if (r < cluster) {
       if (r == rank) in = state;
-      state = apply<VEC, STARTS>(m.cta[(p * cluster + r) * 32 + lane], state);
+      state = apply<VEC, STARTS>(m.cta[(p * cluster + r) * 32], state);
     }
   }
-#pragma unroll
-  for (int j = 0; j < kMaxWarps - 1; ++j)
-    if (j < warp) in = apply<VEC, STARTS>(m.warp[p][j][lane], in);
+#pragma unroll 4
+  for (int j = 0; j < warp; ++j) in = apply<VEC, STARTS>(all[j * 32], in);
   return in;
 }
 
@@ -411,10 +413,9 @@ HS_DEV void barriers_init(uint64_t *full, int warp, int lane) {
 
 // ------------------------------------------------------------------ forward
 template <typename T, int VEC, bool GATED, bool STARTS, bool TMA>
-__global__ void __launch_bounds__(32 * kMaxWarps, kFwdCtas) rec_fwd_kernel(const __grid_constant__ FwdArgs p) {
+__global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid_constant__ FwdArgs p) {
   extern __shared__ __align__(128) unsigned char dyn[];
-  __shared__ Maps<VEC> maps;
-  __shared__ uint64_t full[kStages];
+  __shared__ uint64_t full[kStages], swap[2];
   using C = Cols<VEC>;
   const int lane = threadIdx.x, warp = threadIdx.y, warps = blockDim.y;
   const int cluster = p.s.cluster, rank = (int)(blockIdx.x % cluster), waves = p.s.waves;
@@ -469,7 +470,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, kFwdCtas) rec_fwd_kernel(const
     return w < waves && lane < kRun && t < T_ ? p.starts[t * p.st + row * p.sb] : 0;
   };
 
-  exchange_init(maps, dyn + (kStages * 2 + (TMA ? 1 : 0)) * in.tensor, warps, warp, lane, cluster);
+  const Maps<VEC> maps = exchange_init<VEC>(swap, dyn + (kStages * 2 + (TMA ? 1 : 0)) * in.tensor, warps, warp, lane, cluster);
   if (TMA) barriers_init(full, warp, lane);
   fetch(0);
   fetch(1);
@@ -527,7 +528,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, kFwdCtas) rec_fwd_kernel(const
     // (every warp has read its inputs once all have published)
     publish<VEC, GATED, STARTS>(maps, w, warps, warp, lane, cluster, rank, A, B, mask != 0);
     fetch(w + kStages);
-    C h = resolve<VEC, STARTS>(maps, w, warp, lane, cluster, rank, state, p.status);
+    C h = resolve<VEC, STARTS>(maps, w, warps, warp, lane, cluster, rank, state, p.status);
     if (len > 0) {
       if (p.ckpt && live) {
         float *c = p.ckpt + (t0 / kRun) * p.ckpt_t + row * p.state_b + col;
@@ -585,10 +586,9 @@ __global__ void __launch_bounds__(32 * kMaxWarps, kFwdCtas) rec_fwd_kernel(const
 
 // ------------------------------------------------------------------ backward
 template <typename T, int VEC, bool GATED, bool STARTS, bool TMA>
-__global__ void __launch_bounds__(32 * kMaxWarps, kBwdCtas) rec_bwd_kernel(const __grid_constant__ BwdArgs p) {
+__global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid_constant__ BwdArgs p) {
   extern __shared__ __align__(128) unsigned char dyn[];
-  __shared__ Maps<VEC> maps;
-  __shared__ uint64_t full[kStages];
+  __shared__ uint64_t full[kStages], swap[2];
   using C = Cols<VEC>;
   // float32 keeps both f and 1-f; the 16-bit types keep 1-f alone and take
   // f = 1 - (1-f), whose error (2^-25) only enters u, far below their rounding
@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, kBwdCtas) rec_bwd_kernel(const
     load_state<VEC>(c >= 0 ? p.ckpt : nullptr, c * p.ckpt_t + row * p.state_b + col, h);
   };
 
-  exchange_init(maps, dyn + (kStages * 3 + (TMA ? 2 : 0)) * in.tensor, warps, warp, lane, cluster);
+  const Maps<VEC> maps = exchange_init<VEC>(swap, dyn + (kStages * 3 + (TMA ? 2 : 0)) * in.tensor, warps, warp, lane, cluster);
   if (TMA) barriers_init(full, warp, lane);
   fetch(0);
   fetch(1);
@@ -742,7 +742,7 @@ __global__ void __launch_bounds__(32 * kMaxWarps, kBwdCtas) rec_bwd_kernel(const
     if (w == 0) exchange_ready(cluster);
     publish<VEC, GATED, STARTS>(maps, w, warps, warp, lane, cluster, rank, A, B, mask != 0);
     fetch(w + kStages);
-    C u = resolve<VEC, STARTS>(maps, w, warp, lane, cluster, rank, state, p.status);
+    C u = resolve<VEC, STARTS>(maps, w, warps, warp, lane, cluster, rank, state, p.status);
     if (len > 0) {
       if constexpr (TMA) {
         if (lane == 0) bulk_wait_read();
@@ -808,25 +808,57 @@ struct Plan {
   size_t smem;
 };
 
-// Warps and CTAs along time: up to 4 warps as the sequence has runs for, then
-// the cluster size of the least time in units of one wave: the rounds in
-// which the CTAs pass through the SMs times the waves of a round, with 1.5 for
-// its start and end.
-void split_time(Plan &pl, int nchunk, int inputs, int outputs, int per_sm) {
-  pl.warps = 1;
-  while (pl.warps < kMaxWarps && pl.warps < nchunk) pl.warps *= 2;
-  const int64_t slots = per_sm * 148;
-  const int most = std::min(kMaxCluster, (nchunk + pl.warps - 1) / pl.warps);
-  double best = 0;
-  for (int c = 1; c <= most; ++c) {
-    const int64_t rounds = (pl.groups * c + slots - 1) / slots;
-    const int waves = (nchunk + pl.warps * c - 1) / (pl.warps * c);
-    const double time = (double)rounds * (waves + 1.5);
-    if (c == 1 || time < best) best = time, pl.cluster = c;
+// What a wave takes, in us: `fixed` + `warp` x the CTA's warps from its inputs
+// to its outputs (+ kHop through the cluster), and at least `move` x the
+// resident warps of an SM for their share of the memory bandwidth (10% more where
+// clusters go in step).  Fitted to runs of every split at T = 128..65536 and
+// 4..2048 column groups; its choice is within 10% of the fastest split of most.
+struct Pace {
+  bool backward;
+  int sm_warps;
+  double fixed, warp, move;
+};
+constexpr double kHop = 0.45;
+Pace pace_of(bool backward, int dtype) {
+  if (backward) return {true, kBwdWarps, 0.55, dtype == HS_F32 ? 0.11 : 0.165, 0.24};
+  return {false, kFwdWarps, 0.5, dtype == HS_F32 ? 0.075 : 0.12, 0.14};
+}
+
+// Dynamic shared memory of a CTA.
+size_t smem_of(bool backward, bool tma, int vec, int warps, int cluster) {
+  const int inputs = backward ? 3 : 2, outputs = !tma ? 0 : backward ? 2 : 1;
+  return (size_t)(kStages * inputs + outputs) * warps * kSlab + (size_t)2 * (warps + (cluster > 1 ? cluster : 0)) * 32 * 8 * vec;
+}
+
+// Clusters of c CTAs that run at once (a cluster stays within a GPC, so some
+// SMs are left over), asked once per device.
+int64_t clusters_at_once(const Pace &m, int warps, int c);
+
+// Warps and CTAs along time: the least time by that model.  A sequence of n
+// waves takes n + 1 of them, and what does not fit the SMs at once goes in
+// rounds.  Many columns run as CTAs of 8 or 4 warps, whose phases overlap on an
+// SM; few columns get more warps and CTAs along time.
+void split_time(Plan &pl, int nchunk, const Pace &m) {
+  double best = -1;
+  for (int warps = 1; warps <= m.sm_warps; warps = warps < 4 ? 2 * warps : warps + 4) {
+    if (warps > 1 && warps / 2 >= nchunk) break;
+    if (warps < 4 && warps < nchunk) continue;  // CTAs of under 4 warps: short sequences alone
+    const int most = std::min(kMaxCluster, (nchunk + warps - 1) / warps);
+    for (int c = 1; c <= most; ++c) {
+      const int64_t at_once = clusters_at_once(m, warps, c), full = pl.groups / at_once;
+      const int waves = (nchunk + warps * c - 1) / (warps * c);
+      auto wave = [&](int64_t groups) {
+        const double resident = warps * (double)(groups * c) / 148;
+        return std::max(m.fixed + m.warp * warps + (c > 1 ? kHop : 0.), m.move * (c > 1 ? 1.1 : 1.) * resident);
+      };
+      double time = (double)full * wave(at_once);
+      if (pl.groups % at_once) time += wave(pl.groups % at_once);
+      time *= waves + 1;
+      if (best < 0 || time < 0.999 * best) best = time, pl.warps = warps, pl.cluster = c;
+    }
   }
   pl.waves = (nchunk + pl.warps * pl.cluster - 1) / (pl.warps * pl.cluster);
-  pl.smem = (size_t)(kStages * inputs + (pl.tma ? outputs : 0)) * pl.warps * kSlab;
-  if (pl.cluster > 1) pl.smem += (size_t)2 * pl.cluster * 32 * 8 * pl.vec;
+  pl.smem = smem_of(m.backward, pl.tma, pl.vec, pl.warps, pl.cluster);
 }
 
 struct Tensor3 {  // [T][rows][n] with contiguous n; null: not there
@@ -840,7 +872,7 @@ struct Tensor3 {  // [T][rows][n] with contiguous n; null: not there
 // TMA where bases and strides are multiples of 16 bytes and there is more than
 // one run (a single run, the serving step, is faster without the copies' set-up).
 Plan make_plan(int dtype, const void *starts, int64_t T, int64_t B, int64_t H, const Tensor3 *ts, int n, int nchunk,
-               int inputs, int outputs, int per_sm) {
+               const Pace &pace) {
   Plan pl = {};
   const int64_t es = (int64_t)dtype_bytes(dtype);
   pl.flat = starts == nullptr;
@@ -860,7 +892,7 @@ Plan make_plan(int dtype, const void *starts, int64_t T, int64_t B, int64_t H, c
     if (ts[i].p && (ts[i].t <= 0 || ts[i].t * es >= (int64_t)1 << 40 || (rows > 1 && (ts[i].b <= 0 || ts[i].b * es >= (int64_t)1 << 40)))) pl.tma = false;
   const int per = 32 * pl.vec;
   pl.groups = (cols + per - 1) / per * rows;
-  split_time(pl, nchunk, inputs, outputs, per_sm);
+  split_time(pl, nchunk, pace);
   return pl;
 }
 
@@ -898,10 +930,14 @@ bool encode(CUtensorMap *m, const Tensor3 &t, int dtype, const Plan &pl, int64_t
                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+constexpr size_t kSmemMost = (size_t)(kStages * 3 + 2) * kBwdWarps * kSlab + 2 * (kBwdWarps + kMaxCluster) * 32 * 16;
+static_assert(kSmemMost <= 227 * 1024 && (kStages * 2 + 1) * kFwdWarps * kSlab + 2 * (kFwdWarps + kMaxCluster) * 32 * 16 <= kSmemMost,
+              "shared memory of a CTA");
+
 template <typename Args, typename K>
 int launch(K kernel, const Args &args, const Plan &pl, cudaStream_t st, const char *what,
            std::atomic<unsigned long long> *done) {
-  if (int e = allow_dynamic_smem((const void *)kernel, (size_t)(kStages * 3 + 2) * kMaxWarps * kSlab + 2 * kMaxCluster * 32 * 16, done)) return e;
+  if (int e = allow_dynamic_smem((const void *)kernel, kSmemMost, done)) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(pl.groups * pl.cluster));
   cfg.blockDim = dim3(32, pl.warps);
@@ -916,6 +952,37 @@ int launch(K kernel, const Args &args, const Plan &pl, cudaStream_t st, const ch
   cfg.numAttrs = 1;
   (void)cudaLaunchKernelEx(&cfg, kernel, args);
   return check_launch(what);
+}
+
+int64_t clusters_at_once(const Pace &m, int warps, int c) {
+  const int64_t ctas = (int64_t)(m.sm_warps / warps) * 148;
+  static std::atomic<int> known[64][2][kFwdWarps / 4][kMaxCluster];
+  int dev = 0;
+  if (c == 1 || warps < 4 || cudaGetDevice(&dev) != cudaSuccess) return ctas / c;
+  std::atomic<int> &k = known[dev & 63][m.backward][warps / 4 - 1][c - 1];
+  int n = k.load(std::memory_order_relaxed);
+  if (n) return n;
+  static std::atomic<unsigned long long> done[2];
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(ctas / c * c));
+  cfg.blockDim = dim3(32, warps);
+  cfg.dynamicSmemBytes = smem_of(m.backward, true, 2, warps, c);
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)c;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  auto ask = [&](auto kernel) {
+    return allow_dynamic_smem((const void *)kernel, kSmemMost, &done[m.backward]) == HS_OK &&
+           cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0;
+  };
+  if (!(m.backward ? ask(rec_bwd_kernel<__nv_bfloat16, 2, true, false, true>) : ask(rec_fwd_kernel<__nv_bfloat16, 2, true, false, true>))) {
+    (void)cudaGetLastError();
+    n = (int)(ctas / c);
+  }
+  k.store(n, std::memory_order_relaxed);
+  return n;
 }
 
 template <typename T, int VEC, bool GATED, bool STARTS, bool TMA> struct Kernel {
@@ -987,7 +1054,7 @@ int hs_recurrence_forward(int dtype, int form, const void *z, int64_t z_t, int64
     return fail(HS_ERR_INVALID_ARG, "hs_recurrence_forward: misaligned tensor");
   const int nchunk = (int)((T + kRun - 1) / kRun);
   const Tensor3 ts[3] = {{z, z_t, z_b}, {x, x_t, x_b}, {h, h_t, h_b}};
-  const Plan pl = make_plan(dtype, starts, T, B, H, ts, 3, nchunk, 2, 1, kFwdCtas);
+  const Plan pl = make_plan(dtype, starts, T, B, H, ts, 3, nchunk, pace_of(false, dtype));
   if (pl.groups * pl.cluster > 0x7fffffff) return fail(HS_ERR_UNSUPPORTED, "hs_recurrence_forward: too many columns");
   FwdArgs a = {};
   a.s = shape_of(pl, T, B, H, nchunk);
@@ -1025,7 +1092,7 @@ int hs_recurrence_backward(int dtype, int form, const void *z, int64_t z_t, int6
     return fail(HS_ERR_INVALID_ARG, "hs_recurrence_backward: misaligned tensor");
   const int nchunk = (int)((T + kRun - 1) / kRun);
   const Tensor3 ts[5] = {{z, z_t, z_b}, {x, x_t, x_b}, {dh, dh_t, dh_b}, {dz, dz_t, dz_b}, {dx, dx_t, dx_b}};
-  const Plan pl = make_plan(dtype, starts, T, B, H, ts, 5, nchunk, 3, 2, kBwdCtas);
+  const Plan pl = make_plan(dtype, starts, T, B, H, ts, 5, nchunk, pace_of(true, dtype));
   if (pl.groups * pl.cluster > 0x7fffffff) return fail(HS_ERR_UNSUPPORTED, "hs_recurrence_backward: too many columns");
   BwdArgs a = {};
   a.s = shape_of(pl, T, B, H, nchunk);
