@@ -402,6 +402,17 @@ template <typename T, int VEC, bool TMA, int N> struct Inputs {
   }
 };
 
+// The starts among the steps t .. t+15 as bits.  A warp reads those of its next
+// 32 waves at once, one wave per lane: read wave by wave, the load's latency
+// showed in every one of them (25% of the forward's time, 40% of the backward's).
+HS_DEV unsigned start_mask(const unsigned char *starts, int64_t stride, int64_t t, int64_t T) {
+  unsigned m = 0;
+#pragma unroll
+  for (int k = 0; k < kRun; ++k)
+    if (t + k < T && starts[(t + k) * stride]) m |= 1u << k;
+  return m;
+}
+
 HS_DEV void barriers_init(uint64_t *full, int warp, int lane) {
   if (warp == 0 && lane == 0) {
     for (int i = 0; i < kStages; ++i) mbar_init(full + i);
@@ -465,16 +476,13 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
       cp_commit();
     }
   };
-  auto fetch_starts = [&](int w) -> unsigned {
-    const int64_t t = start_of(w) + lane;
-    return w < waves && lane < kRun && t < T_ ? p.starts[t * p.st + row * p.sb] : 0;
-  };
+  auto starts_from = [&](int w) { return w + lane < waves ? start_mask(p.starts + row * p.sb, p.st, start_of(w + lane), T_) : 0u; };
 
   const Maps<VEC> maps = exchange_init<VEC>(swap, dyn + (kStages * 2 + (TMA ? 1 : 0)) * in.tensor, warps, warp, lane, cluster);
   if (TMA) barriers_init(full, warp, lane);
   fetch(0);
   fetch(1);
-  unsigned next = STARTS ? fetch_starts(0) : 0;
+  unsigned masks = 0;
   float s0[VEC];
   load_state<VEC>(p.h0, row * p.state_b + col, s0);
   C state = C::of(s0);
@@ -484,8 +492,8 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
     const int len = (int)max((int64_t)0, min((int64_t)kRun, T_ - t0));
     unsigned mask = 0;
     if (STARTS) {
-      mask = __ballot_sync(0xffffffffu, next != 0);
-      next = fetch_starts(w + 1);
+      if (w % 32 == 0) masks = starts_from(w);
+      mask = __shfl_sync(0xffffffffu, masks, w % 32);
     }
     in.wait(w);
     const unsigned d = in.at(w);
@@ -650,9 +658,9 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
       cp_commit();
     }
   };
-  auto fetch_starts = [&](int w) -> unsigned {
-    const int64_t t = (int64_t)chunk_of(w) * kRun + lane;
-    return w < waves && lane < kRun && t >= 0 && t < T_ ? p.starts[t * p.st + row * p.sb] : 0;
+  auto starts_from = [&](int w) {
+    const int c = chunk_of(w + lane);
+    return w + lane < waves && c >= 0 ? start_mask(p.starts + row * p.sb, p.st, (int64_t)c * kRun, T_) : 0u;
   };
   auto fetch_ckpt = [&](int w, float *h) {
     const int c = w < waves ? chunk_of(w) : -1;
@@ -665,7 +673,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
   fetch(1);
   float next_h[VEC], s0[VEC];
   fetch_ckpt(0, next_h);
-  unsigned next_start = STARTS ? fetch_starts(0) : 0;
+  unsigned masks = 0;
   load_state<VEC>(p.dh_n, row * p.state_b + col, s0);
   C state = C::of(s0);
   const C one = C::all(1.f), zero = C::all(0.f);
@@ -673,8 +681,8 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
   for (int w = 0; w < waves; ++w) {
     unsigned mask = 0;
     if (STARTS) {
-      mask = __ballot_sync(0xffffffffu, next_start != 0);
-      next_start = fetch_starts(w + 1);
+      if (w % 32 == 0) masks = starts_from(w);
+      mask = __shfl_sync(0xffffffffu, masks, w % 32);
     }
     C s = C::of(next_h);
     fetch_ckpt(w + 1, next_h);
