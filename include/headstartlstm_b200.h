@@ -530,8 +530,8 @@ HS_API int hs_embedding_backward(int dtype, const void *dout, int token_bits, co
                                  int64_t D, void *workspace, size_t workspace_bytes, int *dev_status,
                                  hs_stream_t stream);
 
-/* Log probabilities of given tokens under softmax(logits / temperature), with
- * the distribution's entropy and its `top` (0 to HS_MAX_TOP) most likely
+/* Log probabilities of given tokens under softmax(logits / temperature)
+ * (temperature from 1e-30 to 1e30), with the distribution's entropy and its `top` (0 to HS_MAX_TOP) most likely
  * tokens.  logits [N,V], rows logits_ld elements apart.  logprob and entropy
  * [N] in nats; top_logprob, top_index [N,top], ordered by logit, equal ones by
  * the lower index; stats [N,2] for the backward (any of these but logprob may

@@ -332,8 +332,8 @@ def token_logprobs(logits, tokens, top: int = 0, temperature: float = 1.0, ignor
     V = logits.shape[-1]
     if not 0 <= top <= min(_MAX_TOP, V):
         raise RuntimeError(f"{who}: top must be in 0..{min(_MAX_TOP, V)}; got {top}")
-    if not 0 < temperature < float("inf"):
-        raise RuntimeError(f"{who}: the temperature must be positive and finite; got {temperature}")
+    if not 1e-30 <= temperature <= 1e30:
+        raise RuntimeError(f"{who}: the temperature must be positive (1e-30 to 1e30); got {temperature}")
     shape = tokens.shape
     tokens = _tokens(who, tokens).view(-1)
     rows = logits if logits.dim() == 2 else logits.reshape(-1, V) if V else logits.reshape(tokens.numel(), 0)

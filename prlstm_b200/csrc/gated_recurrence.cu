@@ -152,49 +152,6 @@ HS_DEV void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memo
 HS_DEV void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 HS_DEV void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// The columns of one lane: one float32, or two as one pair of registers that
-// sm_100a's packed float32 instructions take at once.
-template <int VEC> struct Cols;
-template <> struct Cols<1> {
-  float v;
-  HS_DEV static Cols all(float a) { return {a}; }
-  HS_DEV static Cols of(const float *a) { return {a[0]}; }
-  HS_DEV void get(float *a) const { a[0] = v; }
-};
-template <> struct Cols<2> {
-  unsigned long long v;
-  HS_DEV static Cols of(const float *a) {
-    Cols r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a[0]), "f"(a[1]));
-    return r;
-  }
-  HS_DEV static Cols all(float a) {
-    const float t[2] = {a, a};
-    return of(t);
-  }
-  HS_DEV void get(float *a) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a[0]), "=f"(a[1]) : "l"(v)); }
-};
-HS_DEV Cols<1> operator+(Cols<1> a, Cols<1> b) { return {a.v + b.v}; }
-HS_DEV Cols<1> operator-(Cols<1> a, Cols<1> b) { return {a.v - b.v}; }
-HS_DEV Cols<1> operator*(Cols<1> a, Cols<1> b) { return {__fmul_rn(a.v, b.v)}; }
-HS_DEV Cols<1> fma(Cols<1> a, Cols<1> b, Cols<1> c) { return {fmaf(a.v, b.v, c.v)}; }
-HS_DEV Cols<2> fma(Cols<2> a, Cols<2> b, Cols<2> c) {
-  Cols<2> r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return r;
-}
-HS_DEV Cols<2> operator+(Cols<2> a, Cols<2> b) {
-  Cols<2> r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-HS_DEV Cols<2> operator*(Cols<2> a, Cols<2> b) {
-  Cols<2> r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
-HS_DEV Cols<2> operator-(Cols<2> a, Cols<2> b) { return fma(b, Cols<2>::all(-1.f), a); }
-
 // f = 1/(1+e^-z) and 1-f = e^-z/(1+e^-z), each to a few float32 ulps of its own
 // size.  e^-z is held to 2^126, so that both stay finite (f is 0 to float32's
 // smallest normal number there); a NaN stays one.  The reciprocal is refined by

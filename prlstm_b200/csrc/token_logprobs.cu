@@ -1,16 +1,17 @@
 // Log probabilities of given tokens with entropy and top alternatives, and
 // the gradient of the logits.
 //
-// With c = log2(e) / temperature, m = max x, t_v = (x_v - m) c (base-2 logits):
-//   S = sum 2^t_v, U = sum t_v 2^t_v
-//   log p_v = ln2 (t_v - log2 S),  entropy = ln2 (log2 S - U / S)
+// With c = log2(e) / temperature, m = max x, d_v = x_v - m:
+//   S = sum 2^(c d_v), U = sum d_v 2^(c d_v)
+//   log p_v = d_v / temperature - ln S,  entropy = ln S - U / (S temperature)
 //   dx_v = (1/temperature) (sum of the gradients that name v - p_v (G + ge (log p_v + entropy))),
 //   G the sum of all gradients of the row's log probabilities, ge the entropy's.
 //
 // Bound: memory, the logits read once (and, for the gradient, read once more
 // and written once).  The forward keeps a running maximum per thread and
 // rescales S and U where a batch of values exceeds it; each value costs one
-// hardware exp2 and a few FMAs, below the memory time for 16-bit logits too.
+// hardware exp2 and about four other instructions (sums two at a time), below
+// the memory time for 16-bit logits too.
 //
 // Top alternatives cost the pass nothing: the running maximum already says
 // where each thread's best value lies.  The k-th best of the threads' bests
@@ -31,7 +32,7 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr float kFloor = -150.f;  // 2^-150 is 0 in float32: smaller exponents change nothing
+constexpr float kFloor = -150.f;  // 2^-150 is 0 in float32: a smaller exponent changes nothing
 
 HS_DEV float max_nan(float a, float b) {  // the maximum, NaN if either is
   float r;
@@ -46,23 +47,28 @@ HS_DEV float ex2(float x) {
 constexpr float kNegInf = -__builtin_huge_valf();
 
 // Running (maximum, S, U) of a set of values; S and U are relative to m.
+// Differences are held to `floor` = -150 / c, where 2^(c d) is 0: a masked -inf
+// adds 0 to both sums, and a NaN stays one.
 struct Stat {
   float m, s, u;
 };
-HS_DEV float rel(float m) { return m == kNegInf ? 0.f : m; }  // nothing but -inf so far: 2^(-inf) terms, all 0
-// Moves (s, u) from reference `from` to the larger reference `to`.
-HS_DEV void rescale(Stat &a, float to, float c) {
+struct Scale {
+  float c, floor;
+};
+HS_DEV float rel(float m) { return m == kNegInf ? 0.f : m; }  // nothing but -inf so far: every term is 0
+// Moves (s, u) from its reference to the larger reference `to`.
+HS_DEV void rescale(Stat &a, float to, Scale k) {
   const bool none = a.m == kNegInf;
-  const float d = none ? 0.f : max_nan((a.m - to) * c, kFloor);
-  const float f = none ? 0.f : ex2(d);  // (a NaN s stays NaN)
+  const float d = none ? 0.f : max_nan(a.m - to, k.floor);
+  const float f = none ? 0.f : ex2(d * k.c);  // (a NaN s stays NaN)
   a.u = (a.u + d * a.s) * f;
   a.s *= f;
   a.m = to;
 }
-HS_DEV void merge(Stat &a, Stat b, float c) {
+HS_DEV void merge(Stat &a, Stat b, Scale k) {
   const float m = fmaxf(a.m, b.m);
-  if (a.m != m) rescale(a, m, c);
-  if (b.m != m) rescale(b, m, c);
+  if (a.m != m) rescale(a, m, k);
+  if (b.m != m) rescale(b, m, k);
   a.s += b.s;
   a.u += b.u;
 }
@@ -87,8 +93,9 @@ HS_DEV Key order_pair(Key k, int o, bool keep_max) {
   const Key other = __shfl_xor_sync(0xffffffffu, k, o);
   return ((k > other) == keep_max) ? k : other;
 }
-// The warp's 32 keys in descending order of lanes (bitonic network).
-HS_DEV Key sort_desc(Key k, int lane) {
+// The warp's 32 keys in descending order of lanes (bitonic network).  A
+// function of its own, as its code is long and used in several places.
+__device__ __noinline__ Key sort_desc(Key k, int lane) {
 #pragma unroll
   for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
@@ -96,7 +103,7 @@ HS_DEV Key sort_desc(Key k, int lane) {
   return k;
 }
 // The 32 largest of two descending lists, descending.
-HS_DEV Key merge_desc(Key a, Key b, int lane) {
+__device__ __noinline__ Key merge_desc(Key a, Key b, int lane) {
   const Key r = __shfl_sync(0xffffffffu, b, 31 - lane);
   Key k = a > r ? a : r;  // bitonic
 #pragma unroll
@@ -143,7 +150,8 @@ struct FwdArgs {
   const void *tok;
   int token64;
   int64_t ignore;
-  float c, inv_t;  // log2(e) / temperature, 1 / temperature
+  Scale k;      // c = log2(e) / temperature
+  float inv_t;  // 1 / temperature
   int top;
   float *lp, *ent, *top_lp;
   int64_t *top_id;
@@ -157,57 +165,84 @@ HS_DEV int64_t token_at(const void *tok, int token64, int64_t n) {
   return token64 ? static_cast<const int64_t *>(tok)[n] : (int64_t)static_cast<const int *>(tok)[n];
 }
 
-// What a thread knows of its values.
+// The largest of a 16-byte vector's values, NaN left out.
+template <typename T> HS_DEV float vec_max(const uint4 &q) {
+  if constexpr (sizeof(T) == 4) {
+    return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
+  } else {
+    float v[2];
+    unpack_word<T>(word_max<T>(word_max<T>(q.x, q.y), word_max<T>(q.z, q.w)), v);
+    return fmaxf(v[0], v[1]);
+  }
+}
+
+// What a thread knows of its values.  S and U are kept as two partial sums
+// each, for even and odd values.
 template <typename T> struct Scan {
-  Stat a{kNegInf, 0.f, 0.f};
+  float m = kNegInf;
+  Cols<2> s = Cols<2>::all(0.f), u = Cols<2>::all(0.f);
   int best = -1;  // where the maximum was first met: vector i as i, head scalar as -2, tail scalar as -3
-  HS_DEV void scalar(float v, float c, int where) {
+  HS_DEV Stat stat() const {
+    float a[2], b[2];
+    s.get(a);
+    u.get(b);
+    return {m, a[0] + a[1], b[0] + b[1]};
+  }
+  HS_DEV void raise(float to, Scale k) {
+    float a[2], b[2];
+    s.get(a);
+    u.get(b);
+    Stat x{m, a[0], b[0]}, y{m, a[1], b[1]};
+    rescale(x, to, k);
+    rescale(y, to, k);
+    a[0] = x.s, a[1] = y.s, b[0] = x.u, b[1] = y.u;
+    s = Cols<2>::of(a);
+    u = Cols<2>::of(b);
+    m = to;
+  }
+  HS_DEV void add(const float *v, Cols<2> minus, Scale k) {
+    float d[2];
+    (Cols<2>::of(v) + minus).get(d);
+    d[0] = max_nan(d[0], k.floor);
+    d[1] = max_nan(d[1], k.floor);
+    const Cols<2> dd = Cols<2>::of(d);
+    float t[2];
+    (dd * Cols<2>::all(k.c)).get(t);
+    t[0] = ex2(t[0]);
+    t[1] = ex2(t[1]);
+    const Cols<2> e = Cols<2>::of(t);
+    s = s + e;
+    u = fma(e, dd, u);
+  }
+  HS_DEV void scalar(float v, Scale k, int where) {
     if (best == -1) best = where;
-    if (v > a.m) {
-      rescale(a, v, c);
+    if (v > m) {
+      raise(v, k);
       best = where;
     }
-    const float t = max_nan((v - rel(a.m)) * c, kFloor), e = ex2(t);
-    a.s += e;
-    a.u = fmaf(e, t, a.u);
+    const float two[2] = {v, kNegInf};
+    add(two, Cols<2>::all(-rel(m)), k);
   }
-  // U vectors, the first at index i0, `stride` apart; n of them are there
-  template <int U> HS_DEV void vectors(const uint4 (&q)[U], int n, int i0, int stride, float c) {
+  // U vectors, the first at index i0, `stride` apart
+  template <int U> HS_DEV void vectors(const uint4 (&q)[U], int i0, int stride, Scale k) {
     constexpr int E = Row<T>::E;
     if (best == -1) best = i0;
-    float bm = kNegInf;
+    float top[U], bm = kNegInf;
 #pragma unroll
-    for (int k = 0; k < U; ++k) {
-      if (k >= n) break;
-      float v[E];
-      unpack_vec<T>(q[k], v);
+    for (int j = 0; j < U; ++j) bm = fmaxf(bm, top[j] = vec_max<T>(q[j]));
+    if (bm > m) {
+      raise(bm, k);
 #pragma unroll
-      for (int e = 0; e < E; ++e) bm = fmaxf(bm, v[e]);
+      for (int j = U - 1; j >= 0; --j)
+        if (top[j] == bm) best = i0 + j * stride;
     }
-    if (bm > a.m) {
-      rescale(a, bm, c);
+    const Cols<2> minus = Cols<2>::all(-rel(m));
 #pragma unroll
-      for (int k = U - 1; k >= 0; --k) {
-        if (k >= n) continue;
-        float v[E], m = kNegInf;
-        unpack_vec<T>(q[k], v);
-#pragma unroll
-        for (int e = 0; e < E; ++e) m = fmaxf(m, v[e]);
-        if (m == bm) best = i0 + k * stride;
-      }
-    }
-    const float r = rel(a.m);
-#pragma unroll
-    for (int k = 0; k < U; ++k) {
-      if (k >= n) break;
+    for (int j = 0; j < U; ++j) {
       float v[E];
-      unpack_vec<T>(q[k], v);
+      unpack_vec<T>(q[j], v);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float t = max_nan((v[e] - r) * c, kFloor), p = ex2(t);
-        a.s += p;
-        a.u = fmaf(p, t, a.u);
-      }
+      for (int e = 0; e < E; e += 2) add(v + e, minus, k);
     }
   }
 };
@@ -264,21 +299,24 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) logprobs_fwd_kernel(con
   if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   const Row<T> r(row, p.V, rank, C);
   Scan<T> scan;
-  if (tid < r.head) scan.scalar(to_f32<T>(row[tid]), p.c, -2);
-  for (int i = r.lo + tid; i < r.hi; i += U * NT) {
+  if (tid < r.head) scan.scalar(to_f32<T>(row[tid]), p.k, -2);
+  int i = r.lo + tid;
+  for (; i + (U - 1) * NT < r.hi; i += U * NT) {
     uint4 q[U];
-    const int left = (r.hi - i + NT - 1) / NT, here = left < U ? left : U;
 #pragma unroll
-    for (int k = 0; k < U; ++k)
-      if (k < here) q[k] = __ldg(r.vec(i + k * NT));
-    scan.template vectors<U>(q, here, i, NT, p.c);
+    for (int k = 0; k < U; ++k) q[k] = __ldg(r.vec(i + k * NT));
+    scan.template vectors<U>(q, i, NT, p.k);
   }
-  if (tid < r.ntail) scan.scalar(to_f32<T>(row[r.tail0 + tid]), p.c, -3);
+  for (; i < r.hi; i += NT) {
+    const uint4 q[1] = {__ldg(r.vec(i))};
+    scan.template vectors<1>(q, i, NT, p.k);
+  }
+  if (tid < r.ntail) scan.scalar(to_f32<T>(row[r.tail0 + tid]), p.k, -3);
 
   // the row's statistics
-  Stat a = scan.a;
+  Stat a = scan.stat();
 #pragma unroll
-  for (int o = 16; o; o >>= 1) merge(a, shfl_xor(a, o), p.c);
+  for (int o = 16; o; o >>= 1) merge(a, shfl_xor(a, o), p.k);
   if (W > 1) {
     if (lane == 0) sh.stat[warp] = a;
     if (threadIdx.x == 0) sh.nchosen = 0;
@@ -296,7 +334,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) logprobs_fwd_kernel(con
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const Key k = make_key(v[e], r.index(scan.best, e));
-        if (v[e] == scan.a.m && k > mine) mine = k;
+        if (v[e] == scan.m && k > mine) mine = k;
       }
       if (mine == 0) mine = make_key(kNegInf, r.index(scan.best, 0));  // NaN alone (the row's results are NaN)
     }
@@ -370,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) logprobs_fwd_kernel(con
     if (warp == 0) {
       a = sh.stat[lane & (W - 1)];
 #pragma unroll
-      for (int o = W / 2; o; o >>= 1) merge(a, shfl_xor(a, o), p.c);
+      for (int o = W / 2; o; o >>= 1) merge(a, shfl_xor(a, o), p.k);
     }
     if (C > 1) {
       asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA has started
@@ -385,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) logprobs_fwd_kernel(con
       asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
       if (rank != 0 || warp != 0) return;
       a = sh.cstat[0];
-      for (int j = 1; j < C; ++j) merge(a, sh.cstat[j], p.c);
+      for (int j = 1; j < C; ++j) merge(a, sh.cstat[j], p.k);
       if (TOP) {
         list = sh.clist[0][lane];
         for (int j = 1; j < C; ++j) list = merge_desc(list, sh.clist[j][lane], lane);
@@ -403,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) logprobs_fwd_kernel(con
       p.lp[n] = __int_as_float(0x7fc00000);
       set_status(p.status, HS_ERR_INDEX);
     }
-    if (p.ent) p.ent[n] = empty ? 0.f : kLn2 * (ls - a.u / a.s);
+    if (p.ent) p.ent[n] = empty ? 0.f : kLn2 * ls - p.inv_t * (a.u / a.s);
     if (p.stats) {
       p.stats[2 * n] = bad ? a.s : a.m;
       p.stats[2 * n + 1] = ls;
@@ -455,9 +493,21 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs p)
   const float ge = p.ge && !zero ? p.ge[n] : 0.f;
   // dx = -inv_t p (sum + ge (ln2 t + entropy)) = p (k0 + k1 t)
   const float k0 = ge != 0.f ? -p.inv_t * fmaf(ge, p.ent[n], sum) : -p.inv_t * sum, k1 = -p.inv_t * ge * kLn2;
+  const Cols<2> minus = Cols<2>::all(-m), cc = Cols<2>::all(p.c), mls = Cols<2>::all(-ls), kk0 = Cols<2>::all(k0),
+                kk1 = Cols<2>::all(k1);
+  auto grad2 = [&](float *v) {  // two logits to their gradients
+    float t[2], e[2];
+    fma(Cols<2>::of(v) + minus, cc, mls).get(t);
+    t[0] = max_nan(t[0], kFloor);
+    t[1] = max_nan(t[1], kFloor);
+    e[0] = ex2(t[0]);
+    e[1] = ex2(t[1]);
+    (Cols<2>::of(e) * fma(kk1, Cols<2>::of(t), kk0)).get(v);
+  };
   auto grad = [&](float x) {
-    const float t = max_nan(fmaf(x - m, p.c, -ls), kFloor);
-    return ex2(t) * fmaf(k1, t, k0);
+    float v[2] = {x, x};
+    grad2(v);
+    return v[0];
   };
   const Row<T> r(row, p.V, rank, C);
   // vectors where the output's row is aligned like the input's, else one value at a time
@@ -465,23 +515,26 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs p)
   if (tid < r.head) out[tid] = from_f32<T>(zero ? 0.f : grad(to_f32<T>(row[tid])));
   if (vec) {
     uint4 *o = reinterpret_cast<uint4 *>(out + r.base);
-    for (int i = r.lo + tid; i < r.hi; i += U * NT) {
-      uint4 q[U];
+    auto one = [&](const uint4 &q) {
+      float v[E];
+      unpack_vec<T>(q, v);
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
-        q[k] = uint4{};
-        if (!zero && i + k * NT < r.hi) q[k] = __ldg(r.vec(i + k * NT));
+      for (int e = 0; e < E; e += 2) grad2(v + e);
+      constexpr int P = PerWord<T>::value;
+      return make_uint4(pack_word<T>(v), pack_word<T>(v + P), pack_word<T>(v + 2 * P), pack_word<T>(v + 3 * P));
+    };
+    int i = r.lo + tid;
+    if (zero) {
+      for (; i < r.hi; i += NT) o[i] = uint4{};
+    } else {
+      for (; i + (U - 1) * NT < r.hi; i += U * NT) {
+        uint4 q[U];
+#pragma unroll
+        for (int k = 0; k < U; ++k) q[k] = __ldg(r.vec(i + k * NT));
+#pragma unroll
+        for (int k = 0; k < U; ++k) o[i + k * NT] = one(q[k]);
       }
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        if (i + k * NT >= r.hi) break;
-        float v[E];
-        unpack_vec<T>(q[k], v);
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = zero ? 0.f : grad(v[e]);
-        constexpr int P = PerWord<T>::value;
-        o[i + k * NT] = make_uint4(pack_word<T>(v), pack_word<T>(v + P), pack_word<T>(v + 2 * P), pack_word<T>(v + 3 * P));
-      }
+      for (; i < r.hi; i += NT) o[i] = one(__ldg(r.vec(i)));
     }
   } else {
     for (int i = r.index(r.lo, 0) + tid; i < r.index(r.hi, 0); i += NT) out[i] = from_f32<T>(zero ? 0.f : grad(to_f32<T>(row[i])));
@@ -520,7 +573,8 @@ int check_rows(const char *who, int dtype, const void *x, int64_t ld, int token_
   if (token_bits != 32 && token_bits != 64) return fail(HS_ERR_INVALID_ARG, "%s: token_bits is 32 or 64", who);
   if (N < 0 || V < 0) return fail(HS_ERR_INVALID_ARG, "%s: negative N or V", who);
   if (V > (int64_t)1 << 30 || N > (int64_t)1 << 27) return fail(HS_ERR_UNSUPPORTED, "%s: V above 2^30 or N above 2^27", who);
-  if (!(temperature > 0.f) || !(temperature < 3.0e38f)) return fail(HS_ERR_INVALID_ARG, "%s: the temperature must be positive", who);
+  if (!(temperature >= 1e-30f) || !(temperature <= 1e30f))
+    return fail(HS_ERR_INVALID_ARG, "%s: the temperature must be positive (1e-30 to 1e30)", who);
   if (top < 0 || top > HS_MAX_TOP || top > V) return fail(HS_ERR_INVALID_ARG, "%s: top=%d outside 0..min(%d, V)", who, top, HS_MAX_TOP);
   if (N == 0) return HS_OK;
   if (V == 0) return fail(HS_ERR_INVALID_ARG, "%s: rows of no logits", who);
@@ -552,7 +606,8 @@ int hs_token_logprobs_forward(int dtype, const void *logits, int64_t logits_ld, 
     return fail(HS_ERR_INVALID_ARG, "hs_token_logprobs_forward: null output or dev_status");
   FwdArgs a = {};
   a.x = logits, a.ld = logits_ld, a.tok = tokens, a.token64 = token_bits == 64, a.ignore = ignore_index;
-  a.c = (float)(1.4426950408889634 / (double)temperature), a.inv_t = (float)(1.0 / (double)temperature);
+  a.k.c = (float)(1.4426950408889634 / (double)temperature), a.k.floor = kFloor / a.k.c;
+  a.inv_t = (float)(1.0 / (double)temperature);
   a.top = top, a.lp = logprob, a.ent = entropy, a.top_lp = top_logprob, a.top_id = top_index, a.stats = stats;
   a.N = N, a.V = V, a.status = dev_status;
   const int64_t bytes = V * (int64_t)dtype_bytes(dtype);
