@@ -60,6 +60,12 @@ template <> HS_DEV unsigned word_max<__half>(unsigned a, unsigned b) {
   return r;
 }
 
+// A word of -inf.
+template <typename T> __host__ __device__ constexpr unsigned minus_inf_word();
+template <> __host__ __device__ constexpr unsigned minus_inf_word<float>() { return 0xff800000u; }
+template <> __host__ __device__ constexpr unsigned minus_inf_word<__nv_bfloat16>() { return 0xff80ff80u; }
+template <> __host__ __device__ constexpr unsigned minus_inf_word<__half>() { return 0xfc00fc00u; }
+
 template <typename T> struct PerWord { static constexpr int value = 4 / (int)sizeof(T); };
 
 // One float32, or two as one pair of registers that sm_100a's packed float32

@@ -13,14 +13,15 @@
 // hardware exp2 and about four other instructions (sums two at a time), below
 // the memory time for 16-bit logits too.
 //
-// Top alternatives cost the pass nothing: the running maximum already says
-// where each thread's best value lies.  The k-th best of the threads' bests
-// (k distinct values are at least that) bounds the k-th best of the row from
-// below, and only the k threads whose best reaches it can hold alternatives.
-// Those threads' values, k / 256 of the row, are read again (from L2) and
-// merged into a warp-wide list of 32 sorted keys.  A key is the value's
-// monotone 32-bit image with the complement of its index below it, so the
-// order is by value and, for equal values, by the lower index.
+// Top alternatives cost the pass nothing: each thread already knows its
+// largest value.  A value that k of the threads' largest reach bounds the k-th
+// best of the row from below (found by bisection, a vote per step), and only
+// threads whose largest reaches it can hold alternatives.  Those threads'
+// values, little more than k / 256 of the row, are read again (from L2), the few
+// that reach the bound are collected, and one warp sorts them.  Where equal
+// values make more than fit, the whole row is read again into a list per warp.
+// A key is the value's monotone 32-bit image with the complement of its index
+// below it, so the order is by value and, for equal values, by the lower index.
 //
 // Split: a CTA of 256 threads per row, a cluster of CTAs per row where there
 // are few rows (the parts meet in distributed shared memory), a warp per row
@@ -72,8 +73,16 @@ HS_DEV void merge(Stat &a, Stat b, Scale k) {
   a.s += b.s;
   a.u += b.u;
 }
-HS_DEV Stat shfl_xor(const Stat &a, int o) {
-  return {__shfl_xor_sync(0xffffffffu, a.m, o), __shfl_xor_sync(0xffffffffu, a.s, o), __shfl_xor_sync(0xffffffffu, a.u, o)};
+// Over groups of n lanes: the maximum first, so that each lane moves its sums once.
+HS_DEV Stat reduce(Stat a, int n, Scale k) {
+  float m = a.m;
+  for (int o = n / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (a.m != m) rescale(a, m, k);
+  for (int o = n / 2; o; o >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, o);
+    a.u += __shfl_xor_sync(0xffffffffu, a.u, o);
+  }
+  return a;
 }
 
 // ------------------------------------------------------------------ keys
@@ -181,23 +190,18 @@ template <typename T> HS_DEV float vec_max(const uint4 &q) {
 template <typename T> struct Scan {
   float m = kNegInf;
   Cols<2> s = Cols<2>::all(0.f), u = Cols<2>::all(0.f);
-  int best = -1;  // where the maximum was first met: vector i as i, head scalar as -2, tail scalar as -3
   HS_DEV Stat stat() const {
     float a[2], b[2];
     s.get(a);
     u.get(b);
     return {m, a[0] + a[1], b[0] + b[1]};
   }
+  // Moves the sums to the reference `to` >= m (from none, m = -inf, they are 0).
   HS_DEV void raise(float to, Scale k) {
-    float a[2], b[2];
-    s.get(a);
-    u.get(b);
-    Stat x{m, a[0], b[0]}, y{m, a[1], b[1]};
-    rescale(x, to, k);
-    rescale(y, to, k);
-    a[0] = x.s, a[1] = y.s, b[0] = x.u, b[1] = y.u;
-    s = Cols<2>::of(a);
-    u = Cols<2>::of(b);
+    const float d = max_nan(m - to, k.floor);
+    const Cols<2> f = Cols<2>::all(ex2(d * k.c));
+    u = fma(Cols<2>::all(d), s, u) * f;
+    s = s * f;
     m = to;
   }
   HS_DEV void add(const float *v, Cols<2> minus, Scale k) {
@@ -214,28 +218,17 @@ template <typename T> struct Scan {
     s = s + e;
     u = fma(e, dd, u);
   }
-  HS_DEV void scalar(float v, Scale k, int where) {
-    if (best == -1) best = where;
-    if (v > m) {
-      raise(v, k);
-      best = where;
-    }
+  HS_DEV void scalar(float v, Scale k) {
+    if (v > m) raise(v, k);
     const float two[2] = {v, kNegInf};
     add(two, Cols<2>::all(-rel(m)), k);
   }
-  // U vectors, the first at index i0, `stride` apart
-  template <int U> HS_DEV void vectors(const uint4 (&q)[U], int i0, int stride, Scale k) {
+  template <int U> HS_DEV void vectors(const uint4 (&q)[U], Scale k) {
     constexpr int E = Row<T>::E;
-    if (best == -1) best = i0;
-    float top[U], bm = kNegInf;
+    float bm = kNegInf;
 #pragma unroll
-    for (int j = 0; j < U; ++j) bm = fmaxf(bm, top[j] = vec_max<T>(q[j]));
-    if (bm > m) {
-      raise(bm, k);
-#pragma unroll
-      for (int j = U - 1; j >= 0; --j)
-        if (top[j] == bm) best = i0 + j * stride;
-    }
+    for (int j = 0; j < U; ++j) bm = fmaxf(bm, vec_max<T>(q[j]));
+    if (bm > m) raise(bm, k);
     const Cols<2> minus = Cols<2>::all(-rel(m));
 #pragma unroll
     for (int j = 0; j < U; ++j) {
@@ -247,16 +240,30 @@ template <typename T> struct Scan {
   }
 };
 
-// Shared memory of a CTA per row (a warp per row uses none of it).
-struct Shared {
-  Stat stat[kWarps];
-  Key list[kWarps][32];
-  int chosen[32];
-  int nchosen;
-  Key bound;
-  Stat cstat[kMaxCluster];          // written by the cluster's CTAs
-  Key clist[kMaxCluster][32];
+constexpr int kChosen = 64, kFound = 64;  // threads read again, values collected: at most
+
+// What finding the alternatives of one row needs.
+struct Finder {
+  Key found[kFound];
+  int nfound, nchosen;
+  int chosen[kChosen];
 };
+// Shared memory of a CTA: one row's, or the finders of a row per warp.
+template <int W, bool TOP> struct Shared {
+  Finder f[TOP ? kWarps / W : 1];
+  Stat stat[kWarps];
+  unsigned lowest[kWarps];
+  Key list[TOP && W > 1 ? kWarps : 1][32];
+  Stat cstat[kMaxCluster];  // written by the cluster's CTAs
+  Key clist[TOP ? kMaxCluster : 1][32];
+};
+
+template <int W> HS_DEV void row_sync() {
+  if (W == 1) __syncwarp(); else __syncthreads();
+}
+template <int W> HS_DEV int row_count(bool p) {
+  return W == 1 ? __popc(__ballot_sync(0xffffffffu, p)) : __syncthreads_count(p);
+}
 
 HS_DEV unsigned remote(const void *p, int rank) {
   unsigned r;
@@ -272,8 +279,8 @@ HS_DEV void st_remote(const Key *p, int rank, Key v) {
 
 // W: warps per row (1 or kWarps).
 template <typename T, int W, bool TOP>
-__global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) logprobs_fwd_kernel(const FwdArgs p) {
-  __shared__ Shared sh;
+__global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(const FwdArgs p) {
+  __shared__ Shared<W, TOP> sh;
   constexpr int NT = 32 * W, U = 4, E = Row<T>::E;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int tid = W == 1 ? lane : (int)threadIdx.x;
@@ -299,105 +306,127 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) logprobs_fwd_kernel(con
   if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   const Row<T> r(row, p.V, rank, C);
   Scan<T> scan;
-  if (tid < r.head) scan.scalar(to_f32<T>(row[tid]), p.k, -2);
-  int i = r.lo + tid;
-  for (; i + (U - 1) * NT < r.hi; i += U * NT) {
-    uint4 q[U];
+  if (tid < r.head) scan.scalar(to_f32<T>(row[tid]), p.k);
+  // U vectors at a time, the next ones on their way meanwhile; -inf, which adds
+  // nothing, past the end
+  auto load = [&](uint4 (&q)[U], int i) {
+    if (i + (U - 1) * NT < r.hi) {
 #pragma unroll
-    for (int k = 0; k < U; ++k) q[k] = __ldg(r.vec(i + k * NT));
-    scan.template vectors<U>(q, i, NT, p.k);
+      for (int k = 0; k < U; ++k) q[k] = __ldg(r.vec(i + k * NT));
+    } else {
+      constexpr unsigned w = minus_inf_word<T>();
+#pragma unroll
+      for (int k = 0; k < U; ++k) q[k] = i + k * NT < r.hi ? __ldg(r.vec(i + k * NT)) : make_uint4(w, w, w, w);
+    }
+  };
+  int at = r.lo + tid;
+  if (at < r.hi) {
+    uint4 q[2][U];
+    load(q[0], at);
+    while (true) {
+      if ((at += U * NT) < r.hi) load(q[1], at);
+      scan.template vectors<U>(q[0], p.k);
+      if (at >= r.hi) break;
+      if ((at += U * NT) < r.hi) load(q[0], at);
+      scan.template vectors<U>(q[1], p.k);
+      if (at >= r.hi) break;
+    }
   }
-  for (; i < r.hi; i += NT) {
-    const uint4 q[1] = {__ldg(r.vec(i))};
-    scan.template vectors<1>(q, i, NT, p.k);
-  }
-  if (tid < r.ntail) scan.scalar(to_f32<T>(row[r.tail0 + tid]), p.k, -3);
+  if (tid < r.ntail) scan.scalar(to_f32<T>(row[r.tail0 + tid]), p.k);
 
   // the row's statistics
-  Stat a = scan.stat();
-#pragma unroll
-  for (int o = 16; o; o >>= 1) merge(a, shfl_xor(a, o), p.k);
-  if (W > 1) {
-    if (lane == 0) sh.stat[warp] = a;
-    if (threadIdx.x == 0) sh.nchosen = 0;
-  }
+  Stat a = reduce(scan.stat(), 32, p.k);
+  if (W > 1 && lane == 0) sh.stat[warp] = a;
 
   Key list = 0;
   if constexpr (TOP) {
-    // this thread's best value and its lowest index
-    Key mine = 0;
-    if (scan.best == -2) mine = make_key(to_f32<T>(row[tid]), tid);
-    if (scan.best == -3) mine = make_key(to_f32<T>(row[r.tail0 + tid]), r.tail0 + tid);
-    if (scan.best >= 0) {
-      float v[E];
-      unpack_vec<T>(*r.vec(scan.best), v);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const Key k = make_key(v[e], r.index(scan.best, e));
-        if (v[e] == scan.m && k > mine) mine = k;
-      }
-      if (mine == 0) mine = make_key(kNegInf, r.index(scan.best, 0));  // NaN alone (the row's results are NaN)
-    }
-    Key bests = sort_desc(mine, lane);
+    Finder &f = sh.f[W == 1 ? warp : 0];
+    if (tid == 0) f.nfound = f.nchosen = 0;
+    const bool some = tid < r.head || r.lo + tid < r.hi || tid < r.ntail;  // this thread holds values
+    const unsigned mine = some ? order_bits(scan.m) : 0;
+    // a bound that at least `top` threads reach, and not many more
+    const unsigned least = __reduce_min_sync(0xffffffffu, some ? mine : 0xffffffffu);
+    unsigned lo = least, hi = order_bits(a.m);
     if (W > 1) {
-      sh.list[warp][lane] = bests;
+      if (lane == 0) sh.lowest[warp] = least;
       __syncthreads();
 #pragma unroll
-      for (int half = W / 2; half; half >>= 1) {
-        if (warp < half) {
-          bests = merge_desc(bests, sh.list[warp + half][lane], lane);
-          sh.list[warp][lane] = bests;
-        }
-        __syncthreads();
+      for (int w = 0; w < W; ++w) {
+        lo = min(lo, sh.lowest[w]);
+        hi = max(hi, order_bits(sh.stat[w].m));
       }
-      if (warp == 0 && lane == p.top - 1) sh.bound = bests;
-      __syncthreads();
     }
-    const Key bound = W > 1 ? sh.bound : __shfl_sync(0xffffffffu, bests, p.top - 1);
-    // read the sets of the threads that reach the bound (0: fewer sets than alternatives, all of them)
-    auto add = [&](Key k) {
-      if (__ballot_sync(0xffffffffu, k >= bound && k > 0) == 0) return;
-      list = merge_desc(list, sort_desc(k >= bound ? k : 0, lane), lane);
+    hi += 1;
+    int c = row_count<W>(mine >= lo && some);
+    while (c > p.top + 8 && hi - lo > 1) {
+      const unsigned mid = lo + (hi - lo) / 2;
+      const int n = row_count<W>(mine >= mid);
+      if (n >= p.top) lo = mid, c = n; else hi = mid;
+    }
+    if (c < p.top) lo = 1;  // fewer threads with values than alternatives: all of them
+    if (some && mine >= lo) {
+      const int at = atomicAdd(&f.nchosen, 1);  // in any order: the keys are sorted
+      if (at < kChosen) f.chosen[at] = tid;
+    }
+    row_sync<W>();
+    const int nchosen = f.nchosen;
+    auto collect = [&](float v, int at) {
+      const unsigned b = order_bits(v);
+      if (b < lo || isnan(v)) return;
+      const int k = atomicAdd(&f.nfound, 1);
+      if (k < kFound) f.found[k] = make_key(v, at);
     };
-    auto read_set = [&](int t) {
-      if (t < r.head) add(lane == 0 ? make_key(to_f32<T>(row[t]), t) : 0);
-      for (int i0 = r.lo + t; i0 < r.hi; i0 += 32 * NT) {
-        const int i = i0 + lane * NT;
+    if (nchosen <= kChosen) {
+      if (mine >= lo && tid < r.head) collect(to_f32<T>(row[tid]), tid);
+      if (mine >= lo && tid < r.ntail) collect(to_f32<T>(row[r.tail0 + tid]), r.tail0 + tid);
+      const int per = (r.hi - r.lo + NT - 1) / NT;  // vectors of a thread
+      for (int j = tid; j < nchosen * per; j += NT) {
+        const int t = j / per, i = r.lo + f.chosen[t] + (j - t * per) * NT;
+        if (i >= r.hi) continue;
+        const uint4 q = __ldg(r.vec(i));
+        if (order_bits(vec_max<T>(q)) < lo) continue;
         float v[E];
-        const bool ok = i < r.hi;
-        if (ok) unpack_vec<T>(__ldg(r.vec(i)), v);
+        unpack_vec<T>(q, v);
 #pragma unroll
-        for (int e = 0; e < E; ++e) add(ok && !isnan(v[e]) ? make_key(v[e], r.index(i, e)) : 0);
+        for (int e = 0; e < E; ++e) collect(v[e], r.index(i, e));
       }
-      if (t < r.ntail) add(lane == 0 ? make_key(to_f32<T>(row[r.tail0 + t]), r.tail0 + t) : 0);
-    };
-    if (W == 1) {
-      unsigned who = __ballot_sync(0xffffffffu, mine >= bound && mine > 0);
-      while (who) {
-        const int t = __ffs(who) - 1;
-        who &= who - 1;
-        read_set(t);
+    }
+    row_sync<W>();
+    const int n = f.nfound;
+    if (nchosen <= kChosen && n <= kFound) {
+      if (W == 1 || warp == 0) {
+        list = sort_desc(lane < n ? f.found[lane] : 0, lane);
+        if (n > 32) list = merge_desc(list, sort_desc(32 + lane < n ? f.found[32 + lane] : 0, lane), lane);
       }
-    } else {
-      if (mine >= bound && mine > 0) {
-        const int at = atomicAdd(&sh.nchosen, 1);  // the order does not matter: keys are merged
-        if (at < 32) sh.chosen[at] = (int)threadIdx.x;
+    } else {  // too many equal values
+      auto add = [&](float v, int at, bool ok) {
+        const Key k = ok && !isnan(v) ? make_key(v, at) : 0;
+        if (__any_sync(0xffffffffu, k > __shfl_sync(0xffffffffu, list, 31))) list = merge_desc(list, sort_desc(k, lane), lane);
+      };
+      if (W == 1 || warp == 0) {
+        add(lane < r.head ? to_f32<T>(row[lane]) : 0.f, lane, lane < r.head);
+        add(lane < r.ntail ? to_f32<T>(row[r.tail0 + lane]) : 0.f, r.tail0 + lane, lane < r.ntail);
       }
-      __syncthreads();
-      if (bound > 0) {
-        for (int j = warp; j < min(sh.nchosen, 32); j += W) read_set(sh.chosen[j]);
-      } else {
-        for (int t = warp; t < NT; t += W) read_set(t);
-      }
-      sh.list[warp][lane] = list;
-      __syncthreads();
+      for (int i0 = r.lo + (W == 1 ? 0 : warp * 32); i0 < r.hi; i0 += NT) {
+        const int i = i0 + lane;
+        const uint4 q = i < r.hi ? __ldg(r.vec(i)) : uint4{};
+        const Key last = __shfl_sync(0xffffffffu, list, 31);
+        if (!__any_sync(0xffffffffu, i < r.hi && order_bits(vec_max<T>(q)) >= (unsigned)(last >> 32))) continue;
+        float v[E];
+        unpack_vec<T>(q, v);
+#pragma unroll 1
+        for (int e = 0; e < E; ++e) {
+          float x = v[0];
 #pragma unroll
-      for (int half = W / 2; half; half >>= 1) {
-        if (warp < half) {
-          list = merge_desc(list, sh.list[warp + half][lane], lane);
-          sh.list[warp][lane] = list;
+          for (int o = 1; o < E; ++o) x = e == o ? v[o] : x;
+          add(x, r.index(i, e), i < r.hi);
         }
+      }
+      if (W > 1) {
+        sh.list[warp][lane] = list;
         __syncthreads();
+        if (warp == 0)
+          for (int w = 1; w < W; ++w) list = merge_desc(list, sh.list[w][lane], lane);
       }
     }
   } else if (W > 1) {
@@ -406,9 +435,7 @@ __global__ void __launch_bounds__(kThreads, TOP ? 4 : 5) logprobs_fwd_kernel(con
   if (W > 1) {
     if (warp != 0 && C == 1) return;
     if (warp == 0) {
-      a = sh.stat[lane & (W - 1)];
-#pragma unroll
-      for (int o = W / 2; o; o >>= 1) merge(a, shfl_xor(a, o), p.k);
+      a = reduce(sh.stat[lane & (W - 1)], W, p.k);
     }
     if (C > 1) {
       asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA has started
@@ -527,14 +554,22 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs p)
     if (zero) {
       for (; i < r.hi; i += NT) o[i] = uint4{};
     } else {
-      for (; i + (U - 1) * NT < r.hi; i += U * NT) {
+      for (; i < r.hi; i += U * NT) {
         uint4 q[U];
+        if (i + (U - 1) * NT < r.hi) {
 #pragma unroll
-        for (int k = 0; k < U; ++k) q[k] = __ldg(r.vec(i + k * NT));
+          for (int k = 0; k < U; ++k) q[k] = __ldg(r.vec(i + k * NT));
 #pragma unroll
-        for (int k = 0; k < U; ++k) o[i + k * NT] = one(q[k]);
+          for (int k = 0; k < U; ++k) o[i + k * NT] = one(q[k]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < U - 1; ++k)
+            if (i + k * NT < r.hi) q[k] = __ldg(r.vec(i + k * NT));
+#pragma unroll
+          for (int k = 0; k < U - 1; ++k)
+            if (i + k * NT < r.hi) o[i + k * NT] = one(q[k]);
+        }
       }
-      for (; i < r.hi; i += NT) o[i] = one(__ldg(r.vec(i)));
     }
   } else {
     for (int i = r.index(r.lo, 0) + tid; i < r.index(r.hi, 0); i += NT) out[i] = from_f32<T>(zero ? 0.f : grad(to_f32<T>(row[i])));
