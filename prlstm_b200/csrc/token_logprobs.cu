@@ -17,7 +17,7 @@
 // largest value.  A value that k of the threads' largest reach bounds the k-th
 // best of the row from below (found by bisection, a vote per step), and only
 // threads whose largest reaches it can hold alternatives.  Those threads'
-// values, little more than k / 256 of the row, are read again (from L2), the few
+// values, little more than k / (threads) of the row, are read again (from L2), the few
 // that reach the bound are collected, and one warp sorts them.  Where equal
 // values make more than fit, the whole row is read again into a list per warp.
 // A key is the value's monotone 32-bit image with the complement of its index
@@ -31,7 +31,8 @@
 namespace hs {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kShortRows = 8;  // rows of a CTA where each warp takes one
+template <int W> constexpr int threads_of() { return 32 * (W == 1 ? kShortRows : W); }
 constexpr int kMaxCluster = 8;
 constexpr float kFloor = -150.f;  // 2^-150 is 0 in float32: a smaller exponent changes nothing
 
@@ -250,10 +251,10 @@ struct Finder {
 };
 // Shared memory of a CTA: one row's, or the finders of a row per warp.
 template <int W, bool TOP> struct Shared {
-  Finder f[TOP ? kWarps / W : 1];
-  Stat stat[kWarps];
-  unsigned lowest[kWarps];
-  Key list[TOP && W > 1 ? kWarps : 1][32];
+  Finder f[TOP && W == 1 ? kShortRows : 1];
+  Stat stat[W];
+  unsigned lowest[W];
+  Key list[TOP && W > 1 ? W : 1][32];
   Stat cstat[kMaxCluster];  // written by the cluster's CTAs
   Key clist[TOP ? kMaxCluster : 1][32];
 };
@@ -277,15 +278,15 @@ HS_DEV void st_remote(const Key *p, int rank, Key v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote(p, rank)), "l"(v) : "memory");
 }
 
-// W: warps per row (1 or kWarps).
+// W: warps per row.
 template <typename T, int W, bool TOP>
-__global__ void __launch_bounds__(kThreads, 4) logprobs_fwd_kernel(const FwdArgs p) {
+__global__ void __launch_bounds__(threads_of<W>(), 1024 / threads_of<W>()) logprobs_fwd_kernel(const FwdArgs p) {
   __shared__ Shared<W, TOP> sh;
   constexpr int NT = 32 * W, U = 4, E = Row<T>::E;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int tid = W == 1 ? lane : (int)threadIdx.x;
   const int C = W == 1 ? 1 : p.cluster, rank = (int)(blockIdx.x % C);
-  const int64_t n = W == 1 ? (int64_t)blockIdx.x * kWarps + warp : blockIdx.x / C;
+  const int64_t n = W == 1 ? (int64_t)blockIdx.x * kShortRows + warp : blockIdx.x / C;
   if (W == 1 && n >= p.N) return;
   const T *row = static_cast<const T *>(p.x) + n * p.ld;
   const int64_t tok = token_at(p.tok, p.token64, n);
@@ -498,12 +499,12 @@ struct BwdArgs {
 };
 
 template <typename T, int W>
-__global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs p) {
+__global__ void __launch_bounds__(threads_of<W>()) logprobs_bwd_kernel(const BwdArgs p) {
   constexpr int NT = 32 * W, U = 4, E = Row<T>::E;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int tid = W == 1 ? lane : (int)threadIdx.x;
   const int C = W == 1 ? 1 : p.parts, rank = (int)(blockIdx.x % C);
-  const int64_t n = W == 1 ? (int64_t)blockIdx.x * kWarps + warp : blockIdx.x / C;
+  const int64_t n = W == 1 ? (int64_t)blockIdx.x * kShortRows + warp : blockIdx.x / C;
   if (W == 1 && n >= p.N) return;
   const T *row = static_cast<const T *>(p.x) + n * p.ld;
   T *out = static_cast<T *>(p.dx) + n * p.dld;
@@ -591,14 +592,22 @@ __global__ void __launch_bounds__(kThreads) logprobs_bwd_kernel(const BwdArgs p)
 }
 
 // ------------------------------------------------------------------ launch
-// Rows up to this many bytes are taken by one warp each.
-constexpr int64_t kShortRow = 4096;
+// Warps per row.  One up to 4 KB (4096 rows of 1 KB: 3.5 us, with four warps
+// 10.5), in the forward of many rows up to 8 KB (8192 of 8 KB: 16.8 against 23.5
+// us); four up to 64 KB (16384 of 64 KB: 174 us, with eight 195); else eight
+// (the gradient of 2047 rows of 100 KB: 77 us, with four 81).
+int warps_of(bool forward, int64_t N, int64_t row_bytes) {
+  if (row_bytes <= 4096 || (forward && row_bytes <= 8192 && N >= 2048)) return 1;
+  return row_bytes <= 65536 ? 4 : 8;
+}
 
-int parts_of(int64_t N, int64_t row_bytes, int most) {
-  // CTAs per row: until the rows fill the SMs several times over, and no
-  // part below 8 KB
+// CTAs per row, of 8 KB at least.  The forward's meet in a cluster, which
+// pays where the rows alone leave SMs idle (24 rows of 512 KB: 7.1 us on
+// eight CTAs each, 20 on one; 300 rows of 100 KB: 15.5 on one, 20.5 on two); the
+// gradient's are independent.
+int parts_of(bool forward, int64_t N, int64_t row_bytes) {
   int c = 1;
-  while (c < most && N * c < 4 * 148 && row_bytes / (2 * c) >= 8192) c *= 2;
+  while (c < (forward ? kMaxCluster : 256) && (forward ? 2 * N * c <= 2 * 148 : N * c < 4 * 148) && row_bytes / (2 * c) >= 8192) c *= 2;
   return c;
 }
 
@@ -646,15 +655,16 @@ int hs_token_logprobs_forward(int dtype, const void *logits, int64_t logits_ld, 
   a.top = top, a.lp = logprob, a.ent = entropy, a.top_lp = top_logprob, a.top_id = top_index, a.stats = stats;
   a.N = N, a.V = V, a.status = dev_status;
   const int64_t bytes = V * (int64_t)dtype_bytes(dtype);
-  const bool short_row = bytes <= kShortRow;
-  a.cluster = short_row ? 1 : parts_of(N, bytes, kMaxCluster);
+  const int warps = warps_of(true, N, bytes);
+  a.cluster = warps == 1 ? 1 : parts_of(true, N, bytes);
   return by_type(dtype, [&](auto tag) -> int {
     using T = decltype(tag);
-    auto kernel = short_row ? (top ? logprobs_fwd_kernel<T, 1, true> : logprobs_fwd_kernel<T, 1, false>)
-                            : (top ? logprobs_fwd_kernel<T, kWarps, true> : logprobs_fwd_kernel<T, kWarps, false>);
+    auto kernel = warps == 1   ? (top ? logprobs_fwd_kernel<T, 1, true> : logprobs_fwd_kernel<T, 1, false>)
+                  : warps == 4 ? (top ? logprobs_fwd_kernel<T, 4, true> : logprobs_fwd_kernel<T, 4, false>)
+                               : (top ? logprobs_fwd_kernel<T, 8, true> : logprobs_fwd_kernel<T, 8, false>);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(short_row ? (N + kWarps - 1) / kWarps : N * a.cluster));
-    cfg.blockDim = dim3(kThreads);
+    cfg.gridDim = dim3((unsigned)(warps == 1 ? (N + kShortRows - 1) / kShortRows : N * a.cluster));
+    cfg.blockDim = dim3(warps == 1 ? 32 * kShortRows : 32 * warps);
     cfg.stream = (cudaStream_t)stream;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -685,15 +695,17 @@ int hs_token_logprobs_backward(int dtype, const void *logits, int64_t logits_ld,
   a.g = dlogprob, a.ge = dentropy, a.gt = top ? dtop_logprob : nullptr;
   a.dx = dlogits, a.dld = dlogits_ld, a.N = N, a.V = V;
   const int64_t bytes = V * (int64_t)dtype_bytes(dtype);
-  const bool short_row = bytes <= kShortRow;
-  a.parts = short_row ? 1 : parts_of(N, bytes, 256);
-  const unsigned grid = (unsigned)(short_row ? (N + kWarps - 1) / kWarps : N * a.parts);
+  const int warps = warps_of(false, N, bytes);
+  a.parts = warps == 1 ? 1 : parts_of(false, N, bytes);
+  const unsigned grid = (unsigned)(warps == 1 ? (N + kShortRows - 1) / kShortRows : N * a.parts);
   return by_type(dtype, [&](auto tag) -> int {
     using T = decltype(tag);
-    if (short_row)
-      logprobs_bwd_kernel<T, 1><<<grid, kThreads, 0, (cudaStream_t)stream>>>(a);
+    if (warps == 1)
+      logprobs_bwd_kernel<T, 1><<<grid, threads_of<1>(), 0, (cudaStream_t)stream>>>(a);
+    else if (warps == 4)
+      logprobs_bwd_kernel<T, 4><<<grid, threads_of<4>(), 0, (cudaStream_t)stream>>>(a);
     else
-      logprobs_bwd_kernel<T, kWarps><<<grid, kThreads, 0, (cudaStream_t)stream>>>(a);
+      logprobs_bwd_kernel<T, 8><<<grid, threads_of<8>(), 0, (cudaStream_t)stream>>>(a);
     return check_launch("logprobs_bwd_kernel");
   });
 }
