@@ -30,6 +30,7 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortCluster = 8;   // CTAs of the sorting cluster at most
 constexpr int kMaxBits = 9;       // bits of a sorting pass at most
+constexpr int kAhead = 8;         // groups of 32 entries that a sorting warp loads at once
 
 template <int BYTES> struct Chunk;  // one lane's bytes of a row
 template <> struct Chunk<16> { using type = uint4; };
@@ -78,12 +79,13 @@ __global__ void __launch_bounds__(256) emb_lookup_kernel(const char *w, int64_t 
   using C = typename Chunk<BYTES>::type;
   constexpr int E = BYTES / (int)sizeof(T);
   const int64_t i0 = (int64_t)blockIdx.x * (256 * 4) + threadIdx.x;
+  const bool small = total <= 0xffffffffll;  // a 32-bit division will do
   C c[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int64_t i = i0 + k * 256;
     if (i < total) {
-      const int64_t n = i / chunks;
+      const int64_t n = small ? (int64_t)((unsigned)i / (unsigned)chunks) : i / chunks;
       const int64_t t = (int64_t)tok[n];
       if (t >= 0 && t < V) {
         c[k] = *reinterpret_cast<const C *>(w + t * ld_bytes + (i - n * chunks) * BYTES);
@@ -121,7 +123,7 @@ HS_DEV void st_cluster_u32(const void *p, int rank, unsigned v) {
 struct SortArgs {
   const void *tok;
   int64_t N, V, pad;
-  unsigned *key[2], *pos[2];
+  uint2 *pair[2];     // {key, position}
   unsigned *seen;     // bitmap of the ids that occur
   int passes, bits;
   int *status;
@@ -148,24 +150,37 @@ __global__ void __launch_bounds__(kSortThreads, 1) emb_sort_kernel(const SortArg
   const TOK *tok = static_cast<const TOK *>(p.tok);
   for (int pass = 0; pass < p.passes; ++pass) {
     const int shift = pass * p.bits;
-    const unsigned *ksrc = p.key[(pass + 1) & 1], *psrc = p.pos[(pass + 1) & 1];
-    unsigned *kdst = p.key[pass & 1], *pdst = p.pos[pass & 1];
-    auto key_at = [&](int64_t i) -> unsigned {
-      if (pass) return __ldcg(ksrc + i);
-      const int64_t t = (int64_t)tok[i];
-      if (t >= 0 && t < p.V) return t == p.pad ? (unsigned)p.V : (unsigned)t;
-      set_status(p.status, HS_ERR_INDEX);
-      return (unsigned)p.V;
+    const uint2 *src = p.pair[(pass + 1) & 1];
+    uint2 *dst = p.pair[pass & 1];
+    // kAhead groups of 32 entries, all loads in flight at once; V past the end
+    auto load = [&](uint2 (&e)[kAhead], int64_t b) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int64_t i = b + u * 32 + lane;
+        e[u] = {0u, 0u};
+        if (i < hi) {
+          if (pass) {
+            e[u] = __ldcg(src + i);
+          } else {
+            const int64_t t = (int64_t)tok[i];
+            const bool inside = t >= 0 && t < p.V;
+            if (!inside) set_status(p.status, HS_ERR_INDEX);
+            e[u] = {inside && t != p.pad ? (unsigned)t : (unsigned)p.V, (unsigned)i};
+          }
+        }
+      }
     };
     unsigned *h = hist + warp * D;
     for (int i = lane; i < D; i += 32) h[i] = 0;
     __syncwarp();
-    for (int64_t b = lo; b < hi; b += 32) {
-      const bool ok = b + lane < hi;
-      const unsigned dig = ok ? (key_at(b + lane) >> shift) & (D - 1) : 0xffffffffu;
-      const unsigned same = __match_any_sync(0xffffffffu, dig);
-      if (ok && lane == __ffs(same) - 1) h[dig] += __popc(same);
-      __syncwarp();
+    for (int64_t b = lo; b < hi; b += 32 * kAhead) {
+      uint2 e[kAhead];
+      load(e, b);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (b + u * 32 >= hi) break;
+        if (b + u * 32 + lane < hi) atomicAdd(h + ((e[u].x >> shift) & (D - 1)), 1u);
+      }
     }
     if (pass == 0 && C > 1) cluster_sync_all();  // every CTA has started before its memory is written
     __syncthreads();
@@ -204,35 +219,44 @@ __global__ void __launch_bounds__(kSortThreads, 1) emb_sort_kernel(const SortArg
       base[tid] = less + inc - all + before;
     }
     __syncthreads();
-    for (int64_t b = lo; b < hi; b += 32) {
-      const bool ok = b + lane < hi;
-      const int64_t i = b + lane;
-      const unsigned key = ok ? key_at(i) : 0u;
-      const unsigned pos = ok ? (pass ? __ldcg(psrc + i) : (unsigned)i) : 0u;
-      const unsigned dig = ok ? (key >> shift) & (D - 1) : 0xffffffffu;
-      const unsigned same = __match_any_sync(0xffffffffu, dig);
-      unsigned at = 0;
-      if (ok) at = base[dig] + h[dig] + __popc(same & ((1u << lane) - 1u));
-      __syncwarp();
-      if (ok && lane == __ffs(same) - 1) h[dig] += __popc(same);
-      __syncwarp();
-      if (ok) {
-        kdst[at] = key;
-        pdst[at] = pos;
+    for (int64_t b = lo; b < hi; b += 32 * kAhead) {
+      uint2 e[kAhead];
+      load(e, b);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (b + u * 32 >= hi) break;
+        const bool ok = b + u * 32 + lane < hi;
+        const unsigned dig = (e[u].x >> shift) & (D - 1);
+        // the lanes of the same digit, by a vote on each of its bits (a match
+        // instruction in its place took three times as long)
+        unsigned same = __ballot_sync(0xffffffffu, ok);
+#pragma unroll
+        for (int bit = 0; bit < kMaxBits; ++bit) {
+          const unsigned set = __ballot_sync(0xffffffffu, (dig >> bit) & 1);
+          same &= ((dig >> bit) & 1) ? set : ~set;
+        }
+        unsigned at = 0;
+        if (ok) at = base[dig] + h[dig] + __popc(same & ((1u << lane) - 1u));
+        __syncwarp();
+        if (ok && lane == __ffs(same) - 1) h[dig] += __popc(same);
+        __syncwarp();
+        if (ok) dst[at] = e[u];
       }
     }
     if (C > 1) cluster_sync_all(); else __syncthreads();
   }
-  const unsigned *sk = p.key[(p.passes + 1) & 1];
+  const uint2 *sorted = p.pair[(p.passes + 1) & 1];
+#pragma unroll 4
   for (int64_t i = lo + lane; i < hi; i += 32) {
-    const unsigned k = __ldcg(sk + i);
-    if (k < (unsigned)p.V && (i == 0 || __ldcg(sk + i - 1) != k)) atomicOr(p.seen + (k >> 5), 1u << (k & 31));
+    const unsigned k = __ldcg(&sorted[i].x);
+    if (k < (unsigned)p.V && (i == 0 || __ldcg(&sorted[i - 1].x) != k)) atomicOr(p.seen + (k >> 5), 1u << (k & 31));
   }
 }
 
 // ------------------------------------------------------------------ sums of runs
 struct SumArgs {
-  const unsigned *key, *pos, *seen;
+  const uint2 *pair;   // {key, position}, sorted
+  const unsigned *seen;
   const char *dout;
   char *dw;
   float *head, *tail;  // [pieces][D]: the part of a run that came in / goes on
@@ -271,10 +295,10 @@ __global__ void __launch_bounds__(256) emb_sum_kernel(const SumArgs p) {
   const bool live = chunk < p.chunks;
   const int64_t first = piece * kPiece, mine = first + lane;
   const unsigned none = (unsigned)p.V;
-  const unsigned key = mine < p.N ? p.key[mine] : none;
-  const unsigned pos = mine < p.N ? p.pos[mine] : 0u;
-  const unsigned prev = first > 0 ? p.key[first - 1] : none;
-  const unsigned next = first + kPiece < p.N ? p.key[first + kPiece] : none;
+  const uint2 entry = mine < p.N ? p.pair[mine] : uint2{none, 0u};
+  const unsigned key = entry.x, pos = entry.y;
+  const unsigned prev = first > 0 ? p.pair[first - 1].x : none;
+  const unsigned next = first + kPiece < p.N ? p.pair[first + kPiece].x : none;
   const int count = __popc(__ballot_sync(0xffffffffu, key != none));  // valid entries come first
   float acc[E];
 #pragma unroll
@@ -324,7 +348,7 @@ __global__ void __launch_bounds__(256) emb_sum_kernel(const SumArgs p) {
 // A warp per piece whose last run goes on into the next piece and began in
 // this one: it adds the run's parts in order.  Runs over more than kLong
 // pieces are left to the whole CTA, each warp adding a contiguous share.
-constexpr int kJoinWarps = 16, kLong = 32;
+constexpr int kJoinWarps = 8, kLong = 8;
 
 template <typename T, int BYTES>
 __global__ void __launch_bounds__(32 * kJoinWarps) emb_join_kernel(const SumArgs p) {
@@ -343,14 +367,15 @@ __global__ void __launch_bounds__(32 * kJoinWarps) emb_join_kernel(const SumArgs
   __syncthreads();
   auto add_heads = [&](int64_t a, int64_t b, float *acc) {  // head parts of pieces a..b
     int64_t j = a;
-    for (; j + 4 <= b + 1; j += 4) {
-      float v[4][E];
+    constexpr int U = E > 4 ? 4 : 8;
+    for (; j + U <= b + 1; j += U) {
+      float v[U][E];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int e = 0; e < E; ++e) v[u][e] = live ? p.head[(j + u) * p.D + (int64_t)chunk * E + e] : 0.f;
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] += v[u][e];
     }
@@ -366,27 +391,28 @@ __global__ void __launch_bounds__(32 * kJoinWarps) emb_join_kernel(const SumArgs
   };
   const int64_t end = (piece + 1) * kPiece;
   if (piece < p.pieces && end < p.N) {
-    const unsigned k = p.key[end - 1];
-    const bool crosses = k != none && p.key[end] == k;
-    const bool began = p.key[piece * kPiece] != k || piece == 0 || p.key[piece * kPiece - 1] != k;
+    const unsigned k = p.pair[end - 1].x;
+    const bool crosses = k != none && p.pair[end].x == k;
+    const bool began = p.pair[piece * kPiece].x != k || piece == 0 || p.pair[piece * kPiece - 1].x != k;
     if (crosses && began) {
-      // last piece whose first entry is still k: by groups of 32, then halving
-      auto starts_with = [&](int64_t j) { return j < p.pieces && p.key[j * kPiece] == k; };
+      // the run's last piece: the last whose first entry is still k (the pieces
+      // of a run are consecutive)
+      auto starts_with = [&](int64_t j) { return j < p.pieces && p.pair[j * kPiece].x == k; };
       const unsigned run = __ballot_sync(0xffffffffu, starts_with(piece + 1 + lane));
-      if (run != 0xffffffffu) {
-        const int64_t last = piece + __popc(run);  // the pieces of a run are consecutive
+      if (__popc(run) <= kLong) {
+        const int64_t last = piece + __popc(run);
         float acc[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = live ? p.tail[piece * p.D + (int64_t)chunk * E + e] : 0.f;
         add_heads(piece + 1, last, acc);
         write_row(k, acc);
       } else if (lane == 0) {
-        int64_t a = piece + kLong, b = p.pieces;  // starts_with(a), not starts_with(b)
+        int64_t a = piece + __popc(run), b = run == 0xffffffffu ? p.pieces : a + 1;  // starts_with(a), not starts_with(b)
         while (b - a > 1) {
           const int64_t m = (a + b) / 2;
           if (starts_with(m)) a = m; else b = m;
         }
-        long_first = piece;  // 16 pieces hold the beginning of one such run at most
+        long_first = piece;  // kJoinWarps <= kLong + 1 pieces hold the beginning of one such run at most
         long_last = a;
         long_key = k;
       }
@@ -413,7 +439,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) emb_join_kernel(const SumArgs
 
 // ------------------------------------------------------------------ host side
 struct Layout {
-  size_t key[2], pos[2], seen, head, tail, total;
+  size_t pair[2], seen, head, tail, total;
 };
 Layout layout(int64_t N, int64_t V, int64_t D) {
   Layout l;
@@ -423,7 +449,7 @@ Layout layout(int64_t N, int64_t V, int64_t D) {
     at += round_up(bytes, 256);
     return o;
   };
-  for (int i = 0; i < 2; ++i) l.key[i] = take((size_t)N * 4), l.pos[i] = take((size_t)N * 4);
+  for (int i = 0; i < 2; ++i) l.pair[i] = take((size_t)N * sizeof(uint2));
   l.seen = take((size_t)((V + 31) / 32) * 4);
   const size_t parts = (size_t)((N + kPiece - 1) / kPiece) * (size_t)D * sizeof(float);
   l.head = take(parts);
@@ -527,7 +553,7 @@ int hs_embedding_backward(int dtype, const void *dout, int token_bits, const voi
 
   SortArgs s = {};
   s.tok = tokens, s.N = N, s.V = V, s.pad = padding_idx, s.status = dev_status;
-  for (int i = 0; i < 2; ++i) s.key[i] = (unsigned *)(ws + l.key[i]), s.pos[i] = (unsigned *)(ws + l.pos[i]);
+  for (int i = 0; i < 2; ++i) s.pair[i] = (uint2 *)(ws + l.pair[i]);
   s.seen = (unsigned *)(ws + l.seen);
   int key_bits = 1;
   while ((V >> key_bits) != 0) ++key_bits;  // ids 0..V
@@ -555,7 +581,7 @@ int hs_embedding_backward(int dtype, const void *dout, int token_bits, const voi
   if (cudaLaunchKernelExC(&cfg, sort, args) != cudaSuccess) return check_launch("emb_sort_kernel");
 
   SumArgs p = {};
-  p.key = s.key[(s.passes + 1) & 1], p.pos = s.pos[(s.passes + 1) & 1], p.seen = s.seen;
+  p.pair = s.pair[(s.passes + 1) & 1], p.seen = s.seen;
   p.dout = (const char *)dout, p.dw = (char *)dweight;
   p.head = (float *)(ws + l.head), p.tail = (float *)(ws + l.tail);
   p.N = N, p.V = V, p.D = D, p.pieces = (N + kPiece - 1) / kPiece, p.scale = make_scale(scale);
