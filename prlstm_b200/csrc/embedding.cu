@@ -5,16 +5,18 @@
 // Bound: memory.  The lookup reads N rows and writes N rows; the gradient
 // reads the N rows of dout once and writes the V rows of dW once.
 //
-// Gradient, three launches:
-//   1. One cluster sorts the N ids with their positions (stable, least
-//      significant digit first, up to 9 bits a pass: two passes for any vocabulary
-//      below 2^18) and marks the ids that occur in a bitmap.
+// Gradient:
+//   1. The ids are sorted with their positions (stable, least significant
+//      digit first, up to 9 bits a pass: two passes for any vocabulary below
+//      2^18); in one launch of one cluster up to 16384 tokens, in two launches
+//      per pass over the GPU beyond.
 //   2. Pieces of 32 consecutive sorted entries x 32 lanes of up to 16 bytes:
 //      each warp sums the runs of equal ids in its piece in float32.  A run
 //      inside the piece is a finished row of dW; one that crosses a piece
 //      boundary leaves its part in the workspace.  The work of a warp does not depend on
 //      how often a token occurs, so a frequent token costs no more than rare
-//      ones.  Further CTAs write the zero rows of the ids that do not occur.
+//      ones.  Further CTAs write the zero rows of the ids that a search in
+//      the sorted entries does not find.
 //   3. The parts of each crossing run are added in order.
 // dW is therefore written once (no clearing pass), there are no atomics on
 // floating-point data, and the order of every sum follows from the tokens alone.
@@ -124,88 +126,73 @@ struct SortArgs {
   const void *tok;
   int64_t N, V, pad;
   uint2 *pair[2];     // {key, position}
-  unsigned *seen;     // bitmap of the ids that occur
+  unsigned *counts;   // [CTAs][digits] of a pass (grid form)
   int passes, bits;
   int *status;
 };
 
-// A stable counting sort per pass.  Every warp owns a contiguous part of the
-// entries: it counts its digits, the counts are added up over warps, CTAs and
-// digits, and it then places its entries in order, so entries of one digit
+// One pass of a stable counting sort.  Every warp owns a contiguous part of
+// the entries: it counts its digits, the counts are added up over warps, CTAs
+// and digits, and it then places its entries in order, so entries of one digit
 // keep their order.  Ids out of range and the padding id sort as V, last.
-template <typename TOK>
-__global__ void __launch_bounds__(kSortThreads, 1) emb_sort_kernel(const SortArgs p) {
-  extern __shared__ __align__(16) unsigned sm[];
-  const int D = 1 << p.bits;
-  unsigned *hist = sm;                         // [warps][D]
-  unsigned *tot = hist + kSortWarps * D;       // [cluster][D], written by the cluster's CTAs
-  unsigned *base = tot + kSortCluster * D;     // [D]
-  __shared__ unsigned wsum[kSortWarps];
-  const int C = gridDim.x, rank = blockIdx.x;  // one cluster
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t per = (p.N + (int64_t)C * kSortThreads - 1) / ((int64_t)C * kSortThreads) * 32;
-  const int64_t lo = min(p.N, ((int64_t)rank * kSortWarps + warp) * per), hi = min(p.N, lo + per);
-  const int64_t words = (p.V + 31) / 32;
-  for (int64_t i = (int64_t)rank * kSortThreads + tid; i < words; i += (int64_t)C * kSortThreads) p.seen[i] = 0;
-  const TOK *tok = static_cast<const TOK *>(p.tok);
-  for (int pass = 0; pass < p.passes; ++pass) {
-    const int shift = pass * p.bits;
+template <typename TOK> struct Pass {
+  const SortArgs &p;
+  int pass, shift, D;
+  int lane, warp;
+  int64_t lo, hi;  // this warp's entries
+  HS_DEV Pass(const SortArgs &a, int pass_, int ctas, int rank)
+      : p(a), pass(pass_), shift(pass_ * a.bits), D(1 << a.bits), lane(threadIdx.x & 31), warp(threadIdx.x >> 5) {
+    const int64_t per = (p.N + (int64_t)ctas * kSortThreads - 1) / ((int64_t)ctas * kSortThreads) * 32;
+    lo = min(p.N, ((int64_t)rank * kSortWarps + warp) * per);
+    hi = min(p.N, lo + per);
+  }
+  // kAhead groups of 32 entries, all loads in flight at once
+  HS_DEV void load(uint2 (&e)[kAhead], int64_t b) const {
     const uint2 *src = p.pair[(pass + 1) & 1];
-    uint2 *dst = p.pair[pass & 1];
-    // kAhead groups of 32 entries, all loads in flight at once; V past the end
-    auto load = [&](uint2 (&e)[kAhead], int64_t b) {
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int64_t i = b + u * 32 + lane;
-        e[u] = {0u, 0u};
-        if (i < hi) {
-          if (pass) {
-            e[u] = __ldcg(src + i);
-          } else {
-            const int64_t t = (int64_t)tok[i];
-            const bool inside = t >= 0 && t < p.V;
-            if (!inside) set_status(p.status, HS_ERR_INDEX);
-            e[u] = {inside && t != p.pad ? (unsigned)t : (unsigned)p.V, (unsigned)i};
-          }
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t i = b + u * 32 + lane;
+      e[u] = {0u, 0u};
+      if (i < hi) {
+        if (pass) {
+          e[u] = __ldcg(src + i);
+        } else {
+          const int64_t t = (int64_t)static_cast<const TOK *>(p.tok)[i];
+          const bool inside = t >= 0 && t < p.V;
+          if (!inside) set_status(p.status, HS_ERR_INDEX);
+          e[u] = {inside && t != p.pad ? (unsigned)t : (unsigned)p.V, (unsigned)i};
         }
       }
-    };
-    unsigned *h = hist + warp * D;
-    for (int i = lane; i < D; i += 32) h[i] = 0;
-    __syncwarp();
+    }
+  }
+  HS_DEV unsigned digit(uint2 e) const { return (e.x >> shift) & (D - 1); }
+  // Whether the warp's entries are few enough to stay in registers from
+  // counting to placing.
+  HS_DEV bool once() const { return hi - lo <= 32 * kAhead; }
+  // adds this warp's digits to h; e: its last (or only) entries
+  HS_DEV void count(unsigned *h, uint2 (&e)[kAhead]) const {
     for (int64_t b = lo; b < hi; b += 32 * kAhead) {
-      uint2 e[kAhead];
       load(e, b);
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        if (b + u * 32 >= hi) break;
-        if (b + u * 32 + lane < hi) atomicAdd(h + ((e[u].x >> shift) & (D - 1)), 1u);
-      }
+      for (int u = 0; u < kAhead; ++u)
+        if (b + u * 32 + lane < hi) atomicAdd(h + digit(e[u]), 1u);
     }
-    if (pass == 0 && C > 1) cluster_sync_all();  // every CTA has started before its memory is written
-    __syncthreads();
-    if (tid < D) {  // over the warps of this CTA, then to every CTA
-      unsigned run = 0;
-      for (int w = 0; w < kSortWarps; ++w) {
-        const unsigned c = hist[w * D + tid];
-        hist[w * D + tid] = run;
-        run += c;
-      }
-      if (C == 1)
-        tot[tid] = run;
-      else
-        for (int r = 0; r < C; ++r) st_cluster_u32(tot + rank * D + tid, r, run);
+  }
+  // the counts of the warps, [kSortWarps][D], to those of the warps before; their sum
+  HS_DEV unsigned over_warps(unsigned *hist) const {
+    unsigned run = 0;
+#pragma unroll 8
+    for (int w = 0; w < kSortWarps; ++w) {
+      const unsigned c = hist[w * D + threadIdx.x];
+      hist[w * D + threadIdx.x] = run;
+      run += c;
     }
-    if (C > 1) cluster_sync_all(); else __syncthreads();
-    unsigned before = 0, all = 0;
-    if (tid < D) {
-      for (int r = 0; r < C; ++r) {
-        const unsigned c = tot[r * D + tid];
-        if (r < rank) before += c;
-        all += c;
-      }
-    }
-    unsigned inc = all;  // exclusive sums over the digits
+    return run;
+  }
+  // base[d]: the place of the CTA's first entry of digit d, from the thread's
+  // digit's counts in all CTAs and in those before this one.  Whole CTA.
+  HS_DEV void bases(unsigned *base, unsigned *wsum, unsigned all, unsigned before) const {
+    unsigned inc = all;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned v = __shfl_up_sync(0xffffffffu, inc, o);
@@ -213,22 +200,24 @@ __global__ void __launch_bounds__(kSortThreads, 1) emb_sort_kernel(const SortArg
     }
     if (lane == 31) wsum[warp] = inc;
     __syncthreads();
-    if (tid < D) {
+    if ((int)threadIdx.x < D) {
       unsigned less = 0;
       for (int w = 0; w < warp; ++w) less += wsum[w];
-      base[tid] = less + inc - all + before;
+      base[threadIdx.x] = less + inc - all + before;
     }
     __syncthreads();
+  }
+  HS_DEV void place(const unsigned *base, unsigned *h, uint2 (&e)[kAhead]) const {
+    uint2 *dst = p.pair[pass & 1];
     for (int64_t b = lo; b < hi; b += 32 * kAhead) {
-      uint2 e[kAhead];
-      load(e, b);
+      if (!once()) load(e, b);
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) {
         if (b + u * 32 >= hi) break;
         const bool ok = b + u * 32 + lane < hi;
-        const unsigned dig = (e[u].x >> shift) & (D - 1);
-        // the lanes of the same digit, by a vote on each of its bits (a match
-        // instruction in its place took three times as long)
+        const unsigned dig = digit(e[u]);
+        // the lanes of the same digit, by a vote on each of its bits (with a
+        // match instruction the whole sort took 82 us in place of 63)
         unsigned same = __ballot_sync(0xffffffffu, ok);
 #pragma unroll
         for (int bit = 0; bit < kMaxBits; ++bit) {
@@ -243,20 +232,102 @@ __global__ void __launch_bounds__(kSortThreads, 1) emb_sort_kernel(const SortArg
         if (ok) dst[at] = e[u];
       }
     }
+  }
+};
+
+// Few tokens: all passes in one launch of one cluster.
+template <typename TOK>
+__global__ void __launch_bounds__(kSortThreads, 1) emb_sort_kernel(const SortArgs p) {
+  extern __shared__ __align__(16) unsigned sm[];
+  __shared__ unsigned wsum[kSortWarps];
+  const int D = 1 << p.bits, C = gridDim.x, rank = blockIdx.x, tid = threadIdx.x;
+  unsigned *hist = sm;                         // [warps][D]
+  unsigned *tot = hist + kSortWarps * D;       // [cluster][D], written by the cluster's CTAs
+  unsigned *base = tot + kSortCluster * D;     // [D]
+  for (int pass = 0; pass < p.passes; ++pass) {
+    const Pass<TOK> q(p, pass, C, rank);
+    unsigned *h = hist + q.warp * D;
+    for (int i = q.lane; i < D; i += 32) h[i] = 0;
+    __syncwarp();
+    uint2 e[kAhead];
+    q.count(h, e);
+    if (pass == 0 && C > 1) cluster_sync_all();  // every CTA has started before its memory is written
+    __syncthreads();
+    if (tid < D) {
+      const unsigned n = q.over_warps(hist);
+      if (C == 1)
+        tot[tid] = n;
+      else
+        for (int r = 0; r < C; ++r) st_cluster_u32(tot + rank * D + tid, r, n);
+    }
+    if (C > 1) cluster_sync_all(); else __syncthreads();
+    unsigned before = 0, all = 0;
+    if (tid < D) {
+      for (int r = 0; r < C; ++r) {
+        const unsigned c = tot[r * D + tid];
+        if (r < rank) before += c;
+        all += c;
+      }
+    }
+    q.bases(base, wsum, all, before);
+    q.place(base, h, e);
     if (C > 1) cluster_sync_all(); else __syncthreads();
   }
-  const uint2 *sorted = p.pair[(p.passes + 1) & 1];
-#pragma unroll 4
-  for (int64_t i = lo + lane; i < hi; i += 32) {
-    const unsigned k = __ldcg(&sorted[i].x);
-    if (k < (unsigned)p.V && (i == 0 || __ldcg(&sorted[i - 1].x) != k)) atomicOr(p.seen + (k >> 5), 1u << (k & 31));
+}
+
+// Many tokens: two launches per pass over up to kSortCtas CTAs (placing
+// writes 32 separate sectors per warp, which binds a single cluster's SMs: 54 us
+// for 131072 tokens there).
+constexpr int kSortCtas = 64;
+
+template <typename TOK>
+__global__ void __launch_bounds__(kSortThreads, 1) emb_count_kernel(const SortArgs p, int pass) {
+  __shared__ unsigned h[1 << kMaxBits];
+  const Pass<TOK> q(p, pass, gridDim.x, blockIdx.x);
+  if ((int)threadIdx.x < q.D) h[threadIdx.x] = 0;
+  __syncthreads();
+  uint2 e[kAhead];
+  q.count(h, e);
+  __syncthreads();
+  if ((int)threadIdx.x < q.D) p.counts[blockIdx.x * q.D + threadIdx.x] = h[threadIdx.x];
+}
+template <typename TOK>
+__global__ void __launch_bounds__(kSortThreads, 1) emb_place_kernel(const SortArgs p, int pass) {
+  extern __shared__ __align__(16) unsigned sm[];
+  __shared__ unsigned wsum[kSortWarps], other[2][1 << kMaxBits];
+  const Pass<TOK> q(p, pass, gridDim.x, blockIdx.x);
+  unsigned *hist = sm, *base = hist + kSortWarps * q.D;
+  unsigned *h = hist + q.warp * q.D;
+  for (int i = q.lane; i < q.D; i += 32) h[i] = 0;
+  __syncwarp();
+  uint2 e[kAhead];
+  q.count(h, e);
+  // the counts of all CTAs and of those before this one, by two threads per
+  // digit (the digits are at most half the threads)
+  const int d = threadIdx.x & (q.D - 1), part = threadIdx.x / q.D, n = gridDim.x;
+  unsigned before = 0, all = 0;
+  if (part < 2) {
+    const int to = part ? n : n / 2;
+#pragma unroll 16
+    for (int r = part ? n / 2 : 0; r < to; ++r) {
+      const unsigned c = __ldcg(p.counts + r * q.D + d);
+      if (r < (int)blockIdx.x) before += c;
+      all += c;
+    }
+    if (part) other[0][d] = before, other[1][d] = all;
   }
+  __syncthreads();
+  if (part == 0) {
+    before += other[0][d], all += other[1][d];
+    q.over_warps(hist);
+  }
+  q.bases(base, wsum, part == 0 ? all : 0u, before);
+  q.place(base, h, e);
 }
 
 // ------------------------------------------------------------------ sums of runs
 struct SumArgs {
   const uint2 *pair;   // {key, position}, sorted
-  const unsigned *seen;
   const char *dout;
   char *dw;
   float *head, *tail;  // [pieces][D]: the part of a run that came in / goes on
@@ -275,10 +346,13 @@ __global__ void __launch_bounds__(256) emb_sum_kernel(const SumArgs p) {
   const int64_t row_bytes = p.D * (int64_t)sizeof(T);
   if ((int64_t)blockIdx.x >= p.sum_blocks) {
     // 32 ids per warp: rows of those that do not occur
-    const int64_t g = ((int64_t)blockIdx.x - p.sum_blocks) * 8 + warp;
-    if (g * 32 >= p.V) return;
-    unsigned none = ~p.seen[g];
-    if (g * 32 + 32 > p.V) none &= (1u << (p.V - g * 32)) - 1u;
+    const int64_t g = ((int64_t)blockIdx.x - p.sum_blocks) * 8 + warp, id = g * 32 + lane;
+    int64_t a = 0, b = p.N;  // first entry not below this lane's id
+    while (a < b) {
+      const int64_t m = (a + b) / 2;
+      if ((int64_t)p.pair[m].x < id) a = m + 1; else b = m;
+    }
+    unsigned none = __ballot_sync(0xffffffffu, id < p.V && (a == p.N || (int64_t)p.pair[a].x != id));
     const C zero = {};
     while (none) {
       const int r = __ffs(none) - 1;
@@ -348,7 +422,7 @@ __global__ void __launch_bounds__(256) emb_sum_kernel(const SumArgs p) {
 // A warp per piece whose last run goes on into the next piece and began in
 // this one: it adds the run's parts in order.  Runs over more than kLong
 // pieces are left to the whole CTA, each warp adding a contiguous share.
-constexpr int kJoinWarps = 8, kLong = 8;
+constexpr int kJoinWarps = 16, kLong = 16;
 
 template <typename T, int BYTES>
 __global__ void __launch_bounds__(32 * kJoinWarps) emb_join_kernel(const SumArgs p) {
@@ -367,7 +441,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) emb_join_kernel(const SumArgs
   __syncthreads();
   auto add_heads = [&](int64_t a, int64_t b, float *acc) {  // head parts of pieces a..b
     int64_t j = a;
-    constexpr int U = E > 4 ? 4 : 8;
+    constexpr int U = 8;
     for (; j + U <= b + 1; j += U) {
       float v[U][E];
 #pragma unroll
@@ -396,24 +470,33 @@ __global__ void __launch_bounds__(32 * kJoinWarps) emb_join_kernel(const SumArgs
     const bool began = p.pair[piece * kPiece].x != k || piece == 0 || p.pair[piece * kPiece - 1].x != k;
     if (crosses && began) {
       // the run's last piece: the last whose first entry is still k (the pieces
-      // of a run are consecutive)
-      auto starts_with = [&](int64_t j) { return j < p.pieces && p.pair[j * kPiece].x == k; };
-      const unsigned run = __ballot_sync(0xffffffffu, starts_with(piece + 1 + lane));
-      if (__popc(run) <= kLong) {
-        const int64_t last = piece + __popc(run);
+      // of a run are consecutive), by 32 probes at a time, further and further
+      // apart, then closer again
+      auto probe = [&](int64_t from, int64_t by) {  // how many of from, from + by, .. (32 of them)
+        const int64_t j = from + lane * by;
+        return __popc(__ballot_sync(0xffffffffu, j < p.pieces && p.pair[j * kPiece].x == k));
+      };
+      int64_t last = piece, by = 1;
+      int n = probe(piece + 1, 1);
+      last += n;
+      while (n == 32) {
+        by *= 32;
+        n = probe(last + by, by);
+        last += n * by;
+      }
+      while (by > 1) {
+        by /= 32;
+        last += probe(last + by, by) * by;
+      }
+      if (last - piece <= kLong) {
         float acc[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] = live ? p.tail[piece * p.D + (int64_t)chunk * E + e] : 0.f;
         add_heads(piece + 1, last, acc);
         write_row(k, acc);
       } else if (lane == 0) {
-        int64_t a = piece + __popc(run), b = run == 0xffffffffu ? p.pieces : a + 1;  // starts_with(a), not starts_with(b)
-        while (b - a > 1) {
-          const int64_t m = (a + b) / 2;
-          if (starts_with(m)) a = m; else b = m;
-        }
         long_first = piece;  // kJoinWarps <= kLong + 1 pieces hold the beginning of one such run at most
-        long_last = a;
+        long_last = last;
         long_key = k;
       }
     }
@@ -438,10 +521,13 @@ __global__ void __launch_bounds__(32 * kJoinWarps) emb_join_kernel(const SumArgs
 }
 
 // ------------------------------------------------------------------ host side
+// Tokens up to this many are sorted by one cluster.
+constexpr int64_t kClusterSort = 16384;
+
 struct Layout {
-  size_t pair[2], seen, head, tail, total;
+  size_t pair[2], counts, head, tail, total;
 };
-Layout layout(int64_t N, int64_t V, int64_t D) {
+Layout layout(int64_t N, int64_t D) {
   Layout l;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -450,7 +536,7 @@ Layout layout(int64_t N, int64_t V, int64_t D) {
     return o;
   };
   for (int i = 0; i < 2; ++i) l.pair[i] = take((size_t)N * sizeof(uint2));
-  l.seen = take((size_t)((V + 31) / 32) * 4);
+  l.counts = take(N > kClusterSort ? sizeof(unsigned) * kSortCtas << kMaxBits : 0);
   const size_t parts = (size_t)((N + kPiece - 1) / kPiece) * (size_t)D * sizeof(float);
   l.head = take(parts);
   l.tail = take(parts);
@@ -496,6 +582,39 @@ int check_ids(const char *who, int dtype, int token_bits, const void *tokens, in
   return HS_OK;
 }
 
+template <typename TOK> int sort(const SortArgs &s, cudaStream_t st) {
+  constexpr size_t kWord = sizeof(unsigned);
+  static std::atomic<unsigned long long> done{0}, done_place{0};
+  if (s.N > kClusterSort) {
+    const size_t smem = kWord * (kSortWarps + 1) << s.bits;
+    if (int e = allow_dynamic_smem((const void *)emb_place_kernel<TOK>, kWord * (kSortWarps + 1) << kMaxBits, &done_place)) return e;
+    const int ctas = (int)std::min<int64_t>(kSortCtas, (s.N + kSortThreads - 1) / kSortThreads);
+    for (int pass = 0; pass < s.passes; ++pass) {
+      emb_count_kernel<TOK><<<ctas, kSortThreads, 0, st>>>(s, pass);
+      if (int e = check_launch("emb_count_kernel")) return e;
+      emb_place_kernel<TOK><<<ctas, kSortThreads, smem, st>>>(s, pass);
+      if (int e = check_launch("emb_place_kernel")) return e;
+    }
+    return HS_OK;
+  }
+  if (int e = allow_dynamic_smem((const void *)emb_sort_kernel<TOK>, kWord * (kSortWarps + kSortCluster + 1) << kMaxBits, &done)) return e;
+  int cluster = 1;
+  while (cluster < kSortCluster && (int64_t)cluster * kSortThreads < s.N) cluster *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cluster);
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = kWord * (kSortWarps + kSortCluster + 1) << s.bits;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  (void)cudaLaunchKernelEx(&cfg, emb_sort_kernel<TOK>, s);
+  return check_launch("emb_sort_kernel");
+}
+
 }  // namespace
 }  // namespace hs
 
@@ -529,7 +648,7 @@ int hs_embedding_forward(int dtype, const void *weight, int64_t weight_ld, int t
 
 size_t hs_embedding_workspace_bytes(int64_t N, int64_t V, int64_t D) {
   if (N <= 0 || V <= 0 || D <= 0) return 0;
-  return hs::layout(N, V, D).total;
+  return hs::layout(N, D).total;
 }
 
 int hs_embedding_backward(int dtype, const void *dout, int token_bits, const void *tokens, int64_t padding_idx,
@@ -546,7 +665,7 @@ int hs_embedding_backward(int dtype, const void *dout, int token_bits, const voi
     const cudaError_t e = cudaMemsetAsync(dweight, 0, (size_t)V * D * es, st);
     return e == cudaSuccess ? HS_OK : fail(HS_ERR_CUDA, "hs_embedding_backward: %s", cudaGetErrorString(e));
   }
-  const Layout l = layout(N, V, D);
+  const Layout l = layout(N, D);
   if (!workspace || workspace_bytes < l.total || !aligned(workspace, 256))
     return fail(HS_ERR_WORKSPACE, "hs_embedding_backward: workspace %zu < %zu bytes, or not 256-byte aligned", workspace_bytes, l.total);
   char *ws = static_cast<char *>(workspace);
@@ -554,34 +673,15 @@ int hs_embedding_backward(int dtype, const void *dout, int token_bits, const voi
   SortArgs s = {};
   s.tok = tokens, s.N = N, s.V = V, s.pad = padding_idx, s.status = dev_status;
   for (int i = 0; i < 2; ++i) s.pair[i] = (uint2 *)(ws + l.pair[i]);
-  s.seen = (unsigned *)(ws + l.seen);
   int key_bits = 1;
   while ((V >> key_bits) != 0) ++key_bits;  // ids 0..V
   s.passes = (key_bits + kMaxBits - 1) / kMaxBits;
   s.bits = (key_bits + s.passes - 1) / s.passes;
-  int cluster = 1;
-  while (cluster < kSortCluster && (int64_t)cluster * kSortThreads < N) cluster *= 2;
-  const void *sort = token_bits == 64 ? (const void *)emb_sort_kernel<int64_t> : (const void *)emb_sort_kernel<int>;
-  static std::atomic<unsigned long long> done64{0}, done32{0};
-  if (int e = allow_dynamic_smem(sort, sizeof(unsigned) * (kSortWarps + kSortCluster + 1) << kMaxBits,
-                                 token_bits == 64 ? &done64 : &done32))
-    return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(cluster);
-  cfg.blockDim = dim3(kSortThreads);
-  cfg.dynamicSmemBytes = sizeof(unsigned) * (kSortWarps + kSortCluster + 1) << s.bits;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = cluster;
-  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  void *args[] = {&s};
-  if (cudaLaunchKernelExC(&cfg, sort, args) != cudaSuccess) return check_launch("emb_sort_kernel");
+  s.counts = (unsigned *)(ws + l.counts);
+  if (int e = token_bits == 64 ? sort<int64_t>(s, st) : sort<int>(s, st)) return e;
 
   SumArgs p = {};
-  p.pair = s.pair[(s.passes + 1) & 1], p.seen = s.seen;
+  p.pair = s.pair[(s.passes + 1) & 1];
   p.dout = (const char *)dout, p.dw = (char *)dweight;
   p.head = (float *)(ws + l.head), p.tail = (float *)(ws + l.tail);
   p.N = N, p.V = V, p.D = D, p.pieces = (N + kPiece - 1) / kPiece, p.scale = make_scale(scale);
