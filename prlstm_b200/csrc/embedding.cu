@@ -73,6 +73,32 @@ template <typename T, int BYTES> HS_DEV typename Chunk<BYTES>::type chunk_of_f32
   return c;
 }
 
+// E float32 of a part of a run, at a multiple of E (whole chunks divide a row).
+template <int E> HS_DEV void load_part(const float *p, float *v) {
+  if constexpr (E % 4 == 0) {
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      const float4 t = *reinterpret_cast<const float4 *>(p + e);
+      v[e] = t.x, v[e + 1] = t.y, v[e + 2] = t.z, v[e + 3] = t.w;
+    }
+  } else if constexpr (E == 2) {
+    const float2 t = *reinterpret_cast<const float2 *>(p);
+    v[0] = t.x, v[1] = t.y;
+  } else {
+    v[0] = *p;
+  }
+}
+template <int E> HS_DEV void store_part(float *p, const float *v) {
+  if constexpr (E % 4 == 0) {
+#pragma unroll
+    for (int e = 0; e < E; e += 4) *reinterpret_cast<float4 *>(p + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+  } else if constexpr (E == 2) {
+    *reinterpret_cast<float2 *>(p) = make_float2(v[0], v[1]);
+  } else {
+    *p = v[0];
+  }
+}
+
 // ------------------------------------------------------------------ lookup
 // One thread per row chunk and four chunks per thread, a CTA's width apart.
 template <typename T, int BYTES, typename TOK>
@@ -338,6 +364,20 @@ struct SumArgs {
   Scale scale;
 };
 
+// The first entry from `a` on with a key of at least `key` (N if none), by 32
+// probes at a time.  Whole warp.
+HS_DEV int64_t first_entry(const SumArgs &p, unsigned key, int64_t a, int lane) {
+  int64_t b = p.N;  // the answer lies in a..b
+  while (a < b) {
+    const int64_t by = (b - a + 31) / 32, j = a + (lane + 1) * by - 1;  // the last of each 32nd
+    const int below = __popc(__ballot_sync(0xffffffffu, j < b && p.pair[j].x < key));
+    const int64_t from = a + below * by;
+    b = min(b, from + by - 1);
+    a = min(from, b);
+  }
+  return a;
+}
+
 template <typename T, int BYTES>
 __global__ void __launch_bounds__(256) emb_sum_kernel(const SumArgs p) {
   using C = typename Chunk<BYTES>::type;
@@ -346,18 +386,28 @@ __global__ void __launch_bounds__(256) emb_sum_kernel(const SumArgs p) {
   const int64_t row_bytes = p.D * (int64_t)sizeof(T);
   if ((int64_t)blockIdx.x >= p.sum_blocks) {
     // 32 ids per warp: rows of those that do not occur
-    const int64_t g = ((int64_t)blockIdx.x - p.sum_blocks) * 8 + warp, id = g * 32 + lane;
-    int64_t a = 0, b = p.N;  // first entry not below this lane's id
-    while (a < b) {
-      const int64_t m = (a + b) / 2;
-      if ((int64_t)p.pair[m].x < id) a = m + 1; else b = m;
+    const int64_t first = (((int64_t)blockIdx.x - p.sum_blocks) * 8 + warp) * 32;
+    if (first >= p.V) return;
+    const unsigned end = (unsigned)min(p.V, first + 32);
+    unsigned none = 0xffffffffu >> (32 - (end - (unsigned)first));
+    const int64_t from = first_entry(p, (unsigned)first, 0, lane), to = first_entry(p, end, from, lane);
+    if (to - from <= 128) {
+      for (int64_t at = from + lane; at - lane < to; at += 32)
+        none &= ~__reduce_or_sync(0xffffffffu, at < to ? 1u << (p.pair[at].x - (unsigned)first) : 0u);
+    } else {  // frequent ids: each lane looks for its own
+      const unsigned id = (unsigned)first + lane;
+      int64_t a = from, b = to;
+      while (a < b) {
+        const int64_t m = (a + b) / 2;
+        if (p.pair[m].x < id) a = m + 1; else b = m;
+      }
+      none &= ~__ballot_sync(0xffffffffu, a < to && p.pair[a].x == id);
     }
-    unsigned none = __ballot_sync(0xffffffffu, id < p.V && (a == p.N || (int64_t)p.pair[a].x != id));
     const C zero = {};
     while (none) {
       const int r = __ffs(none) - 1;
       none &= none - 1;
-      C *row = reinterpret_cast<C *>(p.dw + (g * 32 + r) * row_bytes);
+      C *row = reinterpret_cast<C *>(p.dw + (first + r) * row_bytes);
       for (int c = lane; c < p.chunks; c += 32) row[c] = zero;
     }
     return;
@@ -400,9 +450,7 @@ __global__ void __launch_bounds__(256) emb_sum_kernel(const SumArgs p) {
         const bool goes_on = after == cur;
         if (live) {
           if (from_prev || goes_on) {
-            float *part = (from_prev ? p.head : p.tail) + piece * p.D + (int64_t)chunk * E;
-#pragma unroll
-            for (int e = 0; e < E; ++e) part[e] = acc[e];
+            store_part<E>((from_prev ? p.head : p.tail) + piece * p.D + (int64_t)chunk * E, acc);
           } else {
 #pragma unroll
             for (int e = 0; e < E; ++e) acc[e] = scaled(acc[e], p.scale);
@@ -439,23 +487,32 @@ __global__ void __launch_bounds__(32 * kJoinWarps) emb_join_kernel(const SumArgs
   const unsigned none = (unsigned)p.V;
   if (threadIdx.x == 0) long_first = -1;
   __syncthreads();
+  auto part = [&](const float *of, int64_t j, float *v) {
+    if (live) {
+      load_part<E>(of + j * p.D + (int64_t)chunk * E, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = 0.f;
+    }
+  };
   auto add_heads = [&](int64_t a, int64_t b, float *acc) {  // head parts of pieces a..b
     int64_t j = a;
     constexpr int U = 8;
     for (; j + U <= b + 1; j += U) {
       float v[U][E];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int e = 0; e < E; ++e) v[u][e] = live ? p.head[(j + u) * p.D + (int64_t)chunk * E + e] : 0.f;
+      for (int u = 0; u < U; ++u) part(p.head, j + u, v[u]);
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] += v[u][e];
     }
-    for (; j <= b; ++j)
+    for (; j <= b; ++j) {
+      float v[E];
+      part(p.head, j, v);
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += live ? p.head[j * p.D + (int64_t)chunk * E + e] : 0.f;
+      for (int e = 0; e < E; ++e) acc[e] += v[e];
+    }
   };
   auto write_row = [&](unsigned v, float *acc) {
     if (!live) return;
@@ -490,8 +547,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) emb_join_kernel(const SumArgs
       }
       if (last - piece <= kLong) {
         float acc[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] = live ? p.tail[piece * p.D + (int64_t)chunk * E + e] : 0.f;
+        part(p.tail, piece, acc);
         add_heads(piece + 1, last, acc);
         write_row(k, acc);
       } else if (lane == 0) {
@@ -507,7 +563,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps) emb_join_kernel(const SumArgs
   const int64_t a = long_first + 1 + warp * per, b = min(long_last, a + per - 1);
   float acc[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = warp == 0 && live ? p.tail[long_first * p.D + (int64_t)chunk * E + e] : 0.f;
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  if (warp == 0) part(p.tail, long_first, acc);
   add_heads(a, b, acc);
 #pragma unroll
   for (int e = 0; e < E; ++e) share[warp][e][lane] = acc[e];
