@@ -479,6 +479,9 @@ HS_API int hs_recurrent_backward_bf16(const float *x, const float *w_ih, const f
  * for all `void *` tensors of a call) and aligned to their element; all
  * arithmetic, states and sums are float32.  Extents may be 0.  Every result
  * has one fixed order of operations: the same bits from run to run.
+ * dev_status may also be a word of pinned host memory, which the host can then
+ * read as it is; where HS_ERR_INDEX may be written it should not be the word of
+ * the calls above, whose bounded waits give up at once on a nonzero one.
  * ---------------------------------------------------------------------- */
 enum { HS_F32 = 0, HS_BF16 = 1, HS_F16 = 2 };
 enum {

@@ -147,37 +147,68 @@ def call(name: str, *args):
     return rc
 
 
+_functions = {}
+
+
+def function(name: str):
+    """An entry point of the library, looked up once: called with plain ints,
+    it returns the status code (the calls whose host time counts)."""
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(load(), name)
+    return fn
+
+
+def raise_error(name: str, rc: int):
+    lib = load()
+    msg = lib.hs_last_error_message().decode(errors="replace")
+    raise RuntimeError(f"{name}: {lib.hs_status_string(rc).decode()}: {msg}")
+
+
 # ---------------------------------------------------------------- status word
 _status = {}
 _pending = {}
+_host_status = {}
 
 
-def _status_words(device: torch.device):
-    """Per device: both status words as one tensor, and each as a view.  The
-    first is for bounded waits that gave up (a nonzero one makes later waits
-    give up at once); the second for token ids out of range, which must not
-    disturb them."""
-    idx = device.index if device.index is not None else torch.cuda.current_device()
-    t = _status.get(idx)
-    if t is None:
-        both = torch.zeros(2, dtype=torch.int32, device=torch.device("cuda", idx))
-        t = _status[idx] = (both, both[:1], both[1:])
-    return t
+class HostStatus:
+    """Status words in pinned host memory, which the kernels write and the
+    host reads as plain memory, without a copy or a wait: ``timeout`` for bounded
+    waits, ``token`` for token ids out of range (apart from the device's own
+    word, where a nonzero value makes every later wait give up at once)."""
+
+    def __init__(self):
+        self.words = torch.zeros(2, dtype=torch.int32, pin_memory=True)
+        self.timeout_ptr = self.words.data_ptr()
+        self.token_ptr = self.timeout_ptr + 4
+        self.values = (ctypes.c_int32 * 2).from_address(self.timeout_ptr)
+
+    def check(self):
+        for code in self.values:
+            if code != HS_OK:
+                _raise_status(code)
+
+
+def host_status(index: int) -> HostStatus:
+    s = _host_status.get(index)
+    if s is None:
+        s = _host_status[index] = HostStatus()
+    return s
 
 
 def status_word(device: torch.device) -> torch.Tensor:
     """Per-device sticky device-status int the kernels report bounded-wait
     failures into."""
-    return _status_words(device)[1]
-
-
-def token_status_word(device: torch.device) -> torch.Tensor:
-    """Per-device sticky int the kernels report token ids out of range into."""
-    return _status_words(device)[2]
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    t = _status.get(idx)
+    if t is None:
+        t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+        _status[idx] = t
+    return t
 
 
 def note_launch(device: torch.device):
-    """Queue an asynchronous read-back of the status words; the values are
+    """Queue an asynchronous read-back of the status word; the value is
     checked (without a sync) the next time the library is called.  Skipped
     while the stream is being captured into a CUDA graph (an event query is
     not allowed there): a graphed step reports through check_device_status."""
@@ -185,8 +216,8 @@ def note_launch(device: torch.device):
         return
     idx = device.index if device.index is not None else torch.cuda.current_device()
     poll(device)
-    host = torch.empty(2, dtype=torch.int32, pin_memory=True)
-    host.copy_(_status_words(device)[0], non_blocking=True)
+    host = torch.empty(1, dtype=torch.int32, pin_memory=True)
+    host.copy_(status_word(device), non_blocking=True)
     ev = torch.cuda.Event()
     ev.record()
     _pending[idx] = (host, ev)
@@ -208,26 +239,30 @@ def poll(device: torch.device):
     host, ev = item
     if ev.query():
         del _pending[idx]
-        for code in host.tolist():
-            if code != HS_OK:
-                _raise_status(code)
+        if int(host.item()) != HS_OK:
+            _raise_status(int(host.item()))
 
 
 def check_device_status(device=None):
-    """Synchronously read the device status words; raise if a kernel gave up
+    """Synchronously read the device's status words; raise if a kernel gave up
     or met a token id out of range."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    for word in (status_word(device), token_status_word(device)):
-        out = ctypes.c_int(-1)
-        call("hs_read_status", ptr(word), ctypes.byref(out), stream_ptr(device))
-        if out.value != HS_OK:
-            _raise_status(out.value)
+    out = ctypes.c_int(-1)
+    call("hs_read_status", ptr(status_word(device)), ctypes.byref(out), stream_ptr(device))
+    if out.value != HS_OK:
+        _raise_status(out.value)
+    host = _host_status.get(device.index if device.index is not None else torch.cuda.current_device())
+    if host is not None:  # (the read above has waited for the stream)
+        host.check()
 
 
 def clear_device_status(device=None):
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    for word in (status_word(device), token_status_word(device)):
-        call("hs_clear_status", ptr(word), stream_ptr(device))
+    call("hs_clear_status", ptr(status_word(device)), stream_ptr(device))
+    host = _host_status.get(device.index if device.index is not None else torch.cuda.current_device())
+    if host is not None:
+        torch.cuda.current_stream(device).synchronize()
+        host.words.zero_()
     idx = device.index if device.index is not None else torch.cuda.current_device()
     _pending.pop(idx, None)
 

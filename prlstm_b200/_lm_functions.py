@@ -9,7 +9,6 @@ refused, as in ``HeadStartLSTM``.
 
 from __future__ import annotations
 
-import ctypes
 from typing import NamedTuple, Optional
 
 import torch
@@ -20,14 +19,16 @@ from . import _lib
 _CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _GATED, _LINEAR = 0, 1
 _MAX_TOP = 32
+_RUN = 16  # steps between the recurrence's saved states
+
+_raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream() without the Python object (2 us a call)
+_current_device = torch._C._cuda_getDevice
 
 
-def _code(who, t):
-    c = _CODE.get(t.dtype)
-    if c is None:
+def _refuse_dtype(who, t):
+    if t.dtype not in _CODE:
         raise TypeError(f"{who}: prlstm_b200 computes in float32; got dtype {t.dtype} "
                         "(use float32, bfloat16 or float16)")
-    return c
 
 
 def _same_device(who, first, *rest):
@@ -35,62 +36,64 @@ def _same_device(who, first, *rest):
         raise RuntimeError("prlstm_b200 runs on CUDA devices (B200, sm_100a) only; "
                            f"{who} got a tensor on {first.device}")
     for t in rest:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != first.get_device():
             raise RuntimeError(f"{who}: tensors on {first.device} and {t.device}")
 
 
-def _call(name, dev, *args):
-    """The library call on the current stream of `dev`, made with that device
-    current."""
-    if dev.index != torch.cuda.current_device():
-        with torch.cuda.device(dev):
-            return _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
-    return _lib.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
+def _call(name, index, *args):
+    """The library call on the current stream of device `index`, with that
+    device current."""
+    if index != _current_device():
+        with torch.cuda.device(index):
+            rc = _lib.function(name)(*args, _raw_stream(index))
+    else:
+        rc = _lib.function(name)(*args, _raw_stream(index))
+    if rc:
+        _lib.raise_error(name, rc)
 
 
 def _p(t):
     return None if t is None else t.data_ptr()
 
 
-def _wants_grad(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
-
-
 # ------------------------------------------------------------------ recurrence
 def _rows(t):
     """`t` with its last axis contiguous (a copy only where it is not)."""
-    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
 def _strides(t, batch_first):
     """Element strides of a step and of a sequence."""
+    if t is None:
+        return 0, 0
     s = t.stride()
     return (s[1], s[0]) if batch_first else (s[0], s[1])
 
 
+def _extents(z, batch_first):
+    """T, B, H."""
+    a, b, H = z.shape
+    return (b, a, H) if batch_first else (a, b, H)
+
+
 def _recurrence_forward(form, z, x, h0, starts, batch_first, keep, h_n=None):
     """(h, h_n, checkpoints) of checked arguments; z and x have contiguous rows."""
-    B, T = (z.shape[0], z.shape[1]) if batch_first else (z.shape[1], z.shape[0])
-    H, dev = z.shape[2], z.device
-    h = torch.empty(z.shape, dtype=z.dtype, device=dev)
+    T, B, H = _extents(z, batch_first)
+    index = z.get_device()
+    h = torch.empty_like(z) if H else torch.empty(z.shape, dtype=z.dtype, device=z.device)
     if h_n is None:
-        h_n = torch.empty(B, H, device=dev)
-    ckpt = None
-    if keep:
-        nbytes = _lib.load().hs_recurrence_checkpoint_bytes(T, B, H)
-        ckpt = torch.empty(nbytes // 4, device=dev)
-    zs, xs, hs = _strides(z, batch_first), _strides(x, batch_first), _strides(h, batch_first)
-    ss = (0, 0) if starts is None else _strides(starts, batch_first)
-    _call("hs_recurrence_forward", dev, _CODE[z.dtype], form, _p(z), *zs, _p(x), *xs, _p(h0), _p(starts), *ss,
-          _p(h), *hs, _p(h_n), _p(ckpt), T, B, H, _p(_lib.status_word(dev)))
+        h_n = torch.empty((B, H), device=z.device)
+    ckpt = torch.empty(-(-T // _RUN) * B * H, device=z.device) if keep else None
+    _call("hs_recurrence_forward", index, _CODE[z.dtype], form, z.data_ptr(), *_strides(z, batch_first), x.data_ptr(),
+          *_strides(x, batch_first), _p(h0), _p(starts), *_strides(starts, batch_first), h.data_ptr(),
+          *_strides(h, batch_first), h_n.data_ptr(), _p(ckpt), T, B, H, _lib.host_status(index).timeout_ptr)
     return h, h_n, ckpt
 
 
 class RecurrenceFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, z, x, h0, starts, form, batch_first):
-        h, h_n, ckpt = _recurrence_forward(form, z, x, None if h0 is None else h0.float().contiguous(), starts,
-                                           batch_first, True)
+        h, h_n, ckpt = _recurrence_forward(form, z, x, None if h0 is None else _state(h0), starts, batch_first, True)
         ctx.save_for_backward(z, x, starts, ckpt)
         ctx.h0_dtype = None if h0 is None else h0.dtype
         ctx.form, ctx.batch_first = form, batch_first
@@ -101,45 +104,47 @@ class RecurrenceFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dh, dh_n):
         z, x, starts, ckpt = ctx.saved_tensors
-        bf, dev = ctx.batch_first, z.device
-        B, T = (z.shape[0], z.shape[1]) if bf else (z.shape[1], z.shape[0])
-        H = z.shape[2]
+        bf, index = ctx.batch_first, z.get_device()
+        T, B, H = _extents(z, bf)
         dh = None if dh is None else _rows(dh)
-        dh_n = None if dh_n is None else dh_n.float().contiguous()
-        dz, dx = torch.empty(z.shape, dtype=z.dtype, device=dev), torch.empty(x.shape, dtype=x.dtype, device=dev)
-        dh0 = torch.empty(B, H, device=dev) if ctx.h0_dtype is not None and ctx.needs_input_grad[2] else None
-        gs = (0, 0) if dh is None else _strides(dh, bf)
-        ss = (0, 0) if starts is None else _strides(starts, bf)
-        _call("hs_recurrence_backward", dev, _CODE[z.dtype], ctx.form, _p(z), *_strides(z, bf), _p(x),
-              *_strides(x, bf), _p(ckpt), _p(starts), *ss, _p(dh), *gs, _p(dh_n), _p(dz), *_strides(dz, bf),
-              _p(dx), *_strides(dx, bf), _p(dh0), T, B, H, _p(_lib.status_word(dev)))
-        return dz, dx, None if dh0 is None else dh0.to(ctx.h0_dtype), None, None, None
+        dh_n = None if dh_n is None else _state(dh_n)
+        dz, dx = torch.empty_like(z), torch.empty_like(x)
+        dh0 = torch.empty((B, H), device=z.device) if ctx.h0_dtype is not None and ctx.needs_input_grad[2] else None
+        _call("hs_recurrence_backward", index, _CODE[z.dtype], ctx.form, z.data_ptr(), *_strides(z, bf), x.data_ptr(),
+              *_strides(x, bf), ckpt.data_ptr(), _p(starts), *_strides(starts, bf), _p(dh), *_strides(dh, bf), _p(dh_n),
+              dz.data_ptr(), *_strides(dz, bf), dx.data_ptr(), *_strides(dx, bf), _p(dh0), T, B, H,
+              _lib.host_status(index).timeout_ptr)
+        return dz, dx, dh0 if dh0 is None or ctx.h0_dtype is torch.float32 else dh0.to(ctx.h0_dtype), None, None, None
+
+
+def _state(t):
+    """A [B, H] state as the library takes it."""
+    return t if t.dtype is torch.float32 and t.is_contiguous() else t.float().contiguous()
 
 
 def _recurrence(who, form, z, x, h0, starts, batch_first):
-    _code(who, z)
+    _refuse_dtype(who, z)
     _same_device(who, z, x, h0, starts)
     if z.dim() != 3 or x.shape != z.shape:
         raise RuntimeError(f"{who}: both tensors must be [T, B, H] ([B, T, H] with batch_first); got "
                            f"{tuple(z.shape)} and {tuple(x.shape)}")
-    if x.dtype != z.dtype:
+    if x.dtype is not z.dtype:
         raise TypeError(f"{who}: tensors of {z.dtype} and {x.dtype}")
-    B, T = (z.shape[0], z.shape[1]) if batch_first else (z.shape[1], z.shape[0])
     if h0 is not None:
+        B, H = z.shape[0 if batch_first else 1], z.shape[2]
         if h0.dim() == 3 and h0.shape[0] == 1:
             h0 = h0.squeeze(0)
-        if h0.shape != (B, z.shape[2]):
-            raise RuntimeError(f"{who}: h0 must be [{B}, {z.shape[2]}]; got {tuple(h0.shape)}")
-        _code(who, h0)
-    if starts is not None:
-        if starts.shape != z.shape[:2] or starts.dtype not in (torch.bool, torch.uint8):
-            raise RuntimeError(f"{who}: starts must be a bool tensor of shape {tuple(z.shape[:2])}; got "
-                               f"{starts.dtype} {tuple(starts.shape)}")
+        if h0.shape != (B, H):
+            raise RuntimeError(f"{who}: h0 must be [{B}, {H}]; got {tuple(h0.shape)}")
+        _refuse_dtype(who, h0)
+    if starts is not None and (starts.shape != z.shape[:2] or starts.dtype not in (torch.bool, torch.uint8)):
+        raise RuntimeError(f"{who}: starts must be a bool tensor of shape {tuple(z.shape[:2])}; got "
+                           f"{starts.dtype} {tuple(starts.shape)}")
+    _lib.host_status(z.get_device()).check()
     z, x = _rows(z), _rows(x)
-    if _wants_grad(z, x, h0):
+    if torch.is_grad_enabled() and (z.requires_grad or x.requires_grad or (h0 is not None and h0.requires_grad)):
         return RecurrenceFn.apply(z, x, h0, starts, form, batch_first)
-    h0 = None if h0 is None else h0.float().contiguous()
-    h, h_n, _ = _recurrence_forward(form, z, x, h0, starts, batch_first, False)
+    h, h_n, _ = _recurrence_forward(form, z, x, None if h0 is None else _state(h0), starts, batch_first, False)
     return h, h_n
 
 
@@ -162,23 +167,29 @@ def linear_recurrence(a, b, h0=None, starts=None, batch_first: bool = False):
 
 
 def _step(who, form, z, x, h, out_state):
-    _code(who, z)
+    _refuse_dtype(who, z)
     _same_device(who, z, x, h, out_state)
     if z.dim() != 2 or x.shape != z.shape or h.shape != z.shape:
         raise RuntimeError(f"{who}: z, x and h must be [B, H]; got {tuple(z.shape)}, {tuple(x.shape)} and "
                            f"{tuple(h.shape)}")
-    if x.dtype != z.dtype:
+    if x.dtype is not z.dtype:
         raise TypeError(f"{who}: tensors of {z.dtype} and {x.dtype}")
-    if h.dtype != torch.float32:
+    if h.dtype is not torch.float32:
         raise TypeError(f"{who}: the state is float32; got {h.dtype}")
-    if out_state is not None and (out_state.dtype != torch.float32 or out_state.shape != h.shape
-                                  or not out_state.is_contiguous()):
-        raise RuntimeError(f"{who}: out_state must be a contiguous float32 [B, H] tensor")
-    if _wants_grad(z, x, h):
+    if torch.is_grad_enabled() and (z.requires_grad or x.requires_grad or h.requires_grad):
         raise RuntimeError(f"{who} is not differentiable; use the recurrence over [1, B, H], or torch.no_grad()")
-    out, state, _ = _recurrence_forward(form, _rows(z).unsqueeze(0), _rows(x).unsqueeze(0), h.contiguous(), None,
-                                        False, False, out_state)
-    return out[0], state
+    if out_state is None:
+        out_state = torch.empty(h.shape, device=h.device)
+    elif out_state.dtype is not torch.float32 or out_state.shape != h.shape or not out_state.is_contiguous():
+        raise RuntimeError(f"{who}: out_state must be a contiguous float32 [B, H] tensor")
+    z, x, h = _rows(z), _rows(x), h if h.is_contiguous() else h.contiguous()
+    out = torch.empty(z.shape, dtype=z.dtype, device=z.device)
+    index, (B, H) = z.get_device(), z.shape
+    status = _lib.host_status(index)
+    status.check()
+    _call("hs_recurrence_forward", index, _CODE[z.dtype], form, z.data_ptr(), 0, z.stride(0), x.data_ptr(), 0, x.stride(0),
+          h.data_ptr(), None, 0, 0, out.data_ptr(), 0, H, out_state.data_ptr(), None, 1, B, H, status.timeout_ptr)
+    return out, out_state
 
 
 def gated_recurrence_step(z, x, h, out_state=None):
@@ -195,41 +206,43 @@ def linear_recurrence_step(a, b, h, out_state=None):
 
 # ------------------------------------------------------------------ tokens
 def _tokens(who, tokens):
-    if tokens.dtype not in (torch.int64, torch.int32):
+    """(contiguous tokens, their bits)."""
+    bits = 64 if tokens.dtype is torch.int64 else 32 if tokens.dtype is torch.int32 else 0
+    if not bits:
         raise TypeError(f"{who}: tokens must be int64 or int32; got {tokens.dtype}")
-    return tokens if tokens.is_contiguous() else tokens.contiguous()
+    return tokens if tokens.is_contiguous() else tokens.contiguous(), bits
 
 
-def _embedding_forward(tokens, weight, scale):
-    (V, D), dev = weight.shape, weight.device
-    out = torch.empty(*tokens.shape, D, dtype=weight.dtype, device=dev)
-    _call("hs_embedding_forward", dev, _CODE[weight.dtype], _p(weight), weight.stride(0),
-          8 * tokens.element_size(), _p(tokens), scale, _p(out), tokens.numel(), V, D, _p(_lib.token_status_word(dev)))
+def _embedding_forward(tokens, bits, weight, scale):
+    V, D = weight.shape
+    index = weight.get_device()
+    out = torch.empty((*tokens.shape, D), dtype=weight.dtype, device=weight.device)
+    _call("hs_embedding_forward", index, _CODE[weight.dtype], weight.data_ptr(), weight.stride(0), bits,
+          tokens.data_ptr(), scale, out.data_ptr(), tokens.numel(), V, D, _lib.host_status(index).token_ptr)
     return out
 
 
 class EmbeddingFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, weight, tokens, scale, padding_idx):
-        _lib.poll(weight.device)
+    def forward(ctx, weight, tokens, bits, scale, padding_idx):
         ctx.save_for_backward(tokens)
         ctx.table = (weight.shape, weight.dtype)
-        ctx.scale, ctx.padding_idx = scale, padding_idx
-        return _embedding_forward(tokens, weight, scale)
+        ctx.args = (bits, scale, padding_idx)
+        return _embedding_forward(tokens, bits, weight, scale)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         (tokens,) = ctx.saved_tensors
         (V, D), dtype = ctx.table
-        dev, N = dout.device, tokens.numel()
-        dout = dout.contiguous()
-        dweight = torch.empty(V, D, dtype=dtype, device=dev)
-        ws = _lib.workspace(_lib.load().hs_embedding_workspace_bytes(N, V, D), dev)
-        _call("hs_embedding_backward", dev, _CODE[dtype], _p(dout), 8 * tokens.element_size(), _p(tokens),
-              ctx.padding_idx, ctx.scale, _p(dweight), N, V, D, _p(ws), ws.numel(), _p(_lib.token_status_word(dev)))
-        _lib.note_launch(dev)
-        return dweight, None, None, None
+        bits, scale, padding_idx = ctx.args
+        dev, index, N = dout.device, dout.get_device(), tokens.numel()
+        dout = dout if dout.is_contiguous() else dout.contiguous()
+        dweight = torch.empty((V, D), dtype=dtype, device=dev)
+        ws = _lib.workspace(_lib.function("hs_embedding_workspace_bytes")(N, V, D), dev)
+        _call("hs_embedding_backward", index, _CODE[dtype], dout.data_ptr(), bits, tokens.data_ptr(), padding_idx, scale,
+              dweight.data_ptr(), N, V, D, ws.data_ptr(), ws.numel(), _lib.host_status(index).token_ptr)
+        return dweight, None, None, None, None
 
 
 def embedding(tokens, weight, scale: float = 1.0, padding_idx: Optional[int] = None):
@@ -239,24 +252,26 @@ def embedding(tokens, weight, scale: float = 1.0, padding_idx: Optional[int] = N
     The gradient of ``weight`` sums each token's rows in float32, in the order
     of the tokens, and is the same bit for bit from run to run; the row
     ``padding_idx`` gets none.  An id outside [0, V) gives a row of zeros and is
-    reported by ``check_device_status()`` (and by a later training call)."""
+    reported by ``check_device_status()`` and by later calls, until
+    ``clear_device_status()``."""
     who = "embedding"
-    _code(who, weight)
+    _refuse_dtype(who, weight)
     _same_device(who, weight, tokens)
     if weight.dim() != 2:
         raise RuntimeError(f"{who}: weight must be [V, D]; got {tuple(weight.shape)}")
-    tokens = _tokens(who, tokens)
-    weight = _rows(weight)
-    if weight.stride(0) < weight.shape[1]:
+    tokens, bits = _tokens(who, tokens)
+    V, D = weight.shape
+    if weight.stride(0) < D or (D > 1 and weight.stride(1) != 1):
         weight = weight.contiguous()
     pad = -1
     if padding_idx is not None:
-        pad = int(padding_idx) + (weight.shape[0] if padding_idx < 0 else 0)
-        if not 0 <= pad < weight.shape[0]:
-            raise RuntimeError(f"{who}: padding_idx {padding_idx} is outside the table of {weight.shape[0]} rows")
-    if _wants_grad(weight):
-        return EmbeddingFn.apply(weight, tokens, float(scale), pad)
-    return _embedding_forward(tokens, weight, float(scale))
+        pad = padding_idx + (V if padding_idx < 0 else 0)
+        if not 0 <= pad < V:
+            raise RuntimeError(f"{who}: padding_idx {padding_idx} is outside the table of {V} rows")
+    _lib.host_status(weight.get_device()).check()
+    if weight.requires_grad and torch.is_grad_enabled():
+        return EmbeddingFn.apply(weight, tokens, bits, scale, pad)
+    return _embedding_forward(tokens, bits, weight, scale)
 
 
 class TokenLogprobs(NamedTuple):
@@ -268,27 +283,25 @@ class TokenLogprobs(NamedTuple):
     top_index: Optional[torch.Tensor]
 
 
-def _logprobs_forward(logits, tokens, top, temperature, ignore_index, keep):
+def _logprobs_forward(logits, tokens, bits, top, temperature, ignore_index, keep):
     N, V = logits.shape
-    dev = logits.device
-    both = torch.empty(2, N, device=dev)
-    logprob, entropy = both[0], both[1]
-    top_lp = torch.empty(N, top, device=dev) if top else None
-    top_id = torch.empty(N, top, dtype=torch.int64, device=dev) if top else None
-    stats = torch.empty(N, 2, device=dev) if keep else None
-    _call("hs_token_logprobs_forward", dev, _CODE[logits.dtype], _p(logits), logits.stride(0),
-          8 * tokens.element_size(), _p(tokens), ignore_index, temperature, top, _p(logprob), _p(entropy), _p(top_lp),
-          _p(top_id), _p(stats), N, V, _p(_lib.token_status_word(dev)))
+    dev, index = logits.device, logits.get_device()
+    logprob, entropy = torch.empty(N, device=dev), torch.empty(N, device=dev)
+    top_lp = torch.empty((N, top), device=dev) if top else None
+    top_id = torch.empty((N, top), dtype=torch.int64, device=dev) if top else None
+    stats = torch.empty((N, 2), device=dev) if keep else None
+    _call("hs_token_logprobs_forward", index, _CODE[logits.dtype], logits.data_ptr(), logits.stride(0), bits,
+          tokens.data_ptr(), ignore_index, temperature, top, logprob.data_ptr(), entropy.data_ptr(), _p(top_lp), _p(top_id),
+          _p(stats), N, V, _lib.host_status(index).token_ptr)
     return logprob, entropy, top_lp, top_id, stats
 
 
 class TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tokens, top, temperature, ignore_index):
-        _lib.poll(logits.device)
-        logprob, entropy, top_lp, top_id, stats = _logprobs_forward(logits, tokens, top, temperature, ignore_index, True)
+    def forward(ctx, logits, tokens, bits, top, temperature, ignore_index):
+        logprob, entropy, top_lp, top_id, stats = _logprobs_forward(logits, tokens, bits, top, temperature, ignore_index, True)
         ctx.save_for_backward(logits, tokens, entropy, top_id, stats)
-        ctx.args = (top, temperature, ignore_index)
+        ctx.args = (bits, top, temperature, ignore_index)
         ctx.set_materialize_grads(False)
         if top:
             ctx.mark_non_differentiable(top_id)
@@ -298,16 +311,14 @@ class TokenLogprobsFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dlogprob, dentropy, dtop, _dindex):
         logits, tokens, entropy, top_id, stats = ctx.saved_tensors
-        top, temperature, ignore_index = ctx.args
+        bits, top, temperature, ignore_index = ctx.args
         N, V = logits.shape
-        dev = logits.device
-        dlogprob, dentropy, dtop = (None if t is None else t.float().contiguous() for t in (dlogprob, dentropy, dtop))
-        dlogits = torch.empty(N, V, dtype=logits.dtype, device=dev)
-        _call("hs_token_logprobs_backward", dev, _CODE[logits.dtype], _p(logits), logits.stride(0),
-              8 * tokens.element_size(), _p(tokens), ignore_index, temperature, top, _p(stats), _p(entropy), _p(top_id),
-              _p(dlogprob), _p(dentropy), _p(dtop), _p(dlogits), V, N, V)
-        _lib.note_launch(dev)
-        return dlogits, None, None, None, None
+        dlogprob, dentropy, dtop = (None if t is None else _state(t) for t in (dlogprob, dentropy, dtop))
+        dlogits = torch.empty((N, V), dtype=logits.dtype, device=logits.device)
+        _call("hs_token_logprobs_backward", logits.get_device(), _CODE[logits.dtype], logits.data_ptr(), logits.stride(0),
+              bits, tokens.data_ptr(), ignore_index, temperature, top, stats.data_ptr(), entropy.data_ptr(), _p(top_id),
+              _p(dlogprob), _p(dentropy), _p(dtop), dlogits.data_ptr(), V, N, V)
+        return dlogits, None, None, None, None, None
 
 
 def token_logprobs(logits, tokens, top: int = 0, temperature: float = 1.0, ignore_index: int = -100) -> TokenLogprobs:
@@ -318,32 +329,34 @@ def token_logprobs(logits, tokens, top: int = 0, temperature: float = 1.0, ignor
     Differentiable in logits through ``logprob``, ``entropy`` and
     ``top_logprob``; ``-r.logprob.mean()`` is the cross-entropy loss.
     Alternatives are ordered by logit, equal logits by the lower index.  Rows
-    whose token is ``ignore_index`` are not read and give 0 (``top_index`` -1)
-    and no gradient.  Logits of -inf are masked out; a row with nothing left
+    whose token is ``ignore_index`` give 0 (``top_index`` -1) and no gradient,
+    whatever their logits.  Logits of -inf are masked out; a row with nothing left
     gives -inf, entropy 0 and no gradient; a row with a NaN or +inf gives NaN
     (``top_index`` -1).  A token outside [0, V) gives NaN and is reported by
-    ``check_device_status()``."""
+    ``check_device_status()`` and by later calls, until
+    ``clear_device_status()``."""
     who = "token_logprobs"
-    _code(who, logits)
+    _refuse_dtype(who, logits)
     _same_device(who, logits, tokens)
-    if logits.dim() < 1 or logits.shape[:-1] != tokens.shape:
-        raise RuntimeError(f"{who}: logits [..., V] and tokens [...] do not match: {tuple(logits.shape)} and "
-                           f"{tuple(tokens.shape)}")
+    shape = tokens.shape
+    if logits.dim() < 1 or logits.shape[:-1] != shape:
+        raise RuntimeError(f"{who}: logits [..., V] and tokens [...] do not match: {tuple(logits.shape)} and {tuple(shape)}")
     V = logits.shape[-1]
-    if not 0 <= top <= min(_MAX_TOP, V):
+    if not 0 <= top <= _MAX_TOP or top > V:
         raise RuntimeError(f"{who}: top must be in 0..{min(_MAX_TOP, V)}; got {top}")
     if not 1e-30 <= temperature <= 1e30:
         raise RuntimeError(f"{who}: the temperature must be positive (1e-30 to 1e30); got {temperature}")
-    shape = tokens.shape
-    tokens = _tokens(who, tokens).view(-1)
-    rows = logits if logits.dim() == 2 else logits.reshape(-1, V) if V else logits.reshape(tokens.numel(), 0)
-    rows = _rows(rows)
+    tokens, bits = _tokens(who, tokens)
+    if len(shape) != 1:
+        tokens, logits = tokens.view(-1), logits.reshape(tokens.numel(), V)
+    rows = _rows(logits)
     if rows.shape[0] > 1 and rows.stride(0) < V:
         rows = rows.contiguous()
-    if _wants_grad(rows):
-        lp, ent, top_lp, top_id = TokenLogprobsFn.apply(rows, tokens, int(top), float(temperature), int(ignore_index))
+    _lib.host_status(rows.get_device()).check()
+    if rows.requires_grad and torch.is_grad_enabled():
+        lp, ent, top_lp, top_id = TokenLogprobsFn.apply(rows, tokens, bits, top, temperature, ignore_index)
     else:
-        lp, ent, top_lp, top_id, _ = _logprobs_forward(rows, tokens, int(top), float(temperature), int(ignore_index), False)
+        lp, ent, top_lp, top_id, _ = _logprobs_forward(rows, tokens, bits, top, temperature, ignore_index, False)
     if len(shape) != 1:
         lp, ent = lp.view(shape), ent.view(shape)
         if top:

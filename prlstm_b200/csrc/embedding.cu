@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(256) emb_lookup_kernel(const char *w, int64_t 
         c[k] = *reinterpret_cast<const C *>(w + t * ld_bytes + (i - n * chunks) * BYTES);
       } else {
         c[k] = C{};
-        set_status(status, HS_ERR_INDEX);
+        report(status, HS_ERR_INDEX);
       }
     }
   }
@@ -185,7 +185,7 @@ template <typename TOK> struct Pass {
         } else {
           const int64_t t = (int64_t)static_cast<const TOK *>(p.tok)[i];
           const bool inside = t >= 0 && t < p.V;
-          if (!inside) set_status(p.status, HS_ERR_INDEX);
+          if (!inside) report(p.status, HS_ERR_INDEX);
           e[u] = {inside && t != p.pad ? (unsigned)t : (unsigned)p.V, (unsigned)i};
         }
       }

@@ -123,7 +123,7 @@ HS_DEV void mbar_wait(uint64_t *b, unsigned parity, int *status) {
     if ((++n & 63u) == 0) {
       if (ld_status(status) != 0) return;
       if (globaltimer() - t0 > kWaitLimitNs) {
-        set_status(status, HS_ERR_DEVICE_TIMEOUT);
+        report(status, HS_ERR_DEVICE_TIMEOUT);
         return;
       }
     }

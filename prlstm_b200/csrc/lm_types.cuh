@@ -13,6 +13,10 @@ namespace hs {
 inline bool dtype_ok(int dtype) { return dtype == HS_F32 || dtype == HS_BF16 || dtype == HS_F16; }
 inline size_t dtype_bytes(int dtype) { return dtype == HS_F32 ? 4 : 2; }
 
+// Records a failure in a status word that may lie in pinned host memory (a
+// call writes one code only, so a plain store will do).
+HS_DEV void report(int *p, int code) { *reinterpret_cast<volatile int *>(p) = code; }
+
 template <typename T> HS_DEV float to_f32(T v);
 template <> HS_DEV float to_f32<float>(float v) { return v; }
 template <> HS_DEV float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }

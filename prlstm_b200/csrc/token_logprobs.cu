@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(threads_of<W>(), 1024 / threads_of<W>()) logpr
       p.lp[n] = logp(to_f32<T>(row[tok]));
     } else {
       p.lp[n] = __int_as_float(0x7fc00000);
-      set_status(p.status, HS_ERR_INDEX);
+      report(p.status, HS_ERR_INDEX);
     }
     if (p.ent) p.ent[n] = empty ? 0.f : kLn2 * ls - p.inv_t * (a.u / a.s);
     if (p.stats) {

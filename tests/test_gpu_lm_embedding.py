@@ -127,9 +127,9 @@ def test_ids_out_of_range_are_reported_and_harmless():
         # the recurrent layers' own waits are not cut short by it
         m = P.HeadStartLSTM(8, 32, parallel=True).to(DEV)
         x = torch.randn(64, 2, 8, device=DEV)
-        with pytest.raises(RuntimeError, match="token id"):
-            m(x)  # the training step above is reported once
         y = m(x)[0]
+        with pytest.raises(RuntimeError, match="token id"):
+            op(tok[:1], w)  # reported until it is cleared
     finally:
         P.clear_device_status()
     assert torch.allclose(y, m(x)[0], rtol=1e-5, atol=1e-6)
