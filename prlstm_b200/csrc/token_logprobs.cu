@@ -175,15 +175,26 @@ HS_DEV int64_t token_at(const void *tok, int token64, int64_t n) {
   return token64 ? static_cast<const int64_t *>(tok)[n] : (int64_t)static_cast<const int *>(tok)[n];
 }
 
-// The largest of a 16-byte vector's values, NaN left out.
-template <typename T> HS_DEV float vec_max(const uint4 &q) {
+// The largest of U 16-byte vectors' values, NaN left out.
+template <typename T, int U> HS_DEV float vec_max(const uint4 (&q)[U]) {
   if constexpr (sizeof(T) == 4) {
-    return fmaxf(fmaxf(__uint_as_float(q.x), __uint_as_float(q.y)), fmaxf(__uint_as_float(q.z), __uint_as_float(q.w)));
+    float m = kNegInf;
+#pragma unroll
+    for (int j = 0; j < U; ++j)
+      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(q[j].x), __uint_as_float(q[j].y)), fmaxf(__uint_as_float(q[j].z), __uint_as_float(q[j].w))));
+    return m;
   } else {
+    unsigned w = minus_inf_word<T>();
+#pragma unroll
+    for (int j = 0; j < U; ++j) w = word_max<T>(w, word_max<T>(word_max<T>(q[j].x, q[j].y), word_max<T>(q[j].z, q[j].w)));
     float v[2];
-    unpack_word<T>(word_max<T>(word_max<T>(q.x, q.y), word_max<T>(q.z, q.w)), v);
+    unpack_word<T>(w, v);
     return fmaxf(v[0], v[1]);
   }
+}
+template <typename T> HS_DEV float vec_max(const uint4 &q) {
+  const uint4 one[1] = {q};
+  return vec_max<T, 1>(one);
 }
 
 // What a thread knows of its values.  S and U are kept as two partial sums
@@ -226,9 +237,7 @@ template <typename T> struct Scan {
   }
   template <int U> HS_DEV void vectors(const uint4 (&q)[U], Scale k) {
     constexpr int E = Row<T>::E;
-    float bm = kNegInf;
-#pragma unroll
-    for (int j = 0; j < U; ++j) bm = fmaxf(bm, vec_max<T>(q[j]));
+    const float bm = vec_max<T, U>(q);
     if (bm > m) raise(bm, k);
     const Cols<2> minus = Cols<2>::all(-rel(m));
 #pragma unroll
@@ -253,7 +262,7 @@ struct Finder {
 template <int W, bool TOP> struct Shared {
   Finder f[TOP && W == 1 ? kShortRows : 1];
   Stat stat[W];
-  unsigned lowest[W];
+  unsigned group[32];
   Key list[TOP && W > 1 ? W : 1][32];
   Stat cstat[kMaxCluster];  // written by the cluster's CTAs
   Key clist[TOP ? kMaxCluster : 1][32];
@@ -305,6 +314,9 @@ __global__ void __launch_bounds__(threads_of<W>(), 1024 / threads_of<W>()) logpr
     return;
   }
   if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  const bool inside = tok >= 0 && tok < p.V;
+  // the token's logit, loaded before the row: it is there when it is needed
+  const float given = tid == 0 && rank == 0 && inside ? to_f32<T>(row[tok]) : 0.f;
   const Row<T> r(row, p.V, rank, C);
   Scan<T> scan;
   if (tid < r.head) scan.scalar(to_f32<T>(row[tid]), p.k);
@@ -345,20 +357,28 @@ __global__ void __launch_bounds__(threads_of<W>(), 1024 / threads_of<W>()) logpr
     if (tid == 0) f.nfound = f.nchosen = 0;
     const bool some = tid < r.head || r.lo + tid < r.hi || tid < r.ntail;  // this thread holds values
     const unsigned mine = some ? order_bits(scan.m) : 0;
-    // a bound that at least `top` threads reach, and not many more
-    const unsigned least = __reduce_min_sync(0xffffffffu, some ? mine : 0xffffffffu);
-    unsigned lo = least, hi = order_bits(a.m);
-    if (W > 1) {
-      if (lane == 0) sh.lowest[warp] = least;
-      __syncthreads();
+    // A bound that at least `top` threads reach, and not many more: the top-th
+    // largest of the maxima of 32 groups of threads, raised by bisection where
+    // more than a few too many reach it (large `top`, equal values).
+    unsigned v = mine;
 #pragma unroll
-      for (int w = 0; w < W; ++w) {
-        lo = min(lo, sh.lowest[w]);
-        hi = max(hi, order_bits(sh.stat[w].m));
-      }
+    for (int o = 1; o < W; o <<= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (W > 1) {
+      if (lane % W == 0) sh.group[(warp * 32 + lane) / W] = v;
+      __syncthreads();
+      v = sh.group[lane];
     }
+    int above = 0;
+#pragma unroll 8
+    for (int o = 0; o < 32; ++o) {
+      const unsigned w = __shfl_sync(0xffffffffu, v, o);
+      above += w > v || (w == v && o < lane);
+    }
+    unsigned lo = __shfl_sync(0xffffffffu, v, __ffs(__ballot_sync(0xffffffffu, above == p.top - 1)) - 1);
+    unsigned hi = __reduce_max_sync(0xffffffffu, v);
+    if (lo == 0) lo = 1;  // some groups hold nothing
     hi += 1;
-    int c = row_count<W>(mine >= lo && some);
+    int c = row_count<W>(mine >= lo);
     while (c > p.top + 8 && hi - lo > 1) {
       const unsigned mid = lo + (hi - lo) / 2;
       const int n = row_count<W>(mine >= mid);
@@ -463,8 +483,8 @@ __global__ void __launch_bounds__(threads_of<W>(), 1024 / threads_of<W>()) logpr
   const float ls = log2f(a.s);
   auto logp = [&](float x) { return empty ? kNegInf : bad ? a.s : fmaf(x - a.m, p.inv_t, -kLn2 * ls); };
   if (lane == 0) {
-    if (tok >= 0 && tok < p.V) {
-      p.lp[n] = logp(to_f32<T>(row[tok]));
+    if (inside) {
+      p.lp[n] = logp(given);
     } else {
       p.lp[n] = __int_as_float(0x7fc00000);
       report(p.status, HS_ERR_INDEX);
