@@ -160,6 +160,23 @@ def test_optional_inputs_and_gradients(form):
         check_all(got, want, memory, f"{form} {d is None} {dn is None}")
 
 
+def test_broadcast_inputs_and_a_second_backward():
+    """Gates shared by all sequences and a state shared by all columns come in
+    as expanded tensors; their gradients are the sums.  The graph can be walked twice."""
+    T, B, H = 37, 4, 48
+    a, b, h0, s, dh, dh_n = make(T, B, H, torch.float32, "gated", seed=23)
+    a, h0 = a[:, :1], h0[:, :1]
+    want, memory = truth(a.expand(T, B, H), b, h0.expand(B, H), None, dh, dh_n, "gated")
+    z, x, start = (t.to(DEV).requires_grad_(True) for t in (a, b, h0))
+    h, h_n = call("gated")(z.expand(T, B, H), x, start.expand(B, H))
+    check(h.detach(), want["h"], memory, "h")
+    for n in (1, 2):
+        torch.autograd.backward((h, h_n), (dh.to(DEV), dh_n.to(DEV)), retain_graph=True)
+        check(z.grad / n, want["da"].sum(1, keepdim=True), 2 * memory, "da")
+        check(x.grad / n, want["db"], memory, "db")
+        check(start.grad / n, want["dh0"].sum(1, keepdim=True), 2 * memory, "dh0")
+
+
 def test_empty_extents():
     for T, B, H in ((0, 3, 8), (4, 0, 8), (4, 3, 0), (0, 0, 0)):
         z = torch.randn(T, B, H, device=DEV, requires_grad=True)
