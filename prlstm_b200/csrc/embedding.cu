@@ -28,6 +28,7 @@ namespace hs {
 namespace {
 
 constexpr int kPiece = 32;        // sorted entries per warp of the summing kernel
+constexpr int kZeroIds = 8;       // ids per warp that writes zero rows
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortCluster = 8;   // CTAs of the sorting cluster at most
@@ -364,18 +365,29 @@ struct SumArgs {
   Scale scale;
 };
 
-// The first entry from `a` on with a key of at least `key` (N if none), by 32
-// probes at a time.  Whole warp.
-HS_DEV int64_t first_entry(const SumArgs &p, unsigned key, int64_t a, int lane) {
-  int64_t b = p.N;  // the answer lies in a..b
-  while (a < b) {
-    const int64_t by = (b - a + 31) / 32, j = a + (lane + 1) * by - 1;  // the last of each 32nd
-    const int below = __popc(__ballot_sync(0xffffffffu, j < b && p.pair[j].x < key));
-    const int64_t from = a + below * by;
-    b = min(b, from + by - 1);
-    a = min(from, b);
+// The first entries with keys of at least key[0] and key[1] (N if none), by 32
+// probes for each at a time.  Whole warp.
+HS_DEV void first_entries(const SumArgs &p, const unsigned (&key)[2], int lane, int64_t (&a)[2]) {
+  int64_t b[2] = {p.N, p.N};  // the answers lie in a..b
+  a[0] = a[1] = 0;
+  while (a[0] < b[0] || a[1] < b[1]) {
+    int64_t by[2];
+    bool under[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      by[i] = (b[i] - a[i] + 31) / 32;
+      const int64_t j = a[i] + (lane + 1) * by[i] - 1;  // the last of each 32nd
+      under[i] = j < b[i] && p.pair[j].x < key[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int below = __popc(__ballot_sync(0xffffffffu, under[i]));
+      if (a[i] >= b[i]) continue;
+      const int64_t from = a[i] + below * by[i];
+      b[i] = min(b[i], from + by[i] - 1);
+      a[i] = min(from, b[i]);
+    }
   }
-  return a;
 }
 
 template <typename T, int BYTES>
@@ -385,23 +397,24 @@ __global__ void __launch_bounds__(256) emb_sum_kernel(const SumArgs p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row_bytes = p.D * (int64_t)sizeof(T);
   if ((int64_t)blockIdx.x >= p.sum_blocks) {
-    // 32 ids per warp: rows of those that do not occur
-    const int64_t first = (((int64_t)blockIdx.x - p.sum_blocks) * 8 + warp) * 32;
+    // a few ids per warp: rows of those that do not occur
+    const int64_t first = (((int64_t)blockIdx.x - p.sum_blocks) * 8 + warp) * kZeroIds;
     if (first >= p.V) return;
-    const unsigned end = (unsigned)min(p.V, first + 32);
-    unsigned none = 0xffffffffu >> (32 - (end - (unsigned)first));
-    const int64_t from = first_entry(p, (unsigned)first, 0, lane), to = first_entry(p, end, from, lane);
-    if (to - from <= 128) {
-      for (int64_t at = from + lane; at - lane < to; at += 32)
-        none &= ~__reduce_or_sync(0xffffffffu, at < to ? 1u << (p.pair[at].x - (unsigned)first) : 0u);
-    } else {  // frequent ids: each lane looks for its own
+    const unsigned end = (unsigned)min(p.V, first + kZeroIds);
+    unsigned none = (1u << (end - (unsigned)first)) - 1u;
+    int64_t at[2];
+    first_entries(p, {(unsigned)first, end}, lane, at);
+    if (at[1] - at[0] <= 128) {
+      for (int64_t i = at[0] + lane; i - lane < at[1]; i += 32)
+        none &= ~__reduce_or_sync(0xffffffffu, i < at[1] ? 1u << (p.pair[i].x - (unsigned)first) : 0u);
+    } else {  // frequent ids: a lane looks for each
       const unsigned id = (unsigned)first + lane;
-      int64_t a = from, b = to;
+      int64_t a = at[0], b = at[1];
       while (a < b) {
         const int64_t m = (a + b) / 2;
         if (p.pair[m].x < id) a = m + 1; else b = m;
       }
-      none &= ~__ballot_sync(0xffffffffu, a < to && p.pair[a].x == id);
+      none &= ~__ballot_sync(0xffffffffu, a < at[1] && p.pair[a].x == id);
     }
     const C zero = {};
     while (none) {
@@ -745,7 +758,7 @@ int hs_embedding_backward(int dtype, const void *dout, int token_bits, const voi
   const int bytes = chunk_bytes(D * (int64_t)es, {dout, dweight}, 0, es);
   const int64_t chunks = D * (int64_t)es / bytes, slices = (chunks + 31) / 32;
   p.sum_blocks = (p.pieces * slices + 7) / 8;
-  const int64_t zero_blocks = (V + 255) / 256, join_blocks = (p.pieces + kJoinWarps - 1) / kJoinWarps * slices;
+  const int64_t zero_blocks = (V + 8 * kZeroIds - 1) / (8 * kZeroIds), join_blocks = (p.pieces + kJoinWarps - 1) / kJoinWarps * slices;
   if (chunks > 0x7fffffff || p.sum_blocks + zero_blocks > 0x7fffffff || join_blocks > 0x7fffffff)
     return fail(HS_ERR_UNSUPPORTED, "hs_embedding_backward: N * D is too large");
   p.chunks = (int)chunks, p.slices = (int)slices;
