@@ -173,20 +173,21 @@ _host_status = {}
 
 class HostStatus:
     """Status words in pinned host memory, which the kernels write and the
-    host reads as plain memory, without a copy or a wait: ``timeout`` for bounded
-    waits, ``token`` for token ids out of range (apart from the device's own
+    host reads as plain memory, without a copy or a wait: one for bounded waits
+    that gave up, one for token ids out of range (apart from the device's own
     word, where a nonzero value makes every later wait give up at once)."""
 
     def __init__(self):
         self.words = torch.zeros(2, dtype=torch.int32, pin_memory=True)
         self.timeout_ptr = self.words.data_ptr()
         self.token_ptr = self.timeout_ptr + 4
-        self.values = (ctypes.c_int32 * 2).from_address(self.timeout_ptr)
+        self.both = ctypes.c_int64.from_address(self.timeout_ptr)  # both words in one read
 
     def check(self):
-        for code in self.values:
-            if code != HS_OK:
-                _raise_status(code)
+        if self.both.value:
+            for code in self.words.tolist():
+                if code != HS_OK:
+                    _raise_status(code)
 
 
 def host_status(index: int) -> HostStatus:

@@ -25,19 +25,24 @@ _raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream() without the
 _current_device = torch._C._cuda_getDevice
 
 
-def _refuse_dtype(who, t):
-    if t.dtype not in _CODE:
+def _dtype_code(who, t):
+    code = _CODE.get(t.dtype)
+    if code is None:
         raise TypeError(f"{who}: prlstm_b200 computes in float32; got dtype {t.dtype} "
                         "(use float32, bfloat16 or float16)")
+    return code
 
 
-def _same_device(who, first, *rest):
-    if not first.is_cuda:
+def _device_index(who, first, *rest):
+    """The index of the CUDA device that all tensors are on."""
+    index = first.get_device()
+    if index < 0:
         raise RuntimeError("prlstm_b200 runs on CUDA devices (B200, sm_100a) only; "
                            f"{who} got a tensor on {first.device}")
     for t in rest:
-        if t is not None and t.get_device() != first.get_device():
+        if t is not None and t.get_device() != index:
             raise RuntimeError(f"{who}: tensors on {first.device} and {t.device}")
+    return index
 
 
 def _call(name, index, *args):
@@ -62,12 +67,13 @@ def _rows(t):
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
-def _strides(t, batch_first):
-    """Element strides of a step and of a sequence."""
+def _tensor(t, batch_first):
+    """Address and element strides of a step and of a sequence, as the library
+    takes a [T, B, ..] tensor (or none)."""
     if t is None:
-        return 0, 0
-    s = t.stride()
-    return (s[1], s[0]) if batch_first else (s[0], s[1])
+        return None, 0, 0
+    a, b = t.stride()[:2]
+    return (t.data_ptr(), b, a) if batch_first else (t.data_ptr(), a, b)
 
 
 def _extents(z, batch_first):
@@ -76,27 +82,25 @@ def _extents(z, batch_first):
     return (b, a, H) if batch_first else (a, b, H)
 
 
-def _recurrence_forward(form, z, x, h0, starts, batch_first, keep, h_n=None):
+def _recurrence_forward(code, index, form, z, x, h0, starts, batch_first, keep):
     """(h, h_n, checkpoints) of checked arguments; z and x have contiguous rows."""
     T, B, H = _extents(z, batch_first)
-    index = z.get_device()
-    h = torch.empty_like(z) if H else torch.empty(z.shape, dtype=z.dtype, device=z.device)
-    if h_n is None:
-        h_n = torch.empty((B, H), device=z.device)
+    h = torch.empty_like(z)
+    h_n = torch.empty((B, H), device=z.device) if h0 is None else torch.empty_like(h0)
     ckpt = torch.empty(-(-T // _RUN) * B * H, device=z.device) if keep else None
-    _call("hs_recurrence_forward", index, _CODE[z.dtype], form, z.data_ptr(), *_strides(z, batch_first), x.data_ptr(),
-          *_strides(x, batch_first), _p(h0), _p(starts), *_strides(starts, batch_first), h.data_ptr(),
-          *_strides(h, batch_first), h_n.data_ptr(), _p(ckpt), T, B, H, _lib.host_status(index).timeout_ptr)
+    _call("hs_recurrence_forward", index, code, form, *_tensor(z, batch_first), *_tensor(x, batch_first), _p(h0),
+          *_tensor(starts, batch_first), *_tensor(h, batch_first), h_n.data_ptr(), _p(ckpt), T, B, H,
+          _lib.host_status(index).timeout_ptr)
     return h, h_n, ckpt
 
 
 class RecurrenceFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, z, x, h0, starts, form, batch_first):
-        h, h_n, ckpt = _recurrence_forward(form, z, x, None if h0 is None else _state(h0), starts, batch_first, True)
+    def forward(ctx, z, x, h0, starts, code, index, form, batch_first):
+        h, h_n, ckpt = _recurrence_forward(code, index, form, z, x, None if h0 is None else _state(h0), starts, batch_first,
+                                           True)
         ctx.save_for_backward(z, x, starts, ckpt)
-        ctx.h0_dtype = None if h0 is None else h0.dtype
-        ctx.form, ctx.batch_first = form, batch_first
+        ctx.args = (code, index, form, batch_first, None if h0 is None else h0.dtype)
         ctx.set_materialize_grads(False)
         return h, h_n
 
@@ -104,17 +108,18 @@ class RecurrenceFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dh, dh_n):
         z, x, starts, ckpt = ctx.saved_tensors
-        bf, index = ctx.batch_first, z.get_device()
+        code, index, form, bf, h0_dtype = ctx.args
         T, B, H = _extents(z, bf)
         dh = None if dh is None else _rows(dh)
         dh_n = None if dh_n is None else _state(dh_n)
         dz, dx = torch.empty_like(z), torch.empty_like(x)
-        dh0 = torch.empty((B, H), device=z.device) if ctx.h0_dtype is not None and ctx.needs_input_grad[2] else None
-        _call("hs_recurrence_backward", index, _CODE[z.dtype], ctx.form, z.data_ptr(), *_strides(z, bf), x.data_ptr(),
-              *_strides(x, bf), ckpt.data_ptr(), _p(starts), *_strides(starts, bf), _p(dh), *_strides(dh, bf), _p(dh_n),
-              dz.data_ptr(), *_strides(dz, bf), dx.data_ptr(), *_strides(dx, bf), _p(dh0), T, B, H,
+        dh0 = torch.empty((B, H), device=z.device) if h0_dtype is not None and ctx.needs_input_grad[2] else None
+        _call("hs_recurrence_backward", index, code, form, *_tensor(z, bf), *_tensor(x, bf), ckpt.data_ptr(),
+              *_tensor(starts, bf), *_tensor(dh, bf), _p(dh_n), *_tensor(dz, bf), *_tensor(dx, bf), _p(dh0), T, B, H,
               _lib.host_status(index).timeout_ptr)
-        return dz, dx, dh0 if dh0 is None or ctx.h0_dtype is torch.float32 else dh0.to(ctx.h0_dtype), None, None, None
+        if dh0 is not None and h0_dtype is not torch.float32:
+            dh0 = dh0.to(h0_dtype)
+        return dz, dx, dh0, None, None, None, None, None
 
 
 def _state(t):
@@ -123,29 +128,27 @@ def _state(t):
 
 
 def _recurrence(who, form, z, x, h0, starts, batch_first):
-    _refuse_dtype(who, z)
-    _same_device(who, z, x, h0, starts)
-    if z.dim() != 3 or x.shape != z.shape:
+    code, index = _dtype_code(who, z), _device_index(who, z, x, h0, starts)
+    shape = z.shape
+    if len(shape) != 3 or x.shape != shape:
         raise RuntimeError(f"{who}: both tensors must be [T, B, H] ([B, T, H] with batch_first); got "
-                           f"{tuple(z.shape)} and {tuple(x.shape)}")
+                           f"{tuple(shape)} and {tuple(x.shape)}")
     if x.dtype is not z.dtype:
         raise TypeError(f"{who}: tensors of {z.dtype} and {x.dtype}")
     if h0 is not None:
-        B, H = z.shape[0 if batch_first else 1], z.shape[2]
         if h0.dim() == 3 and h0.shape[0] == 1:
             h0 = h0.squeeze(0)
-        if h0.shape != (B, H):
-            raise RuntimeError(f"{who}: h0 must be [{B}, {H}]; got {tuple(h0.shape)}")
-        _refuse_dtype(who, h0)
-    if starts is not None and (starts.shape != z.shape[:2] or starts.dtype not in (torch.bool, torch.uint8)):
-        raise RuntimeError(f"{who}: starts must be a bool tensor of shape {tuple(z.shape[:2])}; got "
+        if h0.shape != (shape[0 if batch_first else 1], shape[2]):
+            raise RuntimeError(f"{who}: h0 must be [{shape[0 if batch_first else 1]}, {shape[2]}]; got {tuple(h0.shape)}")
+        _dtype_code(who, h0)
+    if starts is not None and (starts.shape != shape[:2] or starts.dtype not in (torch.bool, torch.uint8)):
+        raise RuntimeError(f"{who}: starts must be a bool tensor of shape {tuple(shape[:2])}; got "
                            f"{starts.dtype} {tuple(starts.shape)}")
-    _lib.host_status(z.get_device()).check()
+    _lib.host_status(index).check()
     z, x = _rows(z), _rows(x)
     if torch.is_grad_enabled() and (z.requires_grad or x.requires_grad or (h0 is not None and h0.requires_grad)):
-        return RecurrenceFn.apply(z, x, h0, starts, form, batch_first)
-    h, h_n, _ = _recurrence_forward(form, z, x, None if h0 is None else _state(h0), starts, batch_first, False)
-    return h, h_n
+        return RecurrenceFn.apply(z, x, h0, starts, code, index, form, batch_first)
+    return _recurrence_forward(code, index, form, z, x, None if h0 is None else _state(h0), starts, batch_first, False)[:2]
 
 
 def gated_recurrence(z, x, h0=None, starts=None, batch_first: bool = False):
@@ -167,28 +170,27 @@ def linear_recurrence(a, b, h0=None, starts=None, batch_first: bool = False):
 
 
 def _step(who, form, z, x, h, out_state):
-    _refuse_dtype(who, z)
-    _same_device(who, z, x, h, out_state)
-    if z.dim() != 2 or x.shape != z.shape or h.shape != z.shape:
-        raise RuntimeError(f"{who}: z, x and h must be [B, H]; got {tuple(z.shape)}, {tuple(x.shape)} and "
-                           f"{tuple(h.shape)}")
+    code, index = _dtype_code(who, z), _device_index(who, z, x, h, out_state)
+    shape = z.shape
+    if len(shape) != 2 or x.shape != shape or h.shape != shape:
+        raise RuntimeError(f"{who}: z, x and h must be [B, H]; got {tuple(shape)}, {tuple(x.shape)} and {tuple(h.shape)}")
     if x.dtype is not z.dtype:
         raise TypeError(f"{who}: tensors of {z.dtype} and {x.dtype}")
     if h.dtype is not torch.float32:
         raise TypeError(f"{who}: the state is float32; got {h.dtype}")
-    if torch.is_grad_enabled() and (z.requires_grad or x.requires_grad or h.requires_grad):
+    if (z.requires_grad or x.requires_grad or h.requires_grad) and torch.is_grad_enabled():
         raise RuntimeError(f"{who} is not differentiable; use the recurrence over [1, B, H], or torch.no_grad()")
-    if out_state is None:
-        out_state = torch.empty(h.shape, device=h.device)
-    elif out_state.dtype is not torch.float32 or out_state.shape != h.shape or not out_state.is_contiguous():
-        raise RuntimeError(f"{who}: out_state must be a contiguous float32 [B, H] tensor")
     z, x, h = _rows(z), _rows(x), h if h.is_contiguous() else h.contiguous()
-    out = torch.empty(z.shape, dtype=z.dtype, device=z.device)
-    index, (B, H) = z.get_device(), z.shape
+    if out_state is None:
+        out_state = torch.empty_like(h)
+    elif out_state.dtype is not torch.float32 or out_state.shape != shape or not out_state.is_contiguous():
+        raise RuntimeError(f"{who}: out_state must be a contiguous float32 [B, H] tensor")
+    out = torch.empty_like(z)
+    B, H = shape
     status = _lib.host_status(index)
     status.check()
-    _call("hs_recurrence_forward", index, _CODE[z.dtype], form, z.data_ptr(), 0, z.stride(0), x.data_ptr(), 0, x.stride(0),
-          h.data_ptr(), None, 0, 0, out.data_ptr(), 0, H, out_state.data_ptr(), None, 1, B, H, status.timeout_ptr)
+    _call("hs_recurrence_forward", index, code, form, z.data_ptr(), 0, z.stride(0), x.data_ptr(), 0, x.stride(0),
+          h.data_ptr(), None, 0, 0, out.data_ptr(), 0, out.stride(0), out_state.data_ptr(), None, 1, B, H, status.timeout_ptr)
     return out, out_state
 
 
@@ -213,36 +215,34 @@ def _tokens(who, tokens):
     return tokens if tokens.is_contiguous() else tokens.contiguous(), bits
 
 
-def _embedding_forward(tokens, bits, weight, scale):
+def _embedding_forward(code, index, tokens, bits, weight, scale):
     V, D = weight.shape
-    index = weight.get_device()
     out = torch.empty((*tokens.shape, D), dtype=weight.dtype, device=weight.device)
-    _call("hs_embedding_forward", index, _CODE[weight.dtype], weight.data_ptr(), weight.stride(0), bits,
-          tokens.data_ptr(), scale, out.data_ptr(), tokens.numel(), V, D, _lib.host_status(index).token_ptr)
+    _call("hs_embedding_forward", index, code, weight.data_ptr(), weight.stride(0), bits, tokens.data_ptr(), scale,
+          out.data_ptr(), tokens.numel(), V, D, _lib.host_status(index).token_ptr)
     return out
 
 
 class EmbeddingFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, weight, tokens, bits, scale, padding_idx):
+    def forward(ctx, weight, tokens, code, index, bits, scale, padding_idx):
         ctx.save_for_backward(tokens)
-        ctx.table = (weight.shape, weight.dtype)
-        ctx.args = (bits, scale, padding_idx)
-        return _embedding_forward(tokens, bits, weight, scale)
+        ctx.args = (weight.shape, code, index, bits, scale, padding_idx)
+        return _embedding_forward(code, index, tokens, bits, weight, scale)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         (tokens,) = ctx.saved_tensors
-        (V, D), dtype = ctx.table
-        bits, scale, padding_idx = ctx.args
-        dev, index, N = dout.device, dout.get_device(), tokens.numel()
+        shape, code, index, bits, scale, padding_idx = ctx.args
+        V, D = shape
+        N = tokens.numel()
         dout = dout if dout.is_contiguous() else dout.contiguous()
-        dweight = torch.empty((V, D), dtype=dtype, device=dev)
-        ws = _lib.workspace(_lib.function("hs_embedding_workspace_bytes")(N, V, D), dev)
-        _call("hs_embedding_backward", index, _CODE[dtype], dout.data_ptr(), bits, tokens.data_ptr(), padding_idx, scale,
+        dweight = torch.empty(shape, dtype=dout.dtype, device=dout.device)
+        ws = _lib.workspace(_lib.function("hs_embedding_workspace_bytes")(N, V, D), dout.device)
+        _call("hs_embedding_backward", index, code, dout.data_ptr(), bits, tokens.data_ptr(), padding_idx, scale,
               dweight.data_ptr(), N, V, D, ws.data_ptr(), ws.numel(), _lib.host_status(index).token_ptr)
-        return dweight, None, None, None, None
+        return dweight, None, None, None, None, None, None
 
 
 def embedding(tokens, weight, scale: float = 1.0, padding_idx: Optional[int] = None):
@@ -255,8 +255,7 @@ def embedding(tokens, weight, scale: float = 1.0, padding_idx: Optional[int] = N
     reported by ``check_device_status()`` and by later calls, until
     ``clear_device_status()``."""
     who = "embedding"
-    _refuse_dtype(who, weight)
-    _same_device(who, weight, tokens)
+    code, index = _dtype_code(who, weight), _device_index(who, weight, tokens)
     if weight.dim() != 2:
         raise RuntimeError(f"{who}: weight must be [V, D]; got {tuple(weight.shape)}")
     tokens, bits = _tokens(who, tokens)
@@ -268,10 +267,10 @@ def embedding(tokens, weight, scale: float = 1.0, padding_idx: Optional[int] = N
         pad = padding_idx + (V if padding_idx < 0 else 0)
         if not 0 <= pad < V:
             raise RuntimeError(f"{who}: padding_idx {padding_idx} is outside the table of {V} rows")
-    _lib.host_status(weight.get_device()).check()
+    _lib.host_status(index).check()
     if weight.requires_grad and torch.is_grad_enabled():
-        return EmbeddingFn.apply(weight, tokens, bits, scale, pad)
-    return _embedding_forward(tokens, bits, weight, scale)
+        return EmbeddingFn.apply(weight, tokens, code, index, bits, scale, pad)
+    return _embedding_forward(code, index, tokens, bits, weight, scale)
 
 
 class TokenLogprobs(NamedTuple):
@@ -283,25 +282,27 @@ class TokenLogprobs(NamedTuple):
     top_index: Optional[torch.Tensor]
 
 
-def _logprobs_forward(logits, tokens, bits, top, temperature, ignore_index, keep):
+def _logprobs_forward(code, index, logits, tokens, bits, top, temperature, ignore_index, keep):
     N, V = logits.shape
-    dev, index = logits.device, logits.get_device()
-    logprob, entropy = torch.empty(N, device=dev), torch.empty(N, device=dev)
+    dev = logits.device
+    logprob = torch.empty(N, device=dev)
+    entropy = torch.empty_like(logprob)
     top_lp = torch.empty((N, top), device=dev) if top else None
     top_id = torch.empty((N, top), dtype=torch.int64, device=dev) if top else None
     stats = torch.empty((N, 2), device=dev) if keep else None
-    _call("hs_token_logprobs_forward", index, _CODE[logits.dtype], logits.data_ptr(), logits.stride(0), bits,
-          tokens.data_ptr(), ignore_index, temperature, top, logprob.data_ptr(), entropy.data_ptr(), _p(top_lp), _p(top_id),
-          _p(stats), N, V, _lib.host_status(index).token_ptr)
+    _call("hs_token_logprobs_forward", index, code, logits.data_ptr(), logits.stride(0), bits, tokens.data_ptr(),
+          ignore_index, temperature, top, logprob.data_ptr(), entropy.data_ptr(), _p(top_lp), _p(top_id), _p(stats), N, V,
+          _lib.host_status(index).token_ptr)
     return logprob, entropy, top_lp, top_id, stats
 
 
 class TokenLogprobsFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, tokens, bits, top, temperature, ignore_index):
-        logprob, entropy, top_lp, top_id, stats = _logprobs_forward(logits, tokens, bits, top, temperature, ignore_index, True)
+    def forward(ctx, logits, tokens, code, index, bits, top, temperature, ignore_index):
+        logprob, entropy, top_lp, top_id, stats = _logprobs_forward(code, index, logits, tokens, bits, top, temperature,
+                                                                    ignore_index, True)
         ctx.save_for_backward(logits, tokens, entropy, top_id, stats)
-        ctx.args = (bits, top, temperature, ignore_index)
+        ctx.args = (code, index, bits, top, temperature, ignore_index)
         ctx.set_materialize_grads(False)
         if top:
             ctx.mark_non_differentiable(top_id)
@@ -311,14 +312,14 @@ class TokenLogprobsFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dlogprob, dentropy, dtop, _dindex):
         logits, tokens, entropy, top_id, stats = ctx.saved_tensors
-        bits, top, temperature, ignore_index = ctx.args
+        code, index, bits, top, temperature, ignore_index = ctx.args
         N, V = logits.shape
         dlogprob, dentropy, dtop = (None if t is None else _state(t) for t in (dlogprob, dentropy, dtop))
         dlogits = torch.empty((N, V), dtype=logits.dtype, device=logits.device)
-        _call("hs_token_logprobs_backward", logits.get_device(), _CODE[logits.dtype], logits.data_ptr(), logits.stride(0),
-              bits, tokens.data_ptr(), ignore_index, temperature, top, stats.data_ptr(), entropy.data_ptr(), _p(top_id),
-              _p(dlogprob), _p(dentropy), _p(dtop), dlogits.data_ptr(), V, N, V)
-        return dlogits, None, None, None, None, None
+        _call("hs_token_logprobs_backward", index, code, logits.data_ptr(), logits.stride(0), bits, tokens.data_ptr(),
+              ignore_index, temperature, top, stats.data_ptr(), entropy.data_ptr(), _p(top_id), _p(dlogprob), _p(dentropy),
+              _p(dtop), dlogits.data_ptr(), V, N, V)
+        return dlogits, None, None, None, None, None, None, None
 
 
 def token_logprobs(logits, tokens, top: int = 0, temperature: float = 1.0, ignore_index: int = -100) -> TokenLogprobs:
@@ -336,8 +337,7 @@ def token_logprobs(logits, tokens, top: int = 0, temperature: float = 1.0, ignor
     ``check_device_status()`` and by later calls, until
     ``clear_device_status()``."""
     who = "token_logprobs"
-    _refuse_dtype(who, logits)
-    _same_device(who, logits, tokens)
+    code, index = _dtype_code(who, logits), _device_index(who, logits, tokens)
     shape = tokens.shape
     if logits.dim() < 1 or logits.shape[:-1] != shape:
         raise RuntimeError(f"{who}: logits [..., V] and tokens [...] do not match: {tuple(logits.shape)} and {tuple(shape)}")
@@ -352,11 +352,11 @@ def token_logprobs(logits, tokens, top: int = 0, temperature: float = 1.0, ignor
     rows = _rows(logits)
     if rows.shape[0] > 1 and rows.stride(0) < V:
         rows = rows.contiguous()
-    _lib.host_status(rows.get_device()).check()
+    _lib.host_status(index).check()
     if rows.requires_grad and torch.is_grad_enabled():
-        lp, ent, top_lp, top_id = TokenLogprobsFn.apply(rows, tokens, bits, top, temperature, ignore_index)
+        lp, ent, top_lp, top_id = TokenLogprobsFn.apply(rows, tokens, code, index, bits, top, temperature, ignore_index)
     else:
-        lp, ent, top_lp, top_id, _ = _logprobs_forward(rows, tokens, bits, top, temperature, ignore_index, False)
+        lp, ent, top_lp, top_id, _ = _logprobs_forward(code, index, rows, tokens, bits, top, temperature, ignore_index, False)
     if len(shape) != 1:
         lp, ent = lp.view(shape), ent.view(shape)
         if top:

@@ -914,7 +914,7 @@ int launch(K kernel, const Args &args, const Plan &pl, cudaStream_t st, const ch
   at[0].val.clusterDim.y = 1;
   at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = pl.cluster > 1;
   (void)cudaLaunchKernelEx(&cfg, kernel, args);
   return check_launch(what);
 }

@@ -691,7 +691,7 @@ int hs_token_logprobs_forward(int dtype, const void *logits, int64_t logits_ld, 
     at[0].val.clusterDim.x = (unsigned)a.cluster;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = a.cluster > 1;
     (void)cudaLaunchKernelEx(&cfg, kernel, a);
     return check_launch("logprobs_fwd_kernel");
   });
