@@ -400,24 +400,45 @@ __global__ void __launch_bounds__(threads_of<W>(), 1024 / threads_of<W>()) logpr
     if (nchosen <= kChosen) {
       if (mine >= lo && tid < r.head) collect(to_f32<T>(row[tid]), tid);
       if (mine >= lo && tid < r.ntail) collect(to_f32<T>(row[r.tail0 + tid]), r.tail0 + tid);
-      const int per = (r.hi - r.lo + NT - 1) / NT;  // vectors of a thread
-      for (int j = tid; j < nchosen * per; j += NT) {
-        const int t = j / per, i = r.lo + f.chosen[t] + (j - t * per) * NT;
-        if (i >= r.hi) continue;
-        const uint4 q = __ldg(r.vec(i));
-        if (order_bits(vec_max<T>(q)) < lo) continue;
-        float v[E];
-        unpack_vec<T>(q, v);
+      const int per = (r.hi - r.lo + NT - 1) / NT, all = nchosen * per;  // vectors of a thread, of all
+      constexpr int G = W == 1 ? 1 : 3;  // loads at once
+      for (int j0 = tid; j0 < all; j0 += G * NT) {
+        uint4 q[G];
+        int at[G];
 #pragma unroll
-        for (int e = 0; e < E; ++e) collect(v[e], r.index(i, e));
+        for (int k = 0; k < G; ++k) {
+          const int j = j0 + k * NT, t = j / per;
+          at[k] = j < all ? r.lo + f.chosen[t] + (j - t * per) * NT : r.hi;
+          if (at[k] < r.hi) q[k] = __ldg(r.vec(at[k]));
+        }
+#pragma unroll
+        for (int k = 0; k < G; ++k) {
+          if (at[k] >= r.hi || order_bits(vec_max<T>(q[k])) < lo) continue;
+          float v[E];
+          unpack_vec<T>(q[k], v);
+#pragma unroll
+          for (int e = 0; e < E; ++e) collect(v[e], r.index(at[k], e));
+        }
       }
     }
     row_sync<W>();
     const int n = f.nfound;
     if (nchosen <= kChosen && n <= kFound) {
       if (W == 1 || warp == 0) {
-        list = sort_desc(lane < n ? f.found[lane] : 0, lane);
-        if (n > 32) list = merge_desc(list, sort_desc(32 + lane < n ? f.found[32 + lane] : 0, lane), lane);
+        // in order by counting the larger ones
+        const Key a0 = lane < n ? f.found[lane] : 0, a1 = lane + 32 < n ? f.found[lane + 32] : 0;
+        int before0 = 0, before1 = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) {
+          const Key k = f.found[j];
+          before0 += k > a0;
+          before1 += k > a1;
+        }
+        __syncwarp();
+        if (lane < n && before0 < 32) f.found[before0] = a0;
+        if (lane + 32 < n && before1 < 32) f.found[before1] = a1;
+        __syncwarp();
+        list = lane < n ? f.found[lane] : 0;
       }
     } else {  // too many equal values
       auto add = [&](float v, int at, bool ok) {
