@@ -508,10 +508,10 @@ HS_API int hs_recurrence_forward(int dtype, int form, const void *z, int64_t z_t
                                  int *dev_status, hs_stream_t stream);
 /* Its gradient: dh [T,B,H] and dh_n [B,H] (either may be NULL = zeros) to dz,
  * dx [T,B,H] and dh0 [B,H] (NULL = not wanted).  Reads the forward's
- * checkpoints, not h: the states are recomputed in float32. */
+ * checkpoints, not h: the states are recomputed in float32.  with_starts says
+ * whether the forward had starts; they are in the checkpoints. */
 HS_API int hs_recurrence_backward(int dtype, int form, const void *z, int64_t z_t, int64_t z_b, const void *x,
-                                  int64_t x_t, int64_t x_b, const float *checkpoints,
-                                  const unsigned char *starts, int64_t starts_t, int64_t starts_b,
+                                  int64_t x_t, int64_t x_b, const float *checkpoints, int with_starts,
                                   const void *dh, int64_t dh_t, int64_t dh_b, const float *dh_n, void *dz,
                                   int64_t dz_t, int64_t dz_b, void *dx, int64_t dx_t, int64_t dx_b, float *dh0,
                                   int64_t T, int64_t B, int64_t H, int *dev_status, hs_stream_t stream);

@@ -91,7 +91,7 @@ SIGNATURES = {
     "hs_recurrence_checkpoint_bytes": (_sz, [_i64] * 3),
     "hs_recurrence_forward": (_i32, [_i32] * 2 + [_c_p, _i64, _i64] * 2 + [_c_p] + [_c_p, _i64, _i64] * 2
                               + [_c_p] * 2 + [_i64] * 3 + [_c_p] * 2),
-    "hs_recurrence_backward": (_i32, [_i32] * 2 + [_c_p, _i64, _i64] * 2 + [_c_p] + [_c_p, _i64, _i64] * 2 + [_c_p]
+    "hs_recurrence_backward": (_i32, [_i32] * 2 + [_c_p, _i64, _i64] * 2 + [_c_p, _i32] + [_c_p, _i64, _i64] + [_c_p]
                                + [_c_p, _i64, _i64] * 2 + [_c_p] + [_i64] * 3 + [_c_p] * 2),
     "hs_embedding_forward": (_i32, [_i32, _c_p, _i64, _i32, _c_p, _f64, _c_p] + [_i64] * 3 + [_c_p] * 2),
     "hs_embedding_workspace_bytes": (_sz, [_i64] * 3),

@@ -87,7 +87,7 @@ def _recurrence_forward(code, index, form, z, x, h0, starts, batch_first, keep):
     T, B, H = _extents(z, batch_first)
     h = torch.empty_like(z)
     h_n = torch.empty((B, H), device=z.device) if h0 is None else torch.empty_like(h0)
-    ckpt = torch.empty(-(-T // _RUN) * B * H, device=z.device) if keep else None
+    ckpt = torch.empty(-(-T // _RUN) * B * (H + 1), device=z.device) if keep else None  # states, masks of starts
     _call("hs_recurrence_forward", index, code, form, *_tensor(z, batch_first), *_tensor(x, batch_first), _p(h0),
           *_tensor(starts, batch_first), *_tensor(h, batch_first), h_n.data_ptr(), _p(ckpt), T, B, H,
           _lib.host_status(index).timeout_ptr)
@@ -99,23 +99,23 @@ class RecurrenceFn(torch.autograd.Function):
     def forward(ctx, z, x, h0, starts, code, index, form, batch_first):
         h, h_n, ckpt = _recurrence_forward(code, index, form, z, x, None if h0 is None else _state(h0), starts, batch_first,
                                            True)
-        ctx.save_for_backward(z, x, starts, ckpt)
-        ctx.args = (code, index, form, batch_first, None if h0 is None else h0.dtype)
+        ctx.save_for_backward(z, x, ckpt)
+        ctx.args = (code, index, form, batch_first, starts is not None, None if h0 is None else h0.dtype)
         ctx.set_materialize_grads(False)
         return h, h_n
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dh, dh_n):
-        z, x, starts, ckpt = ctx.saved_tensors
-        code, index, form, bf, h0_dtype = ctx.args
+        z, x, ckpt = ctx.saved_tensors
+        code, index, form, bf, with_starts, h0_dtype = ctx.args
         T, B, H = _extents(z, bf)
         dh = None if dh is None else _rows(dh)
         dh_n = None if dh_n is None else _state(dh_n)
         dz, dx = torch.empty_like(z), torch.empty_like(x)
         dh0 = torch.empty((B, H), device=z.device) if h0_dtype is not None and ctx.needs_input_grad[2] else None
         _call("hs_recurrence_backward", index, code, form, *_tensor(z, bf), *_tensor(x, bf), ckpt.data_ptr(),
-              *_tensor(starts, bf), *_tensor(dh, bf), _p(dh_n), *_tensor(dz, bf), *_tensor(dx, bf), _p(dh0), T, B, H,
+              with_starts, *_tensor(dh, bf), _p(dh_n), *_tensor(dz, bf), *_tensor(dx, bf), _p(dh0), T, B, H,
               _lib.host_status(index).timeout_ptr)
         if dh0 is not None and h0_dtype is not torch.float32:
             dh0 = dh0.to(h0_dtype)

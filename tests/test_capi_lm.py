@@ -28,7 +28,7 @@ def rec_forward(lib, dtype=0, form=0, z=P, x=P, h=P, T=4, B=2, H=8, status=P):
 
 
 def rec_backward(lib, dtype=0, z=P, ckpt=P, dz=P, T=4, B=2, H=8, status=P):
-    return lib.hs_recurrence_backward(dtype, 0, z, 16, 8, P, 16, 8, ckpt, None, 0, 0, None, 0, 0, None, dz, 16, 8, P, 16, 8,
+    return lib.hs_recurrence_backward(dtype, 0, z, 16, 8, P, 16, 8, ckpt, 0, None, 0, 0, None, dz, 16, 8, P, 16, 8,
                                       None, T, B, H, status, None)
 
 
@@ -93,9 +93,10 @@ def test_empty_extents_do_nothing(lib):
 
 
 def test_size_queries(lib):
-    assert lib.hs_recurrence_checkpoint_bytes(1, 2, 3) == 4 * 2 * 3
-    assert lib.hs_recurrence_checkpoint_bytes(16, 2, 3) == 4 * 2 * 3
-    assert lib.hs_recurrence_checkpoint_bytes(17, 2, 3) == 2 * 4 * 2 * 3
+    # a float32 state and a word of starts for each sequence and run of 16 steps
+    assert lib.hs_recurrence_checkpoint_bytes(1, 2, 3) == 4 * 2 * (3 + 1)
+    assert lib.hs_recurrence_checkpoint_bytes(16, 2, 3) == 4 * 2 * (3 + 1)
+    assert lib.hs_recurrence_checkpoint_bytes(17, 2, 3) == 2 * 4 * 2 * (3 + 1)
     assert lib.hs_recurrence_checkpoint_bytes(0, 2, 3) == 0
     sizes = [lib.hs_embedding_workspace_bytes(n, 1000, 64) for n in (1, 1000, 16384, 16385, 100000)]
     assert sizes == sorted(sizes) and sizes[0] > 0
