@@ -486,7 +486,7 @@ __global__ void __launch_bounds__(256) emb_sum_kernel(const SumArgs p) {
 constexpr int kJoinWarps = 16, kLong = 16;
 
 template <typename T, int BYTES>
-__global__ void __launch_bounds__(32 * kJoinWarps) emb_join_kernel(const SumArgs p) {
+__global__ void __launch_bounds__(32 * kJoinWarps, 2) emb_join_kernel(const SumArgs p) {
   using C = typename Chunk<BYTES>::type;
   constexpr int E = BYTES / (int)sizeof(T);
   __shared__ float share[kJoinWarps][E][32];
@@ -510,7 +510,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) emb_join_kernel(const SumArgs
   };
   auto add_heads = [&](int64_t a, int64_t b, float *acc) {  // head parts of pieces a..b
     int64_t j = a;
-    constexpr int U = 8;
+    constexpr int U = E > 4 ? 4 : 8;
     for (; j + U <= b + 1; j += U) {
       float v[U][E];
 #pragma unroll
