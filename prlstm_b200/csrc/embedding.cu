@@ -28,7 +28,6 @@ namespace hs {
 namespace {
 
 constexpr int kPiece = 32;        // sorted entries per warp of the summing kernel
-constexpr int kZeroIds = 8;       // ids per warp that writes zero rows
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortCluster = 8;   // CTAs of the sorting cluster at most
@@ -362,6 +361,7 @@ struct SumArgs {
   int slices;          // lane groups of a row
   int chunks;          // lane chunks of a row
   int64_t sum_blocks;  // CTAs of the sums; the others write zero rows
+  int zero_ids;        // ids per warp there: 8 to 32, about 16 KB of rows
   Scale scale;
 };
 
@@ -398,10 +398,10 @@ __global__ void __launch_bounds__(256) emb_sum_kernel(const SumArgs p) {
   const int64_t row_bytes = p.D * (int64_t)sizeof(T);
   if ((int64_t)blockIdx.x >= p.sum_blocks) {
     // a few ids per warp: rows of those that do not occur
-    const int64_t first = (((int64_t)blockIdx.x - p.sum_blocks) * 8 + warp) * kZeroIds;
+    const int64_t first = (((int64_t)blockIdx.x - p.sum_blocks) * 8 + warp) * p.zero_ids;
     if (first >= p.V) return;
-    const unsigned end = (unsigned)min(p.V, first + kZeroIds);
-    unsigned none = (1u << (end - (unsigned)first)) - 1u;
+    const unsigned end = (unsigned)min(p.V, first + p.zero_ids);
+    unsigned none = 0xffffffffu >> (32 - (end - (unsigned)first));
     int64_t at[2];
     first_entries(p, {(unsigned)first, end}, lane, at);
     if (at[1] - at[0] <= 128) {
@@ -758,7 +758,9 @@ int hs_embedding_backward(int dtype, const void *dout, int token_bits, const voi
   const int bytes = chunk_bytes(D * (int64_t)es, {dout, dweight}, 0, es);
   const int64_t chunks = D * (int64_t)es / bytes, slices = (chunks + 31) / 32;
   p.sum_blocks = (p.pieces * slices + 7) / 8;
-  const int64_t zero_blocks = (V + 8 * kZeroIds - 1) / (8 * kZeroIds), join_blocks = (p.pieces + kJoinWarps - 1) / kJoinWarps * slices;
+  p.zero_ids = 8;
+  while (p.zero_ids < 32 && 2 * p.zero_ids * D * (int64_t)es <= 16384) p.zero_ids *= 2;
+  const int64_t zero_blocks = (V + 8 * p.zero_ids - 1) / (8 * p.zero_ids), join_blocks = (p.pieces + kJoinWarps - 1) / kJoinWarps * slices;
   if (chunks > 0x7fffffff || p.sum_blocks + zero_blocks > 0x7fffffff || join_blocks > 0x7fffffff)
     return fail(HS_ERR_UNSUPPORTED, "hs_embedding_backward: N * D is too large");
   p.chunks = (int)chunks, p.slices = (int)slices;
