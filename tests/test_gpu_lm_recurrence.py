@@ -284,6 +284,15 @@ def test_step_equals_the_recurrence(dtype):
     check(h_n, want["h_n"], memory, "h_n")
 
 
+def test_second_derivatives_are_refused():
+    z = torch.randn(5, 2, 8, device=DEV, requires_grad=True)
+    x = torch.randn(5, 2, 8, device=DEV, requires_grad=True)
+    h, _ = call("gated")(z, x)
+    (g,) = torch.autograd.grad(h.square().sum(), z, create_graph=True)  # the first may be asked for with a graph
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
 def test_same_bits_every_run_and_on_another_stream():
     a, b, h0, s, dh, dh_n = make(1500, 2, 200, torch.bfloat16, "gated", seed=17, starts=True)
     first = run(a, b, h0, s, dh, dh_n, "gated")
