@@ -77,7 +77,8 @@ struct FwdArgs {
   int64_t state_b;                         // row stride of h0 and h_n (columns)
   int64_t ckpt_t;                          // columns of one saved state (B * H)
   int *status;
-  CUtensorMap zm, xm, hm;                  // where the tensors suit TMA
+  const char *ze, *xe;                     // ends of the tensors
+  CUtensorMap zm, xm, hm;                  // where the tensors suit tiles
 };
 
 struct BwdArgs {
@@ -91,6 +92,7 @@ struct BwdArgs {
   int64_t zt, zb, xt, xb, gt, gb, dzt, dzb, dxt, dxb;
   int64_t state_b, ckpt_t;
   int *status;
+  const char *ze, *xe, *ge;
   CUtensorMap zm, xm, gm, dzm, dxm;
 };
 
@@ -351,23 +353,67 @@ template <int VEC> HS_DEV void load_state(const float *p, int64_t at, float *v) 
 }
 
 // ------------------------------------------------------------------ inputs
-// Shared memory of a CTA: kStages x [N tensors][warps][16 steps][32 words] of
-// inputs, then [outputs][warps][16 steps][32 words] where TMA writes them.
-// A tile of all warps' runs comes in by one TMA copy per tensor (TMA), or each
-// lane copies and reads its own words (tensors or strides off 16 bytes).
-template <typename T, int VEC, bool TMA, int N> struct Inputs {
+// How tensors move.  kTiles: a tile of all warps' runs comes in by one TMA copy
+// per tensor and each run leaves by one (bases and strides multiples of 16
+// bytes).  kRows: each lane of a warp copies one step's words of the warp's run,
+// the 16-byte granules that they lie in, by one bulk copy (rows 4-byte aligned).
+// kLanes: each lane copies and reads its own words (a single run, where copies
+// that signal a barrier take longer; rows that are only 2-byte aligned; many
+// columns, as an SM starts one row copy in about 17 cycles).
+enum { kLanes, kTiles, kRows };
+constexpr unsigned step_bytes(int move) { return move == kRows ? kStep + 16 : kStep; }
+constexpr unsigned slab_bytes(int move) { return kRun * step_bytes(move); }
+
+// Shared memory of a CTA: kStages x [N tensors][warps][16 steps] of inputs,
+// then [outputs][warps][16 steps] with kTiles.
+template <int MOVE, int N> struct Inputs {
   unsigned base, tensor;  // this lane's first word of its slab; bytes between tensors
-  uint64_t *full;
+  uint64_t *full;         // [kStages], with kRows [kStages][warps]
   int *status;
+  int warp, warps;
   HS_DEV unsigned at(int w) const { return base + (unsigned)(w % kStages) * (N * tensor); }
+  HS_DEV uint64_t *bar(int w) const { return full + (w % kStages) * (MOVE == kRows ? warps : 1) + (MOVE == kRows ? warp : 0); }
   // Waits until wave w is there.
   HS_DEV void wait(int w) const {
-    if constexpr (TMA)
-      mbar_wait(full + w % kStages, (w / kStages) & 1, status);
-    else
+    if constexpr (MOVE == kLanes)
       cp_wait<kStages - 1>();
+    else
+      mbar_wait(bar(w), (w / kStages) & 1, status);
   }
 };
+
+// Where a step's words begin in their 16-byte granule, for the row segment of
+// a warp (the first of its words at `at` elements from base; 16 steps of any
+// stride are whole granules, so every run begins alike).
+template <typename T, int MOVE> struct Shift {
+  unsigned o, r;
+  HS_DEV Shift(const char *base, int64_t at, int64_t stride)
+      : o((unsigned)(reinterpret_cast<uintptr_t>(base) + (uintptr_t)at * sizeof(T))), r((unsigned)(stride * (int64_t)sizeof(T))) {}
+  HS_DEV unsigned operator()(int k) const { return MOVE == kRows ? (o + k * r) & 15 : 0; }
+};
+
+// Copies the granules of `bytes` bytes at src, but none past the tensor's end;
+// what is left of the last one by the lane itself.  Returns the bytes that the
+// barrier is to expect.
+template <typename T> HS_DEV unsigned copy_row(unsigned dst, const char *src, unsigned bytes, const char *end, uint64_t *bar) {
+  const char *from = reinterpret_cast<const char *>(reinterpret_cast<uintptr_t>(src) & ~(uintptr_t)15);
+  unsigned size = (unsigned)(src + bytes - from + 15) & ~15u;
+  if (from + size > end) {
+    size -= 16;
+    const char *q = from + size < src ? src : from + size;
+    for (; q < src + bytes; q += sizeof(T)) {
+      if constexpr (sizeof(T) == 4)
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst + (unsigned)(q - from)), "r"(*reinterpret_cast<const unsigned *>(q)) : "memory");
+      else
+        asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + (unsigned)(q - from)), "h"(*reinterpret_cast<const unsigned short *>(q)) : "memory");
+    }
+  }
+  if (size)
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(from),
+                 "r"(size), "r"(smem_u32(bar))
+                 : "memory");
+  return size;
+}
 
 // The starts among the steps t .. t+15 as bits.  A warp reads those of its next
 // 32 waves at once, one wave per lane: read wave by wave, the load's latency
@@ -382,9 +428,9 @@ HS_DEV unsigned start_mask(const unsigned char *starts, int64_t stride, int64_t 
   return m;
 }
 
-HS_DEV void barriers_init(uint64_t *full, int warp, int lane) {
+HS_DEV void barriers_init(uint64_t *full, int n, int warp, int lane) {
   if (warp == 0 && lane == 0) {
-    for (int i = 0; i < kStages; ++i) mbar_init(full + i);
+    for (int i = 0; i < n; ++i) mbar_init(full + i);
     fence_mbar_init();
     fence_async();
   }
@@ -392,10 +438,10 @@ HS_DEV void barriers_init(uint64_t *full, int warp, int lane) {
 }
 
 // ------------------------------------------------------------------ forward
-template <typename T, int VEC, bool GATED, bool STARTS, bool TMA>
+template <typename T, int VEC, bool GATED, bool STARTS, int MOVE>
 __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid_constant__ FwdArgs p) {
   extern __shared__ __align__(128) unsigned char dyn[];
-  __shared__ uint64_t full[kStages], swap[2];
+  __shared__ uint64_t full[kStages * kFwdWarps], swap[2];
   using C = Cols<VEC>;
   const int lane = threadIdx.x, warp = threadIdx.y, warps = blockDim.y;
   const int cluster = p.s.cluster, rank = (int)(blockIdx.x % cluster), waves = p.s.waves;
@@ -406,16 +452,33 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
   const bool live = col < p.s.n;  // VEC > 1 only where n is a multiple of VEC
   if (!live) col = p.s.n - VEC;   // reads what a live lane reads, writes nothing
   const int64_t T_ = p.s.T;
-  Inputs<T, VEC, TMA, 2> in;
-  in.tensor = warps * kSlab, in.full = full, in.status = p.status;
-  in.base = smem_u32(dyn) + warp * kSlab + lane * 4;
+  constexpr unsigned kPitch = step_bytes(MOVE);
+  Inputs<MOVE, 2> in;
+  in.tensor = warps * slab_bytes(MOVE), in.full = full, in.status = p.status, in.warp = warp, in.warps = warps;
+  in.base = smem_u32(dyn) + warp * slab_bytes(MOVE) + lane * 4;
+  const Shift<T, MOVE> zsh(p.z, row * p.zb + col0, p.zt), xsh(p.x, row * p.xb + col0, p.xt);
   const unsigned slab = in.base + kStages * 2 * in.tensor;  // this lane's words of the outputs
 
   auto start_of = [&](int w) { return ((int64_t)(w * cluster + rank) * warps + warp) * kRun; };
   auto fetch = [&](int w) {
-    if constexpr (TMA) {
+    if constexpr (MOVE == kRows) {
+      if (w < waves) {  // lanes 0..15 the steps of z, 16..31 those of x
+        const int64_t t = start_of(w) + lane % 16;
+        const bool x = lane >= 16;
+        const unsigned bytes = (unsigned)min((int64_t)kStep, (p.s.n - col0) * (int64_t)sizeof(T));
+        unsigned size = 0;
+        if (t < T_) {
+          const int64_t at = row * (x ? p.xb : p.zb) + col0 + t * (x ? p.xt : p.zt);
+          size = copy_row<T>(in.at(w) - lane * 4 + (x ? in.tensor : 0u) + lane % 16 * kPitch, (x ? p.x : p.z) + at * (int64_t)sizeof(T), bytes,
+                             x ? p.xe : p.ze, in.bar(w));
+        }
+        size = __reduce_add_sync(0xffffffffu, size);
+        if (lane == 0) mbar_expect(in.bar(w), size);
+        __syncwarp();
+      }
+    } else if constexpr (MOVE == kTiles) {
       if (warp == 0 && lane == 0 && w < waves) {
-        uint64_t *bar = full + w % kStages;
+        uint64_t *bar = in.bar(w);
         const unsigned d = in.at(w);
         const int t = (int)start_of(w);
         mbar_expect(bar, 2 * in.tensor);
@@ -447,8 +510,8 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
   };
   auto starts_from = [&](int w) { return w + lane < waves ? start_mask(p.starts + row * p.sb, p.st, start_of(w + lane), T_) : 0u; };
 
-  const Maps<VEC> maps = exchange_init<VEC>(swap, dyn + (kStages * 2 + (TMA ? 1 : 0)) * in.tensor, warps, warp, lane, cluster);
-  if (TMA) barriers_init(full, warp, lane);
+  const Maps<VEC> maps = exchange_init<VEC>(swap, dyn + (kStages * 2 + (MOVE == kTiles ? 1 : 0)) * in.tensor, warps, warp, lane, cluster);
+  if (MOVE != kLanes) barriers_init(full, kStages * (MOVE == kRows ? warps : 1), warp, lane);
   fetch(0);
   fetch(1);
   unsigned masks = 0;
@@ -472,8 +535,8 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
 #pragma unroll
     for (int k = 0; k < kRun; ++k) {
       float zv[VEC], xv[VEC];
-      read_word<T, VEC>(d + k * kStep, zv);
-      read_word<T, VEC>(d + in.tensor + k * kStep, xv);
+      read_word<T, VEC>(d + zsh(k) + k * kPitch, zv);
+      read_word<T, VEC>(d + in.tensor + xsh(k) + k * kPitch, xv);
       if (GATED) {
         C om;
         gate<VEC>(zv, f[k], om);
@@ -515,7 +578,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
 #pragma unroll
         for (int i = 0; i < VEC; ++i) c[i] = v[i];
       }
-      if constexpr (TMA) {
+      if constexpr (MOVE == kTiles) {
         if (lane == 0) bulk_wait_read();  // the previous wave's copy has left the slab
         __syncwarp();
       }
@@ -525,7 +588,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
         h = cut ? b[k] : fma(f[k], h, b[k]);
         float v[VEC];
         h.get(v);
-        if constexpr (TMA) {
+        if constexpr (MOVE == kTiles) {
           stage_word<T>(slab + k * kStep, v);
         } else {
           if (live && k < len) write_word<T, VEC>(hq, v);
@@ -539,7 +602,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
 #pragma unroll
         for (int k = 0; k < kRun; ++k) put(k, false);
       }
-      if constexpr (TMA) {
+      if constexpr (MOVE == kTiles) {
         fence_async();
         __syncwarp();
         if (lane == 0) {
@@ -555,7 +618,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
 #pragma unroll
     for (int i = 0; i < VEC; ++i) p.h_n[row * p.state_b + col + i] = v[i];
   }
-  if (TMA && lane == 0) bulk_wait_read();
+  if (MOVE == kTiles && lane == 0) bulk_wait_read();
   if (cluster > 1) {  // no CTA leaves before the others are done with its memory
     cluster_arrive_relaxed();
     cluster_wait();
@@ -563,10 +626,10 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
 }
 
 // ------------------------------------------------------------------ backward
-template <typename T, int VEC, bool GATED, bool STARTS, bool TMA>
+template <typename T, int VEC, bool GATED, bool STARTS, int MOVE>
 __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid_constant__ BwdArgs p) {
   extern __shared__ __align__(128) unsigned char dyn[];
-  __shared__ uint64_t full[kStages], swap[2];
+  __shared__ uint64_t full[kStages * kBwdWarps], swap[2];
   using C = Cols<VEC>;
   // float32 keeps both f and 1-f; the 16-bit types keep 1-f alone and take
   // f = 1 - (1-f), whose error (2^-25) only enters u, far below their rounding
@@ -581,18 +644,38 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
   if (!live) col = p.s.n - VEC;
   const int64_t T_ = p.s.T;
   const bool has_g = p.g != nullptr;
-  Inputs<T, VEC, TMA, 3> in;
-  in.tensor = warps * kSlab, in.full = full, in.status = p.status;
+  constexpr unsigned kPitch = step_bytes(MOVE);
+  Inputs<MOVE, 3> in;
+  in.tensor = warps * slab_bytes(MOVE), in.full = full, in.status = p.status, in.warp = warp, in.warps = warps;
   // warps go back in time, so the first warp's run is the last of a tile
-  in.base = smem_u32(dyn) + (warps - 1 - warp) * kSlab + lane * 4;
+  in.base = smem_u32(dyn) + (warps - 1 - warp) * slab_bytes(MOVE) + lane * 4;
+  const Shift<T, MOVE> zsh(p.z, row * p.zb + col0, p.zt), xsh(p.x, row * p.xb + col0, p.xt), gsh(p.g, row * p.gb + col0, p.gt);
   const unsigned slab = in.base + kStages * 3 * in.tensor;
 
   // chunks from the last to the first; below 0: past the beginning, nothing
   auto chunk_of = [&](int w) { return p.s.nchunk - 1 - ((w * cluster + rank) * warps + warp); };
   auto fetch = [&](int w) {
-    if constexpr (TMA) {
+    if constexpr (MOVE == kRows) {
+      if (w < waves) {  // lanes 0..15 the steps of z, 16..31 those of x, then 0..15 those of g
+        const int c = chunk_of(w);
+        const int64_t t = (int64_t)c * kRun + lane % 16;
+        const unsigned bytes = (unsigned)min((int64_t)kStep, (p.s.n - col0) * (int64_t)sizeof(T));
+        const unsigned d = in.at(w) - lane * 4 + lane % 16 * kPitch;
+        const bool x = lane >= 16;
+        unsigned size = 0;
+        if (c >= 0 && t < T_) {
+          const int64_t at = row * (x ? p.xb : p.zb) + col0 + t * (x ? p.xt : p.zt);
+          size = copy_row<T>(d + (x ? in.tensor : 0u), (x ? p.x : p.z) + at * (int64_t)sizeof(T), bytes, x ? p.xe : p.ze, in.bar(w));
+          if (!x && has_g)
+            size += copy_row<T>(d + 2 * in.tensor, p.g + (row * p.gb + col0 + t * p.gt) * (int64_t)sizeof(T), bytes, p.ge, in.bar(w));
+        }
+        size = __reduce_add_sync(0xffffffffu, size);
+        if (lane == 0) mbar_expect(in.bar(w), size);
+        __syncwarp();
+      }
+    } else if constexpr (MOVE == kTiles) {
       if (warp == warps - 1 && lane == 0 && w < waves) {  // (the warp whose slab is the tile's first)
-        uint64_t *bar = full + w % kStages;
+        uint64_t *bar = in.bar(w);
         const unsigned d = in.at(w);
         const int t = chunk_of(w) * kRun;  // negative in the last wave's tail: zeros
         mbar_expect(bar, (has_g ? 3 : 2) * in.tensor);
@@ -637,8 +720,8 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
     load_state<VEC>(c >= 0 ? p.ckpt : nullptr, c * p.ckpt_t + row * p.state_b + col, h);
   };
 
-  const Maps<VEC> maps = exchange_init<VEC>(swap, dyn + (kStages * 3 + (TMA ? 2 : 0)) * in.tensor, warps, warp, lane, cluster);
-  if (TMA) barriers_init(full, warp, lane);
+  const Maps<VEC> maps = exchange_init<VEC>(swap, dyn + (kStages * 3 + (MOVE == kTiles ? 2 : 0)) * in.tensor, warps, warp, lane, cluster);
+  if (MOVE != kLanes) barriers_init(full, kStages * (MOVE == kRows ? warps : 1), warp, lane);
   fetch(0);
   fetch(1);
   float next_h[VEC], s0[VEC];
@@ -673,9 +756,9 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
 #pragma unroll
     for (int k = 0; k < kRun; ++k) {
       float zv[VEC], xv[VEC];
-      read_word<T, VEC>(d + k * kStep, zv);
-      read_word<T, VEC>(d + in.tensor + k * kStep, xv);
-      raw[k] = read_raw(d + 2 * in.tensor + k * kStep);
+      read_word<T, VEC>(d + zsh(k) + k * kPitch, zv);
+      read_word<T, VEC>(d + in.tensor + xsh(k) + k * kPitch, xv);
+      raw[k] = read_raw(d + 2 * in.tensor + gsh(k) + k * kPitch);
       const C x = C::of(xv);
       if (STARTS && ((mask >> k) & 1)) s = zero;
       if (GATED) {
@@ -722,7 +805,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
     fetch(w + kStages);
     C u = resolve<VEC, STARTS>(maps, w, warps, warp, lane, cluster, rank, state, p.status);
     if (len > 0) {
-      if constexpr (TMA) {
+      if constexpr (MOVE == kTiles) {
         if (lane == 0) bulk_wait_read();
         __syncwarp();
       }
@@ -735,7 +818,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
         float dz[VEC], dx[VEC];
         (e * q[k]).get(dz);
         (GATED ? e * keep[k] : e).get(dx);
-        if constexpr (TMA) {
+        if constexpr (MOVE == kTiles) {
           stage_word<T>(slab + k * kStep, dz);
           stage_word<T>(slab + in.tensor + k * kStep, dx);
         } else {
@@ -754,7 +837,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
 #pragma unroll
         for (int k = kRun - 1; k >= 0; --k) put(k, false);
       }
-      if constexpr (TMA) {
+      if constexpr (MOVE == kTiles) {
         fence_async();
         __syncwarp();
         if (lane == 0) {
@@ -771,7 +854,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
 #pragma unroll
     for (int v = 0; v < VEC; ++v) p.dh0[row * p.state_b + col + v] = last[v];
   }
-  if (TMA && lane == 0) bulk_wait_read();
+  if (MOVE == kTiles && lane == 0) bulk_wait_read();
   if (cluster > 1) {  // no CTA leaves before the others are done with its memory
     cluster_arrive_relaxed();
     cluster_wait();
@@ -781,7 +864,8 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
 // ------------------------------------------------------------------ launch
 struct Plan {
   int vec, warps, cluster, waves;
-  bool flat, tma;
+  bool flat;
+  int move;
   int64_t groups;  // of all rows
   size_t smem;
 };
@@ -803,9 +887,9 @@ Pace pace_of(bool backward, int dtype) {
 }
 
 // Dynamic shared memory of a CTA.
-size_t smem_of(bool backward, bool tma, int vec, int warps, int cluster) {
-  const int inputs = backward ? 3 : 2, outputs = !tma ? 0 : backward ? 2 : 1;
-  return (size_t)(kStages * inputs + outputs) * warps * kSlab + (size_t)2 * (warps + (cluster > 1 ? cluster : 0)) * 32 * 8 * vec;
+size_t smem_of(bool backward, int move, int vec, int warps, int cluster) {
+  const int inputs = backward ? 3 : 2, outputs = move != kTiles ? 0 : backward ? 2 : 1;
+  return (size_t)(kStages * inputs + outputs) * warps * slab_bytes(move) + (size_t)2 * (warps + (cluster > 1 ? cluster : 0)) * 32 * 8 * vec;
 }
 
 // Clusters of c CTAs that run at once (a cluster stays within a GPC, so some
@@ -836,7 +920,7 @@ void split_time(Plan &pl, int nchunk, const Pace &m) {
     }
   }
   pl.waves = (nchunk + pl.warps * pl.cluster - 1) / (pl.warps * pl.cluster);
-  pl.smem = smem_of(m.backward, pl.tma, pl.vec, pl.warps, pl.cluster);
+  pl.smem = smem_of(m.backward, pl.move, pl.vec, pl.warps, pl.cluster);
 }
 
 struct Tensor3 {  // [T][rows][n] with contiguous n; null: not there
@@ -846,9 +930,7 @@ struct Tensor3 {  // [T][rows][n] with contiguous n; null: not there
 
 // One row of B * H columns when every tensor stores its batch rows back to
 // back and no start mask tells them apart; else B rows of H.  16-bit tensors
-// move two columns per lane where every row is 4-byte aligned, and all move by
-// TMA where bases and strides are multiples of 16 bytes and there is more than
-// one run (a single run, the serving step, is faster without the copies' set-up).
+// move two columns per lane where every row is 4-byte aligned.
 Plan make_plan(int dtype, bool starts, int64_t T, int64_t B, int64_t H, const Tensor3 *ts, int n, int nchunk,
                const Pace &pace) {
   Plan pl = {};
@@ -865,13 +947,29 @@ Plan make_plan(int dtype, bool starts, int64_t T, int64_t B, int64_t H, const Te
     return true;
   };
   pl.vec = dtype != HS_F32 && cols % 2 == 0 && fits(4) ? 2 : 1;
-  pl.tma = nchunk > 1 && pl.vec == 4 / es && fits(16) && cols <= 0x7fffffff && B <= 0x7fffffff;
-  for (int i = 0; i < n; ++i)  // strides a tensor map can hold
-    if (ts[i].p && (ts[i].t <= 0 || ts[i].t * es >= (int64_t)1 << 40 || (rows > 1 && (ts[i].b <= 0 || ts[i].b * es >= (int64_t)1 << 40)))) pl.tma = false;
+  bool whole = true, positive = true;  // strides that a tensor map can hold; that grow
+  for (int i = 0; i < n; ++i) {
+    if (!ts[i].p) continue;
+    const int64_t t = ts[i].t * es, b = rows > 1 ? ts[i].b * es : 0;
+    if (t <= 0 || t >= (int64_t)1 << 40 || (rows > 1 && (b <= 0 || b >= (int64_t)1 << 40))) whole = false;
+    if (t < 0 || b < 0 || !aligned(ts[i].p, 16)) positive = false;
+  }
   const int per = 32 * pl.vec;
   pl.groups = (cols + per - 1) / per * rows;
+  // Rows off 16 bytes: one by one where the columns are few (7179 x 1092
+  // float16, 18 groups: 35 us forward and 44 backward, by lanes 54 and 91), by lanes
+  // where they are many (4096 x 7154 bfloat16, 112 groups: 59 and 102, one by one 67 and 137).
+  if (nchunk > 1 && pl.vec == 4 / es) {
+    if (whole && fits(16) && cols <= 0x7fffffff && B <= 0x7fffffff) pl.move = kTiles;
+    else if (positive && pl.groups <= 96) pl.move = kRows;
+  }
   split_time(pl, nchunk, pace);
   return pl;
+}
+
+// One past the tensor's last element.
+const char *end_of(const Tensor3 &t, int dtype, int64_t T, int64_t B, int64_t H) {
+  return t.p ? (const char *)t.p + ((B - 1) * t.b + (T - 1) * t.t + H) * (int64_t)dtype_bytes(dtype) : nullptr;
 }
 
 RecShape shape_of(const Plan &pl, int64_t T, int64_t B, int64_t H, int nchunk) {
@@ -944,7 +1042,7 @@ int64_t clusters_at_once(const Pace &m, int warps, int c) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(ctas / c * c));
   cfg.blockDim = dim3(32, warps);
-  cfg.dynamicSmemBytes = smem_of(m.backward, true, 2, warps, c);
+  cfg.dynamicSmemBytes = smem_of(m.backward, kTiles, 2, warps, c);
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = (unsigned)c;
@@ -955,7 +1053,7 @@ int64_t clusters_at_once(const Pace &m, int warps, int c) {
     return allow_dynamic_smem((const void *)kernel, kSmemMost, &done[m.backward]) == HS_OK &&
            cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) == cudaSuccess && n > 0;
   };
-  if (!(m.backward ? ask(rec_bwd_kernel<__nv_bfloat16, 2, true, false, true>) : ask(rec_fwd_kernel<__nv_bfloat16, 2, true, false, true>))) {
+  if (!(m.backward ? ask(rec_bwd_kernel<__nv_bfloat16, 2, true, false, kTiles>) : ask(rec_fwd_kernel<__nv_bfloat16, 2, true, false, kTiles>))) {
     (void)cudaGetLastError();
     n = (int)(ctas / c);
   }
@@ -963,32 +1061,33 @@ int64_t clusters_at_once(const Pace &m, int warps, int c) {
   return n;
 }
 
-template <typename T, int VEC, bool GATED, bool STARTS, bool TMA> struct Kernel {
+template <typename T, int VEC, bool GATED, bool STARTS, int MOVE> struct Kernel {
   static int run(const FwdArgs &a, const Plan &pl, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
-    return launch(rec_fwd_kernel<T, VEC, GATED, STARTS, TMA>, a, pl, st, "rec_fwd_kernel", &done);
+    return launch(rec_fwd_kernel<T, VEC, GATED, STARTS, MOVE>, a, pl, st, "rec_fwd_kernel", &done);
   }
   static int run(const BwdArgs &a, const Plan &pl, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
-    return launch(rec_bwd_kernel<T, VEC, GATED, STARTS, TMA>, a, pl, st, "rec_bwd_kernel", &done);
+    return launch(rec_bwd_kernel<T, VEC, GATED, STARTS, MOVE>, a, pl, st, "rec_bwd_kernel", &done);
   }
 };
 
-template <typename T, int VEC, bool TMA, typename Args>
+template <typename T, int VEC, int MOVE, typename Args>
 int by_form(int form, const Args &a, const Plan &pl, cudaStream_t st) {
   const bool gated = form == HS_RECURRENCE_GATED, cuts = a.starts != nullptr;
-  if (gated) return cuts ? Kernel<T, VEC, true, true, TMA>::run(a, pl, st) : Kernel<T, VEC, true, false, TMA>::run(a, pl, st);
-  return cuts ? Kernel<T, VEC, false, true, TMA>::run(a, pl, st) : Kernel<T, VEC, false, false, TMA>::run(a, pl, st);
+  if (gated) return cuts ? Kernel<T, VEC, true, true, MOVE>::run(a, pl, st) : Kernel<T, VEC, true, false, MOVE>::run(a, pl, st);
+  return cuts ? Kernel<T, VEC, false, true, MOVE>::run(a, pl, st) : Kernel<T, VEC, false, false, MOVE>::run(a, pl, st);
+}
+template <typename T, typename Args> int by_move(int form, const Args &a, const Plan &pl, cudaStream_t st) {
+  constexpr int V = PerWord<T>::value;
+  if (pl.move == kTiles) return by_form<T, V, kTiles>(form, a, pl, st);
+  if (pl.move == kRows) return by_form<T, V, kRows>(form, a, pl, st);
+  return pl.vec == V ? by_form<T, V, kLanes>(form, a, pl, st) : by_form<T, 1, kLanes>(form, a, pl, st);
 }
 template <typename Args> int dispatch(int dtype, int form, const Args &a, const Plan &pl, cudaStream_t st) {
-  if (dtype == HS_F32) return pl.tma ? by_form<float, 1, true>(form, a, pl, st) : by_form<float, 1, false>(form, a, pl, st);
-  if (dtype == HS_BF16)
-    return pl.tma        ? by_form<__nv_bfloat16, 2, true>(form, a, pl, st)
-           : pl.vec == 2 ? by_form<__nv_bfloat16, 2, false>(form, a, pl, st)
-                         : by_form<__nv_bfloat16, 1, false>(form, a, pl, st);
-  return pl.tma        ? by_form<__half, 2, true>(form, a, pl, st)
-         : pl.vec == 2 ? by_form<__half, 2, false>(form, a, pl, st)
-                       : by_form<__half, 1, false>(form, a, pl, st);
+  if (dtype == HS_F32) return by_move<float>(form, a, pl, st);
+  if (dtype == HS_BF16) return by_move<__nv_bfloat16>(form, a, pl, st);
+  return by_move<__half>(form, a, pl, st);
 }
 
 int check_common(const char *who, int dtype, int form, int64_t T, int64_t B, int64_t H) {
@@ -1037,13 +1136,14 @@ int hs_recurrence_forward(int dtype, int form, const void *z, int64_t z_t, int64
   FwdArgs a = {};
   a.s = shape_of(pl, T, B, H, nchunk);
   a.z = (const char *)z, a.x = (const char *)x, a.h = (char *)h;
+  a.ze = end_of(ts[0], dtype, T, B, H), a.xe = end_of(ts[1], dtype, T, B, H);
   a.h0 = h0, a.h_n = h_n, a.ckpt = checkpoints, a.starts = starts;
   a.zt = z_t, a.zb = z_b, a.xt = x_t, a.xb = x_b, a.ht = h_t, a.hb = h_b, a.st = starts_t, a.sb = starts_b;
   a.state_b = H, a.ckpt_t = B * H, a.status = dev_status;
   if (checkpoints && starts) a.masks = reinterpret_cast<unsigned *>(checkpoints + (int64_t)nchunk * B * H);
   a.masks_t = B;
   const int tile = pl.warps * kRun;
-  if (pl.tma && !(encode(&a.zm, ts[0], dtype, pl, T, B, H, tile) && encode(&a.xm, ts[1], dtype, pl, T, B, H, tile) &&
+  if (pl.move == kTiles && !(encode(&a.zm, ts[0], dtype, pl, T, B, H, tile) && encode(&a.xm, ts[1], dtype, pl, T, B, H, tile) &&
                   encode(&a.hm, ts[2], dtype, pl, T, B, H, kRun)))
     return fail(HS_ERR_CUDA, "hs_recurrence_forward: cannot describe a tensor to TMA");
   return dispatch(dtype, form, a, pl, st);
@@ -1075,6 +1175,7 @@ int hs_recurrence_backward(int dtype, int form, const void *z, int64_t z_t, int6
   if (pl.groups * pl.cluster > 0x7fffffff) return fail(HS_ERR_UNSUPPORTED, "hs_recurrence_backward: too many columns");
   BwdArgs a = {};
   a.s = shape_of(pl, T, B, H, nchunk);
+  a.ze = end_of(ts[0], dtype, T, B, H), a.xe = end_of(ts[1], dtype, T, B, H), a.ge = end_of(ts[2], dtype, T, B, H);
   a.z = (const char *)z, a.x = (const char *)x, a.g = (const char *)dh, a.dz = (char *)dz, a.dx = (char *)dx;
   a.ckpt = checkpoints, a.dh_n = dh_n, a.dh0 = dh0;
   if (with_starts) a.starts = reinterpret_cast<const unsigned *>(checkpoints + (int64_t)nchunk * B * H);
@@ -1083,7 +1184,7 @@ int hs_recurrence_backward(int dtype, int form, const void *z, int64_t z_t, int6
   a.dzt = dz_t, a.dzb = dz_b, a.dxt = dx_t, a.dxb = dx_b;
   a.state_b = H, a.ckpt_t = B * H, a.status = dev_status;
   const int tile = pl.warps * kRun;
-  if (pl.tma && !(encode(&a.zm, ts[0], dtype, pl, T, B, H, tile) && encode(&a.xm, ts[1], dtype, pl, T, B, H, tile) &&
+  if (pl.move == kTiles && !(encode(&a.zm, ts[0], dtype, pl, T, B, H, tile) && encode(&a.xm, ts[1], dtype, pl, T, B, H, tile) &&
                   encode(&a.gm, ts[2], dtype, pl, T, B, H, tile) && encode(&a.dzm, ts[3], dtype, pl, T, B, H, kRun) &&
                   encode(&a.dxm, ts[4], dtype, pl, T, B, H, kRun)))
     return fail(HS_ERR_CUDA, "hs_recurrence_backward: cannot describe a tensor to TMA");

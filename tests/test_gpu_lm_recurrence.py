@@ -344,3 +344,22 @@ def test_refusals():
         P.gated_recurrence_step(z[0], z[0], torch.zeros(2, 8, device=DEV), out_state=torch.zeros(2, 16, device=DEV)[:, ::2])
     with pytest.raises(RuntimeError):
         P.gated_recurrence_step(z[0].requires_grad_(True), z[0], torch.zeros(2, 8, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("T,B,H", [(33, 1, 2), (100, 1, 6), (200, 1, 70), (97, 3, 94), (530, 1, 258), (70, 150, 46)])
+def test_rows_off_16_bytes(T, B, H, dtype):
+    """Rows that are 4-byte but not 16-byte aligned, alone and as slices, down
+    to rows shorter than a granule and up to the tensor's very last bytes."""
+    a, b, h0, s, dh, dh_n = make(T, B, H, dtype, "gated", seed=T + H, starts=True)
+    for starts in (None, s):
+        want, memory = truth(a, b, h0, starts, dh, dh_n, "gated")
+        check_all(run(a, b, h0, starts, dh, dh_n, "gated"), want, memory, f"starts={starts is not None}")
+    both = torch.cat((a, b), 2).to(DEV).requires_grad_(True)  # halves of one tensor
+    z, x = both.chunk(2, 2)
+    want, memory = truth(a, b, h0, None, dh, dh_n, "gated")
+    h, h_n = call("gated")(z, x, h0.to(DEV))
+    torch.autograd.backward((h, h_n), (dh.to(DEV), dh_n.to(DEV)))
+    check(h.detach(), want["h"], memory, "halves")
+    check(both.grad[..., :H], want["da"], memory, "halves da")
+    check(both.grad[..., H:], want["db"], memory, "halves db")
