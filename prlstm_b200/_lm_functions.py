@@ -61,6 +61,11 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
+def _float32(shape, like):
+    """A float32 tensor on the device of `like`, whatever torch's default dtype is."""
+    return torch.empty(shape, dtype=torch.float32, device=like.device)
+
+
 def _once(backward):
     """A backward that may be differentiated no further: ``once_differentiable``
     where a graph of it is asked for, itself (4 us less a call) where not."""
@@ -97,8 +102,8 @@ def _recurrence_forward(code, index, form, z, x, h0, starts, batch_first, keep):
     """(h, h_n, checkpoints) of checked arguments; z and x have contiguous rows."""
     T, B, H = _extents(z, batch_first)
     h = torch.empty_like(z)
-    h_n = torch.empty((B, H), device=z.device) if h0 is None else torch.empty_like(h0)
-    ckpt = torch.empty(-(-T // _RUN) * B * (H + 1), device=z.device) if keep else None  # states, masks of starts
+    h_n = _float32((B, H), z) if h0 is None else torch.empty_like(h0)
+    ckpt = _float32(-(-T // _RUN) * B * (H + 1), z) if keep else None  # states, masks of starts
     _call("hs_recurrence_forward", index, code, form, *_tensor(z, batch_first), *_tensor(x, batch_first), _p(h0),
           *_tensor(starts, batch_first), *_tensor(h, batch_first), h_n.data_ptr(), _p(ckpt), T, B, H,
           _lib.host_status(index).timeout_ptr)
@@ -124,7 +129,7 @@ class RecurrenceFn(torch.autograd.Function):
         dh = None if dh is None else _rows(dh)
         dh_n = None if dh_n is None else _state(dh_n)
         dz, dx = torch.empty_like(z), torch.empty_like(x)
-        dh0 = torch.empty((B, H), device=z.device) if h0_dtype is not None and ctx.needs_input_grad[2] else None
+        dh0 = _float32((B, H), z) if h0_dtype is not None and ctx.needs_input_grad[2] else None
         _call("hs_recurrence_backward", index, code, form, *_tensor(z, bf), *_tensor(x, bf), ckpt.data_ptr(),
               with_starts, *_tensor(dh, bf), _p(dh_n), *_tensor(dz, bf), *_tensor(dx, bf), _p(dh0), T, B, H,
               _lib.host_status(index).timeout_ptr)
@@ -296,12 +301,11 @@ class TokenLogprobs(NamedTuple):
 
 def _logprobs_forward(code, index, logits, tokens, bits, top, temperature, ignore_index, keep):
     N, V = logits.shape
-    dev = logits.device
-    logprob = torch.empty(N, device=dev)
+    logprob = _float32(N, logits)
     entropy = torch.empty_like(logprob)
-    top_lp = torch.empty((N, top), device=dev) if top else None
-    top_id = torch.empty((N, top), dtype=torch.int64, device=dev) if top else None
-    stats = torch.empty((N, 2), device=dev) if keep else None
+    top_lp = _float32((N, top), logits) if top else None
+    top_id = torch.empty((N, top), dtype=torch.int64, device=logits.device) if top else None
+    stats = _float32((N, 2), logits) if keep else None
     _call("hs_token_logprobs_forward", index, code, logits.data_ptr(), logits.stride(0), bits, tokens.data_ptr(),
           ignore_index, temperature, top, logprob.data_ptr(), entropy.data_ptr(), _p(top_lp), _p(top_id), _p(stats), N, V,
           _lib.host_status(index).token_ptr)

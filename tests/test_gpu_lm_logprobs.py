@@ -316,3 +316,26 @@ def test_refusals():
                      ((x, tok.cpu()), {}), ((x[:, :0], tok), {})):
         with pytest.raises(RuntimeError):
             op(*args, **kw)
+
+
+@pytest.mark.parametrize("default", [torch.float64, torch.bfloat16, torch.float16], ids=str)
+def test_results_are_float32_whatever_the_default_dtype(default):
+    x = torch.linspace(-3, 3, 5 * 301, dtype=torch.float32, device=DEV).view(5, 301)
+    tok = torch.arange(5, device=DEV)
+
+    def run():
+        leaf = x.clone().requires_grad_(True)
+        r = op(leaf, tok, top=3)
+        torch.autograd.backward([r.logprob, r.entropy, r.top_logprob],
+                                [torch.ones_like(r.logprob), torch.ones_like(r.entropy), torch.ones_like(r.top_logprob)])
+        return [t.detach() for t in r] + [leaf.grad]
+
+    want = run()
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(default)
+    try:
+        got = run()
+    finally:
+        torch.set_default_dtype(before)
+    for g, w in zip(got, want):
+        assert g.dtype == w.dtype and torch.equal(g, w)

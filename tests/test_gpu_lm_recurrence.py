@@ -363,3 +363,19 @@ def test_rows_off_16_bytes(T, B, H, dtype):
     check(h.detach(), want["h"], memory, "halves")
     check(both.grad[..., :H], want["da"], memory, "halves da")
     check(both.grad[..., H:], want["db"], memory, "halves db")
+
+
+@pytest.mark.parametrize("default", [torch.float64, torch.bfloat16, torch.float16], ids=str)
+def test_states_are_float32_whatever_the_default_dtype(default):
+    a, b, h0, s, dh, dh_n = make(70, 3, 40, torch.float32, "gated", seed=31, starts=True)
+    for start in (h0, None):
+        want = run(a, b, start, s, dh, dh_n, "gated")
+        before = torch.get_default_dtype()
+        torch.set_default_dtype(default)
+        try:
+            got = run(a, b, start, s, dh, dh_n, "gated")
+        finally:
+            torch.set_default_dtype(before)
+        for k, v in want.items():
+            if v is not None:
+                assert got[k].dtype == v.dtype and torch.equal(got[k], v), k
