@@ -26,6 +26,8 @@
 // the gradient, of which the sort takes 26 and the sums 88 (537 MB, 6.1 TB/s);
 // 8192 tokens of 32000 x 512 float32 take 5.3 and 31 us (sort 12: two passes
 // whose steps wait on one another).
+#include <float.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -47,12 +49,18 @@ template <> struct Chunk<8> { using type = uint2; };
 template <> struct Chunk<4> { using type = unsigned; };
 template <> struct Chunk<2> { using type = unsigned short; };
 
-// The scale as a sum of two float32, so that a product with it is rounded
-// once although the scale (the root of a width, say) is no float32.
+// The scale as a sum of two float32, so that a float32 product with it is rounded
+// once although the scale (the root of a width, say) is no float32; v * lo is kept
+// finite, as it would make a NaN of an infinity (with lo = 0, or of the other
+// sign).  A product that is rounded to 16 bits does without lo, which is
+// 2^-25 of it.
 struct Scale {
   float hi, lo;
 };
-HS_DEV float scaled(float v, Scale s) { return fmaf(v, s.hi, v * s.lo); }
+template <typename T> HS_DEV float scaled(float v, Scale s) {
+  if constexpr (sizeof(T) == 2) return v * s.hi;
+  return fmaf(v, s.hi, fmaxf(fminf(v * s.lo, FLT_MAX), -FLT_MAX));
+}
 Scale make_scale(double s) {
   const float hi = (float)s;
   const double lo = s - (double)hi;
@@ -137,7 +145,7 @@ __global__ void __launch_bounds__(256) emb_lookup_kernel(const char *w, int64_t 
       float v[E];
       chunk_to_f32<T, BYTES>(c[k], v);
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = scaled(v[e], scale);
+      for (int e = 0; e < E; ++e) v[e] = scaled<T>(v[e], scale);
       *reinterpret_cast<C *>(out + i * BYTES) = chunk_of_f32<T, BYTES>(v);
     }
   }
@@ -169,7 +177,7 @@ __global__ void __launch_bounds__(256) emb_lookup_rows_kernel(const char *w, int
         float v[E];
         chunk_to_f32<T, BYTES>(c[k], v);
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[e] = scaled(v[e], scale);
+        for (int e = 0; e < E; ++e) v[e] = scaled<T>(v[e], scale);
         dst[c0 + 32 * k] = chunk_of_f32<T, BYTES>(v);
       }
     }
@@ -520,7 +528,7 @@ __global__ void __launch_bounds__(256) emb_sum_kernel(const SumArgs p) {
               store_part<E>((from_prev ? p.head : p.tail) + piece * p.D + (int64_t)(chunk + 32 * q) * E, acc[q]);
             } else {
 #pragma unroll
-              for (int e = 0; e < E; ++e) acc[q][e] = scaled(acc[q][e], p.scale);
+              for (int e = 0; e < E; ++e) acc[q][e] = scaled<T>(acc[q][e], p.scale);
               *reinterpret_cast<C *>(p.dw + (int64_t)cur * row_bytes + (int64_t)(chunk + 32 * q) * BYTES) = chunk_of_f32<T, BYTES>(acc[q]);
             }
           }
@@ -585,7 +593,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps, 2) emb_join_kernel(const SumA
   auto write_row = [&](unsigned v, float *acc) {
     if (!live) return;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = scaled(acc[e], p.scale);
+    for (int e = 0; e < E; ++e) acc[e] = scaled<T>(acc[e], p.scale);
     *reinterpret_cast<C *>(p.dw + (int64_t)v * p.D * (int64_t)sizeof(T) + (int64_t)chunk * BYTES) = chunk_of_f32<T, BYTES>(acc);
   };
   const int64_t end = (piece + 1) * kPiece;

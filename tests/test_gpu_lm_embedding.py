@@ -164,3 +164,27 @@ def test_refusals():
             op(*bad)
     with pytest.raises(RuntimeError):
         op(tok, w, padding_idx=10)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("scale", [1.0, 0.5, -2.0, 20.0 ** 0.5, 0.1, -0.3, 0.0])
+def test_infinities_stay(scale, dtype):
+    """Rows with infinities and NaN, and gradients of them, are what the product in 64 bits gives."""
+    inf, nan = float("inf"), float("nan")
+    row = torch.tensor([inf, -inf, nan, 0.0, 1.0, -1.0, 4.0], dtype=torch.float64)
+    for D in (7, 8, 300):
+        w = row.repeat(D // 7 + 1)[:D].expand(3, D).to(dtype).to(DEV).clone().requires_grad_(True)
+        tok = torch.tensor([0, 2, 2, 1], device=DEV)
+        dout = row.flip(0).repeat(D // 7 + 1)[:D].expand(4, D).to(dtype).to(DEV)
+        out = op(tok, w, scale=scale)
+        out.backward(dout)
+        want = w.detach().double().cpu()[tok.cpu()] * scale
+        grad = torch.stack([dout[0].double().cpu() * n for n in (1, 1, 2)]) * scale
+        for got, t in ((out.detach(), want), (w.grad, grad)):
+            got = got.double().cpu()
+            assert torch.equal(got.isnan(), t.isnan()) and torch.equal(got.isinf(), t.isinf())
+            at = t.isinf()
+            assert torch.equal(got[at], t[at])
+            at = t.isfinite()
+            tol = 4 * 2.0 ** -24 + (UNIT[dtype] if dtype != torch.float32 else 0)
+            assert ((got[at] - t[at]).abs() <= tol * t[at].abs()).all()
