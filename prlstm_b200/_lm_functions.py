@@ -83,6 +83,14 @@ def _rows(t):
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
 
+def _like(t):
+    """An output laid out like `t`, its last axis contiguous.  (torch lays out the
+    like of overlapping rows, windows say, by their strides, the last axis not
+    always innermost.)"""
+    out = torch.empty_like(t)
+    return out if out.stride(-1) == 1 or out.shape[-1] <= 1 else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _tensor(t, batch_first):
     """Address and element strides of a step and of a sequence, as the library
     takes a [T, B, ..] tensor (or none)."""
@@ -101,7 +109,7 @@ def _extents(z, batch_first):
 def _recurrence_forward(code, index, form, z, x, h0, starts, batch_first, keep):
     """(h, h_n, checkpoints) of checked arguments; z and x have contiguous rows."""
     T, B, H = _extents(z, batch_first)
-    h = torch.empty_like(z)
+    h = _like(z)
     h_n = _float32((B, H), z) if h0 is None else torch.empty_like(h0)
     ckpt = _float32(-(-T // _RUN) * B * (H + 1), z) if keep else None  # states, masks of starts
     _call("hs_recurrence_forward", index, code, form, *_tensor(z, batch_first), *_tensor(x, batch_first), _p(h0),
@@ -128,7 +136,7 @@ class RecurrenceFn(torch.autograd.Function):
         T, B, H = _extents(z, bf)
         dh = None if dh is None else _rows(dh)
         dh_n = None if dh_n is None else _state(dh_n)
-        dz, dx = torch.empty_like(z), torch.empty_like(x)
+        dz, dx = _like(z), _like(x)
         dh0 = _float32((B, H), z) if h0_dtype is not None and ctx.needs_input_grad[2] else None
         _call("hs_recurrence_backward", index, code, form, *_tensor(z, bf), *_tensor(x, bf), ckpt.data_ptr(),
               with_starts, *_tensor(dh, bf), _p(dh_n), *_tensor(dz, bf), *_tensor(dx, bf), _p(dh0), T, B, H,
@@ -201,7 +209,7 @@ def _step(who, form, z, x, h, out_state):
         out_state = torch.empty_like(h)
     elif out_state.dtype is not torch.float32 or out_state.shape != shape or not out_state.is_contiguous():
         raise RuntimeError(f"{who}: out_state must be a contiguous float32 [B, H] tensor")
-    out = torch.empty_like(z)
+    out = _like(z)
     B, H = shape
     status = _lib.host_status(index)
     status.check()

@@ -379,3 +379,25 @@ def test_states_are_float32_whatever_the_default_dtype(default):
         for k, v in want.items():
             if v is not None:
                 assert got[k].dtype == v.dtype and torch.equal(got[k], v), k
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_overlapping_rows(dtype):
+    """Windows of a signal: every step's row a few elements on, fewer steps than columns and more."""
+    for T, H, hop in ((70, 64, 8), (5, 64, 1), (40, 33, 1), (20, 130, 1)):
+        signal = make(T * hop + H + 8 - H % 8, 2, 1, dtype, "gated", seed=T)
+        a, b = (t[:, :, 0].t().contiguous().to(DEV).unfold(1, H, hop)[:, :T].transpose(0, 1) for t in signal[:2])
+        assert a.shape == (T, 2, H) and a.stride(0) == hop
+        _, _, h0, _, dh, dh_n = make(T, 2, H, dtype, "gated", seed=T + 1)
+        want, memory = truth(a, b, h0, None, dh, dh_n, "gated")
+        z, x = a.detach().requires_grad_(True), b.detach().requires_grad_(True)
+        h, h_n = call("gated")(z, x, h0.to(DEV))
+        torch.autograd.backward([h, h_n], [dh.to(DEV), dh_n.to(DEV)])
+        check_all(dict(h=h.detach(), h_n=h_n.detach(), da=z.grad, db=x.grad, dh0=None), want, memory, f"T={T} H={H}")
+    import prlstm_b200 as P
+
+    rows = a[:, 0]  # the single step on overlapping rows
+    out, state = P.gated_recurrence_step(rows, b[:, 0], torch.zeros(T, H, device=DEV))
+    want, memory = truth(rows[None], b[:, 0][None], torch.zeros(T, H), None, None, None, "gated")
+    check(out, want["h"][0], memory, "step")
+    check(state, want["h_n"], memory, "step state", torch.float32)
