@@ -186,6 +186,7 @@ __global__ void __launch_bounds__(256) emb_lookup_rows_kernel(const char *w, int
 
 // ------------------------------------------------------------------ sort
 HS_DEV void cluster_sync_all() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 HS_DEV void st_cluster_u32(const void *p, int rank, unsigned v) {

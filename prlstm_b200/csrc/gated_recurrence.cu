@@ -268,6 +268,7 @@ HS_DEV Maps<VEC> exchange_init(uint64_t *bar, unsigned char *behind, int warps, 
       mbar_init(&m.bar[1]);
       fence_mbar_init();
     }
+    __syncwarp();
     cluster_arrive();
   }
   return m;
@@ -620,6 +621,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
   }
   if (MOVE == kTiles && lane == 0) bulk_wait_read();
   if (cluster > 1) {  // no CTA leaves before the others are done with its memory
+    __syncwarp();
     cluster_arrive_relaxed();
     cluster_wait();
   }
@@ -856,6 +858,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
   }
   if (MOVE == kTiles && lane == 0) bulk_wait_read();
   if (cluster > 1) {  // no CTA leaves before the others are done with its memory
+    __syncwarp();
     cluster_arrive_relaxed();
     cluster_wait();
   }

@@ -320,6 +320,7 @@ __global__ void __launch_bounds__(threads_of<W>(), 1024 / threads_of<W>()) logpr
     }
     return;
   }
+  __syncwarp();
   if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   const bool inside = tok >= 0 && tok < p.V;
   // the token's logit, loaded before the row: it is there when it is needed
@@ -487,6 +488,7 @@ __global__ void __launch_bounds__(threads_of<W>(), 1024 / threads_of<W>()) logpr
       a = reduce(sh.stat[lane & (W - 1)], W, p.k);
     }
     if (C > 1) {
+      __syncwarp();
       asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA has started
       if (warp == 0) {
         if (lane == 0) {
@@ -496,6 +498,7 @@ __global__ void __launch_bounds__(threads_of<W>(), 1024 / threads_of<W>()) logpr
         }
         if (TOP) st_remote(&sh.clist[rank][lane], 0, list);
       }
+      __syncwarp();
       asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
       if (rank != 0 || warp != 0) return;
       a = sh.cstat[0];
