@@ -13,26 +13,31 @@
 // hardware exp2 and about four other instructions (sums two at a time), below
 // the memory time for 16-bit logits too.
 //
-// Top alternatives cost the pass nothing: each thread already knows its
-// largest value.  A value that k of the threads' largest reach bounds the k-th
-// best of the row from below (found by bisection, a vote per step), and only
-// threads whose largest reaches it can hold alternatives.  Those threads'
-// values, little more than k / (threads) of the row, are read again (from L2), the few
-// that reach the bound are collected, and one warp sorts them.  Where equal
-// values make more than fit, the whole row is read again into a list per warp.
+// Top alternatives: each thread keeps its largest value, the batch of 4 vectors
+// that held it (in shared memory) and the largest value outside that batch.  A
+// value that k of the threads' largest reach bounds the k-th best of the row
+// from below (from the maxima of 32 groups of threads, then by bisection, a vote
+// per step), and only threads whose largest reaches it can hold alternatives:
+// most of them in the kept batch; the values of those whose second reaches it
+// too are read again (from L2; reading all of them again took 78 us in place of
+// 65 for 20 alternatives of 4096 rows of 32000 bfloat16).  The few values that reach the
+// bound are collected, and one warp sorts them.  Where equal values make more than
+// fit, the whole row is read again into a list per warp.
 // A key is the value's monotone 32-bit image with the complement of its index
 // below it, so the order is by value and, for equal values, by the lower index.
 //
-// Split: a CTA of 256 threads per row, a cluster of CTAs per row where there
-// are few rows (the parts meet in distributed shared memory), a warp per row
-// where the rows are short.
+// Split: a CTA of 128 or 256 threads per row, a cluster of CTAs per row where
+// there are few rows (the parts meet in distributed shared memory), a warp per
+// row where the rows are short.
 //
 // Measured on one B200 (plain copy 6.53 TB/s): 16384 rows of 32000 bfloat16
 // logits take 159-172 us forward (6.1-6.6 TB/s) and 323-333 for the gradient (6.3-6.5);
-// 2047 rows of 50021 take 43 us, with 5 alternatives 53, with 20 60: the
-// search adds 3 to 4 us to each row's own time, which other rows' passes
+// 2047 rows of 50021 take 41 us, with 5 alternatives 48, with 20 52: the
+// search adds about 3 us to each row's own time, which other rows' passes
 // only partly cover.  24 rows of 131072 float32 logits with 20 alternatives, on
-// eight CTAs each, take 10.4 us.
+// eight CTAs each, take 9.9 us.
+#include <type_traits>
+
 #include "lm_types.cuh"
 
 namespace hs {
@@ -257,13 +262,16 @@ template <typename T> struct Scan {
   }
 };
 
-constexpr int kChosen = 64, kFound = 64;  // threads read again, values collected: at most
+constexpr int kChosen = 64, kFound = 128;  // threads read again, values collected: at most
+constexpr int kBatch = 4;                 // vectors of a thread at a time
 
-// What finding the alternatives of one row needs.
+// What finding the alternatives of one row needs (chosen: the threads whose
+// values are read again).
 struct Finder {
   Key found[kFound];
-  int nfound, nchosen;
+  int nfound, nchosen, nkept;
   int chosen[kChosen];
+  int2 whose[kChosen];  // threads whose best batch holds all they have, and its first vector
 };
 // Shared memory of a CTA: one row's, or the finders of a row per warp.
 template <int W, bool TOP> struct Shared {
@@ -273,6 +281,7 @@ template <int W, bool TOP> struct Shared {
   Key list[TOP && W > 1 ? W : 1][32];
   Stat cstat[kMaxCluster];  // written by the cluster's CTAs
   Key clist[TOP ? kMaxCluster : 1][32];
+  uint4 kept[TOP ? kBatch : 1][TOP ? threads_of<W>() : 1];  // each thread's batch with its largest value
 };
 
 template <int W> HS_DEV void row_sync() {
@@ -298,7 +307,7 @@ HS_DEV void st_remote(const Key *p, int rank, Key v) {
 template <typename T, int W, bool TOP>
 __global__ void __launch_bounds__(threads_of<W>(), 1024 / threads_of<W>()) logprobs_fwd_kernel(const FwdArgs p) {
   __shared__ Shared<W, TOP> sh;
-  constexpr int NT = 32 * W, U = 4, E = Row<T>::E;
+  constexpr int NT = 32 * W, U = kBatch, E = Row<T>::E;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int tid = W == 1 ? lane : (int)threadIdx.x;
   const int C = W == 1 ? 1 : p.cluster, rank = (int)(blockIdx.x % C);
@@ -327,7 +336,8 @@ __global__ void __launch_bounds__(threads_of<W>(), 1024 / threads_of<W>()) logpr
   const float given = tid == 0 && rank == 0 && inside ? to_f32<T>(row[tok]) : 0.f;
   const Row<T> r(row, p.V, rank, C);
   Scan<T> scan;
-  if (tid < r.head) scan.scalar(to_f32<T>(row[tid]), p.k);
+  float second = kNegInf;  // the largest of the thread's vectors outside its best batch
+  int best = -1;           // that batch's first vector
   // U vectors at a time, the next ones on their way meanwhile; -inf, which adds
   // nothing, past the end
   auto load = [&](uint4 (&q)[U], int i) {
@@ -340,19 +350,32 @@ __global__ void __launch_bounds__(threads_of<W>(), 1024 / threads_of<W>()) logpr
       for (int k = 0; k < U; ++k) q[k] = i + k * NT < r.hi ? __ldg(r.vec(i + k * NT)) : make_uint4(w, w, w, w);
     }
   };
+  auto take = [&](const uint4 (&q)[U], int i) {
+    if constexpr (TOP) {
+      const float bm = vec_max<T, U>(q);
+      second = fmaxf(second, fminf(bm, scan.m));
+      if (bm > scan.m) {
+        best = i;
+#pragma unroll
+        for (int k = 0; k < U; ++k) sh.kept[k][threadIdx.x] = q[k];
+      }
+    }
+    scan.template vectors<U>(q, p.k);
+  };
   int at = r.lo + tid;
   if (at < r.hi) {
     uint4 q[2][U];
     load(q[0], at);
     while (true) {
       if ((at += U * NT) < r.hi) load(q[1], at);
-      scan.template vectors<U>(q[0], p.k);
+      take(q[0], at - U * NT);
       if (at >= r.hi) break;
       if ((at += U * NT) < r.hi) load(q[0], at);
-      scan.template vectors<U>(q[1], p.k);
+      take(q[1], at - U * NT);
       if (at >= r.hi) break;
     }
   }
+  if (tid < r.head) scan.scalar(to_f32<T>(row[tid]), p.k);
   if (tid < r.ntail) scan.scalar(to_f32<T>(row[r.tail0 + tid]), p.k);
 
   // the row's statistics
@@ -362,7 +385,7 @@ __global__ void __launch_bounds__(threads_of<W>(), 1024 / threads_of<W>()) logpr
   Key list = 0;
   if constexpr (TOP) {
     Finder &f = sh.f[W == 1 ? warp : 0];
-    if (tid == 0) f.nfound = f.nchosen = 0;
+    if (tid == 0) f.nfound = f.nchosen = f.nkept = 0;
     const bool some = tid < r.head || r.lo + tid < r.hi || tid < r.ntail;  // this thread holds values
     const unsigned mine = some ? order_bits(scan.m) : 0;
     // A bound that at least `top` threads reach, and not many more: the top-th
@@ -376,14 +399,14 @@ __global__ void __launch_bounds__(threads_of<W>(), 1024 / threads_of<W>()) logpr
       __syncthreads();
       v = sh.group[lane];
     }
-    int above = 0;
-#pragma unroll 8
-    for (int o = 0; o < 32; ++o) {
-      const unsigned w = __shfl_sync(0xffffffffu, v, o);
-      above += w > v || (w == v && o < lane);
-    }
-    unsigned lo = __shfl_sync(0xffffffffu, v, __ffs(__ballot_sync(0xffffffffu, above == p.top - 1)) - 1);
-    unsigned hi = __reduce_max_sync(0xffffffffu, v);
+#pragma unroll
+    for (int size = 2; size <= 32; size <<= 1)  // in descending order of lanes
+#pragma unroll
+      for (int o = size >> 1; o; o >>= 1) {
+        const unsigned w = __shfl_xor_sync(0xffffffffu, v, o);
+        v = ((lane & o) == 0) == ((lane & size) == 0) ? max(v, w) : min(v, w);
+      }
+    unsigned lo = __shfl_sync(0xffffffffu, v, p.top - 1), hi = __shfl_sync(0xffffffffu, v, 0);
     if (lo == 0) lo = 1;  // some groups hold nothing
     hi += 1;
     int c = row_count<W>(mine >= lo);
@@ -393,59 +416,92 @@ __global__ void __launch_bounds__(threads_of<W>(), 1024 / threads_of<W>()) logpr
       if (n >= p.top) lo = mid, c = n; else hi = mid;
     }
     if (c < p.top) lo = 1;  // fewer threads with values than alternatives: all of them
-    if (some && mine >= lo) {
-      const int at = atomicAdd(&f.nchosen, 1);  // in any order: the keys are sorted
-      if (at < kChosen) f.chosen[at] = tid;
-    }
-    row_sync<W>();
-    const int nchosen = f.nchosen;
+    // the bound as a value (below -inf's image: everything but NaN)
+    const float bound = lo <= order_bits(kNegInf) ? kNegInf : value_of((Key)lo << 32);
     auto collect = [&](float v, int at) {
-      const unsigned b = order_bits(v);
-      if (b < lo || isnan(v)) return;
-      const int k = atomicAdd(&f.nfound, 1);
+      if (!(v >= bound)) return;
+      const int k = atomicAdd(&f.nfound, 1);  // in any order: the keys are sorted
       if (k < kFound) f.found[k] = make_key(v, at);
     };
-    if (nchosen <= kChosen) {
-      if (mine >= lo && tid < r.head) collect(to_f32<T>(row[tid]), tid);
-      if (mine >= lo && tid < r.ntail) collect(to_f32<T>(row[r.tail0 + tid]), r.tail0 + tid);
-      const int per = (r.hi - r.lo + NT - 1) / NT, all = nchosen * per;  // vectors of a thread, of all
+    auto vector = [&](const uint4 &q, int at) {
+      float v[E];
+      unpack_vec<T>(q, v);
+      unsigned hit = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) hit |= v[e] >= bound ? 1u << e : 0u;
+      if (!hit) return;
+      int k = atomicAdd(&f.nfound, __popc(hit));
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if ((hit >> e) & 1) {
+          if (k < kFound) f.found[k] = make_key(v[e], r.index(at, e));
+          ++k;
+        }
+    };
+    if (some && scan.m >= bound) {
+      if (tid < r.head) collect(to_f32<T>(row[tid]), tid);
+      if (tid < r.ntail) collect(to_f32<T>(row[r.tail0 + tid]), r.tail0 + tid);
+      if (second >= bound) {  // beyond the best batch too
+        const int at = atomicAdd(&f.nchosen, 1);
+        if (at < kChosen) f.chosen[at] = tid;
+      } else if (best >= 0) {
+        const int at = atomicAdd(&f.nkept, 1);
+        if (at < kChosen) f.whose[at] = make_int2(threadIdx.x, best);
+      }
+    }
+    row_sync<W>();
+    const int nchosen = f.nchosen, nkept = f.nkept;
+    if (nchosen <= kChosen && nkept <= kChosen) {
+      // the vectors of the chosen threads from memory, then the kept batches
+      const int per = (r.hi - r.lo + NT - 1) / NT, all = nchosen * per, items = all + nkept * U;
       constexpr int G = W == 1 ? 1 : 3;  // loads at once
-      for (int j0 = tid; j0 < all; j0 += G * NT) {
+      for (int j0 = tid; j0 < items; j0 += G * NT) {
         uint4 q[G];
         int at[G];
 #pragma unroll
         for (int k = 0; k < G; ++k) {
-          const int j = j0 + k * NT, t = j / per;
-          at[k] = j < all ? r.lo + f.chosen[t] + (j - t * per) * NT : r.hi;
-          if (at[k] < r.hi) q[k] = __ldg(r.vec(at[k]));
+          const int j = j0 + k * NT;
+          at[k] = r.hi;
+          if (j < all) {
+            const int t = j / per;
+            at[k] = r.lo + f.chosen[t] + (j - t * per) * NT;
+            if (at[k] < r.hi) q[k] = __ldg(r.vec(at[k]));
+          } else if (j < items) {
+            const int2 o = f.whose[(j - all) / U];
+            at[k] = o.y + (j - all) % U * NT;
+            q[k] = sh.kept[(j - all) % U][o.x];
+          }
         }
 #pragma unroll
-        for (int k = 0; k < G; ++k) {
-          if (at[k] >= r.hi || order_bits(vec_max<T>(q[k])) < lo) continue;
-          float v[E];
-          unpack_vec<T>(q[k], v);
-#pragma unroll
-          for (int e = 0; e < E; ++e) collect(v[e], r.index(at[k], e));
-        }
+        for (int k = 0; k < G; ++k)
+          if (at[k] < r.hi) vector(q[k], at[k]);
       }
     }
     row_sync<W>();
     const int n = f.nfound;
-    if (nchosen <= kChosen && n <= kFound) {
+    if (nchosen <= kChosen && nkept <= kChosen && n <= kFound) {
       if (W == 1 || warp == 0) {
         // in order by counting the larger ones
-        const Key a0 = lane < n ? f.found[lane] : 0, a1 = lane + 32 < n ? f.found[lane + 32] : 0;
-        int before0 = 0, before1 = 0;
+        auto rank = [&](auto keys) {
+          constexpr int M = decltype(keys)::value;  // of a lane
+          Key a[M];
+          int before[M] = {};
+#pragma unroll
+          for (int i = 0; i < M; ++i) a[i] = lane + 32 * i < n ? f.found[lane + 32 * i] : 0;
 #pragma unroll 4
-        for (int j = 0; j < n; ++j) {
-          const Key k = f.found[j];
-          before0 += k > a0;
-          before1 += k > a1;
-        }
-        __syncwarp();
-        if (lane < n && before0 < 32) f.found[before0] = a0;
-        if (lane + 32 < n && before1 < 32) f.found[before1] = a1;
-        __syncwarp();
+          for (int j = 0; j < n; ++j) {
+            const Key k = f.found[j];
+#pragma unroll
+            for (int i = 0; i < M; ++i) before[i] += k > a[i];
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < M; ++i)
+            if (lane + 32 * i < n && before[i] < 32) f.found[before[i]] = a[i];
+          __syncwarp();
+        };
+        if (n <= 64) rank(std::integral_constant<int, 2>{});
+        else rank(std::integral_constant<int, kFound / 32>{});
         list = lane < n ? f.found[lane] : 0;
       }
     } else {  // too many equal values
@@ -645,11 +701,14 @@ __global__ void __launch_bounds__(threads_of<W>()) logprobs_bwd_kernel(const Bwd
 // ------------------------------------------------------------------ launch
 // Warps per row.  One up to 4 KB (4096 rows of 1 KB: 3.5 us, with four warps
 // 10.5), in the forward of many rows up to 8 KB (8192 of 8 KB: 16.8 against 23.5
-// us); four up to 64 KB (16384 of 64 KB: 174 us, with eight 195); else eight
-// (the gradient of 2047 rows of 100 KB: 77 us, with four 81).
+// us); four up to 64 KB (16384 of 64 KB: 174 us, with eight 195), in the forward
+// of any longer rows where they alone fill the SMs (600 rows of 100 KB with 5
+// alternatives: 20.8 us, with eight 24.4; 2047: 48.5 and 53.8; but 500 of 600
+// KB: 68 and 60); else eight (the gradient of 2047 rows of 100 KB: 77 us, with
+// four 81).
 int warps_of(bool forward, int64_t N, int64_t row_bytes) {
   if (row_bytes <= 4096 || (forward && row_bytes <= 8192 && N >= 2048)) return 1;
-  return row_bytes <= 65536 ? 4 : 8;
+  return row_bytes <= 65536 || (forward && N >= 4 * 148) ? 4 : 8;
 }
 
 // CTAs per row, of 8 KB at least.  The forward's meet in a cluster, which

@@ -339,3 +339,24 @@ def test_results_are_float32_whatever_the_default_dtype(default):
         torch.set_default_dtype(before)
     for g, w in zip(got, want):
         assert g.dtype == w.dtype and torch.equal(g, w)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("N,V", [(2, 20000), (600, 20011), (9, 1500), (2048, 3000), (600, 40000)])
+def test_alternatives_wherever_they_lie(N, V, dtype):
+    """The largest values next to one another, or one thread's vectors, batches or rows' parts apart."""
+    strides = [1, 2, 3, 4, 8, 32, 64, 128, 256, 512, 1000, 1024, 2048, 4096, 8192]
+    x = torch.zeros(N, V, device=DEV)
+    g = torch.Generator().manual_seed(V)
+    want = torch.empty(N, 32, dtype=torch.int64)
+    for n in range(N):
+        stride = strides[n % len(strides)]
+        at = (torch.arange(32) * stride + int(torch.randint(V, (1,), generator=g))) % V
+        if len(at.unique()) < 32:  # the stride divides the row: wrap to neighbours
+            at = torch.arange(32) + n % (V - 32)
+        want[n] = at[torch.randperm(32, generator=g)] if n % 3 else at if n % 2 else at.flip(0)
+    value = torch.arange(132, 100, -1, dtype=torch.float32, device=DEV)  # exact in every type
+    x.scatter_(1, want.to(DEV), value.expand(N, 32))
+    for top in (1, 5, 32):
+        r = op(x.to(dtype), torch.zeros(N, dtype=torch.int64, device=DEV), top=top)
+        assert torch.equal(r.top_index.cpu(), want[:, :top]), top
