@@ -416,16 +416,28 @@ template <typename T> HS_DEV unsigned copy_row(unsigned dst, const char *src, un
   return size;
 }
 
-// The starts among the steps t .. t+15 as bits.  A warp reads those of its next
-// 32 waves at once, one wave per lane: read wave by wave, the load's latency
-// showed in every one of them (25% of the forward's time, 40% of the backward's).
+// The starts among the 16 steps of each of a warp's next 32 waves, as bits, one
+// wave per lane.  Read wave by wave, the load's latency showed in every one of
+// them (25% of the forward's time, 40% of the backward's).  The two halves of
+// the warp read the steps of two waves at a time (neighbours in memory, where a lane
+// per wave touched 32 lines a load).
 // The forward leaves the masks with the saved states: the backward loads one
 // word per run in place of 16 bytes (257 -> 244 us at T=16384, B=8, H=1024 bf16).
-HS_DEV unsigned start_mask(const unsigned char *starts, int64_t stride, int64_t t, int64_t T) {
+template <typename F>
+HS_DEV unsigned start_masks(const unsigned char *starts, int64_t stride, int w, int waves, int lane, int64_t T, F start_of) {
   unsigned m = 0;
+  bool cut[16];
 #pragma unroll
-  for (int k = 0; k < kRun; ++k)
-    if (t + k < T && starts[(t + k) * stride]) m |= 1u << k;
+  for (int j = 0; j < 16; ++j) {
+    const int wave = w + 2 * j + lane / 16;
+    const int64_t t = start_of(wave) + lane % 16;
+    cut[j] = wave < waves && t < T && starts[t * stride] != 0;
+  }
+#pragma unroll
+  for (int j = 0; j < 16; ++j) {
+    const unsigned two = __ballot_sync(0xffffffffu, cut[j]);
+    if (lane / 2 == j) m = lane & 1 ? two >> 16 : two & 0xffffu;
+  }
   return m;
 }
 
@@ -509,7 +521,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
       cp_commit();
     }
   };
-  auto starts_from = [&](int w) { return w + lane < waves ? start_mask(p.starts + row * p.sb, p.st, start_of(w + lane), T_) : 0u; };
+  auto starts_from = [&](int w) { return start_masks(p.starts + row * p.sb, p.st, w, waves, lane, T_, start_of); };
 
   const Maps<VEC> maps = exchange_init<VEC>(swap, dyn + (kStages * 2 + (MOVE == kTiles ? 1 : 0)) * in.tensor, warps, warp, lane, cluster);
   if (MOVE != kLanes) barriers_init(full, kStages * (MOVE == kRows ? warps : 1), warp, lane);
