@@ -220,16 +220,26 @@ template <typename T, int VEC> HS_DEV void write_word(char *dst, const float *v)
     *reinterpret_cast<T *>(dst) = from_f32<T>(v[0]);
 }
 
-// The map h -> a h + b of a run of steps, of one lane's columns.  a = +inf
-// marks a run that a start lies in: nothing passes it, the map is b alone.  (A
-// product of gates is at most 1; one of given coefficients is held to the
-// largest finite value, so that it leaves a zero state zero as step by step.)
+// The map h -> a h + b of a run of steps, of one lane's columns.  a = -0 marks
+// a run that a start lies in: nothing passes it, the map is b alone.  For a
+// finite h that is what a h + b gives, so maps are chained without a look at the marks,
+// and a chain that ends in NaN is gone through once more with them (with a
+// look at each: 80 us in place of 74 at T=16384, B=2, H=1024 float32).  (A product of
+// gates is at most 1; one of given coefficients is held to the largest finite
+// value, so that it leaves a zero state zero as step by step.)
 template <int VEC> struct __align__(8 * VEC) Map {
   float a[VEC], b[VEC];
+  HS_DEV bool cut() const { return __float_as_uint(a[0]) == 0x80000000u; }
 };
-template <int VEC, bool STARTS> HS_DEV Cols<VEC> apply(const Map<VEC> &m, Cols<VEC> h) {
-  const Cols<VEC> b = Cols<VEC>::of(m.b), r = fma(Cols<VEC>::of(m.a), h, b);
-  return STARTS && m.a[0] == __int_as_float(0x7f800000) ? b : r;
+template <int VEC> HS_DEV Cols<VEC> apply(const Map<VEC> &m, Cols<VEC> h) { return fma(Cols<VEC>::of(m.a), h, Cols<VEC>::of(m.b)); }
+template <int VEC> HS_DEV Cols<VEC> apply_marked(const Map<VEC> &m, Cols<VEC> h) { return m.cut() ? Cols<VEC>::of(m.b) : apply(m, h); }
+template <int VEC> HS_DEV bool any_nan(Cols<VEC> h) {
+  float v[VEC];
+  h.get(v);
+  bool r = false;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) r |= v[i] != v[i];
+  return r;
 }
 template <int VEC, bool GATED> HS_DEV Cols<VEC> held(Cols<VEC> a) {
   if (GATED) return a;
@@ -285,27 +295,36 @@ HS_DEV void publish(const Maps<VEC> &m, int w, int warps, int warp, int lane, in
   Map<VEC> mine;
   held<VEC, GATED>(A).get(mine.a);
   B.get(mine.b);
-  if (STARTS && cut) mine.a[0] = __int_as_float(0x7f800000);
+  if (STARTS) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) mine.a[i] = cut ? -0.f : GATED ? mine.a[i] : mine.a[i] + 0.f;  // (a -0 by itself: +0)
+  }
   const Map<VEC> *all = m.warp + p * warps * 32;
   m.warp[(p * warps + warp) * 32] = mine;
   __syncthreads();
   if (cluster == 1) return;
   if (warp == 0 && lane == 0) mbar_expect(&m.bar[p], cluster * 32 * (unsigned)sizeof(Map<VEC>));
   if (warp == warps - 1) {  // the CTA's map, to every CTA of the cluster
-    const Cols<VEC> none = Cols<VEC>::all(0.f);
-    Cols<VEC> ta = Cols<VEC>::all(1.f), tb = none;
+    Cols<VEC> ta = Cols<VEC>::all(1.f), tb = Cols<VEC>::all(0.f);
     bool any = false;
 #pragma unroll 4
     for (int j = 0; j < warps; ++j) {
       const Map<VEC> e = all[j * 32];
-      if (STARTS && e.a[0] == __int_as_float(0x7f800000)) any = true;
-      tb = apply<VEC, STARTS>(e, tb);
+      if (STARTS) any |= e.cut();
+      tb = apply(e, tb);
       ta = held<VEC, GATED>(Cols<VEC>::of(e.a) * ta);
+    }
+    if (STARTS && any && any_nan(tb)) {
+      tb = Cols<VEC>::all(0.f);
+      for (int j = 0; j < warps; ++j) tb = apply_marked(all[j * 32], tb);
     }
     Map<VEC> t;
     ta.get(t.a);
     tb.get(t.b);
-    if (STARTS && any) t.a[0] = __int_as_float(0x7f800000);
+    if (STARTS) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) t.a[i] = any ? -0.f : GATED ? t.a[i] : t.a[i] + 0.f;
+    }
     for (int r = 0; r < cluster; ++r) {
       const unsigned to = cluster_addr(&m.cta[(p * cluster + rank) * 32], r), bar = cluster_addr(&m.bar[p], r);
       if constexpr (VEC == 2)
@@ -326,25 +345,42 @@ template <int VEC, bool STARTS>
 HS_DEV Cols<VEC> resolve(const Maps<VEC> &m, int w, int warps, int warp, int lane, int cluster, int rank, Cols<VEC> &state, int *status) {
   const int p = w & 1;
   const Map<VEC> *all = m.warp + p * warps * 32;
+  const Cols<VEC> entry = state;
   Cols<VEC> in = state;
   if (cluster == 1) {
 #pragma unroll 4
     for (int j = 0; j < warps; ++j) {
       if (j == warp) in = state;
-      state = apply<VEC, STARTS>(all[j * 32], state);
+      state = apply(all[j * 32], state);
+    }
+    if (STARTS && any_nan(state)) {
+      state = entry;
+      for (int j = 0; j < warps; ++j) {
+        if (j == warp) in = state;
+        state = apply_marked(all[j * 32], state);
+      }
     }
     return in;
   }
   mbar_wait(&m.bar[p], (w >> 1) & 1, status);
+  const Map<VEC> *ctas = m.cta + p * cluster * 32;
 #pragma unroll
   for (int r = 0; r < kMaxCluster; ++r) {
     if (r < cluster) {
       if (r == rank) in = state;
-      state = apply<VEC, STARTS>(m.cta[(p * cluster + r) * 32], state);
+      state = apply(ctas[r * 32], state);
     }
   }
 #pragma unroll 4
-  for (int j = 0; j < warp; ++j) in = apply<VEC, STARTS>(all[j * 32], in);
+  for (int j = 0; j < warp; ++j) in = apply(all[j * 32], in);
+  if (STARTS && (any_nan(state) || any_nan(in))) {
+    state = in = entry;
+    for (int r = 0; r < cluster; ++r) {
+      if (r == rank) in = state;
+      state = apply_marked(ctas[r * 32], state);
+    }
+    for (int j = 0; j < warp; ++j) in = apply_marked(all[j * 32], in);
+  }
   return in;
 }
 

@@ -401,3 +401,21 @@ def test_overlapping_rows(dtype):
     want, memory = truth(rows[None], b[:, 0][None], torch.zeros(T, H), None, None, None, "gated")
     check(out, want["h"][0], memory, "step")
     check(state, want["h_n"], memory, "step state", torch.float32)
+
+
+@pytest.mark.parametrize("zero", [0.0, -0.0])
+def test_a_zero_coefficient_is_no_start(zero):
+    """An infinite state times a zero of either sign is NaN, step by step; a start drops it."""
+    T, H = 3000, 40
+    a, b = torch.ones(T, 1, H, device=DEV), torch.zeros(T, 1, H, device=DEV)
+    a[1000], b[2000] = zero, 3.0
+    s = torch.zeros(T, 1, dtype=torch.bool, device=DEV)
+    s[2000] = True
+    h0 = torch.full((1, H), float("inf"), device=DEV)
+    for starts in (s, torch.zeros_like(s)):
+        h, h_n = call("linear")(a, b, h0, starts=starts)
+        assert h[:1000].isposinf().all() and h[1000:2000].isnan().all()
+        if starts is s:
+            assert (h[2000:] == 3.0).all() and (h_n == 3.0).all()
+        else:
+            assert h[2000:].isnan().all() and h_n.isnan().all()
