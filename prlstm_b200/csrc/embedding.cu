@@ -22,9 +22,9 @@
 // floating-point data, and the order of every sum follows from the tokens alone.
 //
 // Measured on one B200 (plain copy 6.53 TB/s), ids as skewed as text: 131072
-// tokens of a 131072 x 1024 bfloat16 table take 61 us for the lookup and 132 for
+// tokens of a 131072 x 1024 bfloat16 table take 60 us for the lookup and 131 for
 // the gradient, of which the sort takes 26 and the sums 88 (537 MB, 6.1 TB/s);
-// 8192 tokens of 32000 x 512 float32 take 5.3 and 31 us (sort 12: two passes
+// 8192 tokens of 32000 x 512 float32 take 5.4 and 31 us (sort 12: two passes
 // whose steps wait on one another).
 #include <float.h>
 
