@@ -102,9 +102,20 @@ HS_DEV void cp_async4(unsigned dst, const void *src) {
 }
 HS_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> HS_DEV void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-HS_DEV void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
-HS_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-HS_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// The aligned forms are for a whole warp at once, whatever its lanes did before
+// (polled a barrier, say, each for itself).
+HS_DEV void cluster_arrive_relaxed() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+HS_DEV void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+HS_DEV void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 HS_DEV void fence_mbar_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 HS_DEV void mbar_init(uint64_t *b) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(b)) : "memory");
@@ -278,7 +289,6 @@ HS_DEV Maps<VEC> exchange_init(uint64_t *bar, unsigned char *behind, int warps, 
       mbar_init(&m.bar[1]);
       fence_mbar_init();
     }
-    __syncwarp();
     cluster_arrive();
   }
   return m;
@@ -410,12 +420,14 @@ template <int MOVE, int N> struct Inputs {
   int warp, warps;
   HS_DEV unsigned at(int w) const { return base + (unsigned)(w % kStages) * (N * tensor); }
   HS_DEV uint64_t *bar(int w) const { return full + (w % kStages) * (MOVE == kRows ? warps : 1) + (MOVE == kRows ? warp : 0); }
-  // Waits until wave w is there.
+  // Waits until wave w is there; a warp's lanes, which poll each for itself, go on together.
   HS_DEV void wait(int w) const {
-    if constexpr (MOVE == kLanes)
+    if constexpr (MOVE == kLanes) {
       cp_wait<kStages - 1>();
-    else
+    } else {
       mbar_wait(bar(w), (w / kStages) & 1, status);
+      __syncwarp();
+    }
   }
 };
 
@@ -669,7 +681,6 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
   }
   if (MOVE == kTiles && lane == 0) bulk_wait_read();
   if (cluster > 1) {  // no CTA leaves before the others are done with its memory
-    __syncwarp();
     cluster_arrive_relaxed();
     cluster_wait();
   }
@@ -906,7 +917,6 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
   }
   if (MOVE == kTiles && lane == 0) bulk_wait_read();
   if (cluster > 1) {  // no CTA leaves before the others are done with its memory
-    __syncwarp();
     cluster_arrive_relaxed();
     cluster_wait();
   }

@@ -1,0 +1,25 @@
+"""What the language-model operators' sources have to hold to and a run would
+show by chance only (CPU only)."""
+
+import os
+import re
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "prlstm_b200", "csrc")
+
+
+def source(name):
+    with open(os.path.join(CSRC, name)) as f:
+        return f.read()
+
+
+@pytest.mark.parametrize("name", ["gated_recurrence.cu", "token_logprobs.cu", "embedding.cu"])
+def test_warps_meet_before_aligned_cluster_barriers(name):
+    """An aligned barrier is one instruction of the whole warp: whatever stands
+    before it, the lanes are brought together first."""
+    lines = source(name).splitlines()
+    at = [i for i, line in enumerate(lines) if re.search(r"barrier\.cluster\.\w+\.\w+\.aligned", line)]
+    assert at
+    for i in at:
+        assert "__syncwarp();" in lines[i - 1], f"{name}:{i + 1}"
