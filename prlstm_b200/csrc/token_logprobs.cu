@@ -386,6 +386,7 @@ __global__ void __launch_bounds__(threads_of<W>(), 1024 / threads_of<W>()) logpr
   if constexpr (TOP) {
     Finder &f = sh.f[W == 1 ? warp : 0];
     if (tid == 0) f.nfound = f.nchosen = f.nkept = 0;
+    if (W == 1) __syncwarp();  // before any lane counts (shuffles and votes order no memory)
     const bool some = tid < r.head || r.lo + tid < r.hi || tid < r.ntail;  // this thread holds values
     const unsigned mine = some ? order_bits(scan.m) : 0;
     // A bound that at least `top` threads reach, and not many more: the top-th

@@ -360,3 +360,15 @@ def test_alternatives_wherever_they_lie(N, V, dtype):
     for top in (1, 5, 32):
         r = op(x.to(dtype), torch.zeros(N, dtype=torch.int64, device=DEV), top=top)
         assert torch.equal(r.top_index.cpu(), want[:, :top]), top
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("V", [33, 300, 1000])
+def test_alternatives_of_many_short_rows(V, dtype):
+    """A warp per row, many rows after one another in the same shared memory."""
+    N = 20000
+    x, tok = normal(N, V, dtype, seed=V)
+    for top in (1, 6, 32):
+        r = op(x, tok, top=top)
+        want = torch.sort(x.double(), dim=1, descending=True, stable=True).indices[:, :top]
+        assert torch.equal(r.top_index, want), top

@@ -23,3 +23,13 @@ def test_warps_meet_before_aligned_cluster_barriers(name):
     assert at
     for i in at:
         assert "__syncwarp();" in lines[i - 1], f"{name}:{i + 1}"
+
+
+def test_counters_are_zero_before_any_lane_counts():
+    """The finder of a row's alternatives: one lane clears the counters, others
+    add to them; between the two memory is ordered for a warp per row (votes do not
+    order it) and for a CTA per row."""
+    text = source("token_logprobs.cu")
+    clear = text.index("f.nfound = f.nchosen = f.nkept = 0;")
+    between = text[clear:text.index("atomicAdd(&f.", clear)]
+    assert "if (W == 1) __syncwarp();" in between and "__syncthreads();" in between
