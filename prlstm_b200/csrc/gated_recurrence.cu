@@ -456,6 +456,7 @@ template <typename T> HS_DEV unsigned copy_row(unsigned dst, const char *src, un
       else
         asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + (unsigned)(q - from)), "h"(*reinterpret_cast<const unsigned short *>(q)) : "memory");
     }
+    fence_async();  // these stores before the bulk copies that fill the place in later waves (the backward's)
   }
   if (size)
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(from),

@@ -33,3 +33,13 @@ def test_counters_are_zero_before_any_lane_counts():
     clear = text.index("f.nfound = f.nchosen = f.nkept = 0;")
     between = text[clear:text.index("atomicAdd(&f.", clear)]
     assert "if (W == 1) __syncwarp();" in between and "__syncthreads();" in between
+
+
+def test_stores_precede_bulk_copies_into_the_same_place():
+    """The rows' copies write some bytes by the lanes themselves; a later wave's
+    bulk copy goes into the same bytes by another path, which only a fence orders."""
+    text = source("gated_recurrence.cu")
+    body = text[text.index("HS_DEV unsigned copy_row("):]
+    body = body[:body.index("\n}\n")]
+    stores, fence = body.rindex("st.shared.u16"), body.find("fence_async();")
+    assert stores < fence < body.index("cp.async.bulk.shared::cluster")
