@@ -499,7 +499,10 @@ enum {
  * or NaN, reaches it.  h_n [B,H] (NULL = not wanted) is the state after the
  * last step; it may be h0 itself.  checkpoints (NULL = no backward will
  * follow): hs_recurrence_checkpoint_bytes(T, B, H) bytes for the backward.
- * T = 1 is the single-token step of serving. */
+ * T = 1 is the single-token step of serving.
+ * Given coefficients may be of any size: states stay what steps taken one by one
+ * give although a product of coefficients in between passes float32's range; a
+ * state beyond it is an infinity from that step on. */
 HS_API size_t hs_recurrence_checkpoint_bytes(int64_t T, int64_t B, int64_t H);
 HS_API int hs_recurrence_forward(int dtype, int form, const void *z, int64_t z_t, int64_t z_b, const void *x,
                                  int64_t x_t, int64_t x_b, const float *h0, const unsigned char *starts,

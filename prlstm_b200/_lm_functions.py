@@ -189,7 +189,8 @@ def gated_recurrence(z, x, h0=None, starts=None, batch_first: bool = False):
 
 def linear_recurrence(a, b, h0=None, starts=None, batch_first: bool = False):
     """``h_t = a_t h_{t-1} + b_t``: ``gated_recurrence`` with both coefficients
-    given, of either sign.  Differentiable in a, b and h0."""
+    given, of either sign and any size (a state beyond float32's range is an infinity
+    from that step on).  Differentiable in a, b and h0."""
     return _recurrence("linear_recurrence", _LINEAR, a, b, h0, starts, batch_first)
 
 

@@ -117,8 +117,11 @@ HS_DEV void cluster_wait() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 HS_DEV void fence_mbar_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
-HS_DEV void mbar_init(uint64_t *b) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_u32(b)) : "memory");
+HS_DEV void mbar_init(uint64_t *b, int count = 1) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(count) : "memory");
+}
+HS_DEV void mbar_arrive(uint64_t *b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory");
 }
 HS_DEV void mbar_expect(uint64_t *b, unsigned bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(b)), "r"(bytes) : "memory");
@@ -234,10 +237,8 @@ template <typename T, int VEC> HS_DEV void write_word(char *dst, const float *v)
 // The map h -> a h + b of a run of steps, of one lane's columns.  a = -0 marks
 // a run that a start lies in: nothing passes it, the map is b alone.  For a
 // finite h that is what a h + b gives, so maps are chained without a look at the marks,
-// and a chain that ends in NaN is gone through once more with them (with a
-// look at each: 80 us in place of 74 at T=16384, B=2, H=1024 float32).  (A product of
-// gates is at most 1; one of given coefficients is held to the largest finite
-// value, so that it leaves a zero state zero as step by step.)
+// and a chain of gates that ends in NaN is gone through once more with them (with a
+// look at each: 80 us in place of 74 at T=16384, B=2, H=1024 float32).
 template <int VEC> struct __align__(8 * VEC) Map {
   float a[VEC], b[VEC];
   HS_DEV bool cut() const { return __float_as_uint(a[0]) == 0x80000000u; }
@@ -252,17 +253,104 @@ template <int VEC> HS_DEV bool any_nan(Cols<VEC> h) {
   for (int i = 0; i < VEC; ++i) r |= v[i] != v[i];
   return r;
 }
-template <int VEC, bool GATED> HS_DEV Cols<VEC> held(Cols<VEC> a) {
-  if (GATED) return a;
+
+// A product of gates is at most 1, and too small a one is as good as 0: nothing
+// grows again.  A product of given coefficients may be no float32 of full precision although
+// the states are: growth by 1.5 a step takes 1e-20 to 1e25 in 256 steps, by a
+// factor of 1e45.  Products are chained as they are all the same, and the states looked at:
+//   - An infinite or NaN product leaves a state that is infinite or NaN, and so do
+//     all maps after it.
+//   - What a subnormal or vanished product loses is about 2^-149 of the state before
+//     it: of states up to kNear below 2^-116, where steps would soon lose as much.
+// Where a state along a chain is beyond kNear, infinite or NaN, the wave is chained once
+// more with exact products, m 2^e with 1 <= |m| < 2 (resolve_exact; with states about 1e11
+// in every wave 16384 x 8 x 1024 bfloat16 takes 252 us forward in place of 158).
+constexpr float kNear = 4294967296.f;
+template <int VEC> HS_DEV void largest(float &top, Cols<VEC> h) {
   float v[VEC];
-  a.get(v);
+  h.get(v);
 #pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-    asm("min.NaN.f32 %0, %0, %1;" : "+f"(v[i]) : "f"(FLT_MAX));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(v[i]) : "f"(-FLT_MAX));
+  for (int i = 0; i < VEC; ++i) top = fmaxf(top, fabsf(v[i]));
+}
+// Of a chain whose states were at most `top`, NaN left out, and that ended in h.
+template <int VEC> HS_DEV bool is_far(float top, Cols<VEC> h) {
+  float v[VEC];
+  h.get(v);
+  bool r = !(top <= kNear);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) r |= !(fabsf(v[i]) <= kNear);
+  return r;
+}
+
+// m 2^e; e = kAll: a map that a start lies in, of no product.
+constexpr int kAll = 0x7fffffff;
+template <int VEC> struct __align__(8 * VEC) Product {
+  float m[VEC];
+  int e[VEC];
+};
+// v = v' 2^x with 1 <= |v'| < 2; e becomes e + x.  Zeros, infinities and NaN stay.
+HS_DEV void split(float &v, int &e) {
+  const bool small = fabsf(v) < FLT_MIN;
+  const unsigned w = __float_as_uint(small ? v * 16777216.f : v);
+  const int x = (int)(w >> 23) & 255;
+  if (x != 0 && x != 255) {
+    v = __uint_as_float((w & 0x807fffffu) | 0x3f800000u);
+    e += x - (small ? 127 + 24 : 127);
   }
+}
+HS_DEV float power_of_two(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+// m 2^e h + b.  Where m 2^e is a float32 of full precision, as a fused product and
+// sum; else h is split too (beyond 2^252 and below 2^-252 the product is infinite and
+// 0 in any case; zeros, infinities and NaN of m and h do as they would).
+HS_DEV float exact_step(float m, int e, float h, float b) {
+  if (e >= -126 && e <= 127) return fmaf(m * power_of_two(e), h, b);
+  split(h, e);
+  e = max(-252, min(252, e));
+  return m * h * power_of_two(e / 2) * power_of_two(e - e / 2) + b;
+}
+template <int VEC> HS_DEV Cols<VEC> exact_step(const Product<VEC> &p, const float *b, Cols<VEC> h) {
+  if (p.e[0] == kAll) return Cols<VEC>::of(b);
+  float v[VEC];
+  h.get(v);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = exact_step(p.m[i], p.e[i], v[i], b[i]);
   return Cols<VEC>::of(v);
 }
+// The product of the 16 coefficients of a run: of four at a time in 64 bits, which no
+// four float32 leave.
+template <int VEC, typename F> HS_DEV Product<VEC> run_product(F coef) {
+  Product<VEC> p;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) p.m[i] = 1.f, p.e[i] = 0;
+#pragma unroll
+  for (int k = 0; k < kRun; k += 4) {
+    double d[VEC];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float c[VEC];
+      coef(k + j).get(c);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) d[i] = j ? d[i] * (double)c[i] : (double)c[i];
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      const int hi = __double2hiint(d[i]), x = (hi >> 20) & 2047;
+      if (x != 0 && x != 2047) {
+        d[i] = __hiloint2double((hi & 0x800fffff) | 0x3ff00000, __double2loint(d[i]));
+        p.e[i] += x - 1023;
+      }
+      p.m[i] *= (float)d[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    split(p.m[i], p.e[i]);
+    if (p.m[i] == 0.f || !(fabsf(p.m[i]) <= FLT_MAX)) p.e[i] = 0;
+  }
+  return p;
+}
+
+template <int VEC> struct __align__(4 * VEC) Exponent { int e[VEC]; };
 
 // The maps of the warps of this CTA and of the CTAs of its cluster, each in
 // two copies for alternate waves: a wave's barrier separates its writes from
@@ -271,30 +359,67 @@ template <int VEC, bool GATED> HS_DEV Cols<VEC> held(Cols<VEC> a) {
 // stores.  A CTA sends the map of wave w+2 only after all of wave w+1 have
 // arrived, and each of those was sent after its sender's last read of wave w.
 template <int VEC> struct Maps {
-  uint64_t *bar;   // [2]
+  uint64_t *bar;   // [2], and two of the exact chains: the runs' products, the CTAs' maps
   Map<VEC> *warp;  // [2][warps][32]
   Map<VEC> *cta;   // [2][cluster][32], where the cluster has more than one CTA
+  // of given coefficients, for a wave that is chained once more (one copy: a wave's
+  // is done with before any warp publishes the next)
+  Product<VEC> *run;   // [warps][32]
+  Map<VEC> *exact;     // [cluster][32], m in the place of a
+  Exponent<VEC> *pow;  // [cluster][32]
 };
+__host__ __device__ constexpr size_t maps_bytes(bool gated, int vec, int warps, int cluster) {
+  return (size_t)32 * vec * (warps * (gated ? 16 : 24) + (cluster > 1 ? cluster * (gated ? 16 : 28) : 0));
+}
 
 // Sets up the maps behind the tiles; met by exchange_ready() before the first publish.
-template <int VEC>
+template <int VEC, bool GATED>
 HS_DEV Maps<VEC> exchange_init(uint64_t *bar, unsigned char *behind, int warps, int warp, int lane, int cluster) {
   Maps<VEC> m;
+  const int ctas = cluster > 1 ? cluster : 0;
   m.bar = bar;
   m.warp = reinterpret_cast<Map<VEC> *>(behind) + lane;
   m.cta = m.warp + 2 * warps * 32;
-  if (cluster > 1) {
-    if (warp == 0 && lane == 0) {
+  m.exact = m.cta + 2 * ctas * 32;
+  m.run = reinterpret_cast<Product<VEC> *>(m.exact - lane + ctas * 32) + lane;
+  m.pow = reinterpret_cast<Exponent<VEC> *>(m.run - lane + warps * 32) + lane;
+  if (warp == 0 && lane == 0) {
+    if (cluster > 1) {
       mbar_init(&m.bar[0]);
       mbar_init(&m.bar[1]);
-      fence_mbar_init();
     }
-    cluster_arrive();
+    if (!GATED) {
+      mbar_init(&m.bar[2], warps);
+      mbar_init(&m.bar[3]);
+    }
+    if (cluster > 1 || !GATED) fence_mbar_init();
   }
+  if (cluster > 1) cluster_arrive();
   return m;
 }
 HS_DEV void exchange_ready(int cluster) {
   if (cluster > 1) cluster_wait();  // every CTA has started and set up its barriers
+}
+
+HS_DEV void send(const void *p, int rank, const void *bar, const Map<2> &t) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(cluster_addr(p, rank)),
+               "f"(t.a[0]), "f"(t.a[1]), "f"(t.b[0]), "f"(t.b[1]), "r"(cluster_addr(bar, rank))
+               : "memory");
+}
+HS_DEV void send(const void *p, int rank, const void *bar, const Map<1> &t) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(cluster_addr(p, rank)),
+               "f"(t.a[0]), "f"(t.b[0]), "r"(cluster_addr(bar, rank))
+               : "memory");
+}
+HS_DEV void send(const void *p, int rank, const void *bar, const Exponent<2> &t) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.s32 [%0], {%1, %2}, [%3];" ::"r"(cluster_addr(p, rank)),
+               "r"(t.e[0]), "r"(t.e[1]), "r"(cluster_addr(bar, rank))
+               : "memory");
+}
+HS_DEV void send(const void *p, int rank, const void *bar, const Exponent<1> &t) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.s32 [%0], %1, [%2];" ::"r"(cluster_addr(p, rank)), "r"(t.e[0]),
+               "r"(cluster_addr(bar, rank))
+               : "memory");
 }
 
 // Publishes this warp's map of wave w.
@@ -303,7 +428,7 @@ HS_DEV void publish(const Maps<VEC> &m, int w, int warps, int warp, int lane, in
                     bool cut) {
   const int p = w & 1;
   Map<VEC> mine;
-  held<VEC, GATED>(A).get(mine.a);
+  A.get(mine.a);
   B.get(mine.b);
   if (STARTS) {
 #pragma unroll
@@ -317,59 +442,127 @@ HS_DEV void publish(const Maps<VEC> &m, int w, int warps, int warp, int lane, in
   if (warp == warps - 1) {  // the CTA's map, to every CTA of the cluster
     Cols<VEC> ta = Cols<VEC>::all(1.f), tb = Cols<VEC>::all(0.f);
     bool any = false;
+    float top = 0.f, grown = 0.f, low = FLT_MAX;
 #pragma unroll 4
     for (int j = 0; j < warps; ++j) {
       const Map<VEC> e = all[j * 32];
       if (STARTS) any |= e.cut();
       tb = apply(e, tb);
-      ta = held<VEC, GATED>(Cols<VEC>::of(e.a) * ta);
+      ta = Cols<VEC>::of(e.a) * ta;
+      if (!GATED) {
+        largest<VEC>(top, tb);
+        largest<VEC>(grown, ta);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) low = fminf(low, fabsf(e.a[i]));
+      }
     }
-    if (STARTS && any && any_nan(tb)) {
+    if (GATED && STARTS && any && any_nan(tb)) {
       tb = Cols<VEC>::all(0.f);
       for (int j = 0; j < warps; ++j) tb = apply_marked(all[j * 32], tb);
     }
     Map<VEC> t;
     ta.get(t.a);
     tb.get(t.b);
-    if (STARTS) {
+    // (a state from before the CTA's steps that grows before a product loses it is not seen
+    // in the states between CTAs)
+    const bool again = !GATED && (is_far<VEC>(top, tb) || (grown > 1024.f && low < FLT_MIN));
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) t.a[i] = any ? -0.f : GATED ? t.a[i] : t.a[i] + 0.f;
-    }
-    for (int r = 0; r < cluster; ++r) {
-      const unsigned to = cluster_addr(&m.cta[(p * cluster + rank) * 32], r), bar = cluster_addr(&m.bar[p], r);
-      if constexpr (VEC == 2)
-        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(to),
-                     "f"(t.a[0]), "f"(t.a[1]), "f"(t.b[0]), "f"(t.b[1]), "r"(bar)
-                     : "memory");
-      else
-        asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(to),
-                     "f"(t.a[0]), "f"(t.b[0]), "r"(bar)
-                     : "memory");
-    }
+    for (int i = 0; i < VEC; ++i) t.a[i] = again ? __int_as_float(0x7f800000) : any ? -0.f : STARTS && !GATED ? t.a[i] + 0.f : t.a[i];
+    for (int r = 0; r < cluster; ++r) send(&m.cta[(p * cluster + rank) * 32], r, &m.bar[p], t);
   }
 }
 
+// Wave w's states with exact products: the state entering this warp's run, and
+// in `state` the wave's entry moved to its end.  All warps of a cluster come here
+// together, as all look at the same maps; should they not (a wait that gave up), the
+// waits here end as all do.
+template <int VEC, typename F>
+HS_DEV Cols<VEC> resolve_exact(const Maps<VEC> &m, int w, int round, int warps, int warp, int lane, int cluster, int rank, bool cut, F coef,
+                               Cols<VEC> &state, int *status) {
+  const Map<VEC> *all = m.warp + (w & 1) * warps * 32;
+  Product<VEC> mine = run_product<VEC>(coef);
+  if (cut) mine.e[0] = kAll;
+  m.run[warp * 32] = mine;
+  __syncwarp();
+  if (lane == 0) mbar_arrive(&m.bar[2]);
+  mbar_wait(&m.bar[2], round & 1, status);
+  auto runs = [&](int from, int to, Cols<VEC> h) {
+#pragma unroll 1
+    for (int j = from; j < to; ++j) h = exact_step<VEC>(m.run[j * 32], all[j * 32].b, h);
+    return h;
+  };
+  if (cluster == 1) {
+    const Cols<VEC> in = runs(0, warp, state);
+    state = runs(warp, warps, in);
+    return in;
+  }
+  if (warp == 0 && lane == 0) mbar_expect(&m.bar[3], cluster * 32 * (unsigned)(sizeof(Map<VEC>) + sizeof(Exponent<VEC>)));
+  if (warp == warps - 1) {
+    Map<VEC> t;
+    Exponent<VEC> x;
+    runs(0, warps, Cols<VEC>::all(0.f)).get(t.b);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) t.a[i] = 1.f, x.e[i] = 0;
+    bool any = false;
+#pragma unroll 1
+    for (int j = 0; j < warps; ++j) {
+      const Product<VEC> q = m.run[j * 32];
+      any |= q.e[0] == kAll;
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) t.a[i] *= q.m[i], x.e[i] += q.e[i];  // (up to 16 factors below 2)
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      split(t.a[i], x.e[i]);
+      if (t.a[i] == 0.f || !(fabsf(t.a[i]) <= FLT_MAX)) x.e[i] = 0;
+      if (any) x.e[i] = kAll;
+    }
+    for (int r = 0; r < cluster; ++r) {
+      send(&m.exact[rank * 32], r, &m.bar[3], t);
+      send(&m.pow[rank * 32], r, &m.bar[3], x);
+    }
+  }
+  mbar_wait(&m.bar[3], round & 1, status);
+  Cols<VEC> in = state;
+#pragma unroll 1
+  for (int r = 0; r < cluster; ++r) {
+    if (r == rank) in = state;
+    const Map<VEC> t = m.exact[r * 32];
+    const Exponent<VEC> x = m.pow[r * 32];
+    Product<VEC> q;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) q.m[i] = t.a[i], q.e[i] = x.e[i];
+    state = exact_step<VEC>(q, t.b, state);
+  }
+  return runs(0, warp, in);
+}
+
 // The state entering this warp's run of wave w; `state`, the same in every
-// thread of a column, moves from the wave's entry to its end.
-template <int VEC, bool STARTS>
-HS_DEV Cols<VEC> resolve(const Maps<VEC> &m, int w, int warps, int warp, int lane, int cluster, int rank, Cols<VEC> &state, int *status) {
+// thread of a column, moves from the wave's entry to its end.  `again`: the lanes
+// that need the exact chain (of given coefficients).
+template <int VEC, bool GATED, bool STARTS>
+HS_DEV Cols<VEC> resolve(const Maps<VEC> &m, int w, int warps, int warp, int lane, int cluster, int rank, Cols<VEC> &state, bool &again, int *status) {
   const int p = w & 1;
   const Map<VEC> *all = m.warp + p * warps * 32;
   const Cols<VEC> entry = state;
   Cols<VEC> in = state;
+  float top = 0.f;
+  if (!GATED) largest<VEC>(top, state);
   if (cluster == 1) {
 #pragma unroll 4
     for (int j = 0; j < warps; ++j) {
       if (j == warp) in = state;
       state = apply(all[j * 32], state);
+      if (!GATED) largest<VEC>(top, state);
     }
-    if (STARTS && any_nan(state)) {
+    if (GATED && STARTS && any_nan(state)) {
       state = entry;
       for (int j = 0; j < warps; ++j) {
         if (j == warp) in = state;
         state = apply_marked(all[j * 32], state);
       }
     }
+    again = !GATED && is_far<VEC>(top, state);
     return in;
   }
   mbar_wait(&m.bar[p], (w >> 1) & 1, status);
@@ -379,17 +572,36 @@ HS_DEV Cols<VEC> resolve(const Maps<VEC> &m, int w, int warps, int warp, int lan
     if (r < cluster) {
       if (r == rank) in = state;
       state = apply(ctas[r * 32], state);
+      if (!GATED) largest<VEC>(top, state);
     }
   }
 #pragma unroll 4
   for (int j = 0; j < warp; ++j) in = apply(all[j * 32], in);
-  if (STARTS && (any_nan(state) || any_nan(in))) {
+  if (GATED && STARTS && (any_nan(state) || any_nan(in))) {
     state = in = entry;
     for (int r = 0; r < cluster; ++r) {
       if (r == rank) in = state;
       state = apply_marked(ctas[r * 32], state);
     }
     for (int j = 0; j < warp; ++j) in = apply_marked(all[j * 32], in);
+  }
+  again = !GATED && is_far<VEC>(top, state);
+  return in;
+}
+
+// The same, whatever the coefficients; `round` counts the exact chains.
+template <int VEC, bool GATED, bool STARTS, typename F>
+HS_DEV Cols<VEC> enter(const Maps<VEC> &m, int w, int &round, int warps, int warp, int lane, int cluster, int rank, bool live, bool cut, F coef,
+                       Cols<VEC> &state, int *status) {
+  Cols<VEC> entry = state;
+  bool again;
+  Cols<VEC> in = resolve<VEC, GATED, STARTS>(m, w, warps, warp, lane, cluster, rank, state, again, status);
+  if constexpr (!GATED) {
+    if (__any_sync(0xffffffffu, again && live)) {
+      const Cols<VEC> exact = resolve_exact<VEC>(m, w, round, warps, warp, lane, cluster, rank, cut, coef, entry, status);
+      if (again) in = exact, state = entry;
+      ++round;
+    }
   }
   return in;
 }
@@ -503,7 +715,7 @@ HS_DEV void barriers_init(uint64_t *full, int n, int warp, int lane) {
 template <typename T, int VEC, bool GATED, bool STARTS, int MOVE>
 __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid_constant__ FwdArgs p) {
   extern __shared__ __align__(128) unsigned char dyn[];
-  __shared__ uint64_t full[kStages * kFwdWarps], swap[2];
+  __shared__ uint64_t full[kStages * kFwdWarps], swap[4];
   using C = Cols<VEC>;
   const int lane = threadIdx.x, warp = threadIdx.y, warps = blockDim.y;
   const int cluster = p.s.cluster, rank = (int)(blockIdx.x % cluster), waves = p.s.waves;
@@ -572,7 +784,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
   };
   auto starts_from = [&](int w) { return start_masks(p.starts + row * p.sb, p.st, w, waves, lane, T_, start_of); };
 
-  const Maps<VEC> maps = exchange_init<VEC>(swap, dyn + (kStages * 2 + (MOVE == kTiles ? 1 : 0)) * in.tensor, warps, warp, lane, cluster);
+  const Maps<VEC> maps = exchange_init<VEC, GATED>(swap, dyn + (kStages * 2 + (MOVE == kTiles ? 1 : 0)) * in.tensor, warps, warp, lane, cluster);
   if (MOVE != kLanes) barriers_init(full, kStages * (MOVE == kRows ? warps : 1), warp, lane);
   fetch(0);
   fetch(1);
@@ -580,6 +792,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
   float s0[VEC];
   load_state<VEC>(p.h0, row * p.state_b + col, s0);
   C state = C::of(s0);
+  int round = 0;
 
   for (int w = 0; w < waves; ++w) {
     const int64_t t0 = start_of(w);
@@ -631,7 +844,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
     // (every warp has read its inputs once all have published)
     publish<VEC, GATED, STARTS>(maps, w, warps, warp, lane, cluster, rank, A, B, mask != 0);
     fetch(w + kStages);
-    C h = resolve<VEC, STARTS>(maps, w, warps, warp, lane, cluster, rank, state, p.status);
+    C h = enter<VEC, GATED, STARTS>(maps, w, round, warps, warp, lane, cluster, rank, live, mask != 0, [&](int k) { return f[k]; }, state, p.status);
     if (len > 0) {
       if (p.ckpt && live) {
         float *c = p.ckpt + (t0 / kRun) * p.ckpt_t + row * p.state_b + col;
@@ -691,7 +904,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
 template <typename T, int VEC, bool GATED, bool STARTS, int MOVE>
 __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid_constant__ BwdArgs p) {
   extern __shared__ __align__(128) unsigned char dyn[];
-  __shared__ uint64_t full[kStages * kBwdWarps], swap[2];
+  __shared__ uint64_t full[kStages * kBwdWarps], swap[4];
   using C = Cols<VEC>;
   // float32 keeps both f and 1-f; the 16-bit types keep 1-f alone and take
   // f = 1 - (1-f), whose error (2^-25) only enters u, far below their rounding
@@ -782,7 +995,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
     load_state<VEC>(c >= 0 ? p.ckpt : nullptr, c * p.ckpt_t + row * p.state_b + col, h);
   };
 
-  const Maps<VEC> maps = exchange_init<VEC>(swap, dyn + (kStages * 3 + (MOVE == kTiles ? 2 : 0)) * in.tensor, warps, warp, lane, cluster);
+  const Maps<VEC> maps = exchange_init<VEC, GATED>(swap, dyn + (kStages * 3 + (MOVE == kTiles ? 2 : 0)) * in.tensor, warps, warp, lane, cluster);
   if (MOVE != kLanes) barriers_init(full, kStages * (MOVE == kRows ? warps : 1), warp, lane);
   fetch(0);
   fetch(1);
@@ -791,6 +1004,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
   unsigned masks = 0;
   load_state<VEC>(p.dh_n, row * p.state_b + col, s0);
   C state = C::of(s0);
+  int round = 0;
   const C one = C::all(1.f), zero = C::all(0.f);
 
   for (int w = 0; w < waves; ++w) {
@@ -865,7 +1079,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
     if (w == 0) exchange_ready(cluster);
     publish<VEC, GATED, STARTS>(maps, w, warps, warp, lane, cluster, rank, A, B, mask != 0);
     fetch(w + kStages);
-    C u = resolve<VEC, STARTS>(maps, w, warps, warp, lane, cluster, rank, state, p.status);
+    C u = enter<VEC, GATED, STARTS>(maps, w, round, warps, warp, lane, cluster, rank, live, mask != 0, coef, state, p.status);
     if (len > 0) {
       if constexpr (MOVE == kTiles) {
         if (lane == 0) bulk_wait_read();
@@ -926,7 +1140,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
 // ------------------------------------------------------------------ launch
 struct Plan {
   int vec, warps, cluster, waves;
-  bool flat;
+  bool flat, gated;
   int move;
   int64_t groups;  // of all rows
   size_t smem;
@@ -949,9 +1163,9 @@ Pace pace_of(bool backward, int dtype) {
 }
 
 // Dynamic shared memory of a CTA.
-size_t smem_of(bool backward, int move, int vec, int warps, int cluster) {
+size_t smem_of(bool backward, bool gated, int move, int vec, int warps, int cluster) {
   const int inputs = backward ? 3 : 2, outputs = move != kTiles ? 0 : backward ? 2 : 1;
-  return (size_t)(kStages * inputs + outputs) * warps * slab_bytes(move) + (size_t)2 * (warps + (cluster > 1 ? cluster : 0)) * 32 * 8 * vec;
+  return (size_t)(kStages * inputs + outputs) * warps * slab_bytes(move) + maps_bytes(gated, vec, warps, cluster);
 }
 
 // Clusters of c CTAs that run at once (a cluster stays within a GPC, so some
@@ -982,7 +1196,7 @@ void split_time(Plan &pl, int nchunk, const Pace &m) {
     }
   }
   pl.waves = (nchunk + pl.warps * pl.cluster - 1) / (pl.warps * pl.cluster);
-  pl.smem = smem_of(m.backward, pl.move, pl.vec, pl.warps, pl.cluster);
+  pl.smem = smem_of(m.backward, pl.gated, pl.move, pl.vec, pl.warps, pl.cluster);
 }
 
 struct Tensor3 {  // [T][rows][n] with contiguous n; null: not there
@@ -993,11 +1207,11 @@ struct Tensor3 {  // [T][rows][n] with contiguous n; null: not there
 // One row of B * H columns when every tensor stores its batch rows back to
 // back and no start mask tells them apart; else B rows of H.  16-bit tensors
 // move two columns per lane where every row is 4-byte aligned.
-Plan make_plan(int dtype, bool starts, int64_t T, int64_t B, int64_t H, const Tensor3 *ts, int n, int nchunk,
+Plan make_plan(int dtype, int form, bool starts, int64_t T, int64_t B, int64_t H, const Tensor3 *ts, int n, int nchunk,
                const Pace &pace) {
   Plan pl = {};
   const int64_t es = (int64_t)dtype_bytes(dtype);
-  pl.flat = !starts;
+  pl.flat = !starts, pl.gated = form == HS_RECURRENCE_GATED;
   for (int i = 0; i < n; ++i)
     if (ts[i].p && ts[i].b != H && B > 1) pl.flat = false;
   const int64_t rows = pl.flat ? 1 : B, cols = pl.flat ? B * H : H;
@@ -1068,9 +1282,11 @@ bool encode(CUtensorMap *m, const Tensor3 &t, int dtype, const Plan &pl, int64_t
                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-constexpr size_t kSmemMost = (size_t)(kStages * 3 + 2) * kBwdWarps * kSlab + 2 * (kBwdWarps + kMaxCluster) * 32 * 16;
-static_assert(kSmemMost <= 227 * 1024 && (kStages * 2 + 1) * kFwdWarps * kSlab + 2 * (kFwdWarps + kMaxCluster) * 32 * 16 <= kSmemMost,
-              "shared memory of a CTA");
+constexpr size_t kSmemMost = (size_t)(kStages * 3 + 2) * kBwdWarps * kSlab + maps_bytes(false, 2, kBwdWarps, kMaxCluster);
+static_assert(kSmemMost + 512 <= 227 * 1024 && (kStages * 2 + 1) * kFwdWarps * kSlab + maps_bytes(false, 2, kFwdWarps, kMaxCluster) <= kSmemMost &&
+                  kStages * 2 * kFwdWarps * slab_bytes(kRows) + maps_bytes(false, 2, kFwdWarps, kMaxCluster) <= kSmemMost &&
+                  kStages * 3 * kBwdWarps * slab_bytes(kRows) + maps_bytes(false, 2, kBwdWarps, kMaxCluster) <= kSmemMost,
+              "shared memory of a CTA, beside its barriers");
 
 template <typename Args, typename K>
 int launch(K kernel, const Args &args, const Plan &pl, cudaStream_t st, const char *what,
@@ -1104,7 +1320,7 @@ int64_t clusters_at_once(const Pace &m, int warps, int c) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(ctas / c * c));
   cfg.blockDim = dim3(32, warps);
-  cfg.dynamicSmemBytes = smem_of(m.backward, kTiles, 2, warps, c);
+  cfg.dynamicSmemBytes = smem_of(m.backward, true, kTiles, 2, warps, c);
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = (unsigned)c;
@@ -1193,7 +1409,7 @@ int hs_recurrence_forward(int dtype, int form, const void *z, int64_t z_t, int64
     return fail(HS_ERR_INVALID_ARG, "hs_recurrence_forward: misaligned tensor");
   const int nchunk = (int)((T + kRun - 1) / kRun);
   const Tensor3 ts[3] = {{z, z_t, z_b}, {x, x_t, x_b}, {h, h_t, h_b}};
-  const Plan pl = make_plan(dtype, starts != nullptr, T, B, H, ts, 3, nchunk, pace_of(false, dtype));
+  const Plan pl = make_plan(dtype, form, starts != nullptr, T, B, H, ts, 3, nchunk, pace_of(false, dtype));
   if (pl.groups * pl.cluster > 0x7fffffff) return fail(HS_ERR_UNSUPPORTED, "hs_recurrence_forward: too many columns");
   FwdArgs a = {};
   a.s = shape_of(pl, T, B, H, nchunk);
@@ -1233,7 +1449,7 @@ int hs_recurrence_backward(int dtype, int form, const void *z, int64_t z_t, int6
     return fail(HS_ERR_INVALID_ARG, "hs_recurrence_backward: misaligned tensor");
   const int nchunk = (int)((T + kRun - 1) / kRun);
   const Tensor3 ts[5] = {{z, z_t, z_b}, {x, x_t, x_b}, {dh, dh_t, dh_b}, {dz, dz_t, dz_b}, {dx, dx_t, dx_b}};
-  const Plan pl = make_plan(dtype, with_starts, T, B, H, ts, 5, nchunk, pace_of(true, dtype));
+  const Plan pl = make_plan(dtype, form, with_starts, T, B, H, ts, 5, nchunk, pace_of(true, dtype));
   if (pl.groups * pl.cluster > 0x7fffffff) return fail(HS_ERR_UNSUPPORTED, "hs_recurrence_backward: too many columns");
   BwdArgs a = {};
   a.s = shape_of(pl, T, B, H, nchunk);

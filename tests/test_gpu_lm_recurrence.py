@@ -419,3 +419,102 @@ def test_a_zero_coefficient_is_no_start(zero):
             assert (h[2000:] == 3.0).all() and (h_n == 3.0).all()
         else:
             assert h[2000:].isnan().all() and h_n.isnan().all()
+
+
+def walk(T, B, H, dtype, kind, seed):
+    """Coefficients of either sign whose products leave float32's range while a
+    state from 2^w_0 moves within it: its logarithm goes from w_t to w_{t+1}."""
+    g = torch.Generator().manual_seed(seed)
+    if kind == "up":
+        w = torch.linspace(-110, 110, T + 1)
+    elif kind == "down and up":
+        w = 90 - 190 * (1 - (torch.linspace(-1, 1, T + 1)).abs())
+    elif kind == "up and down":
+        w = -90 + 190 * (1 - (torch.linspace(-1, 1, T + 1)).abs())
+    elif kind == "saw":  # up by 3 a step for 60 steps, down by 60 a step
+        at = torch.arange(T + 1) % 63
+        w = torch.where(at <= 60, -90 + 3.0 * at, 90 - 60.0 * (at - 60))
+    else:  # steps of up to 2^50 either way
+        w = torch.empty(T + 1)
+        w[0] = 0
+        step = 100 * torch.rand(T, generator=g) - 50
+        for t in range(T):
+            w[t + 1] = w[t] + (step[t] if abs(float(w[t] + step[t])) < 100 else -step[t])
+    a = torch.exp2((w[1:] - w[:-1]).double())[:, None, None] * torch.where(torch.rand(T, B, H, generator=g) < 0.5, -1.0, 1.0)
+    return a.to(dtype), torch.exp2(w[0].double()).float()
+
+
+GROWTH = [(32, 1, 64), (520, 1, 64), (2300, 1, 64), (2300, 1, 33), (900, 3, 70), (700, 40, 256), (2300, 1, 65)]
+
+
+@pytest.mark.parametrize("starts", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("kind", ["up", "down and up", "up and down", "saw", "jumps"])
+@pytest.mark.parametrize("shape", GROWTH, ids=str)
+def test_coefficients_whose_products_leave_the_range(shape, kind, dtype, starts):
+    """Each state is one product of t coefficients and the first state (no
+    cancellation), so it is off by a unit 2^-24 a step, and so is the gradient
+    that reaches a step from the end."""
+    T, B, H = shape
+    a, first = walk(T, B, H, dtype, kind, seed=T + H)
+    h0 = first * (1 + torch.rand(B, H, generator=torch.Generator().manual_seed(1)))
+    b = torch.zeros(T, B, H, dtype=dtype)
+    s = None
+    if starts:  # the sequence begins anew at a step or two, from b
+        s = torch.zeros(T, B, dtype=torch.bool)
+        for t in (T // 3, T // 3 + 20):
+            s[t] = True
+    want_h = torch.empty(T, B, H, dtype=torch.float64)
+    state = h0.double()
+    for t in range(T):
+        state = a[t].double() * state
+        if s is not None and bool(s[t].any()):
+            b[t] = state.to(dtype)
+            state = b[t].double()
+        want_h[t] = state
+    # backward on the coefficients taken from the last to the first, so that it walks the same way
+    ra, rb = a.flip(0), torch.zeros_like(b)
+    rs = None if s is None else s.flip(0)
+    e, want_db, want_da = h0.double(), torch.empty_like(want_h), None
+    for t in range(T - 1, -1, -1):
+        want_db[t] = e
+        e = ra[t].double() * e
+        if rs is not None:
+            e = torch.where(rs[t][:, None], 0.0, e)
+    h, h_n = call("linear")(a.to(DEV), b.to(DEV), h0.to(DEV), starts=None if s is None else s.to(DEV))
+    z, x = ra.to(DEV).requires_grad_(True), rb.to(DEV).requires_grad_(True)
+    start = torch.zeros(B, H, device=DEV, requires_grad=True)
+    _, end = call("linear")(z, x, start, starts=None if rs is None else rs.to(DEV))
+    end.backward(h0.to(DEV))
+
+    def same(got, want, what):
+        got = got.double().cpu()
+        tol = 2 * (T + 8) * 2.0 ** -24 + (UNIT[dtype] if what in ("h", "db") and dtype != torch.float32 else 0)
+        worst = ((got - want).abs() / want.abs().clamp(min=2.0 ** -120)).max()
+        assert float(worst) <= tol, f"{what}: {float(worst):.3e} > {tol:.3e}"
+
+    same(h, want_h, "h")
+    same(h_n, want_h[-1], "h_n")
+    same(x.grad, want_db, "db")
+    same(start.grad, e, "dh0")
+
+
+@pytest.mark.parametrize("T,H", [(3000, 40), (3000, 33), (500, 4096)])
+def test_states_that_overflow_are_infinite(T, H):
+    """Growth past the range is an infinity from that step on, from a zero state nothing."""
+    a, b = torch.full((T, 1, H), 2.0, device=DEV), torch.zeros(T, 1, H, device=DEV)
+    h0 = torch.ones(1, H, device=DEV)
+    h0[:, ::2] = 0
+    h0[:, 1::4] = -1
+    h, h_n = call("linear")(a, b, h0)
+    assert (h[:, :, ::2] == 0).all() and (h_n[:, ::2] == 0).all()
+    assert torch.equal(h[:126, 0, 1], torch.tensor([-2.0 ** n for n in range(1, 127)], device=DEV))
+    assert h[127:, :, 1::4].isneginf().all() and h[127:, :, 3::4].isposinf().all()
+    z, x = a.clone().requires_grad_(True), b.clone().requires_grad_(True)
+    _, end = call("linear")(z, x)
+    end.backward(h0)
+    assert (x.grad[:, :, ::2] == 0).all() and x.grad[:T - 128, :, 3::4].isposinf().all()
+    assert torch.equal(x.grad[T - 100:, 0, 3], torch.tensor([2.0 ** n for n in range(99, -1, -1)], device=DEV))
+    # an infinite state outlasts a product of coefficients that is no float32
+    h, _ = call("linear")(torch.full((T, 1, H), -0.5, device=DEV), b, torch.full((1, H), float("inf"), device=DEV))
+    assert h.isinf().all() and bool((h[::2] < 0).all()) and bool((h[1::2] > 0).all())
