@@ -179,8 +179,8 @@ HS_DEV void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" :
 HS_DEV void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // f = 1/(1+e^-z) and 1-f = e^-z/(1+e^-z), each to a few float32 ulps of its own
-// size.  e^-z is held to 2^126, so that both stay finite (f is 0 to float32's
-// smallest normal number there); a NaN stays one.  The reciprocal is refined by
+// size.  e^-z is held to 2^126, so that both stay finite (f is 2^-126 there and 1-f is 1;
+// shut() makes such an f 0); a NaN stays one.  The reciprocal is refined by
 // one Newton step (as in sigf: its rounding compounds over thousands of steps).
 template <int VEC> HS_DEV void gate(const float *z, Cols<VEC> &f, Cols<VEC> &om) {
   float t[VEC], r[VEC];
@@ -198,6 +198,25 @@ template <int VEC> HS_DEV void gate(const float *z, Cols<VEC> &f, Cols<VEC> &om)
   const Cols<VEC> rr = Cols<VEC>::of(r);
   f = fma(rr, fma(nd, rr, Cols<VEC>::all(1.f)), rr);
   om = e * f;
+}
+
+// Gates below float32's normal range are 0: nothing of the state passes, not even
+// what would show beside an input of 0.
+template <int VEC> HS_DEV Cols<VEC> shut(Cols<VEC> f) {
+  float v[VEC];
+  f.get(v);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = v[i] <= FLT_MIN ? 0.f : v[i];
+  return Cols<VEC>::of(v);
+}
+// Whether a product of gates is so small that one of them may be.
+template <int VEC> HS_DEV bool tiny(Cols<VEC> a) {
+  float v[VEC];
+  a.get(v);
+  bool r = false;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) r |= v[i] <= FLT_MIN;
+  return r;
 }
 
 // One lane's word of a step, copied by the lane itself.
@@ -830,6 +849,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
 #pragma unroll
       for (int k = 0; k < kRun; ++k) {
         const bool cut = (mask >> k) & 1;
+        if (GATED) f[k] = shut<VEC>(f[k]);
         A = cut ? C::all(0.f) : A * f[k];
         B = cut ? b[k] : fma(f[k], B, b[k]);
       }
@@ -838,6 +858,15 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
       for (int k = 0; k < kRun; ++k) {
         A = A * f[k];
         B = fma(f[k], B, b[k]);
+      }
+      if (GATED && tiny<VEC>(A)) {
+        A = C::all(1.f), B = C::all(0.f);
+#pragma unroll
+        for (int k = 0; k < kRun; ++k) {
+          f[k] = shut<VEC>(f[k]);
+          A = A * f[k];
+          B = fma(f[k], B, b[k]);
+        }
       }
     }
     if (w == 0) exchange_ready(cluster);

@@ -518,3 +518,18 @@ def test_states_that_overflow_are_infinite(T, H):
     # an infinite state outlasts a product of coefficients that is no float32
     h, _ = call("linear")(torch.full((T, 1, H), -0.5, device=DEV), b, torch.full((1, H), float("inf"), device=DEV))
     assert h.isinf().all() and bool((h[::2] < 0).all()) and bool((h[1::2] > 0).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("T,H", [(1, 32), (40, 33), (2100, 32), (2100, 34), (600, 4096)])
+def test_nothing_passes_a_gate_that_is_shut(T, H, dtype):
+    """Below float32's range a gate is 0: an input of 0 leaves 0, with and without starts in the run."""
+    g = torch.Generator().manual_seed(T + H)
+    x = torch.randn(T, 1, H, generator=g).to(dtype)
+    x[torch.rand(T, 1, H, generator=g) < 0.2] = 0
+    h0 = 100 * torch.randn(1, H, generator=g)
+    z = torch.full((T, 1, H), -200.0, dtype=dtype)
+    s = torch.rand(T, 1, generator=g) < 0.05
+    for starts in (None, s.to(DEV)):
+        h, h_n = call("gated")(z.to(DEV), x.to(DEV), h0.to(DEV), starts=starts)
+        assert torch.equal(h.cpu(), x) and torch.equal(h_n.cpu(), x[-1].float())
