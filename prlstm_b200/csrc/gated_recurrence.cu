@@ -182,16 +182,10 @@ HS_DEV void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "m
 // size.  e^-z is held to 2^126, so that both stay finite (f is 2^-126 there and 1-f is 1;
 // shut() makes such an f 0); a NaN stays one.  The reciprocal is refined by
 // one Newton step (as in sigf: its rounding compounds over thousands of steps).
-template <int VEC> HS_DEV void gate(const float *z, Cols<VEC> &f, Cols<VEC> &om) {
-  float t[VEC], r[VEC];
-#pragma unroll
-  for (int v = 0; v < VEC; ++v) {
-    float x = z[v] * -1.44269504088896341f;
-    asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(126.f));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t[v]) : "f"(x));
-  }
-  const Cols<VEC> e = Cols<VEC>::of(t), nd = fma(e, Cols<VEC>::all(-1.f), Cols<VEC>::all(-1.f));  // -(1 + e^-z)
-  float dd[VEC];
+// gate_of() gives both from e^-z.
+template <int VEC> HS_DEV void gate_of(Cols<VEC> e, Cols<VEC> &f, Cols<VEC> &om) {
+  const Cols<VEC> nd = fma(e, Cols<VEC>::all(-1.f), Cols<VEC>::all(-1.f));  // -(1 + e^-z)
+  float dd[VEC], r[VEC];
   nd.get(dd);
 #pragma unroll
   for (int v = 0; v < VEC; ++v) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r[v]) : "f"(-dd[v]));
@@ -199,6 +193,17 @@ template <int VEC> HS_DEV void gate(const float *z, Cols<VEC> &f, Cols<VEC> &om)
   f = fma(rr, fma(nd, rr, Cols<VEC>::all(1.f)), rr);
   om = e * f;
 }
+template <int VEC> HS_DEV Cols<VEC> gate_exp(const float *z) {
+  float t[VEC];
+#pragma unroll
+  for (int v = 0; v < VEC; ++v) {
+    float x = z[v] * -1.44269504088896341f;
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(126.f));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(t[v]) : "f"(x));
+  }
+  return Cols<VEC>::of(t);
+}
+template <int VEC> HS_DEV void gate(const float *z, Cols<VEC> &f, Cols<VEC> &om) { gate_of<VEC>(gate_exp<VEC>(z), f, om); }
 
 // Gates below float32's normal range are 0: nothing of the state passes, not even
 // what would show beside an input of 0.
@@ -935,9 +940,10 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
   extern __shared__ __align__(128) unsigned char dyn[];
   __shared__ uint64_t full[kStages * kBwdWarps], swap[4];
   using C = Cols<VEC>;
-  // float32 keeps both f and 1-f; the 16-bit types keep 1-f alone and take
-  // f = 1 - (1-f), whose error (2^-25) only enters u, far below their rounding
-  constexpr bool kBoth = GATED && sizeof(T) == 4;
+  // float32 keeps both f and 1-f.  The 16-bit types, two columns to a lane, have
+  // registers for one value and keep e^-z, from which gate_of() gives both again, the
+  // same bits (1-f alone would leave f with the error 2^-25, all of a small gate)
+  constexpr bool kBoth = GATED && VEC == 1, kExp = GATED && VEC == 2;
   const int lane = threadIdx.x, warp = threadIdx.y, warps = blockDim.y;
   const int cluster = p.s.cluster, rank = (int)(blockIdx.x % cluster), waves = p.s.waves;
   const int64_t gid = blockIdx.x / cluster;
@@ -1049,55 +1055,70 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
     const int64_t t0 = (int64_t)c * kRun;
     const unsigned d = in.at(w);
     const int len = c < 0 ? 0 : (int)min((int64_t)kRun, T_ - t0);
-    // keep: 1-f (gated) or f (linear); q: the factor of e in df; raw: g as stored
+    // keep: 1-f, with kExp e^-z (gated) or f (linear); q: the factor of e in df; raw: g as stored
     C keep[kRun], both[kBoth ? kRun : 1], q[kRun];
     unsigned raw[kRun];
-    auto coef = [&](int k) { return kBoth ? both[kBoth ? k : 0] : GATED ? one - keep[k] : keep[k]; };
+    auto coef = [&](int k) {
+      if constexpr (kExp) {
+        C f, om;
+        gate_of<VEC>(keep[k], f, om);
+        return f;
+      }
+      return kBoth ? both[kBoth ? k : 0] : keep[k];
+    };
     auto grad = [&](int k) {
       float g[VEC];
       unpack_lane<T, VEC>(raw[k], g);
       return C::of(g);
     };
+    C A = one, B = zero;
 #pragma unroll
     for (int k = 0; k < kRun; ++k) {
       float zv[VEC], xv[VEC];
       read_word<T, VEC>(d + zsh(k) + k * kPitch, zv);
       read_word<T, VEC>(d + in.tensor + xsh(k) + k * kPitch, xv);
-      raw[k] = read_raw(d + 2 * in.tensor + gsh(k) + k * kPitch);
+      raw[k] = has_g ? read_raw(d + 2 * in.tensor + gsh(k) + k * kPitch) : 0u;
       const C x = C::of(xv);
       if (STARTS && ((mask >> k) & 1)) s = zero;
       if (GATED) {
+        const C e = gate_exp<VEC>(zv);
         C f, om;
-        gate<VEC>(zv, f, om);
+        gate_of<VEC>(e, f, om);
         q[k] = (s - x) * (f * om);
         s = fma(f, s, om * x);
-        keep[k] = om;
+        keep[k] = kExp ? e : om;
         if (kBoth) both[k] = f;
+        if (kExp) {  // the run's map while f is at hand: B = sum of g_k f_0 .. f_k, up to a start
+          A = STARTS && ((mask >> k) & 1) ? zero : A * f;
+          B = fma(A, grad(k), B);
+        }
       } else {
         q[k] = s;
         keep[k] = C::of(zv);
         s = fma(keep[k], s, x);
       }
     }
-    if (len < kRun || !has_g) {
+    if (len < kRun) {
 #pragma unroll
       for (int k = 0; k < kRun; ++k) {
         if (k >= len) {
           keep[k] = GATED ? zero : one;
           if (kBoth) both[k] = one;
+          raw[k] = 0;
         }
-        if (k >= len || !has_g) raw[k] = 0;
       }
     }
-    C A = one, B = zero;
-    if (STARTS && mask) {
+    // (what a step at a time gives: a part of a run, and gradients that are infinite or NaN)
+    const bool steps = !kExp || len < kRun || any_nan(B);
+    if (steps) A = one, B = zero;
+    if (STARTS && mask && steps) {
 #pragma unroll
       for (int k = kRun - 1; k >= 0; --k) {
         const bool cut = (mask >> k) & 1;
         B = cut ? zero : coef(k) * (grad(k) + B);
         A = cut ? zero : A * coef(k);
       }
-    } else {
+    } else if (steps) {
 #pragma unroll
       for (int k = kRun - 1; k >= 0; --k) {
         const C f = coef(k);
@@ -1119,10 +1140,12 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
       char *dxq = p.dx + (row * p.dxb + col) * (int64_t)sizeof(T) + (t0 + kRun - 1) * dxs;
       auto put = [&](int k, bool cut) {
         const C e = grad(k) + u;
-        u = cut ? zero : coef(k) * e;
+        C f = kExp ? zero : coef(k), om = keep[k];
+        if (kExp) gate_of<VEC>(keep[k], f, om);
+        u = cut ? zero : f * e;
         float dz[VEC], dx[VEC];
         (e * q[k]).get(dz);
-        (GATED ? e * keep[k] : e).get(dx);
+        (GATED ? e * om : e).get(dx);
         if constexpr (MOVE == kTiles) {
           stage_word<T>(slab + k * kStep, dz);
           stage_word<T>(slab + in.tensor + k * kStep, dx);

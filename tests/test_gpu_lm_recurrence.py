@@ -533,3 +533,33 @@ def test_nothing_passes_a_gate_that_is_shut(T, H, dtype):
     for starts in (None, s.to(DEV)):
         h, h_n = call("gated")(z.to(DEV), x.to(DEV), h0.to(DEV), starts=starts)
         assert torch.equal(h.cpu(), x) and torch.equal(h_n.cpu(), x[-1].float())
+
+
+@pytest.mark.parametrize("starts", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("shape", [(1, 1, 64), (5, 1, 64), (16, 1, 64), (48, 2, 66), (48, 2, 33), (700, 1, 64), (3000, 1, 64)], ids=str)
+def test_gradient_through_small_gates(shape, dtype, starts):
+    """A loss on the last state alone: what reaches the steps before a small gate is
+    that gate's size, and as exact as anything else.  Each gate carries a few
+    units 2^-24 of itself, so a gradient is off by those of all steps after it."""
+    T, B, H = shape
+    g = torch.Generator().manual_seed(T + H)
+    z = 5 + 2 * torch.rand(T, B, H, generator=g)
+    z[T // 2] = -20 + 12 * torch.rand(B, H, generator=g)
+    z = z.to(dtype)
+    x, h0 = torch.randn(T, B, H, generator=g).to(dtype), torch.randn(B, H, generator=g)
+    dh_n = 1024 * torch.randn(B, H, generator=g)
+    s = torch.zeros(T, B, dtype=torch.bool) if starts else None
+    if starts and T > 16:
+        s[T // 4] = True
+    want, _ = truth(z, x, h0, s, None, dh_n, "gated")
+    got = run(z, x, h0, s, None, dh_n, "gated")
+    unit = (4 * T + 16) * 2.0 ** -24
+    size = want["h"].abs().max() + x.double().abs().max() + h0.abs().max()  # of the difference that da holds
+    f, om = torch.sigmoid(z.double()), torch.sigmoid(-z.double())
+    e = want["db"] / om
+    own = (UNIT[dtype] if dtype != torch.float32 else 0.0)
+    for name, bound in (("dh0", unit * want["dh0"].abs()), ("db", (unit + own) * want["db"].abs() + TINY[dtype]),
+                        ("da", unit * size * e.abs() * f * om + own * want["da"].abs() + TINY[dtype])):
+        over = (got[name].double().cpu() - want[name]).abs() - bound - 2.0 ** -126
+        assert float(over.max()) <= 0, f"{name}: {float(over.max()):.3e} over"
