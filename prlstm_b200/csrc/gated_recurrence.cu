@@ -214,6 +214,30 @@ template <int VEC> HS_DEV Cols<VEC> shut(Cols<VEC> f) {
   for (int i = 0; i < VEC; ++i) v[i] = v[i] <= FLT_MIN ? 0.f : v[i];
   return Cols<VEC>::of(v);
 }
+template <int VEC> HS_DEV Cols<VEC> least(Cols<VEC> a, Cols<VEC> b) {  // NaN left out
+  float u[VEC], v[VEC];
+  a.get(u);
+  b.get(v);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) u[i] = fminf(u[i], v[i]);
+  return Cols<VEC>::of(u);
+}
+// A product of gates, the least of them `low`: above 0 unless a gate is 0.
+template <int VEC> HS_DEV Cols<VEC> open(Cols<VEC> a, Cols<VEC> low) {
+  float u[VEC], v[VEC];
+  a.get(u);
+  low.get(v);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) u[i] = u[i] == 0.f && v[i] > 0.f ? 0x1p-149f : u[i];
+  return Cols<VEC>::of(u);
+}
+template <int VEC> HS_DEV Cols<VEC> open(Cols<VEC> a) {  // of gates that are all above 0
+  float u[VEC];
+  a.get(u);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(u[i]) : "f"(0x1p-149f));
+  return Cols<VEC>::of(u);
+}
 // Whether a product of gates is so small that one of them may be.
 template <int VEC> HS_DEV bool tiny(Cols<VEC> a) {
   float v[VEC];
@@ -278,8 +302,8 @@ template <int VEC> HS_DEV bool any_nan(Cols<VEC> h) {
   return r;
 }
 
-// A product of gates is at most 1, and too small a one is as good as 0: nothing
-// grows again.  A product of given coefficients may be no float32 of full precision although
+// A product of gates is at most 1, and too small a one is as good as 0, as nothing
+// grows again; but it is held to 2^-149 where no gate is 0, so that an infinite state stays one.  A product of given coefficients may be no float32 of full precision although
 // the states are: growth by 1.5 a step takes 1e-20 to 1e25 in 256 steps, by a
 // factor of 1e45.  Products are chained as they are all the same, and the states looked at:
 //   - An infinite or NaN product leaves a state that is infinite or NaN, and so do
@@ -446,8 +470,8 @@ HS_DEV void send(const void *p, int rank, const void *bar, const Exponent<1> &t)
                : "memory");
 }
 
-// Publishes this warp's map of wave w.
-template <int VEC, bool GATED, bool STARTS>
+// Publishes this warp's map of wave w.  SHUT: gates may be 0 (the forward's).
+template <int VEC, bool GATED, bool STARTS, bool SHUT>
 HS_DEV void publish(const Maps<VEC> &m, int w, int warps, int warp, int lane, int cluster, int rank, Cols<VEC> A, Cols<VEC> B,
                     bool cut) {
   const int p = w & 1;
@@ -464,7 +488,7 @@ HS_DEV void publish(const Maps<VEC> &m, int w, int warps, int warp, int lane, in
   if (cluster == 1) return;
   if (warp == 0 && lane == 0) mbar_expect(&m.bar[p], cluster * 32 * (unsigned)sizeof(Map<VEC>));
   if (warp == warps - 1) {  // the CTA's map, to every CTA of the cluster
-    Cols<VEC> ta = Cols<VEC>::all(1.f), tb = Cols<VEC>::all(0.f);
+    Cols<VEC> ta = Cols<VEC>::all(1.f), tb = Cols<VEC>::all(0.f), least_a = ta;
     bool any = false;
     float top = 0.f, grown = 0.f, low = FLT_MAX;
 #pragma unroll 4
@@ -473,6 +497,7 @@ HS_DEV void publish(const Maps<VEC> &m, int w, int warps, int warp, int lane, in
       if (STARTS) any |= e.cut();
       tb = apply(e, tb);
       ta = Cols<VEC>::of(e.a) * ta;
+      if (GATED && SHUT) least_a = least<VEC>(least_a, Cols<VEC>::of(e.a));
       if (!GATED) {
         largest<VEC>(top, tb);
         largest<VEC>(grown, ta);
@@ -484,6 +509,7 @@ HS_DEV void publish(const Maps<VEC> &m, int w, int warps, int warp, int lane, in
       tb = Cols<VEC>::all(0.f);
       for (int j = 0; j < warps; ++j) tb = apply_marked(all[j * 32], tb);
     }
+    if (GATED) ta = SHUT ? open<VEC>(ta, least_a) : open<VEC>(ta);
     Map<VEC> t;
     ta.get(t.a);
     tb.get(t.b);
@@ -866,17 +892,20 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
       }
       if (GATED && tiny<VEC>(A)) {
         A = C::all(1.f), B = C::all(0.f);
+        C low = A;
 #pragma unroll
         for (int k = 0; k < kRun; ++k) {
           f[k] = shut<VEC>(f[k]);
           A = A * f[k];
           B = fma(f[k], B, b[k]);
+          low = least<VEC>(low, f[k]);
         }
+        A = open<VEC>(A, low);
       }
     }
     if (w == 0) exchange_ready(cluster);
     // (every warp has read its inputs once all have published)
-    publish<VEC, GATED, STARTS>(maps, w, warps, warp, lane, cluster, rank, A, B, mask != 0);
+    publish<VEC, GATED, STARTS, true>(maps, w, warps, warp, lane, cluster, rank, A, B, mask != 0);
     fetch(w + kStages);
     C h = enter<VEC, GATED, STARTS>(maps, w, round, warps, warp, lane, cluster, rank, live, mask != 0, [&](int k) { return f[k]; }, state, p.status);
     if (len > 0) {
@@ -1126,8 +1155,9 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
         A = A * f;
       }
     }
+    if (GATED) A = open<VEC>(A);  // (2^-126 at least)
     if (w == 0) exchange_ready(cluster);
-    publish<VEC, GATED, STARTS>(maps, w, warps, warp, lane, cluster, rank, A, B, mask != 0);
+    publish<VEC, GATED, STARTS, false>(maps, w, warps, warp, lane, cluster, rank, A, B, mask != 0);
     fetch(w + kStages);
     C u = enter<VEC, GATED, STARTS>(maps, w, round, warps, warp, lane, cluster, rank, live, mask != 0, coef, state, p.status);
     if (len > 0) {

@@ -563,3 +563,31 @@ def test_gradient_through_small_gates(shape, dtype, starts):
                         ("da", unit * size * e.abs() * f * om + own * want["da"].abs() + TINY[dtype])):
         over = (got[name].double().cpu() - want[name]).abs() - bound - 2.0 ** -126
         assert float(over.max()) <= 0, f"{name}: {float(over.max()):.3e} over"
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("logit", [2.0, 0.0, -20.0])
+@pytest.mark.parametrize("T,H", [(40, 32), (3000, 32), (3000, 33), (3000, 34), (600, 4096)])
+def test_an_infinite_state_outlasts_any_number_of_gates(T, H, logit, dtype):
+    """Times a gate above 0 it stays infinite, over runs and CTAs whose product of
+    gates is no float32; a start ends it.  The gradient's chain is alike."""
+    inf = float("inf")
+    z = torch.full((T, 1, H), logit, dtype=dtype, device=DEV).requires_grad_(True)
+    x = torch.ones(T, 1, H, dtype=dtype, device=DEV).requires_grad_(True)
+    h0 = torch.full((1, H), inf, device=DEV)
+    h0[:, ::3] = -inf
+    start = torch.zeros(1, H, device=DEV).requires_grad_(True)
+    for at in (None, T // 2 + 3):
+        s = None
+        if at is not None:
+            s = torch.zeros(T, 1, dtype=torch.bool, device=DEV)
+            s[at] = True
+        h, h_n = call("gated")(z, x, h0, starts=s)
+        end = T if at is None else at
+        assert h[:end, :, ::3].isneginf().all() and h[:end, :, 1::3].isposinf().all()
+        assert h[end:].isfinite().all() and (at is not None or torch.equal(h_n, h0))
+        _, h_n = call("gated")(z, x, start, starts=s)
+        dx, d0 = torch.autograd.grad(h_n, (x, start), h0)
+        first = 0 if at is None else at
+        assert dx[first:, :, ::3].isneginf().all() and dx[first:, :, 1::3].isposinf().all()
+        assert not dx[:first].any() and (at is not None or torch.equal(d0, h0))
