@@ -12,6 +12,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -34,7 +35,12 @@ def _dtype_code(who, t):
 
 
 def _device_index(who, first, *rest):
-    """The index of the CUDA device that all tensors are on."""
+    """The index of the CUDA device that all tensors are on.  Tensors that carry a
+    forward-mode tangent are refused here: the results would have lost it."""
+    if forward_ad._current_level >= 0:
+        for t in (first, *rest):
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{who} has no forward-mode derivative (its gradients are reverse-mode)")
     index = first.get_device()
     if index < 0:
         raise RuntimeError("prlstm_b200 runs on CUDA devices (B200, sm_100a) only; "
