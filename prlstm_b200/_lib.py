@@ -178,7 +178,7 @@ class HostStatus:
     word, where a nonzero value makes every later wait give up at once)."""
 
     def __init__(self):
-        self.words = torch.zeros(2, dtype=torch.int32, pin_memory=True)
+        self.words = torch.zeros(2, dtype=torch.int32, device="cpu", pin_memory=True)  # whatever torch's default device is
         self.timeout_ptr = self.words.data_ptr()
         self.token_ptr = self.timeout_ptr + 4
         self.both = ctypes.c_int64.from_address(self.timeout_ptr)  # both words in one read
