@@ -193,7 +193,10 @@ class HostStatus:
 def host_status(index: int) -> HostStatus:
     s = _host_status.get(index)
     if s is None:
-        s = _host_status[index] = HostStatus()
+        with _lock:  # one for all threads: launches hold its address for good
+            s = _host_status.get(index)
+            if s is None:
+                s = _host_status[index] = HostStatus()
     return s
 
 
