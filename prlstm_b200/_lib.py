@@ -261,11 +261,12 @@ def check_device_status(device=None):
 
 
 def clear_device_status(device=None):
+    """Clear the device's status words, after everything launched on it so far."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     call("hs_clear_status", ptr(status_word(device)), stream_ptr(device))
     host = _host_status.get(device.index if device.index is not None else torch.cuda.current_device())
     if host is not None:
-        torch.cuda.current_stream(device).synchronize()
+        torch.cuda.synchronize(device)  # launches on any stream may still write the words
         host.words.zero_()
     idx = device.index if device.index is not None else torch.cuda.current_device()
     _pending.pop(idx, None)

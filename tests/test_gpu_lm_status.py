@@ -31,3 +31,25 @@ assert P.embedding(torch.tensor([1, 0]), z[0]).shape == (2, 8)
 assert P.token_logprobs(z[0], torch.tensor([1, 2]), top=2).top_index.shape == (2, 2)
 P.check_device_status()
 """)
+
+
+def test_clearing_waits_for_every_stream():
+    """A bad id still on its way on another stream is cleared, too, not reported by the next call."""
+    import prlstm_b200 as P
+
+    table, good, bad = torch.randn(10, 8, device=DEV), torch.tensor([1], device=DEV), torch.tensor([99], device=DEV)
+    P.embedding(good, table)
+    P.clear_device_status()
+    side = torch.cuda.Stream(DEV)
+    side.wait_stream(torch.cuda.current_stream(DEV))
+    try:
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(200_000_000)  # about a tenth of a second
+            P.embedding(bad, table)
+        P.clear_device_status()
+        side.synchronize()
+        P.embedding(good, table)
+        P.check_device_status()
+    finally:
+        side.synchronize()
+        P.clear_device_status()
