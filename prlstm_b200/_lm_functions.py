@@ -9,6 +9,7 @@ refused, as in ``HeadStartLSTM``.
 
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import NamedTuple, Optional
 
 import torch
@@ -83,6 +84,18 @@ def _once(backward):
     return run
 
 
+def _apply(fn):
+    """``fn.apply``; the wrapper that torch puts around it is for functorch transforms
+    (which refuse these functions) and left out where none is active, 5 us a call."""
+    plain = super(torch.autograd.Function, fn).apply
+    transforms = torch._C._are_functorch_transforms_active
+
+    def apply(*args):
+        return fn.apply(*args) if transforms() else plain(*args)
+
+    return apply
+
+
 # ------------------------------------------------------------------ recurrence
 def _rows(t):
     """`t` with its last axis contiguous (a copy only where it is not)."""
@@ -152,6 +165,9 @@ class RecurrenceFn(torch.autograd.Function):
         return dz, dx, dh0, None, None, None, None, None
 
 
+_recurrence_apply = _apply(RecurrenceFn)
+
+
 def _state(t):
     """A [B, H] state as the library takes it."""
     return t if t.dtype is torch.float32 and t.is_contiguous() else t.float().contiguous()
@@ -177,7 +193,7 @@ def _recurrence(who, form, z, x, h0, starts, batch_first):
     _lib.host_status(index).check()
     z, x = _rows(z), _rows(x)
     if torch.is_grad_enabled() and (z.requires_grad or x.requires_grad or (h0 is not None and h0.requires_grad)):
-        return RecurrenceFn.apply(z, x, h0, starts, code, index, form, batch_first)
+        return _recurrence_apply(z, x, h0, starts, code, index, form, batch_first)
     return _recurrence_forward(code, index, form, z, x, None if h0 is None else _state(h0), starts, batch_first, False)[:2]
 
 
@@ -254,6 +270,11 @@ def _embedding_forward(code, index, tokens, bits, weight, scale):
     return out
 
 
+@lru_cache(maxsize=64)
+def _embedding_workspace_bytes(N, V, D):
+    return _lib.function("hs_embedding_workspace_bytes")(N, V, D)
+
+
 class EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, tokens, code, index, bits, scale, padding_idx):
@@ -269,12 +290,15 @@ class EmbeddingFn(torch.autograd.Function):
         V, D = shape
         N = tokens.numel()
         dout = dout if dout.is_contiguous() else dout.contiguous()
-        dweight = torch.empty(shape, dtype=dout.dtype, device=dout.device)
-        nbytes = _lib.function("hs_embedding_workspace_bytes")(N, V, D)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dout.device)
+        dweight = dout.new_empty(shape)
+        nbytes = _embedding_workspace_bytes(N, V, D)
+        ws = dout.new_empty(nbytes // dout.element_size())  # (a multiple of 256 bytes)
         _call("hs_embedding_backward", index, code, dout.data_ptr(), bits, tokens.data_ptr(), padding_idx, scale,
               dweight.data_ptr(), N, V, D, ws.data_ptr(), nbytes, _lib.host_status(index).token_ptr)
         return dweight, None, None, None, None, None, None
+
+
+_embedding_apply = _apply(EmbeddingFn)
 
 
 def embedding(tokens, weight, scale: float = 1.0, padding_idx: Optional[int] = None):
@@ -301,7 +325,7 @@ def embedding(tokens, weight, scale: float = 1.0, padding_idx: Optional[int] = N
             raise RuntimeError(f"{who}: padding_idx {padding_idx} is outside the table of {V} rows")
     _lib.host_status(index).check()
     if weight.requires_grad and torch.is_grad_enabled():
-        return EmbeddingFn.apply(weight, tokens, code, index, bits, float(scale), pad)
+        return _embedding_apply(weight, tokens, code, index, bits, float(scale), pad)
     return _embedding_forward(code, index, tokens, bits, weight, float(scale))
 
 
@@ -353,6 +377,9 @@ class TokenLogprobsFn(torch.autograd.Function):
         return dlogits, None, None, None, None, None, None, None
 
 
+_token_logprobs_apply = _apply(TokenLogprobsFn)
+
+
 def token_logprobs(logits, tokens, top: int = 0, temperature: float = 1.0, ignore_index: int = -100) -> TokenLogprobs:
     """Log probabilities (in nats) of ``tokens`` [...] under
     ``softmax(logits / temperature)``, logits [..., V], with the entropy of
@@ -385,7 +412,7 @@ def token_logprobs(logits, tokens, top: int = 0, temperature: float = 1.0, ignor
         rows = rows.contiguous()
     _lib.host_status(index).check()
     if rows.requires_grad and torch.is_grad_enabled():
-        lp, ent, top_lp, top_id = TokenLogprobsFn.apply(rows, tokens, code, index, bits, top, temperature, ignore_index)
+        lp, ent, top_lp, top_id = _token_logprobs_apply(rows, tokens, code, index, bits, top, temperature, ignore_index)
     else:
         lp, ent, top_lp, top_id, _ = _logprobs_forward(code, index, rows, tokens, bits, top, temperature, ignore_index, False)
     if len(shape) != 1:

@@ -45,6 +45,8 @@ def test_forward_mode_is_refused(name):
         torch.func.jvp(call, (t,), (torch.ones_like(t),))
     with pytest.raises((RuntimeError, NotImplementedError)):
         torch.func.vmap(call)(t[None])
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.grad(lambda t: (out := call(t), out if isinstance(out, torch.Tensor) else out[0])[1].sum())(t)
     leaves = [got, want] if isinstance(got, torch.Tensor) else list(zip(got, want))
     for pair in ([leaves] if isinstance(got, torch.Tensor) else leaves):
         assert pair[0] is pair[1] or torch.equal(pair[0], pair[1])
