@@ -512,7 +512,7 @@ HS_API int hs_recurrence_forward(int dtype, int form, const void *z, int64_t z_t
 /* Its gradient: dh [T,B,H] and dh_n [B,H] (either may be NULL = zeros) to dz,
  * dx [T,B,H] and dh0 [B,H] (NULL = not wanted).  Reads the forward's
  * checkpoints, not h: the states are recomputed in float32.  with_starts says
- * whether the forward had starts; they are in the checkpoints. */
+ * whether the forward had starts; they are in the checkpoints.  dh0 may be dh_n itself. */
 HS_API int hs_recurrence_backward(int dtype, int form, const void *z, int64_t z_t, int64_t z_b, const void *x,
                                   int64_t x_t, int64_t x_b, const float *checkpoints, int with_starts,
                                   const void *dh, int64_t dh_t, int64_t dh_b, const float *dh_n, void *dz,

@@ -950,16 +950,18 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
       }
     }
   }
+  if (MOVE == kTiles && lane == 0) bulk_wait_read();
+  // no CTA leaves before the others are done with its memory, nor is the last state
+  // written where it takes the place of the first before all have read that
+  if (cluster > 1) {
+    if (p.h_n && p.h_n == p.h0) cluster_arrive(); else cluster_arrive_relaxed();  // (to release waits for all outputs, 1 us)
+    cluster_wait();
+  }
   if (p.h_n && live && rank == 0 && warp == 0) {
     float v[VEC];
     state.get(v);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) p.h_n[row * p.state_b + col + i] = v[i];
-  }
-  if (MOVE == kTiles && lane == 0) bulk_wait_read();
-  if (cluster > 1) {  // no CTA leaves before the others are done with its memory
-    cluster_arrive_relaxed();
-    cluster_wait();
   }
 }
 
@@ -1206,16 +1208,18 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
       }
     }
   }
+  if (MOVE == kTiles && lane == 0) bulk_wait_read();
+  // no CTA leaves before the others are done with its memory, nor is dh0 written,
+  // where it takes the place of dh_n before all have read that
+  if (cluster > 1) {
+    if (p.dh0 && p.dh0 == p.dh_n) cluster_arrive(); else cluster_arrive_relaxed();
+    cluster_wait();
+  }
   if (p.dh0 && live && rank == 0 && warp == 0) {
     float last[VEC];
     state.get(last);
 #pragma unroll
     for (int v = 0; v < VEC; ++v) p.dh0[row * p.state_b + col + v] = last[v];
-  }
-  if (MOVE == kTiles && lane == 0) bulk_wait_read();
-  if (cluster > 1) {  // no CTA leaves before the others are done with its memory
-    cluster_arrive_relaxed();
-    cluster_wait();
   }
 }
 

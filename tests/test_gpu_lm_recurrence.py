@@ -591,3 +591,28 @@ def test_an_infinite_state_outlasts_any_number_of_gates(T, H, logit, dtype):
         first = 0 if at is None else at
         assert dx[first:, :, ::3].isneginf().all() and dx[first:, :, 1::3].isposinf().all()
         assert not dx[:first].any() and (at is not None or torch.equal(d0, h0))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+@pytest.mark.parametrize("form", ["gated", "linear"])
+@pytest.mark.parametrize("T,H", [(1, 70), (40, 64), (2048, 64), (700, 4096), (2049, 33)])
+def test_states_in_place(T, H, form, dtype):
+    """The library's calls write the last state over the first, and dh0 over dh_n."""
+    from prlstm_b200 import _lib
+    from prlstm_b200 import _lm_functions as F
+
+    a, b, h0, _, dh, dh_n = (None if t is None else t.to(DEV) for t in make(T, 1, H, dtype, form, seed=T))
+    code, kind, index, strides = F._CODE[dtype], 0 if form == "gated" else 1, 0, (H, H)
+    ckpt = torch.empty(_lib.function("hs_recurrence_checkpoint_bytes")(T, 1, H) // 4, dtype=torch.float32, device=DEV)
+    status = _lib.host_status(0).timeout_ptr
+    got = []
+    for here in (False, True):
+        first, grad = h0.clone(), dh_n.clone()
+        last, d0 = (first, grad) if here else (torch.empty_like(h0), torch.empty_like(h0))
+        h, da, db = torch.empty_like(a), torch.empty_like(a), torch.empty_like(a)
+        F._call("hs_recurrence_forward", index, code, kind, a.data_ptr(), *strides, b.data_ptr(), *strides, first.data_ptr(), None, 0, 0,
+                h.data_ptr(), *strides, last.data_ptr(), ckpt.data_ptr(), T, 1, H, status)
+        F._call("hs_recurrence_backward", index, code, kind, a.data_ptr(), *strides, b.data_ptr(), *strides, ckpt.data_ptr(), 0,
+                dh.data_ptr(), *strides, grad.data_ptr(), da.data_ptr(), *strides, db.data_ptr(), *strides, d0.data_ptr(), T, 1, H, status)
+        got.append([t.clone() for t in (h, last, da, db, d0)])
+    assert all(torch.equal(x, y) for x, y in zip(*got))

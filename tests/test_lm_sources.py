@@ -43,3 +43,14 @@ def test_stores_precede_bulk_copies_into_the_same_place():
     body = body[:body.index("\n}\n")]
     stores, fence = body.rindex("st.shared.u16"), body.find("fence_async();")
     assert stores < fence < body.index("cp.async.bulk.shared::cluster")
+
+
+@pytest.mark.parametrize("kernel,store", [("rec_fwd_kernel", "p.h_n[row"), ("rec_bwd_kernel", "p.dh0[row")])
+def test_last_states_are_written_after_all_have_read_the_first(kernel, store):
+    """h_n may be h0 (dh0 may be dh_n), which every CTA of a cluster reads: the store
+    stands behind the barrier that ends the cluster's work."""
+    text = source("gated_recurrence.cu")
+    body = text[text.index(kernel + "(const __grid_constant__"):]
+    at = body.index(store)
+    assert body.rindex("cluster_arrive();", 0, at) < body.rindex("cluster_wait();", 0, at) < at
+    assert "for (int w = 0; w < waves" not in body[body.rindex("cluster_arrive();", 0, at):at]
