@@ -971,10 +971,11 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
   extern __shared__ __align__(128) unsigned char dyn[];
   __shared__ uint64_t full[kStages * kBwdWarps], swap[4];
   using C = Cols<VEC>;
-  // float32 keeps both f and 1-f.  The 16-bit types, two columns to a lane, have
-  // registers for one value and keep e^-z, from which gate_of() gives both again, the
-  // same bits (1-f alone would leave f with the error 2^-25, all of a small gate)
-  constexpr bool kBoth = GATED && VEC == 1, kExp = GATED && VEC == 2;
+  // float32 keeps both f and 1-f.  The 16-bit types have registers for one value (two
+  // columns to a lane, or as many loads on their way) and keep e^-z, from which
+  // gate_of() gives both again, the same bits (1-f alone would leave f with the error
+  // 2^-25, all of a small gate)
+  constexpr bool kBoth = GATED && sizeof(T) == 4, kExp = GATED && sizeof(T) == 2;
   const int lane = threadIdx.x, warp = threadIdx.y, warps = blockDim.y;
   const int cluster = p.s.cluster, rank = (int)(blockIdx.x % cluster), waves = p.s.waves;
   const int64_t gid = blockIdx.x / cluster;
