@@ -587,11 +587,14 @@ HS_DEV Cols<VEC> resolve_exact(const Maps<VEC> &m, int w, int round, int warps, 
   return runs(0, warp, in);
 }
 
+// (Lanes past the last column hold whatever lay in shared memory: what such values
+// call for is not gone into.)
+//
 // The state entering this warp's run of wave w; `state`, the same in every
 // thread of a column, moves from the wave's entry to its end.  `again`: the lanes
 // that need the exact chain (of given coefficients).
 template <int VEC, bool GATED, bool STARTS>
-HS_DEV Cols<VEC> resolve(const Maps<VEC> &m, int w, int warps, int warp, int lane, int cluster, int rank, Cols<VEC> &state, bool &again, int *status) {
+HS_DEV Cols<VEC> resolve(const Maps<VEC> &m, int w, int warps, int warp, int lane, int cluster, int rank, bool live, Cols<VEC> &state, bool &again, int *status) {
   const int p = w & 1;
   const Map<VEC> *all = m.warp + p * warps * 32;
   const Cols<VEC> entry = state;
@@ -605,14 +608,14 @@ HS_DEV Cols<VEC> resolve(const Maps<VEC> &m, int w, int warps, int warp, int lan
       state = apply(all[j * 32], state);
       if (!GATED) largest<VEC>(top, state);
     }
-    if (GATED && STARTS && any_nan(state)) {
+    if (GATED && STARTS && live && any_nan(state)) {
       state = entry;
       for (int j = 0; j < warps; ++j) {
         if (j == warp) in = state;
         state = apply_marked(all[j * 32], state);
       }
     }
-    again = !GATED && is_far<VEC>(top, state);
+    again = !GATED && live && is_far<VEC>(top, state);
     return in;
   }
   mbar_wait(&m.bar[p], (w >> 1) & 1, status);
@@ -627,7 +630,7 @@ HS_DEV Cols<VEC> resolve(const Maps<VEC> &m, int w, int warps, int warp, int lan
   }
 #pragma unroll 4
   for (int j = 0; j < warp; ++j) in = apply(all[j * 32], in);
-  if (GATED && STARTS && (any_nan(state) || any_nan(in))) {
+  if (GATED && STARTS && live && (any_nan(state) || any_nan(in))) {
     state = in = entry;
     for (int r = 0; r < cluster; ++r) {
       if (r == rank) in = state;
@@ -635,7 +638,7 @@ HS_DEV Cols<VEC> resolve(const Maps<VEC> &m, int w, int warps, int warp, int lan
     }
     for (int j = 0; j < warp; ++j) in = apply_marked(all[j * 32], in);
   }
-  again = !GATED && is_far<VEC>(top, state);
+  again = !GATED && live && is_far<VEC>(top, state);
   return in;
 }
 
@@ -645,9 +648,9 @@ HS_DEV Cols<VEC> enter(const Maps<VEC> &m, int w, int &round, int warps, int war
                        Cols<VEC> &state, int *status) {
   Cols<VEC> entry = state;
   bool again;
-  Cols<VEC> in = resolve<VEC, GATED, STARTS>(m, w, warps, warp, lane, cluster, rank, state, again, status);
+  Cols<VEC> in = resolve<VEC, GATED, STARTS>(m, w, warps, warp, lane, cluster, rank, live, state, again, status);
   if constexpr (!GATED) {
-    if (__any_sync(0xffffffffu, again && live)) {
+    if (__any_sync(0xffffffffu, again)) {
       const Cols<VEC> exact = resolve_exact<VEC>(m, w, round, warps, warp, lane, cluster, rank, cut, coef, entry, status);
       if (again) in = exact, state = entry;
       ++round;
@@ -890,7 +893,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps, 1) rec_fwd_kernel(const __grid
         A = A * f[k];
         B = fma(f[k], B, b[k]);
       }
-      if (GATED && tiny<VEC>(A)) {
+      if (GATED && live && tiny<VEC>(A)) {
         A = C::all(1.f), B = C::all(0.f);
         C low = A;
 #pragma unroll
@@ -1141,7 +1144,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1) rec_bwd_kernel(const __grid
       }
     }
     // (what a step at a time gives: a part of a run, and gradients that are infinite or NaN)
-    const bool steps = !kExp || len < kRun || any_nan(B);
+    const bool steps = !kExp || len < kRun || (live && any_nan(B));
     if (steps) A = one, B = zero;
     if (STARTS && mask && steps) {
 #pragma unroll
