@@ -478,7 +478,8 @@ HS_API int hs_recurrent_backward_bf16(const float *x, const float *w_ih, const f
  * Tensors of these calls are float32, bfloat16 or float16 (`dtype`, one type
  * for all `void *` tensors of a call) and aligned to their element; all
  * arithmetic, states and sums are float32.  Extents may be 0.  Every result
- * has one fixed order of operations: the same bits from run to run.
+ * has one fixed order of operations for tensors of one shape, layout and alignment:
+ * the same bits from run to run.
  * dev_status may also be a word of pinned host memory, which the host can then
  * read as it is; where HS_ERR_INDEX may be written it should not be the word of
  * the calls above, whose bounded waits give up at once on a nonzero one.

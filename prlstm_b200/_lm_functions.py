@@ -4,7 +4,8 @@ arguments, allocates tensors and calls the library.
 
 All of them take float32, bfloat16 and float16 CUDA tensors, compute in
 float32 and run on the current stream of the tensors' device.  float64 is
-refused, as in ``HeadStartLSTM``.
+refused, as in ``HeadStartLSTM``.  Gradients are reverse-mode and of first
+order; forward-mode tangents and functorch transforms are refused.
 """
 
 from __future__ import annotations

@@ -26,14 +26,16 @@
 // run, the maps meet in shared memory (distributed over the cluster), and
 // every warp then knows its entering state and writes its outputs from the
 // values it still holds, so every tensor is read and written once.  The order of
-// operations is fixed by the shape alone: results are the same bit for bit
-// from run to run.  No CTA waits on one outside its own cluster.
+// operations follows from the shape, the tensors' strides and alignment, whether there are
+// starts, and the device: a call gives the same bits each time, but not the same as one
+// on another layout.  No CTA waits on one outside its own cluster.
 //
 // Measured on one B200, whose plain copy moves 6.53 TB/s: at T = 16384, B = 8,
-// H = 1024 in bfloat16 the forward with its saved states takes 151 us (5.5 TB/s)
-// and the backward 232 (5.9 TB/s); at T = 16384, B = 1 in float32 the forward
-// takes 33 us (6.0 TB/s).  The forward issues 40 instructions per step of 64
-// bfloat16 columns, two columns to a packed instruction where it can.
+// H = 1024 in bfloat16 the forward with its saved states takes 149 us (5.6 TB/s)
+// and the backward 238 (5.8 TB/s), with starts 168 and 264; at T = 16384, B = 1 in
+// float32 the forward takes 34 us (6.0 TB/s).  Per step of 64 bfloat16 columns the forward
+// issues 43 instructions and the backward 64, two columns to a packed instruction
+// where it can.
 #include <float.h>
 
 #include <algorithm>
@@ -1239,8 +1241,11 @@ struct Plan {
 // What a wave takes, in us: `fixed` + `warp` x the CTA's warps from its inputs
 // to its outputs (+ kHop through the cluster), and at least `move` x the
 // resident warps of an SM for their share of the memory bandwidth (10% more where
-// clusters go in step).  Fitted to runs of every split at T = 128..65536 and
-// 4..2048 column groups; its choice is within 10% of the fastest split of most.
+// clusters go in step).  Fitted to runs of every split of 16-byte-aligned rows at
+// T = 128..65536 and 4..2048 column groups, most of which it is within 10% of the fastest
+// split at.  Rows off 16 bytes go by the same constants, up to a third from the
+// fastest split (2000 x 20 x 301 float16 backward 59.9 us, best 45.9; 7179 x 3 x 364
+// forward 35.4, best 27.1; 4096 x 7 x 1023 float32 133.7, best 95.8).
 struct Pace {
   bool backward;
   int sm_warps;
@@ -1324,7 +1329,8 @@ Plan make_plan(int dtype, int form, bool starts, int64_t T, int64_t B, int64_t H
   pl.groups = (cols + per - 1) / per * rows;
   // Rows off 16 bytes: one by one where the columns are few (7179 x 1092
   // float16, 18 groups: 35 us forward and 44 backward, by lanes 54 and 91), by lanes
-  // where they are many (4096 x 7154 bfloat16, 112 groups: 59 and 102, one by one 67 and 137).
+  // where they are many (4096 x 7154 bfloat16, 112 groups: 59 and 102, one by one 67 and 137);
+  // between those two the bound of 96 groups was not measured.
   if (nchunk > 1 && pl.vec == 4 / es) {
     if (whole && fits(16) && cols <= 0x7fffffff && B <= 0x7fffffff) pl.move = kTiles;
     else if (positive && pl.groups <= 96) pl.move = kRows;
